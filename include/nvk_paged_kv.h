@@ -305,6 +305,106 @@ NVK_API int nvk_lm_head_argmax(const void* hidden, int64_t hidden_stride, const 
                                size_t workspace_bytes, int num_ctas, int* error_word, nvk_stream_t stream);
 
 /*
+ * ---- The KV cache held in 4 bits ----
+ * No counterpart in the reference (its pool is bf16): 144 bytes instead of
+ * 512 per token and KV head, for K and V together.
+ *
+ * A row (128 dims of a token's KV head) is 8 groups of 16 neighbouring dims.
+ * A group has a scale s = e4m3(amax / 6) and 16 codes c = e2m1(x / s), both
+ * rounded to nearest (ties to even) and saturating, of the row x divided by
+ * the layer's constant; it stands for constant * s * c, which bf16 and fp16
+ * hold exactly. k_scale and v_scale are those constants: powers of two in
+ * [2^-60, 2^60] (1 for rows whose groups have maxima between about 0.1 and
+ * 2688; below 6 * 2^-9 precision is lost, above 2688 values saturate). A NaN
+ * makes its group read as NaN, infinities saturate. Every call on a layer
+ * takes the constants that it was appended with.
+ *
+ * kv_cache: ONE layer of the pool, uint8 [num_blocks, num_kv_heads,
+ *   block_size / 16, NVK_FP4_UNIT_BYTES], contiguous, 16-byte aligned; K and V
+ *   together. Slot numbers are those of the bf16 pool. The order of the bytes
+ *   in a unit (16 tokens of one KV head) is described in csrc/fp4_kv.cuh; read
+ *   rows with nvk_fp4_read. Zero-fill the pool once when it is allocated (a
+ *   zero byte is a zero value). Rows past a sequence's context are not used,
+ *   whatever they hold.
+ * Supported: head_dim 128; block_size a power of two in [16, 256]; any number
+ *   of KV heads.
+ */
+#define NVK_FP4_UNIT_TOKENS 16
+#define NVK_FP4_UNIT_BYTES 2304
+
+enum { NVK_DTYPE_BF16 = 0, NVK_DTYPE_FP16 = 1 };
+
+/*
+ * nvk_kv_append into a 4-bit pool: rows of `dtype` [num_tokens, num_kv_heads,
+ * head_dim], 4-byte aligned, key_token_stride / value_token_stride ELEMENTS
+ * between tokens (even). A slot outside the pool is skipped and sets bit 4 of
+ * error_word (may be NULL); a slot must not be given twice with different
+ * rows (it would hold parts of both).
+ */
+NVK_API int nvk_fp4_append(const void* key, const void* value, int64_t key_token_stride, int64_t value_token_stride,
+                           void* kv_cache, const int64_t* slot_mapping, int64_t num_tokens, int num_blocks,
+                           int block_size, int num_kv_heads, int head_dim, int dtype, float k_scale, float v_scale,
+                           int* error_word, nvk_stream_t stream);
+
+/*
+ * The rows that a 4-bit pool holds at slot_mapping, as `dtype` rows key /
+ * value [num_tokens, num_kv_heads, head_dim], contiguous, 16-byte aligned
+ * (exact in bf16; in fp16 unless the constants lead out of its range). A slot
+ * outside the pool gives zeros and sets bit 4 of error_word (may be NULL).
+ */
+NVK_API int nvk_fp4_read(void* key, void* value, const void* kv_cache, const int64_t* slot_mapping,
+                         int64_t num_tokens, int num_blocks, int block_size, int num_kv_heads, int head_dim,
+                         int dtype, float k_scale, float v_scale, int* error_word, nvk_stream_t stream);
+
+/*
+ * nvk_qk_norm_rope_append into a 4-bit pool: query_out as there, the rotated k
+ * and v (bf16) appended as by nvk_fp4_append. The mean square is summed in 64
+ * bits, so that the bf16 rows, and with them the codes, do not hang on the
+ * order of a sum.
+ */
+NVK_API int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, const void* value, int64_t query_stride,
+                                        int64_t key_stride, int64_t value_stride, const void* q_weight,
+                                        const void* k_weight, float eps, const float* cos_table,
+                                        const float* sin_table, int max_position, const int64_t* positions,
+                                        void* query_out, void* kv_cache, const int64_t* slot_mapping,
+                                        int64_t num_tokens, int num_blocks, int block_size, int num_heads,
+                                        int num_kv_heads, int head_dim, float k_scale, float v_scale,
+                                        int* error_word, nvk_stream_t stream);
+
+/*
+ * nvk_paged_decode over a 4-bit pool: softmax(scale * q . K^T) . V over the
+ * values that the first context_lens[b] tokens' codes stand for. out, query:
+ * bf16 [batch, num_heads, head_dim], contiguous; num_heads / num_kv_heads any
+ * of 1 to 8; scale > 0. block_tables and context_lens (device memory) as in
+ * nvk_paged_decode; a length of 0 (or below) yields zeros.
+ * workspace: nvk_fp4_paged_decode_workspace_size bytes, zeroed once; every
+ * call leaves it ready for the next one of any batch, with as many heads, KV
+ * heads and CTAs or with others, as long as it is large enough. Calls that
+ * share one must be ordered on one stream. Its first int is the error word
+ * (bits as for nvk_paged_decode; blocks outside the pool read as zeros).
+ */
+NVK_API int nvk_fp4_paged_decode_workspace_size(int num_heads, int num_kv_heads, int head_dim, int num_ctas,
+                                                size_t* bytes);
+NVK_API int nvk_fp4_paged_decode(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
+                                 const int32_t* block_tables, int block_table_stride, int max_blocks_per_seq,
+                                 const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,
+                                 int head_dim, float scale, float k_scale, float v_scale, int num_ctas,
+                                 void* workspace, size_t workspace_bytes, nvk_stream_t stream);
+
+/*
+ * nvk_paged_prefill over a 4-bit pool (same masking; num_heads any multiple
+ * of num_kv_heads; scale > 0). A sequence longer than max_blocks_per_seq
+ * blocks sets bit 8 of error_word (may be NULL), a block id outside the pool
+ * bit 2; the keys that they would lead to count as rows of zeros. A sequence
+ * whose query rows do not lie in [0, total_q) is skipped and sets bit 8.
+ */
+NVK_API int nvk_fp4_paged_prefill(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
+                                  const int32_t* block_tables, int block_table_stride, int max_blocks_per_seq,
+                                  const int32_t* cu_seqlens_q, const int32_t* kv_lens, int batch, int total_q,
+                                  int max_q_len, int num_heads, int num_kv_heads, int head_dim, float scale,
+                                  float k_scale, float v_scale, int* error_word, nvk_stream_t stream);
+
+/*
  * ---- Prefix-cache index (host code) ----
  * The chained exact-content block keys and key -> cached-blocks map behind
  * BlockManager's prefix cache (src/nanovllm_ascend/npu/block_manager.py:57-65,

@@ -96,7 +96,37 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _i32,
          _i32, _f32, _i32, _c_void_p, _size_t, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p],
     ),
+    "nvk_fp4_append": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _f32,
+         _c_void_p, _c_void_p],
+    ),
+    "nvk_fp4_read": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _c_void_p,
+         _c_void_p],
+    ),
+    "nvk_fp4_qk_norm_rope_append": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _f32, _c_void_p, _c_void_p, _i32,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _c_void_p,
+         _c_void_p],
+    ),
+    "nvk_fp4_paged_decode_workspace_size": (_i32, [_i32, _i32, _i32, _i32, ctypes.POINTER(_size_t)]),
+    "nvk_fp4_paged_decode": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _i32, _i32, _f32,
+         _f32, _f32, _i32, _c_void_p, _size_t, _c_void_p],
+    ),
+    "nvk_fp4_paged_prefill": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32,
+         _i32, _i32, _i32, _f32, _f32, _f32, _c_void_p, _c_void_p],
+    ),
 }
+
+FP4_UNIT_TOKENS = 16
+FP4_UNIT_BYTES = 2304
 
 MAX_PEERS = 8
 PEER_HANDLE_BYTES = 64

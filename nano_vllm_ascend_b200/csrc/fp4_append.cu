@@ -1,0 +1,445 @@
+// Rows into and out of the 4-bit KV pool: the quantising append, the read of
+// rows back, and the attention prologue (per-head RMSNorm of q and k, rotary
+// embedding, append) that writes the pool. The format is in fp4_kv.cuh.
+//
+// HBM-bound byte movement with some arithmetic: per (token, KV head) the
+// append reads 512 B and writes 144 B, the read the other way round. Eight
+// lanes take a row, lane g its dims {16 j + 2 g, 16 j + 2 g + 1}: a group's
+// maximum is three shuffles, each 4-byte load of the eight lanes is one whole
+// 32-byte sector, a lane's eight code bytes are what it stores, and the
+// rotation pairs (i, i + 64) sit in one lane.
+#include "fp4_kv.cuh"
+
+namespace nvk {
+namespace fp4 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRowsPerBlock = kThreads / 8;
+
+template <typename T>
+__device__ __forceinline__ float2 pair_to_f32(uint32_t w);
+template <>
+__device__ __forceinline__ float2 pair_to_f32<__nv_bfloat16>(uint32_t w) {
+  return make_float2(bf16lo_to_f32(w), bf16hi_to_f32(w));
+}
+template <>
+__device__ __forceinline__ float2 pair_to_f32<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t f32_to_pair(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t f32_to_pair<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t f32_to_pair<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct AppendArgs {
+  const uint8_t* key;
+  const uint8_t* value;
+  int64_t key_stride, value_stride;  // bytes between tokens
+  uint8_t* pool;
+  const int64_t* slots;
+  int64_t num_tokens, num_slots;
+  int kvh, upb_log2;
+  float k_inv, v_inv;
+  int* err;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int g = threadIdx.x & 7;
+  const int64_t rows = a.num_tokens * 2 * a.kvh;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRowsPerBlock;
+  // the bound is a whole warp's: its lanes exchange words
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 5) * 4; r0 < rows;
+       r0 += stride) {
+    const int64_t r = r0 + ((threadIdx.x >> 3) & 3);
+    const bool live = r < rows;
+    const int64_t t = live ? r / (2 * a.kvh) : 0;
+    const int kr = live ? static_cast<int>(r - t * 2 * a.kvh) : 0;
+    const bool is_v = kr >= a.kvh;
+    const int head = is_v ? kr - a.kvh : kr;
+    const int64_t slot = live ? a.slots[t] : -1;
+    const bool ok = slot >= 0 && slot < a.num_slots;
+    if (live && !ok && kr == 0 && g == 0 && a.err) atomicOr(a.err, kErrBadSlot);
+    const uint8_t* src = (is_v ? a.value + t * a.value_stride : a.key + t * a.key_stride) + head * (kD * 2) + 4 * g;
+    const float inv = is_v ? a.v_inv : a.k_inv;
+    uint32_t raw[kGroups];
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) raw[j] = ok ? *reinterpret_cast<const uint32_t*>(src + 32 * j) : 0u;
+    float2 x[kGroups];
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      x[j] = pair_to_f32<T>(raw[j]);
+      x[j].x *= inv;
+      x[j].y *= inv;
+    }
+    uint32_t w0, w1, s0, s1;
+    quantise_row(x, w0, w1, s0, s1);
+    store_row(ok ? unit_of(a.pool, slot, head, a.kvh, a.upb_log2) : a.pool, static_cast<int>(slot & 15), is_v, ok, g,
+              w0, w1, s0, s1);
+  }
+}
+
+struct ReadArgs {
+  uint8_t* key;  // [tokens, kvh, 128] contiguous
+  uint8_t* value;
+  uint8_t* pool;
+  const int64_t* slots;
+  int64_t num_tokens, num_slots;
+  int kvh, upb_log2;
+  float k_scale, v_scale;
+  int* err;
+};
+
+// One row a group of eight lanes; the rows of a bad slot come out as zeros.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int g = threadIdx.x & 7;
+  const int64_t rows = a.num_tokens * 2 * a.kvh;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRowsPerBlock;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 3); r < rows; r += stride) {
+    const int64_t t = r / (2 * a.kvh);
+    const int kr = static_cast<int>(r - t * 2 * a.kvh);
+    const bool is_v = kr >= a.kvh;
+    const int head = is_v ? kr - a.kvh : kr;
+    const int64_t slot = a.slots[t];
+    const bool ok = slot >= 0 && slot < a.num_slots;
+    if (!ok && kr == 0 && g == 0 && a.err) atomicOr(a.err, kErrBadSlot);
+    uint2 w = make_uint2(0, 0), sw = make_uint2(0, 0);
+    const int i = static_cast<int>(slot & 15);
+    if (ok) {
+      const uint8_t* unit = unit_of(a.pool, slot, head, a.kvh, a.upb_log2);
+      if (is_v) {
+        w = *reinterpret_cast<const uint2*>(unit + kOffV + 256 * (i >> 2) + 32 * g + 8 * (i & 3));
+        const uint8_t* s = unit + kOffVScale + 32 * (i >> 2) + (i & 3);
+        sw.x = s[0] | (s[4] << 8) | (s[8] << 16) | (static_cast<uint32_t>(s[12]) << 24);
+        sw.y = s[16] | (s[20] << 8) | (s[24] << 16) | (static_cast<uint32_t>(s[28]) << 24);
+      } else {
+        w = *reinterpret_cast<const uint2*>(unit + 64 * i + 8 * g);
+        sw = *reinterpret_cast<const uint2*>(unit + kOffKScale + 8 * i);
+      }
+    }
+    uint32_t c[8], s[4];
+    e2m1_to_half2(w.x, c[0], c[1], c[2], c[3]);
+    e2m1_to_half2(w.y, c[4], c[5], c[6], c[7]);
+    e4m3_to_half2(sw.x, s[0], s[1]);
+    e4m3_to_half2(sw.y, s[2], s[3]);
+    const float mul = is_v ? a.v_scale : a.k_scale;
+    auto scale_of = [&](int j) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&s[j >> 1]);
+      return ((j & 1) ? __high2float(h) : __low2float(h)) * mul;
+    };
+    auto value = [&](int k, float sc) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&c[k]));
+      return f32_to_pair<T>(f.x * sc, f.y * sc);
+    };
+    uint8_t* dst = (is_v ? a.value : a.key) + (t * a.kvh + head) * (kD * 2);
+    if (is_v) {  // byte j: dims 16 j + 2 g and + 1
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) *reinterpret_cast<uint32_t*>(dst + 32 * j + 4 * g) = value(j, scale_of(j));
+    } else {  // bytes 2 k and 2 k + 1: dims 16 j + 4 t .. + 3 of group j = 4 (g % 2) + k, t = g / 2
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float sc = (g & 1) ? scale_of(4 + k) : scale_of(k);
+        *reinterpret_cast<uint2*>(dst + 32 * (4 * (g & 1) + k) + 8 * (g >> 1)) =
+            make_uint2(value(2 * k, sc), value(2 * k + 1, sc));
+      }
+    }
+  }
+}
+
+struct NormArgs {
+  const uint8_t* q;
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t q_stride, k_stride, v_stride;  // bytes between tokens
+  const uint8_t* q_weight;
+  const uint8_t* k_weight;
+  const float* cos_table;  // [max_pos, 128]
+  const float* sin_table;
+  int max_pos;
+  const int64_t* positions;
+  const int64_t* slots;
+  uint8_t* q_out;  // [T, H, 128] contiguous
+  uint8_t* pool;
+  int64_t num_tokens, num_slots;
+  int num_heads, kvh, upb_log2;
+  int chunk;  // head rows per warp item, a multiple of 4
+  float eps, k_inv, v_inv;
+  int* err;
+};
+
+__device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+
+// One warp per chunk of head rows (q heads, then k, then v) of one token, four
+// rows at a time. The rows' arithmetic is the separate operators':
+//   y   = bf16(x * rsqrt(mean(x^2) + eps) * w)
+//   out = bf16(y * cos + rotate_half(y) * sin),  cos and sin cast to bf16.
+// The mean square is summed in 64 bits and its root is correctly rounded, so
+// the bf16 row does not hang on the order of the sum: a row that differed in
+// one bf16 bit could be stored one whole e2m1 step away.
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, g = lane & 7, sub = lane >> 3;
+  const int nrows = a.num_heads + 2 * a.kvh, nqk = a.num_heads + a.kvh;
+  const int chunks = (nrows + a.chunk - 1) / a.chunk;
+  const int64_t items = a.num_tokens * chunks;
+  uint32_t wq[kGroups], wk[kGroups];
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j) {
+    wq[j] = *reinterpret_cast<const uint32_t*>(a.q_weight + 32 * j + 4 * g);
+    wk[j] = *reinterpret_cast<const uint32_t*>(a.k_weight + 32 * j + 4 * g);
+  }
+  const int64_t nw = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += nw) {
+    const int64_t t = w / chunks;
+    const int lo = static_cast<int>(w - t * chunks) * a.chunk, hi = min(lo + a.chunk, nrows);
+    const int64_t slot = a.slots[t];
+    const bool slot_ok = slot >= 0 && slot < a.num_slots;
+    if (!slot_ok && lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrBadSlot);
+    uint32_t cs[kGroups], sn[kGroups];  // bf16 pairs
+    if (lo < nqk) {
+      int64_t p = a.positions[t];
+      if (p < 0 || p >= a.max_pos) {
+        if (lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrContextTooLong);
+        p = p < 0 ? 0 : a.max_pos - 1;
+      }
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        const float* c = a.cos_table + p * kD + 16 * j + 2 * g;
+        const float* s = a.sin_table + p * kD + 16 * j + 2 * g;
+        cs[j] = pack_bf16x2(c[0], c[1]);
+        sn[j] = pack_bf16x2(s[0], s[1]);
+      }
+    }
+    for (int r0 = lo; r0 < hi; r0 += 4) {
+      const int r = r0 + sub;
+      const bool live = r < hi;
+      const bool is_q = r < a.num_heads, is_v = r >= nqk;
+      const uint8_t* src = is_q ? a.q + t * a.q_stride + r * 256
+                           : is_v ? a.v + t * a.v_stride + (r - nqk) * 256
+                                  : a.k + t * a.k_stride + (r - a.num_heads) * 256;
+      uint32_t raw[kGroups];
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+        raw[j] = live ? *reinterpret_cast<const uint32_t*>(src + 32 * j + 4 * g) : 0u;
+      float2 x[kGroups];
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) x[j] = pair_to_f32<__nv_bfloat16>(raw[j]);
+      if (r0 < nqk) {  // some row of this round is normalised (the warp sums together)
+        double ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          const double u = x[j].x, v = x[j].y;
+          ss = fma(v, v, fma(u, u, ss));
+        }
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        const float rinv = __frsqrt_rn(static_cast<float>(ss * (1.0 / kD) + static_cast<double>(a.eps)));
+        if (!is_v) {
+          float2 y[kGroups];
+#pragma unroll
+          for (int j = 0; j < kGroups; ++j) {
+            const float2 wt = pair_to_f32<__nv_bfloat16>(is_q ? wq[j] : wk[j]);
+            y[j].x = round_bf16(x[j].x * rinv * wt.x);
+            y[j].y = round_bf16(x[j].y * rinv * wt.y);
+          }
+          // out[i] = y[i] cos[i] - y[i+64] sin[i];  out[i+64] = y[i+64] cos[i+64] + y[i] sin[i+64]
+          // (products of bf16 are exact in fp32: one rounding each, contracted or not)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 c0 = pair_to_f32<__nv_bfloat16>(cs[j]), c1 = pair_to_f32<__nv_bfloat16>(cs[j + 4]);
+            const float2 n0 = pair_to_f32<__nv_bfloat16>(sn[j]), n1 = pair_to_f32<__nv_bfloat16>(sn[j + 4]);
+            raw[j] = pack_bf16x2(y[j].x * c0.x - y[j + 4].x * n0.x, y[j].y * c0.y - y[j + 4].y * n0.y);
+            raw[j + 4] = pack_bf16x2(y[j + 4].x * c1.x + y[j].x * n1.x, y[j + 4].y * c1.y + y[j].y * n1.y);
+          }
+#pragma unroll
+          for (int j = 0; j < kGroups; ++j) x[j] = pair_to_f32<__nv_bfloat16>(raw[j]);
+        }
+      }
+      if (live && is_q) {
+        uint8_t* dst = a.q_out + (t * a.num_heads + r) * 256 + 4 * g;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) *reinterpret_cast<uint32_t*>(dst + 32 * j) = raw[j];
+      }
+      if (r0 + 3 >= a.num_heads) {  // some row of this round goes to the pool
+        const int head = is_v ? r - nqk : r - a.num_heads;
+        const float inv = is_v ? a.v_inv : a.k_inv;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          x[j].x *= inv;
+          x[j].y *= inv;
+        }
+        uint32_t w0, w1, s0, s1;
+        quantise_row(x, w0, w1, s0, s1);
+        const bool store = live && !is_q && slot_ok;
+        store_row(store ? unit_of(a.pool, slot, head, a.kvh, a.upb_log2) : a.pool, static_cast<int>(slot & 15), is_v,
+                  store, g, w0, w1, s0, s1);
+      }
+    }
+  }
+}
+
+int sm_count() {
+  int sms = 148, dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+}  // namespace
+}  // namespace fp4
+}  // namespace nvk
+
+extern "C" int nvk_fp4_append(const void* key, const void* value, int64_t key_token_stride,
+                              int64_t value_token_stride, void* kv_cache, const int64_t* slot_mapping,
+                              int64_t num_tokens, int num_blocks, int block_size, int num_kv_heads, int head_dim,
+                              int dtype, float k_scale, float v_scale, int* error_word, nvk_stream_t stream) {
+  using namespace nvk;
+  using namespace nvk::fp4;
+  const char* who = "fp4_append";
+  if (num_tokens < 0) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: %lld tokens", who, (long long)num_tokens);
+  int rc = check_pool(kv_cache, num_blocks, block_size, num_kv_heads, head_dim, k_scale, v_scale, who);
+  if (rc != NVK_OK) return rc;
+  if (dtype != NVK_DTYPE_BF16 && dtype != NVK_DTYPE_FP16)
+    return fail(NVK_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or fp16 rows only)", who, dtype);
+  if (num_tokens == 0) return NVK_OK;
+  if (!key || !value || !slot_mapping) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * kD;
+  if (!aligned4(key) || !aligned4(value) || key_token_stride % 2 || value_token_stride % 2 ||
+      (num_tokens > 1 && (key_token_stride < row || value_token_stride < row)))
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: rows must be 4-byte aligned and token strides (%lld, %lld) cover a row",
+                who, (long long)key_token_stride, (long long)value_token_stride);
+  AppendArgs a;
+  a.key = static_cast<const uint8_t*>(key);
+  a.value = static_cast<const uint8_t*>(value);
+  a.key_stride = key_token_stride * 2;
+  a.value_stride = value_token_stride * 2;
+  a.pool = static_cast<uint8_t*>(kv_cache);
+  a.slots = slot_mapping;
+  a.num_tokens = num_tokens;
+  a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
+  a.kvh = num_kv_heads;
+  a.upb_log2 = units_log2(block_size);
+  a.k_inv = 1.f / k_scale;
+  a.v_inv = 1.f / v_scale;
+  a.err = error_word;
+  const int64_t want = (num_tokens * 2 * num_kv_heads + kRowsPerBlock - 1) / kRowsPerBlock;
+  const int64_t most = int64_t(sm_count()) * 8;
+  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return check_cuda(dtype == NVK_DTYPE_BF16 ? launch_pdl(append_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, a)
+                                            : launch_pdl(append_kernel<__half>, grid, dim3(kThreads), 0, st, a),
+                    "fp4_append launch");
+}
+
+extern "C" int nvk_fp4_read(void* key, void* value, const void* kv_cache, const int64_t* slot_mapping,
+                            int64_t num_tokens, int num_blocks, int block_size, int num_kv_heads, int head_dim,
+                            int dtype, float k_scale, float v_scale, int* error_word, nvk_stream_t stream) {
+  using namespace nvk;
+  using namespace nvk::fp4;
+  const char* who = "fp4_read";
+  if (num_tokens < 0) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: %lld tokens", who, (long long)num_tokens);
+  int rc = check_pool(kv_cache, num_blocks, block_size, num_kv_heads, head_dim, k_scale, v_scale, who);
+  if (rc != NVK_OK) return rc;
+  if (dtype != NVK_DTYPE_BF16 && dtype != NVK_DTYPE_FP16)
+    return fail(NVK_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or fp16 rows only)", who, dtype);
+  if (num_tokens == 0) return NVK_OK;
+  if (!key || !value || !slot_mapping) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (!aligned16(key) || !aligned16(value))
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: the rows must be 16-byte aligned", who);
+  ReadArgs a;
+  a.key = static_cast<uint8_t*>(key);
+  a.value = static_cast<uint8_t*>(value);
+  a.pool = static_cast<uint8_t*>(const_cast<void*>(kv_cache));
+  a.slots = slot_mapping;
+  a.num_tokens = num_tokens;
+  a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
+  a.kvh = num_kv_heads;
+  a.upb_log2 = units_log2(block_size);
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.err = error_word;
+  const int64_t want = (num_tokens * 2 * num_kv_heads + kRowsPerBlock - 1) / kRowsPerBlock;
+  const int64_t most = int64_t(sm_count()) * 8;
+  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return check_cuda(dtype == NVK_DTYPE_BF16 ? launch_pdl(read_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, a)
+                                            : launch_pdl(read_kernel<__half>, grid, dim3(kThreads), 0, st, a),
+                    "fp4_read launch");
+}
+
+extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, const void* value,
+                                           int64_t query_stride, int64_t key_stride, int64_t value_stride,
+                                           const void* q_weight, const void* k_weight, float eps,
+                                           const float* cos_table, const float* sin_table, int max_position,
+                                           const int64_t* positions, void* query_out, void* kv_cache,
+                                           const int64_t* slot_mapping, int64_t num_tokens, int num_blocks,
+                                           int block_size, int num_heads, int num_kv_heads, int head_dim,
+                                           float k_scale, float v_scale, int* error_word, nvk_stream_t stream) {
+  using namespace nvk;
+  using namespace nvk::fp4;
+  const char* who = "fp4_qk_norm_rope_append";
+  if (num_tokens < 0 || num_heads <= 0 || max_position <= 0)
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: bad sizes (tokens=%lld heads=%d max_position=%d)", who,
+                (long long)num_tokens, num_heads, max_position);
+  int rc = check_pool(kv_cache, num_blocks, block_size, num_kv_heads, head_dim, k_scale, v_scale, who);
+  if (rc != NVK_OK) return rc;
+  if (num_tokens == 0) return NVK_OK;
+  if (!query || !key || !value || !q_weight || !k_weight || !cos_table || !sin_table || !positions || !query_out ||
+      !slot_mapping)
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (!aligned4(query) || !aligned4(key) || !aligned4(value) || !aligned4(q_weight) || !aligned4(k_weight) ||
+      !aligned4(query_out) || query_stride % 2 || key_stride % 2 || value_stride % 2 ||
+      (num_tokens > 1 && (query_stride < int64_t(num_heads) * kD || key_stride < int64_t(num_kv_heads) * kD ||
+                          value_stride < int64_t(num_kv_heads) * kD)))
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: rows must be 4-byte aligned and strides cover a row", who);
+  NormArgs a;
+  a.q = static_cast<const uint8_t*>(query);
+  a.k = static_cast<const uint8_t*>(key);
+  a.v = static_cast<const uint8_t*>(value);
+  a.q_stride = query_stride * 2;
+  a.k_stride = key_stride * 2;
+  a.v_stride = value_stride * 2;
+  a.q_weight = static_cast<const uint8_t*>(q_weight);
+  a.k_weight = static_cast<const uint8_t*>(k_weight);
+  a.cos_table = cos_table;
+  a.sin_table = sin_table;
+  a.max_pos = max_position;
+  a.positions = positions;
+  a.slots = slot_mapping;
+  a.q_out = static_cast<uint8_t*>(query_out);
+  a.pool = static_cast<uint8_t*>(kv_cache);
+  a.num_tokens = num_tokens;
+  a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
+  a.num_heads = num_heads;
+  a.kvh = num_kv_heads;
+  a.upb_log2 = units_log2(block_size);
+  a.eps = eps;
+  a.k_inv = 1.f / k_scale;
+  a.v_inv = 1.f / v_scale;
+  a.err = error_word;
+  const int sms = sm_count();
+  const int nrows = num_heads + 2 * num_kv_heads;
+  // a whole token per warp (cos and sin loaded once) when the tokens alone give every SM 16 warps
+  a.chunk = num_tokens >= int64_t(sms) * 16 ? (nrows + 3) / 4 * 4 : 4;
+  const int64_t items = num_tokens * ((nrows + a.chunk - 1) / a.chunk);
+  const int64_t want = (items + kThreads / 32 - 1) / (kThreads / 32);
+  const int64_t most = int64_t(sms) * 8;
+  return check_cuda(launch_pdl(norm_rope_kernel, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kThreads),
+                               0, reinterpret_cast<cudaStream_t>(stream), a),
+                    "fp4_qk_norm_rope_append launch");
+}

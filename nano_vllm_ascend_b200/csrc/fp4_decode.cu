@@ -1,0 +1,568 @@
+// Paged decode attention over the 4-bit KV pool, one query token a sequence:
+//   out[b, h] = softmax(scale * q[b, h] . K_b^T) . V_b
+// with K and V the values that the codes of fp4_kv.cuh stand for.
+//
+// HBM-bound: 144 bytes per (token, KV head) are read once. Tensor-core
+// operands are made in registers, on the legacy m16n8k16 path: an A fragment
+// can be filled straight from the packed codes (tcgen05 would need a second
+// trip of four times the bytes through shared memory), and eight query heads
+// are all the columns that there are.
+//   S^T[16 tokens x 8 heads] = K[16 x 128] . Q^T, eight steps of one group each
+//   O^T[16 dims x 8 heads] (8 tiles) += V^T[16 dims x 16 tokens] . P^T
+// K and V are e2m1 -> fp16 (one conversion for two values) times their group's
+// e4m3 scale: exact. Q is scaled by a power of two into fp16's range (entries
+// 2^14 below the row's largest lose bits that a sum of 128 terms does not
+// show); P is kept as 2^7 p in fp16, so 11 bits down to p = 2^-21. Scores,
+// maxima, sums and O are fp32.
+//
+// Schedule: the units (16 tokens) of all (sequence, KV head) pairs, sequence
+// major, are cut into equal contiguous ranges, one per CTA, each cut into
+// equal ranges of its warps. A warp keeps its own running maximum, sum and O;
+// pairs that lie in one warp are written by it, the others' pieces meet in
+// shared memory at the end, and pairs split over CTAs in the workspace, where
+// the CTA that arrives last (a ticket) joins them. Nothing waits for another
+// CTA.
+#include "fp4_kv.cuh"
+
+namespace nvk {
+namespace fp4 {
+namespace {
+
+constexpr int kWarps = 16;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxSeqs = 1024;   // sequences per launch (their prefix of units sits in shared memory)
+constexpr int kMaxCtas = 1024;
+constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
+constexpr int kMinUnits = 2;     // units per warp below which fewer CTAs are used
+constexpr float kRescale = 8.f;  // log2 by which a score may pass the running maximum before O is rescaled
+constexpr float kPShift = 7.f;   // P is held as 2^7 p: p up to 2^8 fits fp16
+constexpr size_t kTicketOffset = 256;
+constexpr size_t kMlOffset = kTicketOffset + kMaxCtas * sizeof(int);
+
+struct DecodeArgs {
+  __nv_bfloat16* out;
+  const __nv_bfloat16* q;
+  const uint8_t* pool;
+  const int32_t* tables;
+  const int32_t* ctx;
+  int* err;
+  int* tickets;  // [CTAs], at zero between calls
+  float2* ws_ml; // [CTAs][2][group] (maximum, sum) of a split pair's piece
+  float* ws_o;   // [CTAs][2][group][128]
+  int batch, heads, kvh, group;
+  int bt_stride, max_blocks, num_blocks, upb_log2;
+  float scale_log2;  // scale * log2(e) * k_scale
+  float v_scale;
+};
+
+// One lane's eight 16-byte-or-less words of a unit.
+struct UnitRegs {
+  uint4 ka, kb, va, vb, vsa, vsb;
+  uint2 ksa, ksb;
+};
+
+struct Smem {
+  int pre[kMaxSeqs + 1];  // units before each sequence (of one KV head)
+  int scan[kWarps];
+  int piece_pair[2 * kWarps];
+  int last[2];
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t dup_lo(uint32_t v) { return __byte_perm(v, v, 0x1010); }
+__device__ __forceinline__ uint32_t dup_hi(uint32_t v) { return __byte_perm(v, v, 0x3232); }
+
+struct State {
+  uint32_t q[kGroups][2];  // the B fragments of Q^T: head lane / 4, dims 16 j + 4 t + {0, 1} and {2, 3}
+  float sc[2];             // log2 factor of the scores of heads 2 t and 2 t + 1
+  float m[2], l[2];        // their running maximum and this lane's part of the sum (times 2^7)
+  float o[kGroups][4];     // O^T: dims 16 j + 2 g (heads 2 t, 2 t + 1), then 16 j + 2 g + 1 (the same)
+};
+
+// Q's rows of one pair as fragments; g = lane / 4, t = lane % 4.
+__device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g, int t, State& st) {
+  uint2 raw[kGroups];
+  const bool live = g < a.group;
+  const __nv_bfloat16* row = a.q + (static_cast<int64_t>(b) * a.heads + h * a.group + (live ? g : 0)) * kD + 4 * t;
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j)
+    raw[j] = live ? *reinterpret_cast<const uint2*>(row + 16 * j) : make_uint2(0, 0);
+  // the row's largest exponent: bf16 magnitudes order as integers
+  uint32_t big = 0;
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j) {
+    big = max(big, max(raw[j].x & 0x7fffu, (raw[j].x >> 16) & 0x7fffu));
+    big = max(big, max(raw[j].y & 0x7fffu, (raw[j].y >> 16) & 0x7fffu));
+  }
+  big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+  big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+  const int e = min(max(static_cast<int>(big >> 7), 27), 227) - 127;  // within 2^+-100
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j) {
+    st.q[j][0] = half2_of(bf16lo_to_f32(raw[j].x) * down, bf16hi_to_f32(raw[j].x) * down);
+    st.q[j][1] = half2_of(bf16lo_to_f32(raw[j].y) * down, bf16hi_to_f32(raw[j].y) * down);
+  }
+  st.sc[0] = __shfl_sync(0xffffffffu, up, 8 * t) * a.scale_log2;
+  st.sc[1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * a.scale_log2;
+  st.m[0] = st.m[1] = -INFINITY;
+  st.l[0] = st.l[1] = 0.f;
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) st.o[j][c] = 0.f;
+}
+
+// One unit: its first `valid` tokens are the sequence's.
+__device__ __forceinline__ void attend(State& st, UnitRegs& u, int valid, int g, int t) {
+  // rows g and g + 8 of the S tile are tokens ta and ta + 2, so that the
+  // transposed P has tokens 4 t .. 4 t + 3 in lane t, whose V words hold them
+  const int ta = 4 * (g >> 1) + (g & 1);
+  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+  {
+    uint32_t sa[4], sb[4];
+    e4m3_to_half2(u.ksa.x, sa[0], sa[1]);
+    e4m3_to_half2(u.ksa.y, sa[2], sa[3]);
+    e4m3_to_half2(u.ksb.x, sb[0], sb[1]);
+    e4m3_to_half2(u.ksb.y, sb[2], sb[3]);
+    const uint32_t wa[4] = {u.ka.x, u.ka.y, u.ka.z, u.ka.w}, wb[4] = {u.kb.x, u.kb.y, u.kb.z, u.kb.w};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {  // a word holds groups 2 w and 2 w + 1
+      uint32_t x[4], y[4];
+      e2m1_to_half2(wa[w], x[0], x[1], x[2], x[3]);
+      e2m1_to_half2(wb[w], y[0], y[1], y[2], y[3]);
+      const uint32_t a0 = dup_lo(sa[w]), a1 = dup_hi(sa[w]), b0 = dup_lo(sb[w]), b1 = dup_hi(sb[w]);
+      mma_16816(s0, hmul2(x[0], a0), hmul2(y[0], b0), hmul2(x[1], a0), hmul2(y[1], b0), st.q[2 * w][0],
+                st.q[2 * w][1]);
+      mma_16816(s1, hmul2(x[2], a1), hmul2(y[2], b1), hmul2(x[3], a1), hmul2(y[3], b1), st.q[2 * w + 1][0],
+                st.q[2 * w + 1][1]);
+    }
+  }
+  float x[4];  // token ta: heads 2 t, 2 t + 1; token ta + 2: the same
+#pragma unroll
+  for (int c = 0; c < 4; ++c) x[c] = (s0[c] + s1[c]) * st.sc[c & 1];
+  if (valid < kUnitTokens) {
+    if (ta >= valid) x[0] = x[1] = -INFINITY;
+    if (ta + 2 >= valid) x[2] = x[3] = -INFINITY;
+    // nor may what these tokens' scale bytes hold get into the sum
+    const int n = min(max(valid - 4 * t, 0), 4);
+    const uint32_t keep = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
+    u.vsa.x &= keep, u.vsa.y &= keep, u.vsa.z &= keep, u.vsa.w &= keep;
+    u.vsb.x &= keep, u.vsb.y &= keep, u.vsb.z &= keep, u.vsb.w &= keep;
+  }
+  const float hi0 = fmaxf(x[0], x[2]), hi1 = fmaxf(x[1], x[3]);
+  if (__any_sync(0xffffffffu, hi0 > st.m[0] + kRescale || hi1 > st.m[1] + kRescale)) {
+    float n0 = hi0, n1 = hi1;
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, off));
+      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
+    }
+    n0 = fmaxf(n0, st.m[0]);
+    n1 = fmaxf(n1, st.m[1]);
+    const float f0 = st.m[0] == -INFINITY ? 0.f : fast_exp2(st.m[0] - n0);
+    const float f1 = st.m[1] == -INFINITY ? 0.f : fast_exp2(st.m[1] - n1);
+    st.m[0] = n0, st.m[1] = n1;
+    st.l[0] *= f0, st.l[1] *= f1;
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+      st.o[j][0] *= f0, st.o[j][2] *= f0;
+      st.o[j][1] *= f1, st.o[j][3] *= f1;
+    }
+  }
+  const float r0 = st.m[0] == -INFINITY ? 0.f : st.m[0] - kPShift;
+  const float r1 = st.m[1] == -INFINITY ? 0.f : st.m[1] - kPShift;
+  const float p0 = fast_exp2(x[0] - r0), p1 = fast_exp2(x[1] - r1);
+  const float p2 = fast_exp2(x[2] - r0), p3 = fast_exp2(x[3] - r1);
+  st.l[0] += p0 + p2;
+  st.l[1] += p1 + p3;
+  const uint32_t b0 = movmatrix(half2_of(p0, p1)), b1 = movmatrix(half2_of(p2, p3));
+  const uint32_t sv[8] = {u.vsa.x, u.vsa.y, u.vsa.z, u.vsa.w, u.vsb.x, u.vsb.y, u.vsb.z, u.vsb.w};
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {  // groups 4 w .. 4 w + 3; tokens 4 t .. 4 t + 3
+    const uint32_t c0 = w ? u.va.y : u.va.x, c1 = w ? u.va.w : u.va.z;
+    const uint32_t c2 = w ? u.vb.y : u.vb.x, c3 = w ? u.vb.w : u.vb.z;
+    constexpr uint32_t kLow = 0x0f0f0f0fu;
+    uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
+    auto spread = [](uint32_t v, uint32_t (&r)[4]) { e2m1_to_half2(v, r[0], r[1], r[2], r[3]); };
+    spread((c0 & kLow) | ((c1 << 4) & ~kLow), lo01);
+    spread(((c0 >> 4) & kLow) | (c1 & ~kLow), hi01);
+    spread((c2 & kLow) | ((c3 << 4) & ~kLow), lo23);
+    spread(((c2 >> 4) & kLow) | (c3 & ~kLow), hi23);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t s01, s23;
+      e4m3_to_half2(sv[4 * w + k], s01, s23);
+      mma_16816(st.o[4 * w + k], hmul2(lo01[k], s01), hmul2(hi01[k], s01), hmul2(lo23[k], s23), hmul2(hi23[k], s23),
+                b0, b1);
+    }
+  }
+}
+
+__device__ __forceinline__ void load_unit(const uint8_t* p, int g, int t, UnitRegs& u) {
+  const int ta = 4 * (g >> 1) + (g & 1);
+  u.ka = *reinterpret_cast<const uint4*>(p + 64 * ta + 16 * t);
+  u.kb = *reinterpret_cast<const uint4*>(p + 64 * (ta + 2) + 16 * t);
+  u.ksa = *reinterpret_cast<const uint2*>(p + kOffKScale + 8 * ta);
+  u.ksb = *reinterpret_cast<const uint2*>(p + kOffKScale + 8 * (ta + 2));
+  u.va = *reinterpret_cast<const uint4*>(p + kOffV + 256 * t + 32 * g);
+  u.vb = *reinterpret_cast<const uint4*>(p + kOffV + 256 * t + 32 * g + 16);
+  u.vsa = *reinterpret_cast<const uint4*>(p + kOffVScale + 32 * t);
+  u.vsb = *reinterpret_cast<const uint4*>(p + kOffVScale + 32 * t + 16);
+}
+
+__device__ __forceinline__ int seq_units(const DecodeArgs& a, int b, bool report) {
+  int n = a.ctx[b];
+  const int64_t most = static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4);
+  if (n > most) {
+    if (report) atomicOr(a.err, kErrContextTooLong);
+    n = static_cast<int>(most);
+  }
+  return n <= 0 ? 0 : (n + kUnitTokens - 1) / kUnitTokens;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  // pieces of pairs that are not one warp's: [2 * kWarps][group] (m, l), then [2 * kWarps][group][128]
+  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + (sizeof(Smem) + 15) / 16 * 16);
+  float* piece_o = reinterpret_cast<float*>(piece_ml + 2 * kWarps * a.group);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- the prefix of units: two sequences a thread ----
+  {
+    const int b = 2 * tid;
+    const int u0 = b < a.batch ? seq_units(a, b, blockIdx.x == 0) : 0;
+    const int u1 = b + 1 < a.batch ? seq_units(a, b + 1, blockIdx.x == 0) : 0;
+    int sum = u0 + u1;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += v;
+    }
+    if (lane == 31) sm.scan[warp] = sum;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < warp; ++w) before += sm.scan[w];
+    const int at = before + sum - u0 - u1;
+    if (b <= a.batch) sm.pre[b] = at;
+    if (b + 1 <= a.batch) sm.pre[b + 1] = at + u0;
+    if (b + 2 == a.batch) sm.pre[b + 2] = at + u0 + u1;
+    if (tid < 2 * kWarps) sm.piece_pair[tid] = -1;
+    if (tid < 2) sm.last[tid] = 0;
+    __syncthreads();
+  }
+  // sequences without context: zeros
+  for (int b = blockIdx.x * kWarps + warp; b < a.batch; b += gridDim.x * kWarps) {
+    if (sm.pre[b + 1] != sm.pre[b]) continue;
+    uint32_t* row = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(b) * a.heads * kD);
+    for (int i = lane; i < a.heads * (kD / 2); i += 32) row[i] = 0;
+  }
+  const int64_t total = static_cast<int64_t>(sm.pre[a.batch]) * a.kvh;
+  if (total == 0) return;
+  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits)));
+  const int c = blockIdx.x;
+  if (c >= ctas) return;
+  const int64_t clo = total * c / ctas, chi = total * (c + 1) / ctas;
+  const int64_t lo = clo + (chi - clo) * warp / kWarps, hi = clo + (chi - clo) * (warp + 1) / kWarps;
+
+  auto find_seq = [&](int64_t x) {  // the sequence that unit x belongs to
+    int b0 = 0, b1 = a.batch;       // pre[b0] * kvh <= x < pre[b1] * kvh
+    while (b1 - b0 > 1) {
+      const int mid = (b0 + b1) >> 1;
+      if (static_cast<int64_t>(sm.pre[mid]) * a.kvh <= x) b0 = mid;
+      else b1 = mid;
+    }
+    return b0;
+  };
+
+  // Writes this warp's result of a pair as a piece (index 2 * warp + slot), or as the output.
+  State st;
+  auto finish = [&](int b, int h, bool whole, int slot) {
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], off);
+      st.l[1] += __shfl_xor_sync(0xffffffffu, st.l[1], off);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int head = 2 * t + e;
+      if (head >= a.group) continue;
+      if (whole) {
+        const float inv = st.l[e] == 0.f ? 0.f : a.v_scale / st.l[e];
+        __nv_bfloat16* row = a.out + (static_cast<int64_t>(b) * a.heads + h * a.group + head) * kD + 2 * g;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j)
+          *reinterpret_cast<uint32_t*>(row + 16 * j) = pack_bf16x2(st.o[j][e] * inv, st.o[j][2 + e] * inv);
+      } else {
+        const int at = (2 * warp + slot) * a.group + head;
+        if (g == 0) piece_ml[at] = make_float2(st.m[e], st.l[e]);
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j)
+          *reinterpret_cast<float2*>(piece_o + at * kD + 16 * j + 2 * g) = make_float2(st.o[j][e], st.o[j][2 + e]);
+      }
+    }
+    if (!whole && lane == 0) sm.piece_pair[2 * warp + slot] = b * a.kvh + h;
+  };
+
+  // ---- this warp's units ----
+  int64_t x = lo;
+  int b = lo < hi ? find_seq(lo) : 0;
+  while (x < hi) {
+    while (sm.pre[b + 1] == sm.pre[b] || static_cast<int64_t>(sm.pre[b + 1]) * a.kvh <= x) ++b;
+    const int units = sm.pre[b + 1] - sm.pre[b];
+    const int64_t in_seq = x - static_cast<int64_t>(sm.pre[b]) * a.kvh;
+    const int h = static_cast<int>(in_seq / units);
+    const int u_lo = static_cast<int>(in_seq - static_cast<int64_t>(h) * units);
+    const int u_hi = static_cast<int>(min(static_cast<int64_t>(units), u_lo + (hi - x)));
+    const int n_tok = min(a.ctx[b], units * kUnitTokens);
+    load_q(a, b, h, g, t, st);
+    for (int u = u_lo; u < u_hi; ++u) {
+      const int blk = a.tables[static_cast<int64_t>(b) * a.bt_stride + (u >> a.upb_log2)];
+      UnitRegs r;
+      if (blk < 0 || blk >= a.num_blocks) {  // reads as zeros
+        if (lane == 0) atomicOr(a.err, kErrBadBlockId);
+        r.ka = r.kb = r.va = r.vb = r.vsa = r.vsb = make_uint4(0, 0, 0, 0);
+        r.ksa = r.ksb = make_uint2(0, 0);
+      } else {
+        const int64_t unit = (((static_cast<int64_t>(blk) * a.kvh + h) << a.upb_log2) + (u & ((1 << a.upb_log2) - 1)));
+        load_unit(a.pool + unit * kUnitBytes, g, t, r);
+      }
+      attend(st, r, min(n_tok - u * kUnitTokens, kUnitTokens), g, t);
+    }
+    finish(b, h, u_lo == 0 && u_hi == units, x == lo ? 0 : 1);
+    x += u_hi - u_lo;
+  }
+  __syncthreads();
+
+  // ---- pieces of one pair meet: lane p of every warp looks at piece p ----
+  const int mine = sm.piece_pair[lane];
+  const uint32_t valid = __ballot_sync(0xffffffffu, mine >= 0);
+  const uint32_t below = valid & ((1u << lane) - 1);
+  const int prev = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
+  const uint32_t starts = __ballot_sync(0xffffffffu, mine >= 0 && (below == 0 || prev != mine));
+  const int tasks = __popc(starts) * a.group;
+  for (int k = warp; k < tasks; k += kWarps) {
+    const int run = k / a.group, head = k - run * a.group;
+    const int first = __fns(starts, 0, run + 1);
+    const int pair = __shfl_sync(0xffffffffu, mine, first);
+    const uint32_t members = __ballot_sync(0xffffffffu, mine == pair);
+    const float2 ml = mine == pair ? piece_ml[lane * a.group + head] : make_float2(-INFINITY, 0.f);
+    float m = ml.x;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - m);
+    float l = ml.y * w;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t left = members; left; left &= left - 1) {
+      const int p = __ffs(left) - 1;
+      const float wp = __shfl_sync(0xffffffffu, w, p);
+      const float4 v = *reinterpret_cast<const float4*>(piece_o + (p * a.group + head) * kD + 4 * lane);
+      o.x += wp * v.x, o.y += wp * v.y, o.z += wp * v.z, o.w += wp * v.w;
+    }
+    const int pb = pair / a.kvh, ph = pair - pb * a.kvh;
+    const int units = sm.pre[pb + 1] - sm.pre[pb];
+    const int64_t plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * units;
+    if (plo >= clo && plo + units <= chi) {
+      const float inv = l == 0.f ? 0.f : a.v_scale / l;
+      *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
+          make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    } else {
+      const int64_t at = (static_cast<int64_t>(c) * 2 + (plo < clo ? 0 : 1)) * a.group + head;
+      if (lane == 0) a.ws_ml[at] = make_float2(m, l);
+      *reinterpret_cast<float4*>(a.ws_o + at * kD + 4 * lane) = o;
+      __threadfence();
+    }
+  }
+  // ---- pairs split over CTAs: the first and the last of this CTA's units ----
+  auto cta_of = [&](int64_t unit) { return static_cast<int>(((unit + 1) * ctas - 1) / total); };
+  auto pair_of = [&](int64_t unit, int& pb, int& ph, int64_t& plo, int& units) {
+    pb = find_seq(unit);
+    while (sm.pre[pb + 1] == sm.pre[pb]) ++pb;
+    units = sm.pre[pb + 1] - sm.pre[pb];
+    ph = static_cast<int>((unit - static_cast<int64_t>(sm.pre[pb]) * a.kvh) / units);
+    plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * units;
+  };
+  __syncthreads();
+  if (tid < 2) {
+    int pb, ph, units;
+    int64_t plo;
+    pair_of(tid == 0 ? clo : chi - 1, pb, ph, plo, units);
+    // end 0: a pair that began before this CTA; end 1: one that begins here and goes on
+    const bool split = tid == 0 ? plo < clo : plo >= clo && plo + units > chi;
+    if (split) {
+      const int c0 = cta_of(plo), c1 = cta_of(plo + units - 1);
+      __threadfence();
+      if (atomicAdd(a.tickets + c0, 1) == c1 - c0) {
+        a.tickets[c0] = 0;  // every piece is in: nobody else touches it in this call
+        sm.last[tid] = 1;
+      }
+    }
+  }
+  __syncthreads();
+  for (int end = 0; end < 2; ++end) {
+    if (!sm.last[end]) continue;
+    __threadfence();
+    int pb, ph, units;
+    int64_t plo;
+    pair_of(end == 0 ? clo : chi - 1, pb, ph, plo, units);
+    const int c0 = cta_of(plo), c1 = cta_of(plo + units - 1);
+    for (int head = warp; head < a.group; head += kWarps) {
+      // the pair's piece in CTA k: its end 1 where it begins, its end 0 after that
+      auto at = [&](int k) { return (static_cast<int64_t>(k) * 2 + (k == c0 ? 1 : 0)) * a.group + head; };
+      float m = -INFINITY;
+      for (int k = c0 + lane; k <= c1; k += 32) m = fmaxf(m, __ldcg(&a.ws_ml[at(k)].x));
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+      float l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int k = c0; k <= c1; ++k) {
+        const float2 ml = __ldcg(&a.ws_ml[at(k)]);
+        const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - m);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(k) * kD + 4 * lane));
+        l += w * ml.y;
+        o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+      }
+      const float inv = l == 0.f ? 0.f : a.v_scale / l;
+      *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
+          make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    }
+  }
+}
+
+size_t workspace_bytes(int group, int ctas) {
+  return kMlOffset + static_cast<size_t>(ctas) * 2 * group * (sizeof(float2) + kD * sizeof(float));
+}
+
+int resolve_ctas(int num_ctas, int* out) {
+  int ctas = num_ctas;
+  if (ctas == 0) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&ctas, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return check_cuda(e, "fp4_paged_decode: SM count");
+  }
+  *out = ctas < kMaxCtas ? ctas : kMaxCtas;
+  return NVK_OK;
+}
+
+int check_heads(int num_heads, int num_kv_heads, int num_ctas, const char* who) {
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_ctas < 0)
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: bad sizes (heads=%d kv_heads=%d ctas=%d)", who, num_heads, num_kv_heads,
+                num_ctas);
+  if (num_heads % num_kv_heads != 0 || num_heads / num_kv_heads > kMaxGroup)
+    return fail(NVK_ERR_UNSUPPORTED, "%s: %d query heads over %d KV heads (a GQA group of 1 to %d)", who, num_heads,
+                num_kv_heads, kMaxGroup);
+  return NVK_OK;
+}
+
+}  // namespace
+}  // namespace fp4
+}  // namespace nvk
+
+extern "C" int nvk_fp4_paged_decode_workspace_size(int num_heads, int num_kv_heads, int head_dim, int num_ctas,
+                                                   size_t* bytes) {
+  using namespace nvk;
+  using namespace nvk::fp4;
+  const char* who = "fp4_paged_decode_workspace_size";
+  if (!bytes) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (head_dim != kD) return fail(NVK_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (128 only)", who, head_dim);
+  int rc = check_heads(num_heads, num_kv_heads, num_ctas, who), ctas = 0;
+  if (rc != NVK_OK || (rc = resolve_ctas(num_ctas, &ctas)) != NVK_OK) return rc;
+  *bytes = workspace_bytes(num_heads / num_kv_heads, ctas);
+  return NVK_OK;
+}
+
+extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv_cache, int num_blocks,
+                                    int block_size, const int32_t* block_tables, int block_table_stride,
+                                    int max_blocks_per_seq, const int32_t* context_lens, int batch, int num_heads,
+                                    int num_kv_heads, int head_dim, float scale, float k_scale, float v_scale,
+                                    int num_ctas, void* workspace, size_t workspace_bytes_given,
+                                    nvk_stream_t stream) {
+  using namespace nvk;
+  using namespace nvk::fp4;
+  const char* who = "fp4_paged_decode";
+  if (batch < 0) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: batch %d", who, batch);
+  int rc = check_heads(num_heads, num_kv_heads, num_ctas, who);
+  if (rc != NVK_OK) return rc;
+  if ((rc = check_pool(kv_cache, num_blocks, block_size, num_kv_heads, head_dim, k_scale, v_scale, who)) != NVK_OK)
+    return rc;
+  if (!(scale > 0.f)) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: scale %g is not positive", who, double(scale));
+  if (max_blocks_per_seq <= 0 || block_table_stride < max_blocks_per_seq)
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: block table stride %d below its %d columns", who, block_table_stride,
+                max_blocks_per_seq);
+  if (batch == 0) return NVK_OK;
+  if (!out || !query || !block_tables || !context_lens || !workspace)
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (!aligned16(out) || !aligned16(query) || !aligned16(workspace))
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: q, out and workspace must be 16-byte aligned", who);
+  const int upb_log2 = units_log2(block_size);
+  const int64_t seqs = batch < kMaxSeqs ? batch : kMaxSeqs;
+  if (((seqs * max_blocks_per_seq) << upb_log2) > 0x7fffffffll ||
+      (static_cast<int64_t>(max_blocks_per_seq) << upb_log2) > 0x7fffffffll / kUnitTokens)
+    return fail(NVK_ERR_UNSUPPORTED, "%s: %d blocks of %d tokens a sequence are above the kernel's range", who,
+                max_blocks_per_seq, block_size);
+  int ctas = 0;
+  if ((rc = resolve_ctas(num_ctas, &ctas)) != NVK_OK) return rc;
+  const int group = num_heads / num_kv_heads;
+  if (workspace_bytes_given < workspace_bytes(group, ctas))
+    return fail(NVK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes_given,
+                workspace_bytes(group, ctas));
+  const size_t smem =
+      (sizeof(Smem) + 15) / 16 * 16 + static_cast<size_t>(2 * kWarps) * group * (sizeof(float2) + kD * sizeof(float));
+  const size_t most = (sizeof(Smem) + 15) / 16 * 16 +
+                      static_cast<size_t>(2 * kWarps) * kMaxGroup * (sizeof(float2) + kD * sizeof(float));
+  if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&decode_kernel), most)) != NVK_OK) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  DecodeArgs a;
+  a.pool = static_cast<const uint8_t*>(kv_cache);
+  a.err = reinterpret_cast<int*>(ws);
+  a.tickets = reinterpret_cast<int*>(ws + kTicketOffset);
+  a.ws_ml = reinterpret_cast<float2*>(ws + kMlOffset);
+  a.ws_o = reinterpret_cast<float*>(ws + kMlOffset + static_cast<size_t>(ctas) * 2 * group * sizeof(float2));
+  a.heads = num_heads;
+  a.kvh = num_kv_heads;
+  a.group = group;
+  a.bt_stride = block_table_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_blocks = num_blocks;
+  a.upb_log2 = upb_log2;
+  a.scale_log2 = scale * 1.4426950408889634f * k_scale;
+  a.v_scale = v_scale;
+  for (int b0 = 0; b0 < batch; b0 += kMaxSeqs) {
+    a.batch = batch - b0 < kMaxSeqs ? batch - b0 : kMaxSeqs;
+    a.out = static_cast<__nv_bfloat16*>(out) + static_cast<int64_t>(b0) * num_heads * kD;
+    a.q = static_cast<const __nv_bfloat16*>(query) + static_cast<int64_t>(b0) * num_heads * kD;
+    a.tables = block_tables + static_cast<int64_t>(b0) * block_table_stride;
+    a.ctx = context_lens + b0;
+    if ((rc = check_cuda(launch_pdl(decode_kernel, dim3(ctas), dim3(kThreads), smem,
+                                    reinterpret_cast<cudaStream_t>(stream), a),
+                         "fp4_paged_decode launch")) != NVK_OK)
+      return rc;
+  }
+  return NVK_OK;
+}
