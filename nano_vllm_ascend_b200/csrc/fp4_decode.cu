@@ -15,6 +15,11 @@
 // show); P is kept as 2^7 p in fp16, so 11 bits down to p = 2^-21. Scores,
 // maxima, sums and O are fp32.
 //
+// Data: every warp streams its units through a ring of its own in shared
+// memory, one bulk copy (2304 contiguous bytes) a unit, four in flight. With
+// 16 warps that is 147 KB in flight an SM, three times what hides the latency
+// of HBM at full rate, and no warp waits for another one's data.
+//
 // Schedule: the units (16 tokens) of all (sequence, KV head) pairs, sequence
 // major, are cut into equal contiguous ranges, one per CTA, each cut into
 // equal ranges of its warps. A warp keeps its own running maximum, sum and O;
@@ -30,6 +35,7 @@ namespace {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
+constexpr int kStages = 4;       // units in flight a warp
 constexpr int kMaxSeqs = 1024;   // sequences per launch (their prefix of units sits in shared memory)
 constexpr int kMaxCtas = 1024;
 constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
@@ -62,6 +68,8 @@ struct UnitRegs {
 };
 
 struct Smem {
+  alignas(128) uint8_t ring[kWarps][kStages][kUnitBytes];  // a warp's last piece comes here when it has read them
+  uint64_t full[kWarps][kStages];
   int pre[kMaxSeqs + 1];  // units before each sequence (of one KV head)
   int scan[kWarps];
   int piece_pair[2 * kWarps];
@@ -230,6 +238,11 @@ __device__ __forceinline__ void load_unit(const uint8_t* p, int g, int t, UnitRe
   u.vsb = *reinterpret_cast<const uint4*>(p + kOffVScale + 32 * t + 16);
 }
 
+__device__ __forceinline__ void zero_unit(UnitRegs& u) {
+  u.ka = u.kb = u.va = u.vb = u.vsa = u.vsb = make_uint4(0, 0, 0, 0);
+  u.ksa = u.ksb = make_uint2(0, 0);
+}
+
 __device__ __forceinline__ int seq_units(const DecodeArgs& a, int b, bool report) {
   int n = a.ctx[b];
   const int64_t most = static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4);
@@ -241,14 +254,25 @@ __device__ __forceinline__ int seq_units(const DecodeArgs& a, int b, bool report
 }
 
 __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
+  extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-  // pieces of pairs that are not one warp's: [2 * kWarps][group] (m, l), then [2 * kWarps][group][128]
-  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + (sizeof(Smem) + 15) / 16 * 16);
-  float* piece_o = reinterpret_cast<float*>(piece_ml + 2 * kWarps * a.group);
+  // Pieces of pairs that are not one warp's: [2 * kWarps][group] (m, l), and
+  // [group][128] each: a warp's first one in its own place, its last one in
+  // the warp's ring.
+  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Smem));
+  float* piece_first = reinterpret_cast<float*>(piece_ml + 2 * kWarps * a.group);
+  auto piece_o = [&](int p) {
+    return (p & 1) ? reinterpret_cast<float*>(sm.ring[p >> 1]) : piece_first + (p >> 1) * a.group * kD;
+  };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&sm.full[warp][s], 1);
+    fence_mbar_init();
+  }
   pdl_launch_dependents();
-  pdl_wait();
+  // The lengths and the tables are step metadata, which no kernel writes that
+  // lets its dependents start early (see the entry point): they are read, and
+  // the schedule made of them, while the kernel before this one drains.
 
   // ---- the prefix of units: two sequences a thread ----
   {
@@ -273,17 +297,22 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
     if (tid < 2) sm.last[tid] = 0;
     __syncthreads();
   }
-  // sequences without context: zeros
-  for (int b = blockIdx.x * kWarps + warp; b < a.batch; b += gridDim.x * kWarps) {
-    if (sm.pre[b + 1] != sm.pre[b]) continue;
-    uint32_t* row = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(b) * a.heads * kD);
-    for (int i = lane; i < a.heads * (kD / 2); i += 32) row[i] = 0;
-  }
+  auto zero_empty = [&] {  // the rows of sequences without context
+    for (int b = blockIdx.x * kWarps + warp; b < a.batch; b += gridDim.x * kWarps) {
+      if (sm.pre[b + 1] != sm.pre[b]) continue;
+      uint32_t* row = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(b) * a.heads * kD);
+      for (int i = lane; i < a.heads * (kD / 2); i += 32) row[i] = 0;
+    }
+  };
   const int64_t total = static_cast<int64_t>(sm.pre[a.batch]) * a.kvh;
-  if (total == 0) return;
-  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits)));
+  const int ctas =
+      static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits)));
   const int c = blockIdx.x;
-  if (c >= ctas) return;
+  if (c >= ctas) {
+    pdl_wait();
+    zero_empty();
+    return;
+  }
   const int64_t clo = total * c / ctas, chi = total * (c + 1) / ctas;
   const int64_t lo = clo + (chi - clo) * warp / kWarps, hi = clo + (chi - clo) * (warp + 1) / kWarps;
 
@@ -320,39 +349,92 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
         if (g == 0) piece_ml[at] = make_float2(st.m[e], st.l[e]);
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
-          *reinterpret_cast<float2*>(piece_o + at * kD + 16 * j + 2 * g) = make_float2(st.o[j][e], st.o[j][2 + e]);
+          *reinterpret_cast<float2*>(piece_o(2 * warp + slot) + head * kD + 16 * j + 2 * g) = make_float2(st.o[j][e], st.o[j][2 + e]);
       }
     }
     if (!whole && lane == 0) sm.piece_pair[2 * warp + slot] = b * a.kvh + h;
   };
 
   // ---- this warp's units ----
-  int64_t x = lo;
-  int b = lo < hi ? find_seq(lo) : 0;
-  while (x < hi) {
-    while (sm.pre[b + 1] == sm.pre[b] || static_cast<int64_t>(sm.pre[b + 1]) * a.kvh <= x) ++b;
+  const int n = static_cast<int>(hi - lo);
+  constexpr int kFirst = 1 << 8, kLast = 1 << 9, kBad = 1 << 10;
+  // What lane i knows of the batch of 32 units that starts at lo + base: where
+  // unit base + i lies, whose it is, and its tokens with the flags above.
+  const uint8_t* next_at = nullptr;
+  int next_pair = 0, next_info = 0;
+  auto look_up = [&](int base) {
+    if (base + lane >= n) return;
+    const int64_t x = lo + base + lane;
+    const int b = find_seq(x);
     const int units = sm.pre[b + 1] - sm.pre[b];
     const int64_t in_seq = x - static_cast<int64_t>(sm.pre[b]) * a.kvh;
     const int h = static_cast<int>(in_seq / units);
-    const int u_lo = static_cast<int>(in_seq - static_cast<int64_t>(h) * units);
-    const int u_hi = static_cast<int>(min(static_cast<int64_t>(units), u_lo + (hi - x)));
-    const int n_tok = min(a.ctx[b], units * kUnitTokens);
-    load_q(a, b, h, g, t, st);
-    for (int u = u_lo; u < u_hi; ++u) {
-      const int blk = a.tables[static_cast<int64_t>(b) * a.bt_stride + (u >> a.upb_log2)];
-      UnitRegs r;
-      if (blk < 0 || blk >= a.num_blocks) {  // reads as zeros
-        if (lane == 0) atomicOr(a.err, kErrBadBlockId);
-        r.ka = r.kb = r.va = r.vb = r.vsa = r.vsb = make_uint4(0, 0, 0, 0);
-        r.ksa = r.ksb = make_uint2(0, 0);
+    const int u = static_cast<int>(in_seq - static_cast<int64_t>(h) * units);
+    const int blk = a.tables[static_cast<int64_t>(b) * a.bt_stride + (u >> a.upb_log2)];
+    next_pair = b * a.kvh + h;
+    next_info = min(a.ctx[b] - u * kUnitTokens, kUnitTokens) | (u == 0 ? kFirst : 0) | (u == units - 1 ? kLast : 0);
+    if (blk < 0 || blk >= a.num_blocks) next_info |= kBad;
+    next_at = a.pool + ((((static_cast<int64_t>(blk) * a.kvh + h) << a.upb_log2) + (u & ((1 << a.upb_log2) - 1))) *
+                        kUnitBytes);
+  };
+  auto fetch = [&](int i) {  // unit i into its stage
+    const uint8_t* at =
+        reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(next_at), i & 31));
+    const int info = __shfl_sync(0xffffffffu, next_info, i & 31);
+    if (lane == 0) {
+      uint64_t* bar = &sm.full[warp][i % kStages];
+      if (info & kBad) {
+        atomicOr(a.err, kErrBadBlockId);
+        mbar_arrive(bar);
       } else {
-        const int64_t unit = (((static_cast<int64_t>(blk) * a.kvh + h) << a.upb_log2) + (u & ((1 << a.upb_log2) - 1)));
-        load_unit(a.pool + unit * kUnitBytes, g, t, r);
+        mbar_arrive_expect_tx(bar, kUnitBytes);
+        bulk_load(sm.ring[warp][i % kStages], at, kUnitBytes, bar);
       }
-      attend(st, r, min(n_tok - u * kUnitTokens, kUnitTokens), g, t);
     }
-    finish(b, h, u_lo == 0 && u_hi == units, x == lo ? 0 : 1);
-    x += u_hi - u_lo;
+  };
+  look_up(0);
+  pdl_wait();
+  zero_empty();
+  int issued = 0;
+  for (; issued < min(n, kStages); ++issued) fetch(issued);
+  int pair_now = next_pair, info_now = next_info;  // the batch that is being read
+  bool ok = true;
+  int b = 0, h = 0;
+  bool whole = false, open = false;
+  int slot = 0;
+  for (int i = 0; i < n; ++i) {
+    if (i > 0 && (i & 31) == 0) pair_now = next_pair, info_now = next_info;
+    const int info = __shfl_sync(0xffffffffu, info_now, i & 31);
+    if (!open) {
+      const int pair = __shfl_sync(0xffffffffu, pair_now, i & 31);
+      b = pair / a.kvh;
+      h = pair - b * a.kvh;
+      load_q(a, b, h, g, t, st);
+      whole = info & kFirst;
+      slot = i == 0 ? 0 : 1;
+      open = true;
+    }
+    const int stage = i % kStages;
+    if (ok && !__all_sync(0xffffffffu, mbar_wait(&sm.full[warp][stage], (i / kStages) & 1))) {
+      ok = false;
+      if (lane == 0) atomicOr(a.err, kErrWaitTimeout);
+    }
+    UnitRegs r;
+    if (!ok || (info & kBad)) zero_unit(r);  // reads as zeros
+    else load_unit(sm.ring[warp][stage], g, t, r);
+    __syncwarp();
+    if (ok && issued < n) {
+      if ((issued & 31) == 0) look_up(issued);
+      fetch(issued);
+      ++issued;
+    }
+    attend(st, r, info & 0xff, g, t);
+    if ((info & kLast) || i == n - 1) {
+      if (!ok)  // the ring takes the piece only after every copy into it has landed or been given up
+        for (int k = max(i, issued - kStages); k < issued; ++k) (void)mbar_wait(&sm.full[warp][k % kStages], (k / kStages) & 1);
+      finish(b, h, whole && (info & kLast), slot);
+      open = false;
+    }
   }
   __syncthreads();
 
@@ -380,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
     for (uint32_t left = members; left; left &= left - 1) {
       const int p = __ffs(left) - 1;
       const float wp = __shfl_sync(0xffffffffu, w, p);
-      const float4 v = *reinterpret_cast<const float4*>(piece_o + (p * a.group + head) * kD + 4 * lane);
+      const float4 v = *reinterpret_cast<const float4*>(piece_o(p) + head * kD + 4 * lane);
       o.x += wp * v.x, o.y += wp * v.y, o.z += wp * v.z, o.w += wp * v.w;
     }
     const int pb = pair / a.kvh, ph = pair - pb * a.kvh;
@@ -453,6 +535,13 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
     }
   }
 }
+
+size_t smem_bytes(int group) {
+  return sizeof(Smem) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
+}
+static_assert(sizeof(Smem) % 16 == 0 && sizeof(Smem) + kWarps * kMaxGroup * (16 + kD * 4) <= 232448,
+              "decode shared memory exceeds the 227 KB per-CTA limit");
+static_assert(kStages * kUnitBytes >= kMaxGroup * kD * 4, "a warp's ring takes its last piece");
 
 size_t workspace_bytes(int group, int ctas) {
   return kMlOffset + static_cast<size_t>(ctas) * 2 * group * (sizeof(float2) + kD * sizeof(float));
@@ -532,10 +621,8 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   if (workspace_bytes_given < workspace_bytes(group, ctas))
     return fail(NVK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes_given,
                 workspace_bytes(group, ctas));
-  const size_t smem =
-      (sizeof(Smem) + 15) / 16 * 16 + static_cast<size_t>(2 * kWarps) * group * (sizeof(float2) + kD * sizeof(float));
-  const size_t most = (sizeof(Smem) + 15) / 16 * 16 +
-                      static_cast<size_t>(2 * kWarps) * kMaxGroup * (sizeof(float2) + kD * sizeof(float));
+  const size_t smem = smem_bytes(group);
+  const size_t most = smem_bytes(kMaxGroup);
   if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&decode_kernel), most)) != NVK_OK) return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
