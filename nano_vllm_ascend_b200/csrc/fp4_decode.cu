@@ -61,14 +61,15 @@ struct DecodeArgs {
   float v_scale;
 };
 
-// One lane's eight 16-byte-or-less words of a unit.
-struct UnitRegs {
-  uint4 ka, kb, va, vb, vsa, vsb;
-  uint2 ksa, ksb;
+// The scales of one unit, converted once for the whole warp.
+struct Scales {
+  float k[kUnitTokens][kGroups];
+  uint2 v[kGroups / 2][4][2];  // [j / 2][quad][j % 2]: fp16 of the quad's four tokens
 };
 
 struct Smem {
   alignas(128) uint8_t ring[kWarps][kStages][kUnitBytes];  // a warp's last piece comes here when it has read them
+  Scales scales[kWarps];
   uint64_t full[kWarps][kStages];
   int pre[kMaxSeqs + 1];  // units before each sequence (of one KV head)
   int scan[kWarps];
@@ -95,8 +96,6 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t dup_lo(uint32_t v) { return __byte_perm(v, v, 0x1010); }
-__device__ __forceinline__ uint32_t dup_hi(uint32_t v) { return __byte_perm(v, v, 0x3232); }
 
 struct State {
   uint32_t q[kGroups][2];  // the B fragments of Q^T: head lane / 4, dims 16 j + 4 t + {0, 1} and {2, 3}
@@ -140,42 +139,57 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
     for (int c = 0; c < 4; ++c) st.o[j][c] = 0.f;
 }
 
+// A unit's scale bytes into `sc`: lane i converts word i of K's and of V's.
+// Tokens from `valid` on get V scales of 0, so that nothing that their bytes
+// hold (a NaN) meets their weights of 0.
+__device__ __forceinline__ void convert_scales(const uint8_t* unit, Scales& sc, int valid, int lane) {
+  const uint32_t wk = *reinterpret_cast<const uint32_t*>(unit + kOffKScale + 4 * lane);
+  uint32_t wv = *reinterpret_cast<const uint32_t*>(unit + kOffVScale + 4 * lane);
+  const int quad = lane >> 3, j = lane & 7;
+  if (valid < kUnitTokens) {
+    const int n = min(max(valid - 4 * quad, 0), 4);
+    wv &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
+  }
+  uint32_t a, b, c, d;
+  e4m3_to_half2(wk, a, b);
+  e4m3_to_half2(wv, c, d);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  *reinterpret_cast<float4*>(&sc.k[0][0] + 4 * lane) = make_float4(f.x, f.y, h.x, h.y);
+  sc.v[j >> 1][quad][j & 1] = make_uint2(c, d);
+}
+
 // One unit: its first `valid` tokens are the sequence's.
-__device__ __forceinline__ void attend(State& st, UnitRegs& u, int valid, int g, int t) {
+__device__ __forceinline__ void attend(State& st, const uint8_t* unit, const Scales& sc, int valid, int g, int t) {
   // rows g and g + 8 of the S tile are tokens ta and ta + 2, so that the
   // transposed P has tokens 4 t .. 4 t + 3 in lane t, whose V words hold them
   const int ta = 4 * (g >> 1) + (g & 1);
-  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+  float x[4] = {0.f, 0.f, 0.f, 0.f};  // token ta: heads 2 t, 2 t + 1; token ta + 2: the same
   {
-    uint32_t sa[4], sb[4];
-    e4m3_to_half2(u.ksa.x, sa[0], sa[1]);
-    e4m3_to_half2(u.ksa.y, sa[2], sa[3]);
-    e4m3_to_half2(u.ksb.x, sb[0], sb[1]);
-    e4m3_to_half2(u.ksb.y, sb[2], sb[3]);
-    const uint32_t wa[4] = {u.ka.x, u.ka.y, u.ka.z, u.ka.w}, wb[4] = {u.kb.x, u.kb.y, u.kb.z, u.kb.w};
+    const uint4 ka = *reinterpret_cast<const uint4*>(unit + 64 * ta + 16 * t);
+    const uint4 kb = *reinterpret_cast<const uint4*>(unit + 64 * (ta + 2) + 16 * t);
+    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {  // a word holds groups 2 w and 2 w + 1
-      uint32_t x[4], y[4];
-      e2m1_to_half2(wa[w], x[0], x[1], x[2], x[3]);
-      e2m1_to_half2(wb[w], y[0], y[1], y[2], y[3]);
-      const uint32_t a0 = dup_lo(sa[w]), a1 = dup_hi(sa[w]), b0 = dup_lo(sb[w]), b1 = dup_hi(sb[w]);
-      mma_16816(s0, hmul2(x[0], a0), hmul2(y[0], b0), hmul2(x[1], a0), hmul2(y[1], b0), st.q[2 * w][0],
-                st.q[2 * w][1]);
-      mma_16816(s1, hmul2(x[2], a1), hmul2(y[2], b1), hmul2(x[3], a1), hmul2(y[3], b1), st.q[2 * w + 1][0],
-                st.q[2 * w + 1][1]);
+      uint32_t p[4], q[4];
+      e2m1_to_half2(wa[w], p[0], p[1], p[2], p[3]);
+      e2m1_to_half2(wb[w], q[0], q[1], q[2], q[3]);
+      const float2 fa = *reinterpret_cast<const float2*>(&sc.k[ta][2 * w]);
+      const float2 fb = *reinterpret_cast<const float2*>(&sc.k[ta + 2][2 * w]);
+      float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_16816(d, p[0], q[0], p[1], q[1], st.q[2 * w][0], st.q[2 * w][1]);
+      mma_16816(e, p[2], q[2], p[3], q[3], st.q[2 * w + 1][0], st.q[2 * w + 1][1]);
+      x[0] = fmaf(d[0], fa.x, x[0]), x[1] = fmaf(d[1], fa.x, x[1]);
+      x[2] = fmaf(d[2], fb.x, x[2]), x[3] = fmaf(d[3], fb.x, x[3]);
+      x[0] = fmaf(e[0], fa.y, x[0]), x[1] = fmaf(e[1], fa.y, x[1]);
+      x[2] = fmaf(e[2], fb.y, x[2]), x[3] = fmaf(e[3], fb.y, x[3]);
     }
   }
-  float x[4];  // token ta: heads 2 t, 2 t + 1; token ta + 2: the same
 #pragma unroll
-  for (int c = 0; c < 4; ++c) x[c] = (s0[c] + s1[c]) * st.sc[c & 1];
+  for (int c = 0; c < 4; ++c) x[c] *= st.sc[c & 1];
   if (valid < kUnitTokens) {
     if (ta >= valid) x[0] = x[1] = -INFINITY;
     if (ta + 2 >= valid) x[2] = x[3] = -INFINITY;
-    // nor may what these tokens' scale bytes hold get into the sum
-    const int n = min(max(valid - 4 * t, 0), 4);
-    const uint32_t keep = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
-    u.vsa.x &= keep, u.vsa.y &= keep, u.vsa.z &= keep, u.vsa.w &= keep;
-    u.vsb.x &= keep, u.vsb.y &= keep, u.vsb.z &= keep, u.vsb.w &= keep;
   }
   const float hi0 = fmaxf(x[0], x[2]), hi1 = fmaxf(x[1], x[3]);
   if (__any_sync(0xffffffffu, hi0 > st.m[0] + kRescale || hi1 > st.m[1] + kRescale)) {
@@ -204,11 +218,12 @@ __device__ __forceinline__ void attend(State& st, UnitRegs& u, int valid, int g,
   st.l[0] += p0 + p2;
   st.l[1] += p1 + p3;
   const uint32_t b0 = movmatrix(half2_of(p0, p1)), b1 = movmatrix(half2_of(p2, p3));
-  const uint32_t sv[8] = {u.vsa.x, u.vsa.y, u.vsa.z, u.vsa.w, u.vsb.x, u.vsb.y, u.vsb.z, u.vsb.w};
+  const uint4 va = *reinterpret_cast<const uint4*>(unit + kOffV + 256 * t + 32 * g);
+  const uint4 vb = *reinterpret_cast<const uint4*>(unit + kOffV + 256 * t + 32 * g + 16);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {  // groups 4 w .. 4 w + 3; tokens 4 t .. 4 t + 3
-    const uint32_t c0 = w ? u.va.y : u.va.x, c1 = w ? u.va.w : u.va.z;
-    const uint32_t c2 = w ? u.vb.y : u.vb.x, c3 = w ? u.vb.w : u.vb.z;
+    const uint32_t c0 = w ? va.y : va.x, c1 = w ? va.w : va.z;
+    const uint32_t c2 = w ? vb.y : vb.x, c3 = w ? vb.w : vb.z;
     constexpr uint32_t kLow = 0x0f0f0f0fu;
     uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
     auto spread = [](uint32_t v, uint32_t (&r)[4]) { e2m1_to_half2(v, r[0], r[1], r[2], r[3]); };
@@ -217,30 +232,23 @@ __device__ __forceinline__ void attend(State& st, UnitRegs& u, int valid, int g,
     spread((c2 & kLow) | ((c3 << 4) & ~kLow), lo23);
     spread(((c2 >> 4) & kLow) | (c3 & ~kLow), hi23);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t s01, s23;
-      e4m3_to_half2(sv[4 * w + k], s01, s23);
-      mma_16816(st.o[4 * w + k], hmul2(lo01[k], s01), hmul2(hi01[k], s01), hmul2(lo23[k], s23), hmul2(hi23[k], s23),
+    for (int k = 0; k < 4; k += 2) {
+      const uint4 s = *reinterpret_cast<const uint4*>(&sc.v[2 * w + (k >> 1)][t][0]);
+      mma_16816(st.o[4 * w + k], hmul2(lo01[k], s.x), hmul2(hi01[k], s.x), hmul2(lo23[k], s.y), hmul2(hi23[k], s.y),
                 b0, b1);
+      mma_16816(st.o[4 * w + k + 1], hmul2(lo01[k + 1], s.z), hmul2(hi01[k + 1], s.z), hmul2(lo23[k + 1], s.w),
+                hmul2(hi23[k + 1], s.w), b0, b1);
     }
   }
 }
 
-__device__ __forceinline__ void load_unit(const uint8_t* p, int g, int t, UnitRegs& u) {
-  const int ta = 4 * (g >> 1) + (g & 1);
-  u.ka = *reinterpret_cast<const uint4*>(p + 64 * ta + 16 * t);
-  u.kb = *reinterpret_cast<const uint4*>(p + 64 * (ta + 2) + 16 * t);
-  u.ksa = *reinterpret_cast<const uint2*>(p + kOffKScale + 8 * ta);
-  u.ksb = *reinterpret_cast<const uint2*>(p + kOffKScale + 8 * (ta + 2));
-  u.va = *reinterpret_cast<const uint4*>(p + kOffV + 256 * t + 32 * g);
-  u.vb = *reinterpret_cast<const uint4*>(p + kOffV + 256 * t + 32 * g + 16);
-  u.vsa = *reinterpret_cast<const uint4*>(p + kOffVScale + 32 * t);
-  u.vsb = *reinterpret_cast<const uint4*>(p + kOffVScale + 32 * t + 16);
-}
+// Orders this thread's shared-memory writes before later copies into them.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void zero_unit(UnitRegs& u) {
-  u.ka = u.kb = u.va = u.vb = u.vsa = u.vsb = make_uint4(0, 0, 0, 0);
-  u.ksa = u.ksb = make_uint2(0, 0);
+// A unit of zeros in place of one that the table does not lead to (by the whole warp).
+__device__ __forceinline__ void zero_unit(uint8_t* unit, int lane) {
+  for (int i = lane; i < kUnitBytes / 16; i += 32) reinterpret_cast<uint4*>(unit)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
 }
 
 __device__ __forceinline__ int seq_units(const DecodeArgs& a, int b, bool report) {
@@ -419,16 +427,19 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
       ok = false;
       if (lane == 0) atomicOr(a.err, kErrWaitTimeout);
     }
-    UnitRegs r;
-    if (!ok || (info & kBad)) zero_unit(r);  // reads as zeros
-    else load_unit(sm.ring[warp][stage], g, t, r);
+    uint8_t* unit = sm.ring[warp][stage];
+    Scales& sc = sm.scales[warp];
+    if (!ok || (info & kBad)) zero_unit(unit, lane);  // reads as zeros
+    convert_scales(unit, sc, info & 0xff, lane);
     __syncwarp();
+    attend(st, unit, sc, info & 0xff, g, t);
+    if ((info & kBad)) fence_proxy_async();  // before the next copy into it
+    __syncwarp();  // every lane is done with the unit and the scales
     if (ok && issued < n) {
       if ((issued & 31) == 0) look_up(issued);
       fetch(issued);
       ++issued;
     }
-    attend(st, r, info & 0xff, g, t);
     if ((info & kLast) || i == n - 1) {
       if (!ok)  // the ring takes the piece only after every copy into it has landed or been given up
         for (int k = max(i, issued - kStages); k < issued; ++k) (void)mbar_wait(&sm.full[warp][k % kStages], (k / kStages) & 1);
