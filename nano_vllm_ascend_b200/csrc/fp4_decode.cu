@@ -9,16 +9,15 @@
 // are all the columns that there are.
 //   S^T[16 tokens x 8 heads] = K[16 x 128] . Q^T, eight steps of one group each
 //   O^T[16 dims x 8 heads] (8 tiles) += V^T[16 dims x 16 tokens] . P^T
-// K and V are e2m1 -> fp16 (one conversion for two values) times their group's
-// e4m3 scale: exact. Q is scaled by a power of two into fp16's range (entries
-// 2^14 below the row's largest lose bits that a sum of 128 terms does not
-// show); P is kept as 2^7 p in fp16, so 11 bits down to p = 2^-21. Scores,
-// maxima, sums and O are fp32.
+// K and V enter as e2m1 -> fp16 (one conversion for two values): exact. K's
+// scales multiply the fp32 sums of their groups, V's the weights: P s is
+// rounded to fp16 twice (P, then the product: 2^-10 of a weight), with 2^4 p s
+// normal down to 2^-18. Q is scaled by a power of two into fp16's range
+// (entries 2^14 below the row's largest lose bits that a sum of 128 terms does
+// not show). Scores, maxima, sums and O are fp32.
 //
 // Data: every warp streams its units through a ring of its own in shared
-// memory, one bulk copy (2304 contiguous bytes) a unit, four in flight. With
-// 16 warps that is 147 KB in flight an SM, three times what hides the latency
-// of HBM at full rate, and no warp waits for another one's data.
+// memory, one bulk copy (2304 contiguous bytes) a unit, three or four in flight; no warp waits for another one's data.
 //
 // Schedule: the units (16 tokens) of all (sequence, KV head) pairs, sequence
 // major, are cut into equal contiguous ranges, one per CTA, each cut into
@@ -35,13 +34,12 @@ namespace {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 4;       // units in flight a warp
 constexpr int kMaxSeqs = 1024;   // sequences per launch (their prefix of units sits in shared memory)
 constexpr int kMaxCtas = 1024;
 constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
 constexpr int kMinUnits = 2;     // units per warp below which fewer CTAs are used
-constexpr float kRescale = 8.f;  // log2 by which a score may pass the running maximum before O is rescaled
-constexpr float kPShift = 7.f;   // P is held as 2^7 p: p up to 2^8 fits fp16
+constexpr float kRescale = 3.f;  // log2 by which a score may pass the running maximum before O is rescaled
+constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and scales up to 448, P s fits fp16
 constexpr size_t kTicketOffset = 256;
 constexpr size_t kMlOffset = kTicketOffset + kMaxCtas * sizeof(int);
 
@@ -66,10 +64,12 @@ struct Scales {
   float k[kUnitTokens][kGroups];
   uint2 v[kGroups / 2][4][2];  // [j / 2][quad][j % 2]: fp16 of the quad's four tokens
 };
+constexpr int kScalesV = sizeof(float) * kUnitTokens * kGroups;  // offset of v
 
+template <int kStages>  // units in flight a warp
 struct Smem {
   alignas(128) uint8_t ring[kWarps][kStages][kUnitBytes];  // a warp's last piece comes here when it has read them
-  Scales scales[kWarps];
+  Scales scales[kWarps][2];
   uint64_t full[kWarps][kStages];
   int pre[kMaxSeqs + 1];  // units before each sequence (of one KV head)
   int scan[kWarps];
@@ -79,8 +79,7 @@ struct Smem {
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -100,7 +99,7 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
 struct State {
   uint32_t q[kGroups][2];  // the B fragments of Q^T: head lane / 4, dims 16 j + 4 t + {0, 1} and {2, 3}
   float sc[2];             // log2 factor of the scores of heads 2 t and 2 t + 1
-  float m[2], l[2];        // their running maximum and this lane's part of the sum (times 2^7)
+  float m[2], l[2];        // their running maximum and this lane's part of the sum (times 2^4)
   float o[kGroups][4];     // O^T: dims 16 j + 2 g (heads 2 t, 2 t + 1), then 16 j + 2 g + 1 (the same)
 };
 
@@ -139,12 +138,24 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
     for (int c = 0; c < 4; ++c) st.o[j][c] = 0.f;
 }
 
+__device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // A unit's scale bytes into `sc`: lane i converts word i of K's and of V's.
 // Tokens from `valid` on get V scales of 0, so that nothing that their bytes
 // hold (a NaN) meets their weights of 0.
-__device__ __forceinline__ void convert_scales(const uint8_t* unit, Scales& sc, int valid, int lane) {
-  const uint32_t wk = *reinterpret_cast<const uint32_t*>(unit + kOffKScale + 4 * lane);
-  uint32_t wv = *reinterpret_cast<const uint32_t*>(unit + kOffVScale + 4 * lane);
+__device__ __forceinline__ void convert_scales(uint32_t unit, uint32_t sc, int valid, int lane) {
+  const uint32_t wk = ld_shared(unit + kOffKScale + 4 * lane);
+  uint32_t wv = ld_shared(unit + kOffVScale + 4 * lane);
   const int quad = lane >> 3, j = lane & 7;
   if (valid < kUnitTokens) {
     const int n = min(max(valid - 4 * quad, 0), 4);
@@ -155,34 +166,38 @@ __device__ __forceinline__ void convert_scales(const uint8_t* unit, Scales& sc, 
   e4m3_to_half2(wv, c, d);
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&b));
-  *reinterpret_cast<float4*>(&sc.k[0][0] + 4 * lane) = make_float4(f.x, f.y, h.x, h.y);
-  sc.v[j >> 1][quad][j & 1] = make_uint2(c, d);
+  st_shared_v4(sc + 16 * lane, __float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(h.x), __float_as_uint(h.y));
+  st_shared_v2(sc + kScalesV + 64 * (j >> 1) + 16 * quad + 8 * (j & 1), c, d);
 }
 
-// One unit: its first `valid` tokens are the sequence's.
-__device__ __forceinline__ void attend(State& st, const uint8_t* unit, const Scales& sc, int valid, int g, int t) {
-  // rows g and g + 8 of the S tile are tokens ta and ta + 2, so that the
-  // transposed P has tokens 4 t .. 4 t + 3 in lane t, whose V words hold them
+// Scores of one unit in log2 units: x[0], x[1] of token ta's heads 2 t and
+// 2 t + 1, x[2], x[3] of token ta + 2's. Rows g and g + 8 of the S tile are
+// these tokens, so that the transposed P has tokens 4 t .. 4 t + 3 in lane t,
+// whose V words hold them.
+__device__ __forceinline__ void scores(const State& st, uint32_t unit, uint32_t sc, int valid, int g, int t,
+                                       float (&x)[4]) {
   const int ta = 4 * (g >> 1) + (g & 1);
-  float x[4] = {0.f, 0.f, 0.f, 0.f};  // token ta: heads 2 t, 2 t + 1; token ta + 2: the same
-  {
-    const uint4 ka = *reinterpret_cast<const uint4*>(unit + 64 * ta + 16 * t);
-    const uint4 kb = *reinterpret_cast<const uint4*>(unit + 64 * (ta + 2) + 16 * t);
-    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+  const uint4 ka = ld_shared_v4(unit + 64 * ta + 16 * t);
+  const uint4 kb = ld_shared_v4(unit + 64 * (ta + 2) + 16 * t);
+  const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {  // a word holds groups 2 w and 2 w + 1
+  for (int c = 0; c < 4; ++c) x[c] = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // groups 4 h .. 4 h + 3
+    const uint4 fa = ld_shared_v4(sc + 32 * ta + 16 * h), fb = ld_shared_v4(sc + 32 * (ta + 2) + 16 * h);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {  // a word holds two groups
+      const int w = 2 * h + v;
       uint32_t p[4], q[4];
       e2m1_to_half2(wa[w], p[0], p[1], p[2], p[3]);
       e2m1_to_half2(wb[w], q[0], q[1], q[2], q[3]);
-      const float2 fa = *reinterpret_cast<const float2*>(&sc.k[ta][2 * w]);
-      const float2 fb = *reinterpret_cast<const float2*>(&sc.k[ta + 2][2 * w]);
       float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
       mma_16816(d, p[0], q[0], p[1], q[1], st.q[2 * w][0], st.q[2 * w][1]);
       mma_16816(e, p[2], q[2], p[3], q[3], st.q[2 * w + 1][0], st.q[2 * w + 1][1]);
-      x[0] = fmaf(d[0], fa.x, x[0]), x[1] = fmaf(d[1], fa.x, x[1]);
-      x[2] = fmaf(d[2], fb.x, x[2]), x[3] = fmaf(d[3], fb.x, x[3]);
-      x[0] = fmaf(e[0], fa.y, x[0]), x[1] = fmaf(e[1], fa.y, x[1]);
-      x[2] = fmaf(e[2], fb.y, x[2]), x[3] = fmaf(e[3], fb.y, x[3]);
+      const float a0 = __uint_as_float(v ? fa.z : fa.x), a1 = __uint_as_float(v ? fa.w : fa.y);
+      const float b0 = __uint_as_float(v ? fb.z : fb.x), b1 = __uint_as_float(v ? fb.w : fb.y);
+      x[0] = fmaf(d[0], a0, x[0]), x[1] = fmaf(d[1], a0, x[1]), x[2] = fmaf(d[2], b0, x[2]), x[3] = fmaf(d[3], b0, x[3]);
+      x[0] = fmaf(e[0], a1, x[0]), x[1] = fmaf(e[1], a1, x[1]), x[2] = fmaf(e[2], b1, x[2]), x[3] = fmaf(e[3], b1, x[3]);
     }
   }
 #pragma unroll
@@ -191,7 +206,43 @@ __device__ __forceinline__ void attend(State& st, const uint8_t* unit, const Sca
     if (ta >= valid) x[0] = x[1] = -INFINITY;
     if (ta + 2 >= valid) x[2] = x[3] = -INFINITY;
   }
-  const float hi0 = fmaxf(x[0], x[2]), hi1 = fmaxf(x[1], x[3]);
+}
+
+// O += V^T P^T of one unit; b0 and b1 are the fragments of P^T.
+__device__ __forceinline__ void weigh(State& st, uint32_t unit, uint32_t sc, int g, int t, uint32_t b0,
+                                      uint32_t b1) {
+  const uint4 va = ld_shared_v4(unit + kOffV + 256 * t + 32 * g);
+  const uint4 vb = ld_shared_v4(unit + kOffV + 256 * t + 32 * g + 16);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {  // groups 4 w .. 4 w + 3; tokens 4 t .. 4 t + 3
+    const uint32_t c0 = w ? va.y : va.x, c1 = w ? va.w : va.z;
+    const uint32_t c2 = w ? vb.y : vb.x, c3 = w ? vb.w : vb.z;
+    constexpr uint32_t kLow = 0x0f0f0f0fu;
+    uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
+    auto spread = [](uint32_t v, uint32_t (&r)[4]) { e2m1_to_half2(v, r[0], r[1], r[2], r[3]); };
+    spread((c0 & kLow) | ((c1 << 4) & ~kLow), lo01);
+    spread(((c0 >> 4) & kLow) | (c1 & ~kLow), hi01);
+    spread((c2 & kLow) | ((c3 << 4) & ~kLow), lo23);
+    spread(((c2 >> 4) & kLow) | (c3 & ~kLow), hi23);
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+      const uint4 s = ld_shared_v4(sc + kScalesV + 64 * (2 * w + (k >> 1)) + 16 * t);
+      mma_16816(st.o[4 * w + k], lo01[k], hi01[k], lo23[k], hi23[k], hmul2(b0, s.x), hmul2(b1, s.y));
+      mma_16816(st.o[4 * w + k + 1], lo01[k + 1], hi01[k + 1], lo23[k + 1], hi23[k + 1], hmul2(b0, s.z),
+                hmul2(b1, s.w));
+    }
+  }
+}
+
+// N units of one pair; the first valid[u] tokens of unit u are the sequence's.
+template <int N>
+__device__ __forceinline__ void attend(State& st, const uint32_t (&unit)[N], uint32_t sc, const int (&valid)[N],
+                                       int g, int t) {
+  float x[N][4];
+#pragma unroll
+  for (int u = 0; u < N; ++u) scores(st, unit[u], sc + u * uint32_t(sizeof(Scales)), valid[u], g, t, x[u]);
+  float hi0 = fmaxf(x[0][0], x[0][2]), hi1 = fmaxf(x[0][1], x[0][3]);
+  if (N == 2) hi0 = fmax3(hi0, x[N - 1][0], x[N - 1][2]), hi1 = fmax3(hi1, x[N - 1][1], x[N - 1][3]);
   if (__any_sync(0xffffffffu, hi0 > st.m[0] + kRescale || hi1 > st.m[1] + kRescale)) {
     float n0 = hi0, n1 = hi1;
 #pragma unroll
@@ -213,32 +264,14 @@ __device__ __forceinline__ void attend(State& st, const uint8_t* unit, const Sca
   }
   const float r0 = st.m[0] == -INFINITY ? 0.f : st.m[0] - kPShift;
   const float r1 = st.m[1] == -INFINITY ? 0.f : st.m[1] - kPShift;
-  const float p0 = fast_exp2(x[0] - r0), p1 = fast_exp2(x[1] - r1);
-  const float p2 = fast_exp2(x[2] - r0), p3 = fast_exp2(x[3] - r1);
-  st.l[0] += p0 + p2;
-  st.l[1] += p1 + p3;
-  const uint32_t b0 = movmatrix(half2_of(p0, p1)), b1 = movmatrix(half2_of(p2, p3));
-  const uint4 va = *reinterpret_cast<const uint4*>(unit + kOffV + 256 * t + 32 * g);
-  const uint4 vb = *reinterpret_cast<const uint4*>(unit + kOffV + 256 * t + 32 * g + 16);
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {  // groups 4 w .. 4 w + 3; tokens 4 t .. 4 t + 3
-    const uint32_t c0 = w ? va.y : va.x, c1 = w ? va.w : va.z;
-    const uint32_t c2 = w ? vb.y : vb.x, c3 = w ? vb.w : vb.z;
-    constexpr uint32_t kLow = 0x0f0f0f0fu;
-    uint32_t lo01[4], hi01[4], lo23[4], hi23[4];
-    auto spread = [](uint32_t v, uint32_t (&r)[4]) { e2m1_to_half2(v, r[0], r[1], r[2], r[3]); };
-    spread((c0 & kLow) | ((c1 << 4) & ~kLow), lo01);
-    spread(((c0 >> 4) & kLow) | (c1 & ~kLow), hi01);
-    spread((c2 & kLow) | ((c3 << 4) & ~kLow), lo23);
-    spread(((c2 >> 4) & kLow) | (c3 & ~kLow), hi23);
-#pragma unroll
-    for (int k = 0; k < 4; k += 2) {
-      const uint4 s = *reinterpret_cast<const uint4*>(&sc.v[2 * w + (k >> 1)][t][0]);
-      mma_16816(st.o[4 * w + k], hmul2(lo01[k], s.x), hmul2(hi01[k], s.x), hmul2(lo23[k], s.y), hmul2(hi23[k], s.y),
-                b0, b1);
-      mma_16816(st.o[4 * w + k + 1], hmul2(lo01[k + 1], s.z), hmul2(hi01[k + 1], s.z), hmul2(lo23[k + 1], s.w),
-                hmul2(hi23[k + 1], s.w), b0, b1);
-    }
+  for (int u = 0; u < N; ++u) {
+    const float p0 = fast_exp2(x[u][0] - r0), p1 = fast_exp2(x[u][1] - r1);
+    const float p2 = fast_exp2(x[u][2] - r0), p3 = fast_exp2(x[u][3] - r1);
+    st.l[0] += p0 + p2;
+    st.l[1] += p1 + p3;
+    weigh(st, unit[u], sc + u * uint32_t(sizeof(Scales)), g, t, movmatrix(half2_of(p0, p1)),
+          movmatrix(half2_of(p2, p3)));
   }
 }
 
@@ -246,8 +279,8 @@ __device__ __forceinline__ void attend(State& st, const uint8_t* unit, const Sca
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A unit of zeros in place of one that the table does not lead to (by the whole warp).
-__device__ __forceinline__ void zero_unit(uint8_t* unit, int lane) {
-  for (int i = lane; i < kUnitBytes / 16; i += 32) reinterpret_cast<uint4*>(unit)[i] = make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void zero_unit(uint32_t unit, int lane) {
+  for (int i = lane; i < kUnitBytes / 16; i += 32) st_shared_v4(unit + 16 * i, 0, 0, 0, 0);
   __syncwarp();
 }
 
@@ -261,13 +294,15 @@ __device__ __forceinline__ int seq_units(const DecodeArgs& a, int b, bool report
   return n <= 0 ? 0 : (n + kUnitTokens - 1) / kUnitTokens;
 }
 
+template <int kStages>
 __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  using Sm = Smem<kStages>;
+  Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
   // Pieces of pairs that are not one warp's: [2 * kWarps][group] (m, l), and
   // [group][128] each: a warp's first one in its own place, its last one in
   // the warp's ring.
-  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Smem));
+  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Sm));
   float* piece_first = reinterpret_cast<float*>(piece_ml + 2 * kWarps * a.group);
   auto piece_o = [&](int p) {
     return (p & 1) ? reinterpret_cast<float*>(sm.ring[p >> 1]) : piece_first + (p >> 1) * a.group * kD;
@@ -385,19 +420,15 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
     next_at = a.pool + ((((static_cast<int64_t>(blk) * a.kvh + h) << a.upb_log2) + (u & ((1 << a.upb_log2) - 1))) *
                         kUnitBytes);
   };
-  auto fetch = [&](int i) {  // unit i into its stage
-    const uint8_t* at =
-        reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(next_at), i & 31));
-    const int info = __shfl_sync(0xffffffffu, next_info, i & 31);
-    if (lane == 0) {
-      uint64_t* bar = &sm.full[warp][i % kStages];
-      if (info & kBad) {
-        atomicOr(a.err, kErrBadBlockId);
-        mbar_arrive(bar);
-      } else {
-        mbar_arrive_expect_tx(bar, kUnitBytes);
-        bulk_load(sm.ring[warp][i % kStages], at, kUnitBytes, bar);
-      }
+  auto fetch = [&](int i) {  // unit i into its stage, by the lane that knows it
+    if (lane != (i & 31)) return;
+    uint64_t* bar = &sm.full[warp][i % kStages];
+    if (next_info & kBad) {
+      atomicOr(a.err, kErrBadBlockId);
+      mbar_arrive(bar);
+    } else {
+      mbar_arrive_expect_tx(bar, kUnitBytes);
+      bulk_load(sm.ring[warp][i % kStages], next_at, kUnitBytes, bar);
     }
   };
   look_up(0);
@@ -405,14 +436,25 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
   zero_empty();
   int issued = 0;
   for (; issued < min(n, kStages); ++issued) fetch(issued);
-  int pair_now = next_pair, info_now = next_info;  // the batch that is being read
+  int pair_now = next_pair, info_now = next_info, batch_end = 32;  // the batch that is being read
   bool ok = true;
   int b = 0, h = 0;
   bool whole = false, open = false;
   int slot = 0;
-  for (int i = 0; i < n; ++i) {
-    if (i > 0 && (i & 31) == 0) pair_now = next_pair, info_now = next_info;
-    const int info = __shfl_sync(0xffffffffu, info_now, i & 31);
+  auto info_of = [&](int i) {  // of the unit that is read next, or the one after it
+    return __shfl_sync(0xffffffffu, i < batch_end ? info_now : next_info, i & 31);
+  };
+  const uint32_t ring = smem_u32(sm.ring[warp]), sc = smem_u32(sm.scales[warp]);
+  auto landed = [&](int i) {
+    if (ok && !__all_sync(0xffffffffu, mbar_wait(&sm.full[warp][i % kStages], (i / kStages) & 1))) {
+      ok = false;
+      if (lane == 0) atomicOr(a.err, kErrWaitTimeout);
+    }
+    return ring + (i % kStages) * kUnitBytes;
+  };
+  for (int i = 0; i < n;) {
+    if (i >= batch_end) pair_now = next_pair, info_now = next_info, batch_end += 32;
+    const int info = info_of(i);
     if (!open) {
       const int pair = __shfl_sync(0xffffffffu, pair_now, i & 31);
       b = pair / a.kvh;
@@ -422,28 +464,40 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
       slot = i == 0 ? 0 : 1;
       open = true;
     }
-    const int stage = i % kStages;
-    if (ok && !__all_sync(0xffffffffu, mbar_wait(&sm.full[warp][stage], (i / kStages) & 1))) {
-      ok = false;
-      if (lane == 0) atomicOr(a.err, kErrWaitTimeout);
+    const bool two = !(info & kLast) && i + 1 < n;
+    const int info2 = two ? info_of(i + 1) : 0;
+    const uint32_t u0 = landed(i);
+    if (!ok || (info & kBad)) zero_unit(u0, lane);  // reads as zeros
+    convert_scales(u0, sc, info & 0xff, lane);
+    if (two) {
+      const uint32_t u1 = landed(i + 1);
+      if (!ok || (info2 & kBad)) zero_unit(u1, lane);
+      convert_scales(u1, sc + sizeof(Scales), info2 & 0xff, lane);
+      __syncwarp();
+      const uint32_t units[2] = {u0, u1};
+      const int valid[2] = {info & 0xff, info2 & 0xff};
+      attend<2>(st, units, sc, valid, g, t);
+    } else {
+      __syncwarp();
+      const uint32_t units[1] = {u0};
+      const int valid[1] = {info & 0xff};
+      attend<1>(st, units, sc, valid, g, t);
     }
-    uint8_t* unit = sm.ring[warp][stage];
-    Scales& sc = sm.scales[warp];
-    if (!ok || (info & kBad)) zero_unit(unit, lane);  // reads as zeros
-    convert_scales(unit, sc, info & 0xff, lane);
-    __syncwarp();
-    attend(st, unit, sc, info & 0xff, g, t);
-    if ((info & kBad)) fence_proxy_async();  // before the next copy into it
-    __syncwarp();  // every lane is done with the unit and the scales
-    if (ok && issued < n) {
+    if ((info | info2) & kBad) fence_proxy_async();  // before the next copy into it
+    __syncwarp();  // every lane is done with the units and the scales
+    i += two ? 2 : 1;
+    for (int k = 0; k < 2; ++k) {
+      if (!ok || issued >= min(n, i + kStages)) break;
       if ((issued & 31) == 0) look_up(issued);
       fetch(issued);
       ++issued;
     }
-    if ((info & kLast) || i == n - 1) {
+    const int last = two ? info2 : info;
+    if ((last & kLast) || i == n) {
       if (!ok)  // the ring takes the piece only after every copy into it has landed or been given up
-        for (int k = max(i, issued - kStages); k < issued; ++k) (void)mbar_wait(&sm.full[warp][k % kStages], (k / kStages) & 1);
-      finish(b, h, whole && (info & kLast), slot);
+        for (int k = max(i, issued - kStages); k < issued; ++k)
+          (void)mbar_wait(&sm.full[warp][k % kStages], (k / kStages) & 1);
+      finish(b, h, whole && (last & kLast), slot);
       open = false;
     }
   }
@@ -547,12 +601,25 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
   }
 }
 
-size_t smem_bytes(int group) {
-  return sizeof(Smem) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
+template <int kStages>
+constexpr size_t smem_bytes(int group) {
+  return sizeof(Smem<kStages>) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
 }
-static_assert(sizeof(Smem) % 16 == 0 && sizeof(Smem) + kWarps * kMaxGroup * (16 + kD * 4) <= 232448,
+// Four units in flight a warp where their shared memory leaves room for the pieces of the group's heads, else three.
+constexpr int kFewHeads = 4;
+static_assert(sizeof(Smem<3>) % 16 == 0 && sizeof(Smem<4>) % 16 == 0, "the pieces behind it are 16-byte aligned");
+static_assert(smem_bytes<4>(kFewHeads) <= 232448 && smem_bytes<3>(kMaxGroup) <= 232448,
               "decode shared memory exceeds the 227 KB per-CTA limit");
-static_assert(kStages * kUnitBytes >= kMaxGroup * kD * 4, "a warp's ring takes its last piece");
+static_assert(3 * kUnitBytes >= kMaxGroup * kD * 4, "a warp's ring takes its last piece");
+
+template <int kStages>
+int launch(const DecodeArgs& a, int ctas, cudaStream_t stream) {
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&decode_kernel<kStages>),
+                                     smem_bytes<kStages>(kStages == 4 ? kFewHeads : kMaxGroup));
+  if (rc != NVK_OK) return rc;
+  return check_cuda(launch_pdl(decode_kernel<kStages>, dim3(ctas), dim3(kThreads), smem_bytes<kStages>(a.group), stream, a),
+                    "fp4_paged_decode launch");
+}
 
 size_t workspace_bytes(int group, int ctas) {
   return kMlOffset + static_cast<size_t>(ctas) * 2 * group * (sizeof(float2) + kD * sizeof(float));
@@ -632,9 +699,6 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   if (workspace_bytes_given < workspace_bytes(group, ctas))
     return fail(NVK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes_given,
                 workspace_bytes(group, ctas));
-  const size_t smem = smem_bytes(group);
-  const size_t most = smem_bytes(kMaxGroup);
-  if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&decode_kernel), most)) != NVK_OK) return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
   a.pool = static_cast<const uint8_t*>(kv_cache);
@@ -657,9 +721,8 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
     a.q = static_cast<const __nv_bfloat16*>(query) + static_cast<int64_t>(b0) * num_heads * kD;
     a.tables = block_tables + static_cast<int64_t>(b0) * block_table_stride;
     a.ctx = context_lens + b0;
-    if ((rc = check_cuda(launch_pdl(decode_kernel, dim3(ctas), dim3(kThreads), smem,
-                                    reinterpret_cast<cudaStream_t>(stream), a),
-                         "fp4_paged_decode launch")) != NVK_OK)
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if ((rc = group <= kFewHeads ? launch<4>(a, ctas, st) : launch<3>(a, ctas, st)) != NVK_OK)
       return rc;
   }
   return NVK_OK;

@@ -6,8 +6,9 @@ tolerance counts the roundings on the way (relative half steps: bf16 2^-8,
 fp16 2^-11):
 
 * the output's own, 2^-8 |o|;
-* the weights', which are held in fp16 in decode and bf16 in prefill: at most
-  half a step of the weighted mean of |v|, A;
+* the weights', which are held in fp16 in decode (rounded, multiplied by V's
+  scale and rounded again: two half steps) and in bf16 in prefill: of the
+  weighted mean of |v|, A;
 * scores: sums of 128 products in fp32 (in the test's range below 2^7 in log2
   units, so within 2^-14 of them after 128 roundings of 2^-24 relative to the
   sum of magnitudes), the exponential's 2^-22, fp16's floor for entries of q
@@ -27,7 +28,7 @@ pytestmark = pytest.mark.gpu
 
 D = 128
 SCALE = D ** -0.5
-DECODE_A = 2.0 ** -11 + 2.0 ** -11
+DECODE_A = 2 * 2.0 ** -11 + 2.0 ** -11
 PREFILL_A = 2.0 ** -8 + 2.0 ** -11
 
 
