@@ -16,10 +16,13 @@
 // (entries 2^14 below the row's largest lose bits that a sum of 128 terms does
 // not show). Scores, maxima, sums and O are fp32.
 //
-// Data: every warp streams its units through a ring of its own in shared
-// memory, one bulk copy (2304 contiguous bytes) a unit, three or four in flight; no warp waits for another one's data.
+// Data: every warp streams its tiles (two units, 32 tokens) through a ring of
+// its own in shared memory, one bulk copy of 4608 contiguous bytes a tile (two
+// copies where a block is one unit), two in flight: 74 to 147 KB an SM, where
+// about 55 KB hide HBM's latency at full rate. No warp waits for another one's
+// data.
 //
-// Schedule: the units (16 tokens) of all (sequence, KV head) pairs, sequence
+// Schedule: the tiles of all (sequence, KV head) pairs, sequence
 // major, are cut into equal contiguous ranges, one per CTA, each cut into
 // equal ranges of its warps. A warp keeps its own running maximum, sum and O;
 // pairs that lie in one warp are written by it, the others' pieces meet in
@@ -34,10 +37,12 @@ namespace {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxSeqs = 1024;   // sequences per launch (their prefix of units sits in shared memory)
+constexpr int kMaxSeqs = 1024;   // sequences per launch (their prefix of tiles sits in shared memory)
 constexpr int kMaxCtas = 1024;
 constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
-constexpr int kMinUnits = 2;     // units per warp below which fewer CTAs are used
+constexpr int kTileTokens = 2 * kUnitTokens;  // a warp's step
+constexpr int kTileBytes = 2 * kUnitBytes;
+constexpr int kStages = 2;       // tiles in flight a warp
 constexpr float kRescale = 3.f;  // log2 by which a score may pass the running maximum before O is rescaled
 constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and scales up to 448, P s fits fp16
 constexpr size_t kTicketOffset = 256;
@@ -59,23 +64,16 @@ struct DecodeArgs {
   float v_scale;
 };
 
-// The scales of one unit, converted once for the whole warp.
-struct Scales {
-  float k[kUnitTokens][kGroups];
-  uint2 v[kGroups / 2][4][2];  // [j / 2][quad][j % 2]: fp16 of the quad's four tokens
-};
-constexpr int kScalesV = sizeof(float) * kUnitTokens * kGroups;  // offset of v
-
-template <int kStages>  // units in flight a warp
 struct Smem {
-  alignas(128) uint8_t ring[kWarps][kStages][kUnitBytes];  // a warp's last piece comes here when it has read them
-  Scales scales[kWarps][2];
+  alignas(128) uint8_t ring[kWarps][kStages][kTileBytes];  // a warp's last piece comes here when it has read them
+  uint2 vscale[kWarps][2][kGroups / 2][4][2];  // [unit][j / 2][quad][j % 2]: V's scales of the quad's four tokens, fp16
   uint64_t full[kWarps][kStages];
-  int pre[kMaxSeqs + 1];  // units before each sequence (of one KV head)
+  int pre[kMaxSeqs + 1];  // tiles before each sequence (of one KV head)
   int scan[kWarps];
   int piece_pair[2 * kWarps];
   int last[2];
 };
+constexpr uint32_t kVScaleBytes = sizeof(Smem::vscale) / (2 * kWarps);  // of one unit
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
@@ -99,7 +97,9 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
 struct State {
   uint32_t q[kGroups][2];  // the B fragments of Q^T: head lane / 4, dims 16 j + 4 t + {0, 1} and {2, 3}
   float sc[2];             // log2 factor of the scores of heads 2 t and 2 t + 1
-  float m[2], l[2];        // their running maximum and this lane's part of the sum (times 2^4)
+  float ref[2];            // p = 2^(score - ref): their running maximum - kPShift
+  float thr[2];            // the score above which it moves: their running maximum + kRescale (-inf at first)
+  float l[2];              // this lane's part of the sum of p
   float o[kGroups][4];     // O^T: dims 16 j + 2 g (heads 2 t, 2 t + 1), then 16 j + 2 g + 1 (the same)
 };
 
@@ -130,7 +130,8 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
   }
   st.sc[0] = __shfl_sync(0xffffffffu, up, 8 * t) * a.scale_log2;
   st.sc[1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * a.scale_log2;
-  st.m[0] = st.m[1] = -INFINITY;
+  st.ref[0] = st.ref[1] = 0.f;
+  st.thr[0] = st.thr[1] = -INFINITY;
   st.l[0] = st.l[1] = 0.f;
 #pragma unroll
   for (int j = 0; j < kGroups; ++j)
@@ -143,6 +144,11 @@ __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
   asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
 }
@@ -150,66 +156,62 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// A unit's scale bytes into `sc`: lane i converts word i of K's and of V's.
-// Tokens from `valid` on get V scales of 0, so that nothing that their bytes
+// A unit's V scales to fp16, once for the whole warp: lane i converts word i.
+// Tokens from `valid` on get scales of 0, so that nothing that their bytes
 // hold (a NaN) meets their weights of 0.
-__device__ __forceinline__ void convert_scales(uint32_t unit, uint32_t sc, int valid, int lane) {
-  const uint32_t wk = ld_shared(unit + kOffKScale + 4 * lane);
-  uint32_t wv = ld_shared(unit + kOffVScale + 4 * lane);
+template <bool kMask>
+__device__ __forceinline__ void convert_vscales(uint32_t unit, uint32_t to, int valid, int lane) {
+  uint32_t w = ld_shared(unit + kOffVScale + 4 * lane);
   const int quad = lane >> 3, j = lane & 7;
-  if (valid < kUnitTokens) {
+  if (kMask) {
     const int n = min(max(valid - 4 * quad, 0), 4);
-    wv &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
+    w &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
   }
-  uint32_t a, b, c, d;
-  e4m3_to_half2(wk, a, b);
-  e4m3_to_half2(wv, c, d);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
-  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&b));
-  st_shared_v4(sc + 16 * lane, __float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(h.x), __float_as_uint(h.y));
-  st_shared_v2(sc + kScalesV + 64 * (j >> 1) + 16 * quad + 8 * (j & 1), c, d);
+  uint32_t lo, hi;
+  e4m3_to_half2(w, lo, hi);
+  st_shared_v2(to + 64 * (j >> 1) + 16 * quad + 8 * (j & 1), lo, hi);
 }
 
-// Scores of one unit in log2 units: x[0], x[1] of token ta's heads 2 t and
-// 2 t + 1, x[2], x[3] of token ta + 2's. Rows g and g + 8 of the S tile are
-// these tokens, so that the transposed P has tokens 4 t .. 4 t + 3 in lane t,
-// whose V words hold them.
-__device__ __forceinline__ void scores(const State& st, uint32_t unit, uint32_t sc, int valid, int g, int t,
-                                       float (&x)[4]) {
+// Scores of one unit (without the factor sc): x[0], x[1] of token ta's heads
+// 2 t and 2 t + 1, x[2], x[3] of token ta + 2's. Rows g and g + 8 of the S
+// tile are these tokens, so that the transposed P has tokens 4 t .. 4 t + 3 in
+// lane t, whose V words hold them.
+template <bool kMask>
+__device__ __forceinline__ void scores(const State& st, uint32_t unit, int valid, int g, int t, float (&x)[4]) {
   const int ta = 4 * (g >> 1) + (g & 1);
-  const uint4 ka = ld_shared_v4(unit + 64 * ta + 16 * t);
-  const uint4 kb = ld_shared_v4(unit + 64 * (ta + 2) + 16 * t);
+  const uint4 ka = ld_shared_v4(unit + 64 * ta + 16 * t), kb = ld_shared_v4(unit + 64 * (ta + 2) + 16 * t);
+  const uint2 ksa = ld_shared_v2(unit + kOffKScale + 8 * ta), ksb = ld_shared_v2(unit + kOffKScale + 8 * (ta + 2));
   const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+  uint32_t sa[4], sb[4];
+  e4m3_to_half2(ksa.x, sa[0], sa[1]);
+  e4m3_to_half2(ksa.y, sa[2], sa[3]);
+  e4m3_to_half2(ksb.x, sb[0], sb[1]);
+  e4m3_to_half2(ksb.y, sb[2], sb[3]);
 #pragma unroll
   for (int c = 0; c < 4; ++c) x[c] = 0.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {  // groups 4 h .. 4 h + 3
-    const uint4 fa = ld_shared_v4(sc + 32 * ta + 16 * h), fb = ld_shared_v4(sc + 32 * (ta + 2) + 16 * h);
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {  // a word holds two groups
-      const int w = 2 * h + v;
-      uint32_t p[4], q[4];
-      e2m1_to_half2(wa[w], p[0], p[1], p[2], p[3]);
-      e2m1_to_half2(wb[w], q[0], q[1], q[2], q[3]);
-      float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_16816(d, p[0], q[0], p[1], q[1], st.q[2 * w][0], st.q[2 * w][1]);
-      mma_16816(e, p[2], q[2], p[3], q[3], st.q[2 * w + 1][0], st.q[2 * w + 1][1]);
-      const float a0 = __uint_as_float(v ? fa.z : fa.x), a1 = __uint_as_float(v ? fa.w : fa.y);
-      const float b0 = __uint_as_float(v ? fb.z : fb.x), b1 = __uint_as_float(v ? fb.w : fb.y);
-      x[0] = fmaf(d[0], a0, x[0]), x[1] = fmaf(d[1], a0, x[1]), x[2] = fmaf(d[2], b0, x[2]), x[3] = fmaf(d[3], b0, x[3]);
-      x[0] = fmaf(e[0], a1, x[0]), x[1] = fmaf(e[1], a1, x[1]), x[2] = fmaf(e[2], b1, x[2]), x[3] = fmaf(e[3], b1, x[3]);
-    }
+  for (int w = 0; w < 4; ++w) {  // a word holds groups 2 w and 2 w + 1
+    uint32_t p[4], q[4];
+    e2m1_to_half2(wa[w], p[0], p[1], p[2], p[3]);
+    e2m1_to_half2(wb[w], q[0], q[1], q[2], q[3]);
+    float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_16816(d, p[0], q[0], p[1], q[1], st.q[2 * w][0], st.q[2 * w][1]);
+    mma_16816(e, p[2], q[2], p[3], q[3], st.q[2 * w + 1][0], st.q[2 * w + 1][1]);
+    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&sa[w]));
+    const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&sb[w]));
+    x[0] = fmaf(d[0], fa.x, x[0]), x[1] = fmaf(d[1], fa.x, x[1]);
+    x[2] = fmaf(d[2], fb.x, x[2]), x[3] = fmaf(d[3], fb.x, x[3]);
+    x[0] = fmaf(e[0], fa.y, x[0]), x[1] = fmaf(e[1], fa.y, x[1]);
+    x[2] = fmaf(e[2], fb.y, x[2]), x[3] = fmaf(e[3], fb.y, x[3]);
   }
-#pragma unroll
-  for (int c = 0; c < 4; ++c) x[c] *= st.sc[c & 1];
-  if (valid < kUnitTokens) {
+  if (kMask) {
     if (ta >= valid) x[0] = x[1] = -INFINITY;
     if (ta + 2 >= valid) x[2] = x[3] = -INFINITY;
   }
 }
 
 // O += V^T P^T of one unit; b0 and b1 are the fragments of P^T.
-__device__ __forceinline__ void weigh(State& st, uint32_t unit, uint32_t sc, int g, int t, uint32_t b0,
+__device__ __forceinline__ void weigh(State& st, uint32_t unit, uint32_t vscale, int g, int t, uint32_t b0,
                                       uint32_t b1) {
   const uint4 va = ld_shared_v4(unit + kOffV + 256 * t + 32 * g);
   const uint4 vb = ld_shared_v4(unit + kOffV + 256 * t + 32 * g + 16);
@@ -226,7 +228,7 @@ __device__ __forceinline__ void weigh(State& st, uint32_t unit, uint32_t sc, int
     spread(((c2 >> 4) & kLow) | (c3 & ~kLow), hi23);
 #pragma unroll
     for (int k = 0; k < 4; k += 2) {
-      const uint4 s = ld_shared_v4(sc + kScalesV + 64 * (2 * w + (k >> 1)) + 16 * t);
+      const uint4 s = ld_shared_v4(vscale + 64 * (2 * w + (k >> 1)) + 16 * t);
       mma_16816(st.o[4 * w + k], lo01[k], hi01[k], lo23[k], hi23[k], hmul2(b0, s.x), hmul2(b1, s.y));
       mma_16816(st.o[4 * w + k + 1], lo01[k + 1], hi01[k + 1], lo23[k + 1], hi23[k + 1], hmul2(b0, s.z),
                 hmul2(b1, s.w));
@@ -234,75 +236,76 @@ __device__ __forceinline__ void weigh(State& st, uint32_t unit, uint32_t sc, int
   }
 }
 
-// N units of one pair; the first valid[u] tokens of unit u are the sequence's.
-template <int N>
-__device__ __forceinline__ void attend(State& st, const uint32_t (&unit)[N], uint32_t sc, const int (&valid)[N],
-                                       int g, int t) {
-  float x[N][4];
+// One tile: its first `valid` tokens are the sequence's (kMask: fewer than all).
+template <bool kMask>
+__device__ __forceinline__ void attend(State& st, uint32_t tile, uint32_t vscale, int valid, int g, int t, int lane) {
+  __syncwarp();  // the tile before this one is done with vscale
+  convert_vscales<kMask>(tile, vscale, valid, lane);
+  convert_vscales<kMask>(tile + kUnitBytes, vscale + kVScaleBytes, valid - kUnitTokens, lane);
+  float x[2][4];
+  scores<kMask>(st, tile, valid, g, t, x[0]);
+  scores<kMask>(st, tile + kUnitBytes, valid - kUnitTokens, g, t, x[1]);
+  const float hi0 = fmaxf(fmax3(x[0][0], x[0][2], x[1][0]), x[1][2]) * st.sc[0];
+  const float hi1 = fmaxf(fmax3(x[0][1], x[0][3], x[1][1]), x[1][3]) * st.sc[1];
+  if (__any_sync(0xffffffffu, hi0 > st.thr[0] || hi1 > st.thr[1])) {
 #pragma unroll
-  for (int u = 0; u < N; ++u) scores(st, unit[u], sc + u * uint32_t(sizeof(Scales)), valid[u], g, t, x[u]);
-  float hi0 = fmaxf(x[0][0], x[0][2]), hi1 = fmaxf(x[0][1], x[0][3]);
-  if (N == 2) hi0 = fmax3(hi0, x[N - 1][0], x[N - 1][2]), hi1 = fmax3(hi1, x[N - 1][1], x[N - 1][3]);
-  if (__any_sync(0xffffffffu, hi0 > st.m[0] + kRescale || hi1 > st.m[1] + kRescale)) {
-    float n0 = hi0, n1 = hi1;
+    for (int e = 0; e < 2; ++e) {
+      float m = e ? hi1 : hi0;
 #pragma unroll
-    for (int off = 4; off < 32; off <<= 1) {
-      n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, off));
-      n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
-    }
-    n0 = fmaxf(n0, st.m[0]);
-    n1 = fmaxf(n1, st.m[1]);
-    const float f0 = st.m[0] == -INFINITY ? 0.f : fast_exp2(st.m[0] - n0);
-    const float f1 = st.m[1] == -INFINITY ? 0.f : fast_exp2(st.m[1] - n1);
-    st.m[0] = n0, st.m[1] = n1;
-    st.l[0] *= f0, st.l[1] *= f1;
+      for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+      m = fmaxf(m, st.thr[e] - kRescale);
+      const float ref = m == -INFINITY ? 0.f : m - kPShift;
+      const float f = st.thr[e] == -INFINITY ? 0.f : fast_exp2(st.ref[e] - ref);
+      st.ref[e] = ref;
+      st.thr[e] = m + kRescale;
+      st.l[e] *= f;
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      st.o[j][0] *= f0, st.o[j][2] *= f0;
-      st.o[j][1] *= f1, st.o[j][3] *= f1;
+      for (int j = 0; j < kGroups; ++j) st.o[j][e] *= f, st.o[j][2 + e] *= f;
     }
   }
-  const float r0 = st.m[0] == -INFINITY ? 0.f : st.m[0] - kPShift;
-  const float r1 = st.m[1] == -INFINITY ? 0.f : st.m[1] - kPShift;
+  uint32_t b[2][2];
 #pragma unroll
-  for (int u = 0; u < N; ++u) {
-    const float p0 = fast_exp2(x[u][0] - r0), p1 = fast_exp2(x[u][1] - r1);
-    const float p2 = fast_exp2(x[u][2] - r0), p3 = fast_exp2(x[u][3] - r1);
+  for (int u = 0; u < 2; ++u) {
+    const float p0 = fast_exp2(fmaf(x[u][0], st.sc[0], -st.ref[0])), p1 = fast_exp2(fmaf(x[u][1], st.sc[1], -st.ref[1]));
+    const float p2 = fast_exp2(fmaf(x[u][2], st.sc[0], -st.ref[0])), p3 = fast_exp2(fmaf(x[u][3], st.sc[1], -st.ref[1]));
     st.l[0] += p0 + p2;
     st.l[1] += p1 + p3;
-    weigh(st, unit[u], sc + u * uint32_t(sizeof(Scales)), g, t, movmatrix(half2_of(p0, p1)),
-          movmatrix(half2_of(p2, p3)));
+    b[u][0] = movmatrix(half2_of(p0, p1));
+    b[u][1] = movmatrix(half2_of(p2, p3));
   }
+  __syncwarp();  // vscale is written
+  weigh(st, tile, vscale, g, t, b[0][0], b[0][1]);
+  weigh(st, tile + kUnitBytes, vscale + kVScaleBytes, g, t, b[1][0], b[1][1]);
 }
 
 // Orders this thread's shared-memory writes before later copies into them.
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A unit of zeros in place of one that the table does not lead to (by the whole warp).
+// A unit of zeros in place of one that the table does not lead to (by the
+// whole warp), ordered before the next copy into its place.
 __device__ __forceinline__ void zero_unit(uint32_t unit, int lane) {
   for (int i = lane; i < kUnitBytes / 16; i += 32) st_shared_v4(unit + 16 * i, 0, 0, 0, 0);
+  fence_proxy_async();
   __syncwarp();
 }
 
-__device__ __forceinline__ int seq_units(const DecodeArgs& a, int b, bool report) {
+__device__ __forceinline__ int seq_tiles(const DecodeArgs& a, int b, bool report) {
   int n = a.ctx[b];
   const int64_t most = static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4);
   if (n > most) {
     if (report) atomicOr(a.err, kErrContextTooLong);
     n = static_cast<int>(most);
   }
-  return n <= 0 ? 0 : (n + kUnitTokens - 1) / kUnitTokens;
+  return n <= 0 ? 0 : (n + kTileTokens - 1) / kTileTokens;
 }
 
-template <int kStages>
 __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  using Sm = Smem<kStages>;
-  Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   // Pieces of pairs that are not one warp's: [2 * kWarps][group] (m, l), and
   // [group][128] each: a warp's first one in its own place, its last one in
   // the warp's ring.
-  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Sm));
+  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Smem));
   float* piece_first = reinterpret_cast<float*>(piece_ml + 2 * kWarps * a.group);
   auto piece_o = [&](int p) {
     return (p & 1) ? reinterpret_cast<float*>(sm.ring[p >> 1]) : piece_first + (p >> 1) * a.group * kD;
@@ -317,11 +320,11 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
   // lets its dependents start early (see the entry point): they are read, and
   // the schedule made of them, while the kernel before this one drains.
 
-  // ---- the prefix of units: two sequences a thread ----
+  // ---- the prefix of tiles: two sequences a thread ----
   {
     const int b = 2 * tid;
-    const int u0 = b < a.batch ? seq_units(a, b, blockIdx.x == 0) : 0;
-    const int u1 = b + 1 < a.batch ? seq_units(a, b + 1, blockIdx.x == 0) : 0;
+    const int u0 = b < a.batch ? seq_tiles(a, b, blockIdx.x == 0) : 0;
+    const int u1 = b + 1 < a.batch ? seq_tiles(a, b + 1, blockIdx.x == 0) : 0;
     int sum = u0 + u1;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -348,8 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
     }
   };
   const int64_t total = static_cast<int64_t>(sm.pre[a.batch]) * a.kvh;
-  const int ctas =
-      static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits)));
+  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kWarps - 1) / kWarps));
   const int c = blockIdx.x;
   if (c >= ctas) {
     pdl_wait();
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
   const int64_t clo = total * c / ctas, chi = total * (c + 1) / ctas;
   const int64_t lo = clo + (chi - clo) * warp / kWarps, hi = clo + (chi - clo) * (warp + 1) / kWarps;
 
-  auto find_seq = [&](int64_t x) {  // the sequence that unit x belongs to
+  auto find_seq = [&](int64_t x) {  // the sequence that tile x belongs to
     int b0 = 0, b1 = a.batch;       // pre[b0] * kvh <= x < pre[b1] * kvh
     while (b1 - b0 > 1) {
       const int mid = (b0 + b1) >> 1;
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
           *reinterpret_cast<uint32_t*>(row + 16 * j) = pack_bf16x2(st.o[j][e] * inv, st.o[j][2 + e] * inv);
       } else {
         const int at = (2 * warp + slot) * a.group + head;
-        if (g == 0) piece_ml[at] = make_float2(st.m[e], st.l[e]);
+        if (g == 0) piece_ml[at] = make_float2(st.thr[e] - kRescale, st.l[e]);
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
           *reinterpret_cast<float2*>(piece_o(2 * warp + slot) + head * kD + 16 * j + 2 * g) = make_float2(st.o[j][e], st.o[j][2 + e]);
@@ -398,63 +400,70 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
     if (!whole && lane == 0) sm.piece_pair[2 * warp + slot] = b * a.kvh + h;
   };
 
-  // ---- this warp's units ----
+  // ---- this warp's tiles ----
   const int n = static_cast<int>(hi - lo);
-  constexpr int kFirst = 1 << 8, kLast = 1 << 9, kBad = 1 << 10;
-  // What lane i knows of the batch of 32 units that starts at lo + base: where
-  // unit base + i lies, whose it is, and its tokens with the flags above.
-  const uint8_t* next_at = nullptr;
+  constexpr int kFirst = 1 << 8, kLast = 1 << 9, kBad = 1 << 10, kBad2 = 1 << 11;
+  // What lane i knows of the batch of 32 tiles that starts at lo + base: where
+  // the units of tile base + i lie, whose it is, and its tokens with the flags
+  // above.
+  const uint8_t *next_at = nullptr, *next_at2 = nullptr;
   int next_pair = 0, next_info = 0;
   auto look_up = [&](int base) {
     if (base + lane >= n) return;
     const int64_t x = lo + base + lane;
     const int b = find_seq(x);
-    const int units = sm.pre[b + 1] - sm.pre[b];
+    const int tiles = sm.pre[b + 1] - sm.pre[b];
     const int64_t in_seq = x - static_cast<int64_t>(sm.pre[b]) * a.kvh;
-    const int h = static_cast<int>(in_seq / units);
-    const int u = static_cast<int>(in_seq - static_cast<int64_t>(h) * units);
-    const int blk = a.tables[static_cast<int64_t>(b) * a.bt_stride + (u >> a.upb_log2)];
+    const int h = static_cast<int>(in_seq / tiles);
+    const int tile = static_cast<int>(in_seq - static_cast<int64_t>(h) * tiles);
+    const int64_t room = (static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4));
+    const int64_t left = min(static_cast<int64_t>(a.ctx[b]), room) - static_cast<int64_t>(tile) * kTileTokens;
+    const int tokens = static_cast<int>(min(left, static_cast<int64_t>(kTileTokens)));
     next_pair = b * a.kvh + h;
-    next_info = min(a.ctx[b] - u * kUnitTokens, kUnitTokens) | (u == 0 ? kFirst : 0) | (u == units - 1 ? kLast : 0);
-    if (blk < 0 || blk >= a.num_blocks) next_info |= kBad;
-    next_at = a.pool + ((((static_cast<int64_t>(blk) * a.kvh + h) << a.upb_log2) + (u & ((1 << a.upb_log2) - 1))) *
-                        kUnitBytes);
+    next_info = tokens | (tile == 0 ? kFirst : 0) | (tile == tiles - 1 ? kLast : 0);
+    auto place = [&](int unit, int flag) {
+      const int blk = a.tables[static_cast<int64_t>(b) * a.bt_stride + (unit >> a.upb_log2)];
+      if (blk < 0 || blk >= a.num_blocks) next_info |= flag;
+      return a.pool + ((((static_cast<int64_t>(blk) * a.kvh + h) << a.upb_log2) + (unit & ((1 << a.upb_log2) - 1))) *
+                       kUnitBytes);
+    };
+    next_at = place(2 * tile, kBad);
+    // blocks of one unit: the tile's second unit has a block of its own
+    if (a.upb_log2 == 0 && tokens > kUnitTokens) next_at2 = place(2 * tile + 1, kBad2);
+    else if (next_info & kBad) next_info |= kBad2;
   };
-  auto fetch = [&](int i) {  // unit i into its stage, by the lane that knows it
+  auto fetch = [&](int i) {  // tile i into its stage, by the lane that knows it
     if (lane != (i & 31)) return;
     uint64_t* bar = &sm.full[warp][i % kStages];
-    if (next_info & kBad) {
-      atomicOr(a.err, kErrBadBlockId);
-      mbar_arrive(bar);
-    } else {
-      mbar_arrive_expect_tx(bar, kUnitBytes);
-      bulk_load(sm.ring[warp][i % kStages], next_at, kUnitBytes, bar);
+    uint8_t* to = sm.ring[warp][i % kStages];
+    const bool two = (next_info & 0xff) > kUnitTokens;
+    if (a.upb_log2 > 0 && !(next_info & kBad)) {  // one copy
+      mbar_arrive_expect_tx(bar, two ? kTileBytes : kUnitBytes);
+      bulk_load(to, next_at, two ? kTileBytes : kUnitBytes, bar);
+      return;
     }
+    const bool one_ok = !(next_info & kBad), two_ok = two && !(next_info & kBad2);
+    if (!one_ok || (two && !two_ok)) atomicOr(a.err, kErrBadBlockId);
+    if (!one_ok && !two_ok) {
+      mbar_arrive(bar);
+      return;
+    }
+    mbar_arrive_expect_tx(bar, (one_ok ? kUnitBytes : 0) + (two_ok ? kUnitBytes : 0));
+    if (one_ok) bulk_load(to, next_at, kUnitBytes, bar);
+    if (two_ok) bulk_load(to + kUnitBytes, next_at2, kUnitBytes, bar);
   };
   look_up(0);
   pdl_wait();
   zero_empty();
   int issued = 0;
   for (; issued < min(n, kStages); ++issued) fetch(issued);
-  int pair_now = next_pair, info_now = next_info, batch_end = 32;  // the batch that is being read
-  bool ok = true;
-  int b = 0, h = 0;
-  bool whole = false, open = false;
-  int slot = 0;
-  auto info_of = [&](int i) {  // of the unit that is read next, or the one after it
-    return __shfl_sync(0xffffffffu, i < batch_end ? info_now : next_info, i & 31);
-  };
-  const uint32_t ring = smem_u32(sm.ring[warp]), sc = smem_u32(sm.scales[warp]);
-  auto landed = [&](int i) {
-    if (ok && !__all_sync(0xffffffffu, mbar_wait(&sm.full[warp][i % kStages], (i / kStages) & 1))) {
-      ok = false;
-      if (lane == 0) atomicOr(a.err, kErrWaitTimeout);
-    }
-    return ring + (i % kStages) * kUnitBytes;
-  };
-  for (int i = 0; i < n;) {
-    if (i >= batch_end) pair_now = next_pair, info_now = next_info, batch_end += 32;
-    const int info = info_of(i);
+  int pair_now = next_pair, info_now = next_info;  // the batch that is being read
+  bool ok = true, whole = false, open = false;
+  int b = 0, h = 0, slot = 0;
+  const uint32_t ring = smem_u32(sm.ring[warp]), vscale = smem_u32(sm.vscale[warp]);
+  for (int i = 0; i < n; ++i) {
+    if ((i & 31) == 0 && i > 0) pair_now = next_pair, info_now = next_info;
+    const int info = __shfl_sync(0xffffffffu, info_now, i & 31);
     if (!open) {
       const int pair = __shfl_sync(0xffffffffu, pair_now, i & 31);
       b = pair / a.kvh;
@@ -464,40 +473,32 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
       slot = i == 0 ? 0 : 1;
       open = true;
     }
-    const bool two = !(info & kLast) && i + 1 < n;
-    const int info2 = two ? info_of(i + 1) : 0;
-    const uint32_t u0 = landed(i);
-    if (!ok || (info & kBad)) zero_unit(u0, lane);  // reads as zeros
-    convert_scales(u0, sc, info & 0xff, lane);
-    if (two) {
-      const uint32_t u1 = landed(i + 1);
-      if (!ok || (info2 & kBad)) zero_unit(u1, lane);
-      convert_scales(u1, sc + sizeof(Scales), info2 & 0xff, lane);
-      __syncwarp();
-      const uint32_t units[2] = {u0, u1};
-      const int valid[2] = {info & 0xff, info2 & 0xff};
-      attend<2>(st, units, sc, valid, g, t);
-    } else {
-      __syncwarp();
-      const uint32_t units[1] = {u0};
-      const int valid[1] = {info & 0xff};
-      attend<1>(st, units, sc, valid, g, t);
+    const uint32_t tile = ring + (i % kStages) * kTileBytes;
+    uint64_t* bar = &sm.full[warp][i % kStages];
+    const uint32_t parity = (i / kStages) & 1;
+    if (ok && !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)) && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
+      ok = false;
+      if (lane == 0) atomicOr(a.err, kErrWaitTimeout);
     }
-    if ((info | info2) & kBad) fence_proxy_async();  // before the next copy into it
-    __syncwarp();  // every lane is done with the units and the scales
-    i += two ? 2 : 1;
-    for (int k = 0; k < 2; ++k) {
-      if (!ok || issued >= min(n, i + kStages)) break;
+    const int tokens = info & 0xff;
+    if (tokens == kTileTokens && !(info & (kBad | kBad2)) && ok) {
+      attend<false>(st, tile, vscale, tokens, g, t, lane);
+    } else {
+      if (!ok || (info & kBad)) zero_unit(tile, lane);  // reads as zeros
+      if (!ok || (info & kBad2)) zero_unit(tile + kUnitBytes, lane);
+      attend<true>(st, tile, vscale, tokens, g, t, lane);
+    }
+    __syncwarp();  // every lane is done with the tile
+    if (ok && issued < n) {
       if ((issued & 31) == 0) look_up(issued);
       fetch(issued);
       ++issued;
     }
-    const int last = two ? info2 : info;
-    if ((last & kLast) || i == n) {
+    if ((info & kLast) || i == n - 1) {
       if (!ok)  // the ring takes the piece only after every copy into it has landed or been given up
         for (int k = max(i, issued - kStages); k < issued; ++k)
           (void)mbar_wait(&sm.full[warp][k % kStages], (k / kStages) & 1);
-      finish(b, h, whole && (last & kLast), slot);
+      finish(b, h, whole && (info & kLast), slot);
       open = false;
     }
   }
@@ -531,9 +532,9 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
       o.x += wp * v.x, o.y += wp * v.y, o.z += wp * v.z, o.w += wp * v.w;
     }
     const int pb = pair / a.kvh, ph = pair - pb * a.kvh;
-    const int units = sm.pre[pb + 1] - sm.pre[pb];
-    const int64_t plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * units;
-    if (plo >= clo && plo + units <= chi) {
+    const int tiles = sm.pre[pb + 1] - sm.pre[pb];
+    const int64_t plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * tiles;
+    if (plo >= clo && plo + tiles <= chi) {
       const float inv = l == 0.f ? 0.f : a.v_scale / l;
       *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
           make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
@@ -544,24 +545,24 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
       __threadfence();
     }
   }
-  // ---- pairs split over CTAs: the first and the last of this CTA's units ----
-  auto cta_of = [&](int64_t unit) { return static_cast<int>(((unit + 1) * ctas - 1) / total); };
-  auto pair_of = [&](int64_t unit, int& pb, int& ph, int64_t& plo, int& units) {
-    pb = find_seq(unit);
+  // ---- pairs split over CTAs: the first and the last of this CTA's tiles ----
+  auto cta_of = [&](int64_t tile) { return static_cast<int>(((tile + 1) * ctas - 1) / total); };
+  auto pair_of = [&](int64_t tile, int& pb, int& ph, int64_t& plo, int& tiles) {
+    pb = find_seq(tile);
     while (sm.pre[pb + 1] == sm.pre[pb]) ++pb;
-    units = sm.pre[pb + 1] - sm.pre[pb];
-    ph = static_cast<int>((unit - static_cast<int64_t>(sm.pre[pb]) * a.kvh) / units);
-    plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * units;
+    tiles = sm.pre[pb + 1] - sm.pre[pb];
+    ph = static_cast<int>((tile - static_cast<int64_t>(sm.pre[pb]) * a.kvh) / tiles);
+    plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * tiles;
   };
   __syncthreads();
   if (tid < 2) {
-    int pb, ph, units;
+    int pb, ph, tiles;
     int64_t plo;
-    pair_of(tid == 0 ? clo : chi - 1, pb, ph, plo, units);
+    pair_of(tid == 0 ? clo : chi - 1, pb, ph, plo, tiles);
     // end 0: a pair that began before this CTA; end 1: one that begins here and goes on
-    const bool split = tid == 0 ? plo < clo : plo >= clo && plo + units > chi;
+    const bool split = tid == 0 ? plo < clo : plo >= clo && plo + tiles > chi;
     if (split) {
-      const int c0 = cta_of(plo), c1 = cta_of(plo + units - 1);
+      const int c0 = cta_of(plo), c1 = cta_of(plo + tiles - 1);
       __threadfence();
       if (atomicAdd(a.tickets + c0, 1) == c1 - c0) {
         a.tickets[c0] = 0;  // every piece is in: nobody else touches it in this call
@@ -573,10 +574,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
   for (int end = 0; end < 2; ++end) {
     if (!sm.last[end]) continue;
     __threadfence();
-    int pb, ph, units;
+    int pb, ph, tiles;
     int64_t plo;
-    pair_of(end == 0 ? clo : chi - 1, pb, ph, plo, units);
-    const int c0 = cta_of(plo), c1 = cta_of(plo + units - 1);
+    pair_of(end == 0 ? clo : chi - 1, pb, ph, plo, tiles);
+    const int c0 = cta_of(plo), c1 = cta_of(plo + tiles - 1);
     for (int head = warp; head < a.group; head += kWarps) {
       // the pair's piece in CTA k: its end 1 where it begins, its end 0 after that
       auto at = [&](int k) { return (static_cast<int64_t>(k) * 2 + (k == c0 ? 1 : 0)) * a.group + head; };
@@ -601,25 +602,12 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
   }
 }
 
-template <int kStages>
 constexpr size_t smem_bytes(int group) {
-  return sizeof(Smem<kStages>) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
+  return sizeof(Smem) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
 }
-// Four units in flight a warp where their shared memory leaves room for the pieces of the group's heads, else three.
-constexpr int kFewHeads = 4;
-static_assert(sizeof(Smem<3>) % 16 == 0 && sizeof(Smem<4>) % 16 == 0, "the pieces behind it are 16-byte aligned");
-static_assert(smem_bytes<4>(kFewHeads) <= 232448 && smem_bytes<3>(kMaxGroup) <= 232448,
-              "decode shared memory exceeds the 227 KB per-CTA limit");
-static_assert(3 * kUnitBytes >= kMaxGroup * kD * 4, "a warp's ring takes its last piece");
-
-template <int kStages>
-int launch(const DecodeArgs& a, int ctas, cudaStream_t stream) {
-  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&decode_kernel<kStages>),
-                                     smem_bytes<kStages>(kStages == 4 ? kFewHeads : kMaxGroup));
-  if (rc != NVK_OK) return rc;
-  return check_cuda(launch_pdl(decode_kernel<kStages>, dim3(ctas), dim3(kThreads), smem_bytes<kStages>(a.group), stream, a),
-                    "fp4_paged_decode launch");
-}
+static_assert(sizeof(Smem) % 16 == 0, "the pieces behind it are 16-byte aligned");
+static_assert(smem_bytes(kMaxGroup) <= 232448, "decode shared memory exceeds the 227 KB per-CTA limit");
+static_assert(kStages * kTileBytes >= kMaxGroup * kD * 4, "a warp's ring takes its last piece");
 
 size_t workspace_bytes(int group, int ctas) {
   return kMlOffset + static_cast<size_t>(ctas) * 2 * group * (sizeof(float2) + kD * sizeof(float));
@@ -699,6 +687,9 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   if (workspace_bytes_given < workspace_bytes(group, ctas))
     return fail(NVK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes_given,
                 workspace_bytes(group, ctas));
+  if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&decode_kernel), smem_bytes(kMaxGroup))) != NVK_OK)
+    return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
   a.pool = static_cast<const uint8_t*>(kv_cache);
@@ -721,8 +712,8 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
     a.q = static_cast<const __nv_bfloat16*>(query) + static_cast<int64_t>(b0) * num_heads * kD;
     a.tables = block_tables + static_cast<int64_t>(b0) * block_table_stride;
     a.ctx = context_lens + b0;
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if ((rc = group <= kFewHeads ? launch<4>(a, ctas, st) : launch<3>(a, ctas, st)) != NVK_OK)
+    if ((rc = check_cuda(launch_pdl(decode_kernel, dim3(ctas), dim3(kThreads), smem_bytes(group), st, a),
+                         "fp4_paged_decode launch")) != NVK_OK)
       return rc;
   }
   return NVK_OK;
