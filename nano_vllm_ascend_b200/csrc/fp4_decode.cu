@@ -35,14 +35,11 @@ namespace nvk {
 namespace fp4 {
 namespace {
 
-constexpr int kWarps = 16;
-constexpr int kThreads = kWarps * 32;
-constexpr int kMaxSeqs = 1024;   // sequences per launch (their prefix of tiles sits in shared memory)
-constexpr int kMaxCtas = 1024;
-constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
 constexpr int kTileTokens = 2 * kUnitTokens;  // a warp's step
 constexpr int kTileBytes = 2 * kUnitBytes;
 constexpr int kStages = 2;       // tiles in flight a warp
+constexpr int kMaxCtas = 1024;
+constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
 constexpr float kRescale = 3.f;  // log2 by which a score may pass the running maximum before O is rescaled
 constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and scales up to 448, P s fits fp16
 constexpr size_t kTicketOffset = 256;
@@ -64,16 +61,18 @@ struct DecodeArgs {
   float v_scale;
 };
 
+template <int kWarps>
 struct Smem {
   alignas(128) uint8_t ring[kWarps][kStages][kTileBytes];  // a warp's last piece comes here when it has read them
+  uint4 q[kWarps][kGroups / 2][32];  // fragments of Q, fp16
   uint2 vscale[kWarps][2][kGroups / 2][4][2];  // [unit][j / 2][quad][j % 2]: V's scales of the quad's four tokens, fp16
   uint64_t full[kWarps][kStages];
-  int pre[kMaxSeqs + 1];  // tiles before each sequence (of one KV head)
+  int pre[2 * kWarps * 32 + 1];  // tiles before each sequence (of one KV head)
   int scan[kWarps];
-  int piece_pair[2 * kWarps];
+  int piece_pair[32];
   int last[2];
 };
-constexpr uint32_t kVScaleBytes = sizeof(Smem::vscale) / (2 * kWarps);  // of one unit
+constexpr uint32_t kVScaleBytes = kGroups * kUnitTokens * 2;  // of one unit
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
@@ -95,7 +94,7 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
 }
 
 struct State {
-  uint32_t q[kGroups][2];  // the B fragments of Q^T: head lane / 4, dims 16 j + 4 t + {0, 1} and {2, 3}
+  uint32_t q;              // shared address of this lane's B fragments of Q^T (see load_q)
   float sc[2];             // log2 factor of the scores of heads 2 t and 2 t + 1
   float ref[2];            // p = 2^(score - ref): their running maximum - kPShift
   float thr[2];            // the score above which it moves: their running maximum + kRescale (-inf at first)
@@ -103,7 +102,26 @@ struct State {
   float o[kGroups][4];     // O^T: dims 16 j + 2 g (heads 2 t, 2 t + 1), then 16 j + 2 g + 1 (the same)
 };
 
-// Q's rows of one pair as fragments; g = lane / 4, t = lane % 4.
+__device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Q's rows of one pair as fragments: head g = lane / 4, dims 16 j + 4 t + {0, 1}
+// and {2, 3}, t = lane % 4. They stay in shared memory (a lane reads only what
+// it wrote): the 16 registers would cost spills.
 __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g, int t, State& st) {
   uint2 raw[kGroups];
   const bool live = g < a.group;
@@ -125,8 +143,8 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
   const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
   for (int j = 0; j < kGroups; ++j) {
-    st.q[j][0] = half2_of(bf16lo_to_f32(raw[j].x) * down, bf16hi_to_f32(raw[j].x) * down);
-    st.q[j][1] = half2_of(bf16lo_to_f32(raw[j].y) * down, bf16hi_to_f32(raw[j].y) * down);
+    st_shared_v2(st.q + 512 * (j >> 1) + 8 * (j & 1), half2_of(bf16lo_to_f32(raw[j].x) * down, bf16hi_to_f32(raw[j].x) * down),
+                 half2_of(bf16lo_to_f32(raw[j].y) * down, bf16hi_to_f32(raw[j].y) * down));
   }
   st.sc[0] = __shfl_sync(0xffffffffu, up, 8 * t) * a.scale_log2;
   st.sc[1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * a.scale_log2;
@@ -137,23 +155,6 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
   for (int j = 0; j < kGroups; ++j)
 #pragma unroll
     for (int c = 0; c < 4; ++c) st.o[j][c] = 0.f;
-}
-
-__device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
-}
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 // A unit's V scales to fp16, once for the whole warp: lane i converts word i.
@@ -195,8 +196,9 @@ __device__ __forceinline__ void scores(const State& st, uint32_t unit, int valid
     e2m1_to_half2(wa[w], p[0], p[1], p[2], p[3]);
     e2m1_to_half2(wb[w], q[0], q[1], q[2], q[3]);
     float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
-    mma_16816(d, p[0], q[0], p[1], q[1], st.q[2 * w][0], st.q[2 * w][1]);
-    mma_16816(e, p[2], q[2], p[3], q[3], st.q[2 * w + 1][0], st.q[2 * w + 1][1]);
+    const uint4 f = ld_shared_v4(st.q + 512 * w);
+    mma_16816(d, p[0], q[0], p[1], q[1], f.x, f.y);
+    mma_16816(e, p[2], q[2], p[3], q[3], f.z, f.w);
     const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&sa[w]));
     const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&sb[w]));
     x[0] = fmaf(d[0], fa.x, x[0]), x[1] = fmaf(d[1], fa.x, x[1]);
@@ -299,13 +301,15 @@ __device__ __forceinline__ int seq_tiles(const DecodeArgs& a, int b, bool report
   return n <= 0 ? 0 : (n + kTileTokens - 1) / kTileTokens;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a) {
+template <int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  using Sm = Smem<kWarps>;
+  Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
   // Pieces of pairs that are not one warp's: [2 * kWarps][group] (m, l), and
   // [group][128] each: a warp's first one in its own place, its last one in
   // the warp's ring.
-  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Smem));
+  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Sm));
   float* piece_first = reinterpret_cast<float*>(piece_ml + 2 * kWarps * a.group);
   auto piece_o = [&](int p) {
     return (p & 1) ? reinterpret_cast<float*>(sm.ring[p >> 1]) : piece_first + (p >> 1) * a.group * kD;
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
     if (b <= a.batch) sm.pre[b] = at;
     if (b + 1 <= a.batch) sm.pre[b + 1] = at + u0;
     if (b + 2 == a.batch) sm.pre[b + 2] = at + u0 + u1;
-    if (tid < 2 * kWarps) sm.piece_pair[tid] = -1;
+    if (tid < 32) sm.piece_pair[tid] = -1;
     if (tid < 2) sm.last[tid] = 0;
     __syncthreads();
   }
@@ -373,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
 
   // Writes this warp's result of a pair as a piece (index 2 * warp + slot), or as the output.
   State st;
+  st.q = smem_u32(&sm.q[warp][0][lane]);
   auto finish = [&](int b, int h, bool whole, int slot) {
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
@@ -602,12 +607,37 @@ __global__ void __launch_bounds__(kThreads, 1) decode_kernel(const DecodeArgs a)
   }
 }
 
+template <int kWarps>
 constexpr size_t smem_bytes(int group) {
-  return sizeof(Smem) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
+  return sizeof(Smem<kWarps>) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
 }
-static_assert(sizeof(Smem) % 16 == 0, "the pieces behind it are 16-byte aligned");
-static_assert(smem_bytes(kMaxGroup) <= 232448, "decode shared memory exceeds the 227 KB per-CTA limit");
+// 16 warps where shared memory has room for the pieces of the group's heads
+// beside their rings, else 12 (16 against 12 at two heads, 256 contexts of
+// about 4096 tokens: 230 against 244 us).
+constexpr int kFewHeads = 4;
+static_assert(sizeof(Smem<16>) % 16 == 0 && sizeof(Smem<12>) % 16 == 0, "the pieces behind it are 16-byte aligned");
+static_assert(smem_bytes<16>(kFewHeads) <= 232448 && smem_bytes<12>(kMaxGroup) <= 232448,
+              "decode shared memory exceeds the 227 KB per-CTA limit");
 static_assert(kStages * kTileBytes >= kMaxGroup * kD * 4, "a warp's ring takes its last piece");
+
+// The sequences in launches of as many as the kernel's prefix holds.
+template <int kWarps>
+int launch(DecodeArgs a, int batch, int ctas, cudaStream_t stream) {
+  const void* kernel = reinterpret_cast<const void*>(&decode_kernel<kWarps>);
+  int rc = ensure_dynamic_smem(kernel, smem_bytes<kWarps>(kWarps == 16 ? kFewHeads : kMaxGroup));
+  constexpr int kMaxSeqs = 2 * kWarps * 32;
+  for (int left = batch; rc == NVK_OK && left > 0; left -= kMaxSeqs) {
+    a.batch = left < kMaxSeqs ? left : kMaxSeqs;
+    rc = check_cuda(launch_pdl(decode_kernel<kWarps>, dim3(ctas), dim3(kWarps * 32), smem_bytes<kWarps>(a.group),
+                               stream, a),
+                    "fp4_paged_decode launch");
+    a.out += static_cast<int64_t>(kMaxSeqs) * a.heads * kD;
+    a.q += static_cast<int64_t>(kMaxSeqs) * a.heads * kD;
+    a.tables += static_cast<int64_t>(kMaxSeqs) * a.bt_stride;
+    a.ctx += kMaxSeqs;
+  }
+  return rc;
+}
 
 size_t workspace_bytes(int group, int ctas) {
   return kMlOffset + static_cast<size_t>(ctas) * 2 * group * (sizeof(float2) + kD * sizeof(float));
@@ -676,7 +706,7 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   if (!aligned16(out) || !aligned16(query) || !aligned16(workspace))
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: q, out and workspace must be 16-byte aligned", who);
   const int upb_log2 = units_log2(block_size);
-  const int64_t seqs = batch < kMaxSeqs ? batch : kMaxSeqs;
+  const int64_t seqs = batch < 1024 ? batch : 1024;
   if (((seqs * max_blocks_per_seq) << upb_log2) > 0x7fffffffll ||
       (static_cast<int64_t>(max_blocks_per_seq) << upb_log2) > 0x7fffffffll / kUnitTokens)
     return fail(NVK_ERR_UNSUPPORTED, "%s: %d blocks of %d tokens a sequence are above the kernel's range", who,
@@ -687,9 +717,6 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   if (workspace_bytes_given < workspace_bytes(group, ctas))
     return fail(NVK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes_given,
                 workspace_bytes(group, ctas));
-  if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&decode_kernel), smem_bytes(kMaxGroup))) != NVK_OK)
-    return rc;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
   a.pool = static_cast<const uint8_t*>(kv_cache);
@@ -706,15 +733,10 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   a.upb_log2 = upb_log2;
   a.scale_log2 = scale * 1.4426950408889634f * k_scale;
   a.v_scale = v_scale;
-  for (int b0 = 0; b0 < batch; b0 += kMaxSeqs) {
-    a.batch = batch - b0 < kMaxSeqs ? batch - b0 : kMaxSeqs;
-    a.out = static_cast<__nv_bfloat16*>(out) + static_cast<int64_t>(b0) * num_heads * kD;
-    a.q = static_cast<const __nv_bfloat16*>(query) + static_cast<int64_t>(b0) * num_heads * kD;
-    a.tables = block_tables + static_cast<int64_t>(b0) * block_table_stride;
-    a.ctx = context_lens + b0;
-    if ((rc = check_cuda(launch_pdl(decode_kernel, dim3(ctas), dim3(kThreads), smem_bytes(group), st, a),
-                         "fp4_paged_decode launch")) != NVK_OK)
-      return rc;
-  }
-  return NVK_OK;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.q = static_cast<const __nv_bfloat16*>(query);
+  a.tables = block_tables;
+  a.ctx = context_lens;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return group <= kFewHeads ? launch<16>(a, batch, ctas, st) : launch<12>(a, batch, ctas, st);
 }
