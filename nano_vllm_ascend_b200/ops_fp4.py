@@ -34,37 +34,58 @@ def pool_shape(num_blocks: int, block_size: int, num_kv_heads: int) -> tuple[int
     return num_blocks, num_kv_heads, block_size // _lib.FP4_UNIT_TOKENS, _lib.FP4_UNIT_BYTES
 
 
+# A decode step makes a few of these calls a layer, so the checks are written
+# to cost little: tensors' properties are read once, and torch's raw stream
+# handle is asked for instead of a Stream object (3 us less a call).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(dev: torch.device, name: str, *args) -> None:
     """Calls ``name`` on ``dev`` and its current stream (the last argument)."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    index = dev.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            _lib.call(name, *args, _raw_stream(index))
+
+
+def _check_devices(dev: torch.device, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.device != dev or not t.is_cuda:
+            _require_cuda(name, t, dev)
 
 
 def _check_pool(who: str, kv_cache: torch.Tensor) -> tuple[int, int, int]:
     """(blocks, block size, KV heads) of a layer's pool."""
-    if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 4 or kv_cache.shape[3] != _lib.FP4_UNIT_BYTES \
+    shape = kv_cache.shape
+    if kv_cache.dtype != torch.uint8 or len(shape) != 4 or shape[3] != _lib.FP4_UNIT_BYTES \
             or not kv_cache.is_contiguous():
         raise ValueError(f"{who}: kv_cache must be contiguous uint8 [blocks, kv_heads, block_size / 16, "
-                         f"{_lib.FP4_UNIT_BYTES}], got {kv_cache.dtype} {tuple(kv_cache.shape)}")
-    nb, kvh, units, _ = kv_cache.shape
-    return nb, units * _lib.FP4_UNIT_TOKENS, kvh
+                         f"{_lib.FP4_UNIT_BYTES}], got {kv_cache.dtype} {tuple(shape)}")
+    return shape[0], shape[2] * _lib.FP4_UNIT_TOKENS, shape[1]
+
+
+def _row_stride(name: str, t: torch.Tensor) -> int:
+    """The token stride of rows [tokens, heads, 128] whose heads and dims are packed."""
+    stride = t.stride()
+    if len(stride) != 3 or stride[2] != 1 or stride[1] != HEAD_DIM or t.shape[2] != HEAD_DIM:
+        _require_rows(name, t)
+        raise ValueError(f"{name} must have {HEAD_DIM} dims a head, got shape {tuple(t.shape)} stride {stride}")
+    return stride[0]
 
 
 def _check_index(who: str, name: str, t: torch.Tensor, dtype: torch.dtype, count: int) -> torch.Tensor:
     if t.dtype != dtype or t.numel() != count:
         raise ValueError(f"{who}: {name} must be {dtype} with {count} entries, got {t.dtype} {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _error_ptr(who: str, error_word: torch.Tensor | None, dev: torch.device) -> int:
     if error_word is None:
         return 0
-    _require_cuda("error_word", error_word, dev)
-    if error_word.dtype != torch.int32 or error_word.numel() < 1:
-        raise ValueError(f"{who}: error_word must be a device int32")
+    if error_word.device != dev or error_word.dtype != torch.int32 or error_word.numel() < 1:
+        raise ValueError(f"{who}: error_word must be an int32 on {dev}")
     return error_word.data_ptr()
 
 
@@ -76,19 +97,19 @@ def kv_append_fp4(kv_cache: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     of ``error_word``."""
     who = "kv_append_fp4"
     dev = kv_cache.device
-    for name, t in (("kv_cache", kv_cache), ("key", key), ("value", value), ("slot_mapping", slot_mapping)):
-        _require_cuda(name, t, dev)
+    _check_devices(dev, kv_cache=kv_cache, key=key, value=value, slot_mapping=slot_mapping)
     nb, bs, kvh = _check_pool(who, kv_cache)
-    if key.dtype not in _DTYPES or value.dtype != key.dtype:
-        raise ValueError(f"{who}: key and value must both be bfloat16 or float16, got {key.dtype} and {value.dtype}")
-    _require_rows("key", key)
-    _require_rows("value", value)
-    if key.shape != value.shape or key.shape[1] != kvh or key.shape[2] != HEAD_DIM:
-        raise ValueError(f"kv shape mismatch: got {tuple(key.shape)} / {tuple(value.shape)}")
-    slots = _check_index(who, "slot_mapping", slot_mapping, torch.int64, key.shape[0])
-    _call(dev, "nvk_fp4_append", key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0),
-          kv_cache.data_ptr(), slots.data_ptr(), key.shape[0], nb, bs, kvh, HEAD_DIM, _DTYPES[key.dtype], k_scale,
-          v_scale, _error_ptr(who, error_word, dev))
+    dtype, shape = key.dtype, key.shape
+    if dtype not in _DTYPES or value.dtype != dtype:
+        raise ValueError(f"{who}: key and value must both be bfloat16 or float16, got {dtype} and {value.dtype}")
+    k_stride, v_stride = _row_stride("key", key), _row_stride("value", value)
+    tokens = shape[0]
+    if value.shape != shape or shape[1] != kvh:
+        raise ValueError(f"kv shape mismatch: got {tuple(shape)} / {tuple(value.shape)}")
+    slots = _check_index(who, "slot_mapping", slot_mapping, torch.int64, tokens)
+    _call(dev, "nvk_fp4_append", key.data_ptr(), value.data_ptr(), k_stride, v_stride, kv_cache.data_ptr(),
+          slots.data_ptr(), tokens, nb, bs, kvh, HEAD_DIM, _DTYPES[dtype], k_scale, v_scale,
+          _error_ptr(who, error_word, dev))
 
 
 def kv_read_fp4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, k_scale: float = 1.0, v_scale: float = 1.0,
@@ -100,25 +121,23 @@ def kv_read_fp4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, k_scale: flo
     outside the pool gives zeros and sets bit 4 of ``error_word``."""
     who = "kv_read_fp4"
     dev = kv_cache.device
-    for name, t in (("kv_cache", kv_cache), ("slot_mapping", slot_mapping)):
-        _require_cuda(name, t, dev)
+    _check_devices(dev, kv_cache=kv_cache, slot_mapping=slot_mapping)
     nb, bs, kvh = _check_pool(who, kv_cache)
     if dtype not in _DTYPES:
         raise ValueError(f"{who}: dtype must be bfloat16 or float16, got {dtype}")
     tokens = slot_mapping.numel()
     slots = _check_index(who, "slot_mapping", slot_mapping, torch.int64, tokens)
-    outs = []
     for name, t in (("key_out", key_out), ("value_out", value_out)):
-        if t is None:
-            t = torch.empty(tokens, kvh, HEAD_DIM, dtype=dtype, device=dev)
-        else:
-            _require_cuda(name, t, dev)
-            if t.shape != (tokens, kvh, HEAD_DIM) or t.dtype != dtype or not t.is_contiguous():
-                raise ValueError(f"{who}: {name} must be contiguous {dtype} [tokens, kv_heads, {HEAD_DIM}]")
-        outs.append(t)
-    _call(dev, "nvk_fp4_read", outs[0].data_ptr(), outs[1].data_ptr(), kv_cache.data_ptr(), slots.data_ptr(), tokens,
-          nb, bs, kvh, HEAD_DIM, _DTYPES[dtype], k_scale, v_scale, _error_ptr(who, error_word, dev))
-    return outs[0], outs[1]
+        if t is not None and (t.device != dev or t.shape != (tokens, kvh, HEAD_DIM) or t.dtype != dtype
+                              or not t.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be contiguous {dtype} [tokens, kv_heads, {HEAD_DIM}] on {dev}")
+    if key_out is None:
+        key_out = torch.empty((tokens, kvh, HEAD_DIM), dtype=dtype, device=dev)
+    if value_out is None:
+        value_out = torch.empty((tokens, kvh, HEAD_DIM), dtype=dtype, device=dev)
+    _call(dev, "nvk_fp4_read", key_out.data_ptr(), value_out.data_ptr(), kv_cache.data_ptr(), slots.data_ptr(),
+          tokens, nb, bs, kvh, HEAD_DIM, _DTYPES[dtype], k_scale, v_scale, _error_ptr(who, error_word, dev))
+    return key_out, value_out
 
 
 def qk_norm_rope_append_fp4(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q_weight: torch.Tensor,
@@ -131,38 +150,36 @@ def qk_norm_rope_append_fp4(query: torch.Tensor, key: torch.Tensor, value: torch
     kernel. Returns the rotated query [tokens, heads, 128]."""
     who = "qk_norm_rope_append_fp4"
     dev = query.device
-    for name, t in (("query", query), ("key", key), ("value", value), ("q_weight", q_weight),
-                    ("k_weight", k_weight), ("cos_table", cos_table), ("sin_table", sin_table),
-                    ("positions", positions), ("kv_cache", kv_cache), ("slot_mapping", slot_mapping)):
-        _require_cuda(name, t, dev)
-    for name, t in (("query", query), ("key", key), ("value", value)):
-        _require_rows(name, t)
-        if t.dtype != _BF16:
-            raise ValueError(f"{who}: {name} must be bfloat16")
-    tokens, num_heads, head_dim = query.shape
+    _check_devices(dev, query=query, key=key, value=value, q_weight=q_weight, k_weight=k_weight,
+                   cos_table=cos_table, sin_table=sin_table, positions=positions, kv_cache=kv_cache,
+                   slot_mapping=slot_mapping)
+    if query.dtype != _BF16 or key.dtype != _BF16 or value.dtype != _BF16:
+        raise ValueError(f"{who}: query, key and value must be bfloat16")
+    q_stride, k_stride, v_stride = _row_stride("query", query), _row_stride("key", key), _row_stride("value", value)
+    tokens, num_heads, _ = query.shape
     nb, bs, kvh = _check_pool(who, kv_cache)
-    if key.shape != (tokens, kvh, HEAD_DIM) or value.shape != key.shape or head_dim != HEAD_DIM:
-        raise ValueError(f"kv shape mismatch: got {tuple(key.shape)} / {tuple(value.shape)}")
+    shape = key.shape
+    if shape[0] != tokens or shape[1] != kvh or value.shape != shape:
+        raise ValueError(f"kv shape mismatch: got {tuple(shape)} / {tuple(value.shape)}")
     for t in (q_weight, k_weight):
         if t.numel() != HEAD_DIM or t.dtype != _BF16 or not t.is_contiguous():
             raise ValueError(f"{who}: q_weight/k_weight must be contiguous bfloat16 [head_dim]")
-    if cos_table.dtype != torch.float32 or sin_table.dtype != torch.float32 or cos_table.dim() != 2 \
-            or sin_table.shape != cos_table.shape or cos_table.shape[1] != HEAD_DIM \
+    table = cos_table.shape
+    if cos_table.dtype != torch.float32 or sin_table.dtype != torch.float32 or len(table) != 2 \
+            or table[1] != HEAD_DIM or sin_table.shape != table \
             or not (cos_table.is_contiguous() and sin_table.is_contiguous()):
         raise ValueError(f"{who}: cos/sin tables must be contiguous float32 [max_position, head_dim]")
     pos = _check_index(who, "positions", positions, torch.int64, tokens)
     slots = _check_index(who, "slot_mapping", slot_mapping, torch.int64, tokens)
     if query_out is None:
-        query_out = torch.empty(tokens, num_heads, HEAD_DIM, dtype=_BF16, device=dev)
-    else:
-        _require_cuda("query_out", query_out, dev)
-        if query_out.shape != query.shape or not query_out.is_contiguous() or query_out.dtype != _BF16:
-            raise ValueError(f"{who}: query_out must be a contiguous bf16 [tokens, heads, head_dim]")
-    _call(dev, "nvk_fp4_qk_norm_rope_append", query.data_ptr(), key.data_ptr(), value.data_ptr(), query.stride(0),
-          key.stride(0), value.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), eps, cos_table.data_ptr(),
-          sin_table.data_ptr(), cos_table.shape[0], pos.data_ptr(), query_out.data_ptr(), kv_cache.data_ptr(),
-          slots.data_ptr(), tokens, nb, bs, num_heads, kvh, HEAD_DIM, k_scale, v_scale,
-          _error_ptr(who, error_word, dev))
+        query_out = torch.empty((tokens, num_heads, HEAD_DIM), dtype=_BF16, device=dev)
+    elif query_out.device != dev or query_out.shape != query.shape or not query_out.is_contiguous() \
+            or query_out.dtype != _BF16:
+        raise ValueError(f"{who}: query_out must be a contiguous bf16 [tokens, heads, head_dim] on {dev}")
+    _call(dev, "nvk_fp4_qk_norm_rope_append", query.data_ptr(), key.data_ptr(), value.data_ptr(), q_stride, k_stride,
+          v_stride, q_weight.data_ptr(), k_weight.data_ptr(), eps, cos_table.data_ptr(), sin_table.data_ptr(),
+          table[0], pos.data_ptr(), query_out.data_ptr(), kv_cache.data_ptr(), slots.data_ptr(), tokens, nb, bs,
+          num_heads, kvh, HEAD_DIM, k_scale, v_scale, _error_ptr(who, error_word, dev))
     return query_out
 
 
@@ -173,29 +190,26 @@ def decode_fp4_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int 
     return int(out.value)
 
 
-def _table_stride(block_tables: torch.Tensor) -> int:
-    """Elements between the rows (of a single row: its width, whatever its stride says)."""
-    return block_tables.stride(0) if block_tables.shape[0] > 1 else block_tables.shape[1]
-
-
-def _check_attention(who: str, out, query, kv_cache, block_tables, lens) -> tuple[int, int, int, int]:
-    """Checks what decode and prefill share; returns (blocks, block size, KV heads, sequences)."""
-    dev = query.device
-    for name, t in (("out", out), ("query", query), ("kv_cache", kv_cache), ("block_tables", block_tables),
-                    ("lens", lens)):
-        _require_cuda(name, t, dev)
+def _check_attention(who: str, dev, out, query, kv_cache, block_tables, lens) -> tuple:
+    """Checks what decode and prefill share; returns what their calls take: query's shape, the pool's blocks,
+    block size and KV heads, and the table's rows, row stride and columns."""
+    _check_devices(dev, out=out, query=query, kv_cache=kv_cache, block_tables=block_tables, lens=lens)
     if query.dtype != _BF16 or out.dtype != _BF16:
         raise ValueError(f"{who}: query and out must be bfloat16")
-    if query.dim() != 3 or query.shape[2] != HEAD_DIM or out.shape != query.shape \
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM or out.shape != shape \
             or not (query.is_contiguous() and out.is_contiguous()):
         raise ValueError(f"{who}: query and out must be contiguous [tokens, heads, {HEAD_DIM}], got "
-                         f"{tuple(query.shape)} and {tuple(out.shape)}")
+                         f"{tuple(shape)} and {tuple(out.shape)}")
     nb, bs, kvh = _check_pool(who, kv_cache)
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1:
+    stride = block_tables.stride()
+    if block_tables.dtype != torch.int32 or len(stride) != 2 or stride[1] != 1:
         raise ValueError(f"{who}: block_tables must be int32 [batch, max_blocks] with unit column stride")
-    if lens.dtype != torch.int32 or lens.numel() != block_tables.shape[0] or not lens.is_contiguous():
+    batch, width = block_tables.shape
+    if lens.dtype != torch.int32 or lens.numel() != batch or not lens.is_contiguous():
         raise ValueError(f"{who}: the sequences' lengths must be a contiguous int32 [batch] device tensor")
-    return nb, bs, kvh, block_tables.shape[0]
+    # a single row's stride may be anything
+    return shape, nb, bs, kvh, batch, stride[0] if batch > 1 else width, width
 
 
 def paged_decode_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -208,15 +222,15 @@ def paged_decode_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Ten
     ordered on one stream. Its first int32 is the device error word.
     """
     who = "paged_decode_fp4"
-    nb, bs, kvh, batch = _check_attention(who, out, query, kv_cache, block_tables, context_lens)
     dev = query.device
-    _require_cuda("workspace", workspace, dev)
-    if query.shape[0] != batch or not workspace.is_contiguous():
-        raise ValueError(f"{who}: {query.shape[0]} queries for {batch} sequences, or a strided workspace")
+    shape, nb, bs, kvh, batch, stride, width = _check_attention(who, dev, out, query, kv_cache, block_tables,
+                                                                context_lens)
+    _check_devices(dev, workspace=workspace)
+    if shape[0] != batch or not workspace.is_contiguous():
+        raise ValueError(f"{who}: {shape[0]} queries for {batch} sequences, or a strided workspace")
     _call(dev, "nvk_fp4_paged_decode", out.data_ptr(), query.data_ptr(), kv_cache.data_ptr(), nb, bs,
-          block_tables.data_ptr(), _table_stride(block_tables), block_tables.shape[1],
-          context_lens.data_ptr(), batch, query.shape[1], kvh, HEAD_DIM, scale, k_scale, v_scale, num_ctas,
-          workspace.data_ptr(), workspace.numel() * workspace.element_size())
+          block_tables.data_ptr(), stride, width, context_lens.data_ptr(), batch, shape[1], kvh, HEAD_DIM, scale,
+          k_scale, v_scale, num_ctas, workspace.data_ptr(), workspace.nbytes)
     return out
 
 
@@ -226,12 +240,11 @@ def paged_prefill_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Te
                       error_word: torch.Tensor | None = None) -> torch.Tensor:
     """Causal (bottom-right) prefill attention over a 4-bit pool into ``out``."""
     who = "paged_prefill_fp4"
-    nb, bs, kvh, batch = _check_attention(who, out, query, kv_cache, block_tables, kv_lens)
     dev = query.device
-    _require_cuda("cu_seqlens_q", cu_seqlens_q, dev)
+    shape, nb, bs, kvh, batch, stride, width = _check_attention(who, dev, out, query, kv_cache, block_tables, kv_lens)
+    _check_devices(dev, cu_seqlens_q=cu_seqlens_q)
     cu = _check_index(who, "cu_seqlens_q", cu_seqlens_q, torch.int32, batch + 1)
     _call(dev, "nvk_fp4_paged_prefill", out.data_ptr(), query.data_ptr(), kv_cache.data_ptr(), nb, bs,
-          block_tables.data_ptr(), _table_stride(block_tables), block_tables.shape[1],
-          cu.data_ptr(), kv_lens.data_ptr(), batch, query.shape[0], max_q_len, query.shape[1], kvh, HEAD_DIM, scale,
-          k_scale, v_scale, _error_ptr(who, error_word, dev))
+          block_tables.data_ptr(), stride, width, cu.data_ptr(), kv_lens.data_ptr(), batch, shape[0], max_q_len,
+          shape[1], kvh, HEAD_DIM, scale, k_scale, v_scale, _error_ptr(who, error_word, dev))
     return out
