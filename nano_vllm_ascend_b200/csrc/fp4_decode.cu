@@ -61,6 +61,14 @@ struct DecodeArgs {
   float v_scale;
 };
 
+// A pair that a CTA shares with others: end 0 began before the CTA's first tile,
+// end 1 begins in the CTA and goes on behind its last.
+struct End {
+  int pair;    // -1: none
+  int c0, c1;  // the CTAs that have a piece of it
+  int last;    // this CTA's piece came last: it joins them
+};
+
 template <int kWarps>
 struct Smem {
   alignas(128) uint8_t ring[kWarps][kStages][kTileBytes];  // a warp's last piece comes here when it has read them
@@ -70,7 +78,7 @@ struct Smem {
   int pre[2 * kWarps * 32 + 1];  // tiles before each sequence (of one KV head)
   int scan[kWarps];
   int piece_pair[32];
-  int last[2];
+  End end[2];
 };
 constexpr uint32_t kVScaleBytes = kGroups * kUnitTokens * 2;  // of one unit
 
@@ -344,7 +352,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
     if (b + 1 <= a.batch) sm.pre[b + 1] = at + u0;
     if (b + 2 == a.batch) sm.pre[b + 2] = at + u0 + u1;
     if (tid < 32) sm.piece_pair[tid] = -1;
-    if (tid < 2) sm.last[tid] = 0;
     __syncthreads();
   }
   auto zero_empty = [&] {  // the rows of sequences without context
@@ -354,26 +361,42 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
       for (int i = lane; i < a.heads * (kD / 2); i += 32) row[i] = 0;
     }
   };
-  const int64_t total = static_cast<int64_t>(sm.pre[a.batch]) * a.kvh;
-  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (total + kWarps - 1) / kWarps));
+  const int total = sm.pre[a.batch] * a.kvh;  // the entry point keeps it below 2^31
+  const int ctas = min(static_cast<int>(gridDim.x), (total + kWarps - 1) / kWarps);
   const int c = blockIdx.x;
   if (c >= ctas) {
     pdl_wait();
     zero_empty();
     return;
   }
-  const int64_t clo = total * c / ctas, chi = total * (c + 1) / ctas;
-  const int64_t lo = clo + (chi - clo) * warp / kWarps, hi = clo + (chi - clo) * (warp + 1) / kWarps;
+  // Even shares, the first ones a tile larger where it does not come out even.
+  const int share = total / ctas, larger = total - share * ctas;
+  const int clo = share * c + min(c, larger), chi = clo + share + (c < larger ? 1 : 0);
+  const int wshare = (chi - clo) / kWarps, wlarger = (chi - clo) % kWarps;
+  const int lo = clo + wshare * warp + min(warp, wlarger), hi = lo + wshare + (warp < wlarger ? 1 : 0);
 
-  auto find_seq = [&](int64_t x) {  // the sequence that tile x belongs to
-    int b0 = 0, b1 = a.batch;       // pre[b0] * kvh <= x < pre[b1] * kvh
+  auto find_seq = [&](int x) {  // the sequence that tile x belongs to
+    int b0 = 0, b1 = a.batch;   // pre[b0] * kvh <= x < pre[b1] * kvh
     while (b1 - b0 > 1) {
       const int mid = (b0 + b1) >> 1;
-      if (static_cast<int64_t>(sm.pre[mid]) * a.kvh <= x) b0 = mid;
+      if (sm.pre[mid] * a.kvh <= x) b0 = mid;
       else b1 = mid;
     }
     return b0;
   };
+  if (warp == kWarps - 1 && lane < 2) {  // the pairs at this CTA's ends
+    auto cta_of = [&](int x) {
+      const int cut = larger * (share + 1);
+      return x < cut ? x / (share + 1) : larger + (x - cut) / share;
+    };
+    const int x = lane == 0 ? clo : chi - 1;
+    const int b = find_seq(x);
+    const int tiles = sm.pre[b + 1] - sm.pre[b];
+    const int h = (x - sm.pre[b] * a.kvh) / tiles;
+    const int plo = sm.pre[b] * a.kvh + h * tiles, phi = plo + tiles;
+    const bool split = lane == 0 ? plo < clo : plo >= clo && phi > chi;
+    sm.end[lane] = End{split ? b * a.kvh + h : -1, cta_of(plo), cta_of(phi - 1), 0};
+  }
 
   // Writes this warp's result of a pair as a piece (index 2 * warp + slot), or as the output.
   State st;
@@ -406,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
   };
 
   // ---- this warp's tiles ----
-  const int n = static_cast<int>(hi - lo);
+  const int n = hi - lo;
   constexpr int kFirst = 1 << 8, kLast = 1 << 9, kBad = 1 << 10, kBad2 = 1 << 11;
   // What lane i knows of the batch of 32 tiles that starts at lo + base: where
   // the units of tile base + i lie, whose it is, and its tokens with the flags
@@ -415,12 +438,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
   int next_pair = 0, next_info = 0;
   auto look_up = [&](int base) {
     if (base + lane >= n) return;
-    const int64_t x = lo + base + lane;
+    const int x = lo + base + lane;
     const int b = find_seq(x);
     const int tiles = sm.pre[b + 1] - sm.pre[b];
-    const int64_t in_seq = x - static_cast<int64_t>(sm.pre[b]) * a.kvh;
-    const int h = static_cast<int>(in_seq / tiles);
-    const int tile = static_cast<int>(in_seq - static_cast<int64_t>(h) * tiles);
+    const int in_seq = x - sm.pre[b] * a.kvh;
+    const int h = in_seq / tiles;
+    const int tile = in_seq - h * tiles;
     const int64_t room = (static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4));
     const int64_t left = min(static_cast<int64_t>(a.ctx[b]), room) - static_cast<int64_t>(tile) * kTileTokens;
     const int tokens = static_cast<int>(min(left, static_cast<int64_t>(kTileTokens)));
@@ -509,101 +532,100 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
   }
   __syncthreads();
 
-  // ---- pieces of one pair meet: lane p of every warp looks at piece p ----
-  const int mine = sm.piece_pair[lane];
+  // ---- the pieces of one pair meet ----
+  // Piece 2 w of warp w is what it had of a pair that began before it (or all
+  // it had), piece 2 w + 1 of one that goes on behind it. A run of pieces of
+  // one pair is its first one and then pieces 2 w of the warps after that.
+  auto write_out = [&](int pair, int head, float l, const float4& o) {
+    const float inv = l == 0.f ? 0.f : a.v_scale / l;
+    const int pb = pair / a.kvh, ph = pair - pb * a.kvh;
+    *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
+        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  };
+  auto weight = [](float2 ml, float m) {  // a piece whose scores were all -inf or NaN has the latter's NaN in its sum
+    return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - m);
+  };
+  auto warp_max = [](float m) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    return m;
+  };
+  auto warp_sum = [](float l) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    return l;
+  };
+  const int mine = sm.piece_pair[lane];  // lane p of every warp looks at piece p
   const uint32_t valid = __ballot_sync(0xffffffffu, mine >= 0);
   const uint32_t below = valid & ((1u << lane) - 1);
   const int prev = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
-  const uint32_t starts = __ballot_sync(0xffffffffu, mine >= 0 && (below == 0 || prev != mine));
-  const int tasks = __popc(starts) * a.group;
-  for (int k = warp; k < tasks; k += kWarps) {
-    const int run = k / a.group, head = k - run * a.group;
-    const int first = __fns(starts, 0, run + 1);
-    const int pair = __shfl_sync(0xffffffffu, mine, first);
-    const uint32_t members = __ballot_sync(0xffffffffu, mine == pair);
-    const float2 ml = mine == pair ? piece_ml[lane * a.group + head] : make_float2(-INFINITY, 0.f);
-    float m = ml.x;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - m);
-    float l = ml.y * w;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t left = members; left; left &= left - 1) {
-      const int p = __ffs(left) - 1;
-      const float wp = __shfl_sync(0xffffffffu, w, p);
-      const float4 v = *reinterpret_cast<const float4*>(piece_o(p) + head * kD + 4 * lane);
-      o.x += wp * v.x, o.y += wp * v.y, o.z += wp * v.z, o.w += wp * v.w;
-    }
-    const int pb = pair / a.kvh, ph = pair - pb * a.kvh;
-    const int tiles = sm.pre[pb + 1] - sm.pre[pb];
-    const int64_t plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * tiles;
-    if (plo >= clo && plo + tiles <= chi) {
-      const float inv = l == 0.f ? 0.f : a.v_scale / l;
-      *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
-          make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-    } else {
-      const int64_t at = (static_cast<int64_t>(c) * 2 + (plo < clo ? 0 : 1)) * a.group + head;
-      if (lane == 0) a.ws_ml[at] = make_float2(m, l);
-      *reinterpret_cast<float4*>(a.ws_o + at * kD + 4 * lane) = o;
-      __threadfence();
-    }
-  }
-  // ---- pairs split over CTAs: the first and the last of this CTA's tiles ----
-  auto cta_of = [&](int64_t tile) { return static_cast<int>(((tile + 1) * ctas - 1) / total); };
-  auto pair_of = [&](int64_t tile, int& pb, int& ph, int64_t& plo, int& tiles) {
-    pb = find_seq(tile);
-    while (sm.pre[pb + 1] == sm.pre[pb]) ++pb;
-    tiles = sm.pre[pb + 1] - sm.pre[pb];
-    ph = static_cast<int>((tile - static_cast<int64_t>(sm.pre[pb]) * a.kvh) / tiles);
-    plo = static_cast<int64_t>(sm.pre[pb]) * a.kvh + static_cast<int64_t>(ph) * tiles;
-  };
-  __syncthreads();
-  if (tid < 2) {
-    int pb, ph, tiles;
-    int64_t plo;
-    pair_of(tid == 0 ? clo : chi - 1, pb, ph, plo, tiles);
-    // end 0: a pair that began before this CTA; end 1: one that begins here and goes on
-    const bool split = tid == 0 ? plo < clo : plo >= clo && plo + tiles > chi;
-    if (split) {
-      const int c0 = cta_of(plo), c1 = cta_of(plo + tiles - 1);
-      __threadfence();
-      if (atomicAdd(a.tickets + c0, 1) == c1 - c0) {
-        a.tickets[c0] = 0;  // every piece is in: nobody else touches it in this call
-        sm.last[tid] = 1;
-      }
-    }
-  }
-  __syncthreads();
-  for (int end = 0; end < 2; ++end) {
-    if (!sm.last[end]) continue;
-    __threadfence();
-    int pb, ph, tiles;
-    int64_t plo;
-    pair_of(end == 0 ? clo : chi - 1, pb, ph, plo, tiles);
-    const int c0 = cta_of(plo), c1 = cta_of(plo + tiles - 1);
-    for (int head = warp; head < a.group; head += kWarps) {
-      // the pair's piece in CTA k: its end 1 where it begins, its end 0 after that
-      auto at = [&](int k) { return (static_cast<int64_t>(k) * 2 + (k == c0 ? 1 : 0)) * a.group + head; };
-      float m = -INFINITY;
-      for (int k = c0 + lane; k <= c1; k += 32) m = fmaxf(m, __ldcg(&a.ws_ml[at(k)].x));
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-      float l = 0.f;
+  uint32_t starts = __ballot_sync(0xffffffffu, mine >= 0 && (below == 0 || prev != mine));
+  for (int k = warp, at = 0; starts; at += a.group, starts &= starts - 1) {
+    for (; k < at + a.group; k += kWarps) {  // task k: head k - at of this run
+      const int head = k - at, first = __ffs(starts) - 1;
+      const int pair = __shfl_sync(0xffffffffu, mine, first);
+      const int count = __popc(__ballot_sync(0xffffffffu, mine == pair));
+      const float2 ml = mine == pair ? piece_ml[lane * a.group + head] : make_float2(-INFINITY, 0.f);
+      const float m = warp_max(ml.x);
+      const float w = weight(ml, m), l = warp_sum(ml.y * w);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int k = c0; k <= c1; ++k) {
-        const float2 ml = __ldcg(&a.ws_ml[at(k)]);
-        const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - m);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(k) * kD + 4 * lane));
-        l += w * ml.y;
-        o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+      for (int i = 0; i < count; ++i) {
+        const int p = i == 0 ? first : 2 * ((first >> 1) + i);
+        const float wp = __shfl_sync(0xffffffffu, w, p);
+        const float4 v = *reinterpret_cast<const float4*>(piece_o(p) + head * kD + 4 * lane);
+        o.x += wp * v.x, o.y += wp * v.y, o.z += wp * v.z, o.w += wp * v.w;
       }
-      const float inv = l == 0.f ? 0.f : a.v_scale / l;
-      *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
-          make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+      const int end = pair == sm.end[0].pair ? 0 : pair == sm.end[1].pair ? 1 : -1;
+      if (end < 0) {
+        write_out(pair, head, l, o);
+      } else {
+        const int64_t to = (static_cast<int64_t>(c) * 2 + end) * a.group + head;
+        if (lane == 0) a.ws_ml[to] = make_float2(m, l);
+        *reinterpret_cast<float4*>(a.ws_o + to * kD + 4 * lane) = o;
+      }
     }
+  }
+  // ---- pairs split over CTAs: the CTA whose piece comes last joins them ----
+  __syncthreads();
+  if (tid < 2 && sm.end[tid].pair >= 0) {
+    const End e = sm.end[tid];
+    __threadfence();  // the CTA's pieces, which the barrier put before this, are out before the ticket
+    if (atomicAdd(a.tickets + e.c0, 1) == e.c1 - e.c0) {
+      a.tickets[e.c0] = 0;  // every piece is in: nobody else touches it in this call
+      __threadfence();
+      sm.end[tid].last = 1;
+    }
+  }
+  __syncthreads();
+  for (int k = warp; k < 2 * a.group; k += kWarps) {
+    const int end = k & 1, head = k >> 1;
+    const End e = sm.end[end];
+    if (e.pair < 0 || !e.last) continue;
+    // the pair's piece in CTA i: its end 1 where it begins, its end 0 after that
+    const int count = e.c1 - e.c0 + 1;
+    auto at = [&](int i) { return (static_cast<int64_t>(e.c0 + i) * 2 + (i == 0 ? 1 : 0)) * a.group + head; };
+    auto piece = [&](int i) { return __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(i) * kD + 4 * lane)); };
+    float4 ahead[4];  // loads in flight together with those of the maxima
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ahead[i] = i < count ? piece(i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY;
+    for (int i = lane; i < count; i += 32) m = fmaxf(m, __ldcg(&a.ws_ml[at(i)].x));
+    m = warp_max(m);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < count; i0 += 32) {
+      const float2 ml = i0 + lane < count ? __ldcg(&a.ws_ml[at(i0 + lane)]) : make_float2(-INFINITY, 0.f);
+      const float w = weight(ml, m);
+      l += warp_sum(ml.y * w);
+#pragma unroll 4
+      for (int i = i0; i < min(count, i0 + 32); ++i) {
+        const float wp = __shfl_sync(0xffffffffu, w, i - i0);
+        const float4 v = i < 4 ? (i == 0 ? ahead[0] : i == 1 ? ahead[1] : i == 2 ? ahead[2] : ahead[3]) : piece(i);
+        o.x += wp * v.x, o.y += wp * v.y, o.z += wp * v.z, o.w += wp * v.w;
+      }
+    }
+    write_out(e.pair, head, l, o);
   }
 }
 
@@ -707,10 +729,10 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: q, out and workspace must be 16-byte aligned", who);
   const int upb_log2 = units_log2(block_size);
   const int64_t seqs = batch < 1024 ? batch : 1024;
-  if (((seqs * max_blocks_per_seq) << upb_log2) > 0x7fffffffll ||
+  if (((seqs * max_blocks_per_seq * num_kv_heads) << upb_log2) > 0x7fffffffll ||
       (static_cast<int64_t>(max_blocks_per_seq) << upb_log2) > 0x7fffffffll / kUnitTokens)
-    return fail(NVK_ERR_UNSUPPORTED, "%s: %d blocks of %d tokens a sequence are above the kernel's range", who,
-                max_blocks_per_seq, block_size);
+    return fail(NVK_ERR_UNSUPPORTED, "%s: %d blocks of %d tokens a sequence and %d KV heads are above the kernel's range",
+                who, max_blocks_per_seq, block_size, num_kv_heads);
   int ctas = 0;
   if ((rc = resolve_ctas(num_ctas, &ctas)) != NVK_OK) return rc;
   const int group = num_heads / num_kv_heads;
