@@ -370,8 +370,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
     }
   };
   const int total = sm.pre[a.batch] * a.kvh;  // the entry point keeps it below 2^31
-  const int ctas = min(min(static_cast<int>(gridDim.x), (total + kMinTiles - 1) / kMinTiles),
-                       kMostPieces * a.batch * a.kvh);
+  const int64_t useful = static_cast<int64_t>(kMostPieces) * a.batch * a.kvh;
+  const int ctas = static_cast<int>(min(useful, static_cast<int64_t>(min(static_cast<int>(gridDim.x),
+                                                                       (total + kMinTiles - 1) / kMinTiles))));
   const int c = blockIdx.x;
   if (c >= ctas) {
     pdl_wait();
