@@ -17,28 +17,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRowsPerBlock = kThreads / 8;
 
-template <typename T>
-__device__ __forceinline__ float2 pair_to_f32(uint32_t w);
-template <>
-__device__ __forceinline__ float2 pair_to_f32<__nv_bfloat16>(uint32_t w) {
-  return make_float2(bf16lo_to_f32(w), bf16hi_to_f32(w));
-}
-template <>
-__device__ __forceinline__ float2 pair_to_f32<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t f32_to_pair(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t f32_to_pair<__nv_bfloat16>(float lo, float hi) {
-  return pack_bf16x2(lo, hi);
-}
-template <>
-__device__ __forceinline__ uint32_t f32_to_pair<__half>(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 struct AppendArgs {
   const uint8_t* key;
   const uint8_t* value;
@@ -75,17 +53,10 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
     uint32_t raw[kGroups];
 #pragma unroll
     for (int j = 0; j < kGroups; ++j) raw[j] = ok ? *reinterpret_cast<const uint32_t*>(src + 32 * j) : 0u;
-    float2 x[kGroups];
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      x[j] = pair_to_f32<T>(raw[j]);
-      x[j].x *= inv;
-      x[j].y *= inv;
-    }
-    uint32_t w0, w1, s0, s1;
-    quantise_row(x, w0, w1, s0, s1);
+    uint32_t w0, w1, scale;
+    quantise_row<T>(raw, inv, g, w0, w1, scale);
     store_row(ok ? unit_of(a.pool, slot, head, a.kvh, a.upb_log2) : a.pool, static_cast<int>(slot & 15), is_v, ok, g,
-              w0, w1, s0, s1);
+              w0, w1, scale);
   }
 }
 
@@ -175,42 +146,61 @@ struct NormArgs {
   uint8_t* pool;
   int64_t num_tokens, num_slots;
   int num_heads, kvh, upb_log2;
-  int chunk;  // head rows per warp item, a multiple of 4
+  int chunk;  // rounds of four head rows per warp item
   float eps, k_inv, v_inv;
   int* err;
 };
 
-__device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+__device__ __forceinline__ uint64_t f32x2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t bf16x2_to_f32x2(uint32_t w) { return f32x2_pack(bf16lo_to_f32(w), bf16hi_to_f32(w)); }
+__device__ __forceinline__ uint32_t f32x2_to_bf16x2(uint64_t v) {
+  float lo, hi;
+  f32x2_unpack(v, lo, hi);
+  return pack_bf16x2(lo, hi);
+}
 
-// One warp per chunk of head rows (q heads, then k, then v) of one token, four
-// rows at a time. The rows' arithmetic is the separate operators':
+// Rows of one token in rounds of four (eight lanes a row): the q heads, then
+// the k heads, then the v heads; a warp takes `chunk` rounds of a token. The
+// rows' arithmetic is the separate operators':
 //   y   = bf16(x * rsqrt(mean(x^2) + eps) * w)
 //   out = bf16(y * cos + rotate_half(y) * sin),  cos and sin cast to bf16.
 // The mean square is summed in 64 bits and its root is correctly rounded, so
 // the bf16 row does not hang on the order of the sum: a row that differed in
 // one bf16 bit could be stored one whole e2m1 step away.
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormArgs a) {
+// Issue-bound where it is not HBM-bound: two values an instruction (f32x2)
+// throughout, and the next round's row is loaded before this one's arithmetic.
+__global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, g = lane & 7, sub = lane >> 3;
-  const int nrows = a.num_heads + 2 * a.kvh, nqk = a.num_heads + a.kvh;
-  const int chunks = (nrows + a.chunk - 1) / a.chunk;
+  const int rq = (a.num_heads + 3) / 4, rk = (a.kvh + 3) / 4, rounds = rq + 2 * rk;
+  const int chunks = (rounds + a.chunk - 1) / a.chunk;
   const int64_t items = a.num_tokens * chunks;
-  uint32_t wq[kGroups], wk[kGroups];
-#pragma unroll
-  for (int j = 0; j < kGroups; ++j) {
-    wq[j] = *reinterpret_cast<const uint32_t*>(a.q_weight + 32 * j + 4 * g);
-    wk[j] = *reinterpret_cast<const uint32_t*>(a.k_weight + 32 * j + 4 * g);
-  }
   const int64_t nw = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
   for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += nw) {
     const int64_t t = w / chunks;
-    const int lo = static_cast<int>(w - t * chunks) * a.chunk, hi = min(lo + a.chunk, nrows);
+    const int lo = static_cast<int>(w - t * chunks) * a.chunk, hi = min(lo + a.chunk, rounds);
+    // this lane's words of its row of round r
+    auto load = [&](int r, uint32_t (&x)[kGroups]) {
+      const bool is_q = r < rq, is_v = r >= rq + rk;
+      const int head = 4 * (r - (is_q ? 0 : is_v ? rq + rk : rq)) + sub;
+      const bool live = head < (is_q ? a.num_heads : a.kvh);
+      const uint8_t* src = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) +
+                           head * 256 + 4 * g;
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) x[j] = live ? *reinterpret_cast<const uint32_t*>(src + 32 * j) : 0u;
+    };
+    uint32_t next[kGroups];
+    load(lo, next);
     const int64_t slot = a.slots[t];
     const bool slot_ok = slot >= 0 && slot < a.num_slots;
     if (!slot_ok && lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrBadSlot);
-    uint32_t cs[kGroups], sn[kGroups];  // bf16 pairs
-    if (lo < nqk) {
+    uint64_t cs[kGroups], sn[kGroups], wt[kGroups];  // sn of the lower half negated
+    if (lo < rq + rk) {
       int64_t p = a.positions[t];
       if (p < 0 || p >= a.max_pos) {
         if (lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrContextTooLong);
@@ -218,75 +208,62 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) {
-        const float* c = a.cos_table + p * kD + 16 * j + 2 * g;
-        const float* s = a.sin_table + p * kD + 16 * j + 2 * g;
-        cs[j] = pack_bf16x2(c[0], c[1]);
-        sn[j] = pack_bf16x2(s[0], s[1]);
+        const float2 c = *reinterpret_cast<const float2*>(a.cos_table + p * kD + 16 * j + 2 * g);
+        const float2 s = *reinterpret_cast<const float2*>(a.sin_table + p * kD + 16 * j + 2 * g);
+        cs[j] = bf16x2_to_f32x2(pack_bf16x2(c.x, c.y));
+        sn[j] = bf16x2_to_f32x2(j < 4 ? pack_bf16x2(-s.x, -s.y) : pack_bf16x2(s.x, s.y));
       }
     }
-    for (int r0 = lo; r0 < hi; r0 += 4) {
-      const int r = r0 + sub;
-      const bool live = r < hi;
-      const bool is_q = r < a.num_heads, is_v = r >= nqk;
-      const uint8_t* src = is_q ? a.q + t * a.q_stride + r * 256
-                           : is_v ? a.v + t * a.v_stride + (r - nqk) * 256
-                                  : a.k + t * a.k_stride + (r - a.num_heads) * 256;
-      uint32_t raw[kGroups];
+    for (int r = lo; r < hi; ++r) {
+      const bool is_q = r < rq, is_v = r >= rq + rk;
+      const int head = 4 * (r - (is_q ? 0 : is_v ? rq + rk : rq)) + sub;
+      const bool live = head < (is_q ? a.num_heads : a.kvh);
+      if (r == lo || r == rq) {
+        const uint8_t* weight = is_q ? a.q_weight : a.k_weight;
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j)
-        raw[j] = live ? *reinterpret_cast<const uint32_t*>(src + 32 * j + 4 * g) : 0u;
-      float2 x[kGroups];
+        for (int j = 0; j < kGroups; ++j)
+          wt[j] = bf16x2_to_f32x2(*reinterpret_cast<const uint32_t*>(weight + 32 * j + 4 * g));
+      }
+      uint32_t x[kGroups];
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) x[j] = pair_to_f32<__nv_bfloat16>(raw[j]);
-      if (r0 < nqk) {  // some row of this round is normalised (the warp sums together)
+      for (int j = 0; j < kGroups; ++j) x[j] = next[j];
+      if (r + 1 < hi) load(r + 1, next);
+      if (!is_v) {
         double ss = 0.0;
+        uint64_t f[kGroups];
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
-          const double u = x[j].x, v = x[j].y;
-          ss = fma(v, v, fma(u, u, ss));
+          const float2 v = pair_to_f32<__nv_bfloat16>(x[j]);
+          f[j] = f32x2_pack(v.x, v.y);
+          const double d0 = v.x, d1 = v.y;
+          ss = fma(d1, d1, fma(d0, d0, ss));
         }
 #pragma unroll
         for (int off = 1; off < 8; off <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         const float rinv = __frsqrt_rn(static_cast<float>(ss * (1.0 / kD) + static_cast<double>(a.eps)));
-        if (!is_v) {
-          float2 y[kGroups];
+        const uint64_t rr = f32x2_pack(rinv, rinv);
 #pragma unroll
-          for (int j = 0; j < kGroups; ++j) {
-            const float2 wt = pair_to_f32<__nv_bfloat16>(is_q ? wq[j] : wk[j]);
-            y[j].x = round_bf16(x[j].x * rinv * wt.x);
-            y[j].y = round_bf16(x[j].y * rinv * wt.y);
-          }
+        for (int j = 0; j < kGroups; ++j)  // the norm's bf16 result
+          f[j] = bf16x2_to_f32x2(f32x2_to_bf16x2(f32x2_mul(f32x2_mul(f[j], rr), wt[j])));
           // out[i] = y[i] cos[i] - y[i+64] sin[i];  out[i+64] = y[i+64] cos[i+64] + y[i] sin[i+64]
-          // (products of bf16 are exact in fp32: one rounding each, contracted or not)
+          // (products of bf16 are exact in fp32: one rounding each)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 c0 = pair_to_f32<__nv_bfloat16>(cs[j]), c1 = pair_to_f32<__nv_bfloat16>(cs[j + 4]);
-            const float2 n0 = pair_to_f32<__nv_bfloat16>(sn[j]), n1 = pair_to_f32<__nv_bfloat16>(sn[j + 4]);
-            raw[j] = pack_bf16x2(y[j].x * c0.x - y[j + 4].x * n0.x, y[j].y * c0.y - y[j + 4].y * n0.y);
-            raw[j + 4] = pack_bf16x2(y[j + 4].x * c1.x + y[j].x * n1.x, y[j + 4].y * c1.y + y[j].y * n1.y);
-          }
-#pragma unroll
-          for (int j = 0; j < kGroups; ++j) x[j] = pair_to_f32<__nv_bfloat16>(raw[j]);
+        for (int j = 0; j < 4; ++j) {
+          x[j] = f32x2_to_bf16x2(f32x2_fma(f[j], cs[j], f32x2_mul(f[j + 4], sn[j])));
+          x[j + 4] = f32x2_to_bf16x2(f32x2_fma(f[j + 4], cs[j + 4], f32x2_mul(f[j], sn[j + 4])));
         }
       }
-      if (live && is_q) {
-        uint8_t* dst = a.q_out + (t * a.num_heads + r) * 256 + 4 * g;
+      if (is_q) {
+        uint8_t* dst = a.q_out + (t * a.num_heads + head) * 256 + 4 * g;
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) *reinterpret_cast<uint32_t*>(dst + 32 * j) = raw[j];
-      }
-      if (r0 + 3 >= a.num_heads) {  // some row of this round goes to the pool
-        const int head = is_v ? r - nqk : r - a.num_heads;
-        const float inv = is_v ? a.v_inv : a.k_inv;
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-          x[j].x *= inv;
-          x[j].y *= inv;
-        }
-        uint32_t w0, w1, s0, s1;
-        quantise_row(x, w0, w1, s0, s1);
-        const bool store = live && !is_q && slot_ok;
+        for (int j = 0; j < kGroups; ++j)
+          if (live) *reinterpret_cast<uint32_t*>(dst + 32 * j) = x[j];
+      } else {
+        uint32_t w0, w1, scale;
+        quantise_row<__nv_bfloat16>(x, is_v ? a.v_inv : a.k_inv, g, w0, w1, scale);
+        const bool store = live && slot_ok;
         store_row(store ? unit_of(a.pool, slot, head, a.kvh, a.upb_log2) : a.pool, static_cast<int>(slot & 15), is_v,
-                  store, g, w0, w1, s0, s1);
+                  store, g, w0, w1, scale);
       }
     }
   }
@@ -433,10 +410,10 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   a.v_inv = 1.f / v_scale;
   a.err = error_word;
   const int sms = sm_count();
-  const int nrows = num_heads + 2 * num_kv_heads;
+  const int rounds = (num_heads + 3) / 4 + 2 * ((num_kv_heads + 3) / 4);
   // a whole token per warp (cos and sin loaded once) when the tokens alone give every SM 16 warps
-  a.chunk = num_tokens >= int64_t(sms) * 16 ? (nrows + 3) / 4 * 4 : 4;
-  const int64_t items = num_tokens * ((nrows + a.chunk - 1) / a.chunk);
+  a.chunk = num_tokens >= int64_t(sms) * 16 ? rounds : 1;
+  const int64_t items = num_tokens * ((rounds + a.chunk - 1) / a.chunk);
   const int64_t want = (items + kThreads / 32 - 1) / (kThreads / 32);
   const int64_t most = int64_t(sms) * 8;
   return check_cuda(launch_pdl(norm_rope_kernel, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kThreads),

@@ -3,7 +3,8 @@
 // A row (128 dims of one token and KV head) is held as 8 groups of 16
 // neighbouring dims. A group has one e4m3 scale s = rn(amax / 6) and 16 e2m1
 // codes c = rn(x / s) (both round to nearest, ties to even, and saturate); it
-// stands for g * s * c with g a power of two that the whole layer shares.
+// stands for g * s * c with g a power of two that the whole layer shares. The
+// sign of a value that rounds to 0 is not kept.
 // e2m1 has two significant bits and e4m3 four, so s * c is exact in bf16 and
 // fp16: what the attention kernels multiply is exactly what is stored.
 //
@@ -87,74 +88,101 @@ __device__ __forceinline__ uint32_t floats_to_e2m1x2(float lo, float hi) {
   return r;
 }
 
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
-// Rounds a quotient computed as a product with a reciprocal (relative error
-// below 2^-21) to 18 significant bits. The rows are bf16 or fp16 (at most 11
-// significant bits) and every rounding border of e2m1 and e4m3, times s or 6,
-// has at most 7: a quotient that is not exactly on a border is at least 2^-12
-// of it away, and one that is on it lands on it again. So the code that
-// follows is the one that an exact division would give.
+// A pair of 16-bit floats to fp32, and back.
+template <typename T>
+__device__ __forceinline__ float2 pair_to_f32(uint32_t w);
+template <>
+__device__ __forceinline__ float2 pair_to_f32<__nv_bfloat16>(uint32_t w) {
+  return make_float2(bf16lo_to_f32(w), bf16hi_to_f32(w));
+}
+template <>
+__device__ __forceinline__ float2 pair_to_f32<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t f32_to_pair(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t f32_to_pair<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t f32_to_pair<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Quotients are computed as products with a reciprocal (relative error below
+// 2^-21) and moved onto a grid that holds every rounding border before they
+// are rounded, so that the codes are those of an exact division: the rows have
+// at most 11 significant bits and a border times s (or 6) at most 7, so a
+// quotient that is not on a border is at least 2^-11 of it away.
+// The scale: to 18 significant bits, 2^-18 of it.
 __device__ __forceinline__ float snap18(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x20u) & ~0x3fu);  // not for NaN
 }
+// The codes: borders are multiples of 1/4 from 1/4 to 5, so to multiples of
+// 2^-14, by adding and subtracting 768 (its step in fp32).
+constexpr float kGrid = 768.f;
 
-// One row by eight lanes: lane g holds x[j] = dims {16 j + 2 g, 16 j + 2 g +
-// 1} of group j, already divided by the layer's constant. Returns this lane's
-// codes (byte j of w0 | w1) and the row's eight scales (e4m3 bytes).
-// A group with a NaN gets a NaN scale (and so reads back as NaN); infinities
-// saturate to 6 * 448; a group whose scale rounds to 0 gets codes of 0.
-__device__ __forceinline__ void quantise_row(const float2 (&x)[kGroups], uint32_t& w0, uint32_t& w1, uint32_t& s0,
-                                             uint32_t& s1) {
-  float amax[kGroups];
+// One row by eight lanes: word j of lane g holds dims 16 j + 2 g and + 1 of
+// group j as 16-bit floats of type T; `inv` is the reciprocal of the layer's
+// constant. Returns this lane's codes (byte j of w0 | w1) and the e4m3 byte of
+// group g. A group with a NaN gets a NaN scale (and so reads back as NaN);
+// infinities saturate to 6 * 448; a group whose scale rounds to 0 gets zeros.
+template <typename T>
+__device__ __forceinline__ void quantise_row(const uint32_t (&x)[kGroups], float inv, int g, uint32_t& w0,
+                                             uint32_t& w1, uint32_t& scale) {
+  // Magnitudes of 16-bit floats order as integers (NaN above infinity). The
+  // maxima of the eight groups are reduced and scattered: three exchanges,
+  // after which lane g has group g's.
+  uint32_t m[4];  // groups 2 k and 2 k + 1
 #pragma unroll
-  for (int j = 0; j < kGroups; ++j) amax[j] = fmax_nan(fabsf(x[j].x), fabsf(x[j].y));
-#pragma unroll
-  for (int off = 1; off < 8; off <<= 1)
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j) amax[j] = fmax_nan(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], off));
-  uint32_t sc[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    auto sixth = [](float m) { return m == m ? snap18(m * (1.f / 6.f)) : m; };
-    sc[j] = floats_to_e4m3x2(sixth(amax[2 * j]), sixth(amax[2 * j + 1]));
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t a = x[2 * k] & 0x7fff7fffu, b = x[2 * k + 1] & 0x7fff7fffu;
+    m[k] = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
   }
-  s0 = sc[0] | (sc[1] << 16);
-  s1 = sc[2] | (sc[3] << 16);
-  uint32_t h[4];
-  e4m3_to_half2(s0, h[0], h[1]);
-  e4m3_to_half2(s1, h[2], h[3]);
+  const bool up4 = g & 4, up2 = g & 2, up1 = g & 1;
+  const uint32_t r0 = __shfl_xor_sync(0xffffffffu, up4 ? m[0] : m[2], 4);
+  const uint32_t r1 = __shfl_xor_sync(0xffffffffu, up4 ? m[1] : m[3], 4);
+  const uint32_t n0 = __vmaxu2(up4 ? m[2] : m[0], r0), n1 = __vmaxu2(up4 ? m[3] : m[1], r1);
+  const uint32_t r2 = __shfl_xor_sync(0xffffffffu, up2 ? n0 : n1, 2);
+  const uint32_t o = __vmaxu2(up2 ? n1 : n0, r2);
+  const uint32_t both = __vmaxu2(o, __shfl_xor_sync(0xffffffffu, o, 1));
+  const float2 pair = pair_to_f32<T>(both);
+  const float amax = (up1 ? pair.y : pair.x) * inv;
+  scale = floats_to_e4m3x2(amax == amax ? snap18(amax * (1.f / 6.f)) : amax, 0.f);
+  uint32_t lo, hi;
+  e4m3_to_half2(scale, lo, hi);
+  const float s = __low2float(*reinterpret_cast<const __half2*>(&lo));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  r = s > 0.f ? r * inv : 0.f;  // also for a NaN scale: its codes do not matter
+  const uint64_t grid = f32x2_pack(kGrid, kGrid), back = f32x2_pack(-kGrid, -kGrid);
   uint32_t code[kGroups];
 #pragma unroll
   for (int j = 0; j < kGroups; ++j) {
-    const __half2 hs = *reinterpret_cast<const __half2*>(&h[j >> 1]);
-    const float s = (j & 1) ? __high2float(hs) : __low2float(hs);
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-    r = s > 0.f ? r : 0.f;  // also for a NaN scale: its codes do not matter
-    // an infinity times a zero reciprocal cannot happen: its scale is 448
-    code[j] = floats_to_e2m1x2(snap18(x[j].x * r), snap18(x[j].y * r));
+    const float rj = __shfl_sync(0xffffffffu, r, j, 8);
+    const float2 f = pair_to_f32<T>(x[j]);
+    float u, v;
+    f32x2_unpack(f32x2_add(f32x2_fma(f32x2_pack(f.x, f.y), f32x2_pack(rj, rj), grid), back), u, v);
+    code[j] = floats_to_e2m1x2(u, v);
   }
   w0 = code[0] | (code[1] << 8) | (code[2] << 16) | (code[3] << 24);
   w1 = code[4] | (code[5] << 8) | (code[6] << 16) | (code[7] << 24);
 }
 
 // Stores the codes and scales of one row (see quantise_row) as token i of a
-// unit: eight bytes of codes a lane. All lanes of the warp call it (the K
-// order exchanges words between neighbouring lanes); `store` is false for
-// rows that are not written.
+// unit: eight bytes of codes and one scale a lane. All lanes of the warp call
+// it (the K order exchanges words between neighbouring lanes); `store` is
+// false for rows that are not written.
 __device__ __forceinline__ void store_row(uint8_t* unit, int i, bool is_v, bool store, int g, uint32_t w0,
-                                          uint32_t w1, uint32_t s0, uint32_t s1) {
+                                          uint32_t w1, uint32_t scale) {
   // K: byte 2 j + h of a lane pair's 16: the even lane stores groups 0-3 of both lanes, the odd one 4-7
   const bool odd = g & 1;
   const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1);
@@ -162,11 +190,11 @@ __device__ __forceinline__ void store_row(uint8_t* unit, int i, bool is_v, bool 
   if (!store) return;
   if (is_v) {
     *reinterpret_cast<uint2*>(unit + kOffV + 256 * (i >> 2) + 32 * g + 8 * (i & 3)) = make_uint2(w0, w1);
-    unit[kOffVScale + 32 * (i >> 2) + 4 * g + (i & 3)] = static_cast<uint8_t>((g < 4 ? s0 : s1) >> (8 * (g & 3)));
+    unit[kOffVScale + 32 * (i >> 2) + 4 * g + (i & 3)] = static_cast<uint8_t>(scale);
   } else {
     *reinterpret_cast<uint2*>(unit + 64 * i + 8 * g) =
         make_uint2(__byte_perm(e, o, 0x5140), __byte_perm(e, o, 0x7362));
-    if (g == 0) *reinterpret_cast<uint2*>(unit + kOffKScale + 8 * i) = make_uint2(s0, s1);
+    unit[kOffKScale + 8 * i + g] = static_cast<uint8_t>(scale);
   }
 }
 
