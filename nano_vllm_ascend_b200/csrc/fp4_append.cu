@@ -17,14 +17,33 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRowsPerBlock = kThreads / 8;
 
+// n / d for n < 2^31 as a multiplication: m = ceil(2^(31 + l) / d) with l the
+// least such that 2^l >= d; n * (m * d - 2^(31 + l)) < 2^(31 + l), so the
+// product's excess never reaches the next quotient.
+struct Divisor {
+  uint32_t m, shift;
+  int d;
+};
+inline Divisor divisor(int d) {
+  uint32_t l = 1;
+  while ((int64_t(1) << l) < d) ++l;
+  return Divisor{static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d), l - 1, d};
+}
+__device__ __forceinline__ int quotient(int n, const Divisor& v) {
+  return static_cast<int>(__umulhi(static_cast<uint32_t>(n), v.m) >> v.shift);
+}
+constexpr int64_t kMostRows = int64_t(1) << 30;  // rows of a launch (more go in several)
+
 struct AppendArgs {
   const uint8_t* key;
   const uint8_t* value;
   int64_t key_stride, value_stride;  // bytes between tokens
   uint8_t* pool;
   const int64_t* slots;
-  int64_t num_tokens, num_slots;
+  int64_t num_slots;
+  int rows;  // tokens * 2 kvh
   int kvh, upb_log2;
+  Divisor per_token;  // 2 kvh
   float k_inv, v_inv;
   int* err;
 };
@@ -34,15 +53,12 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int g = threadIdx.x & 7;
-  const int64_t rows = a.num_tokens * 2 * a.kvh;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRowsPerBlock;
   // the bound is a whole warp's: its lanes exchange words
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 5) * 4; r0 < rows;
-       r0 += stride) {
-    const int64_t r = r0 + ((threadIdx.x >> 3) & 3);
-    const bool live = r < rows;
-    const int64_t t = live ? r / (2 * a.kvh) : 0;
-    const int kr = live ? static_cast<int>(r - t * 2 * a.kvh) : 0;
+  for (int r0 = blockIdx.x * kRowsPerBlock + (threadIdx.x >> 5) * 4; r0 < a.rows; r0 += gridDim.x * kRowsPerBlock) {
+    const int r = r0 + ((threadIdx.x >> 3) & 3);
+    const bool live = r < a.rows;
+    const int t = live ? quotient(r, a.per_token) : 0;
+    const int kr = live ? r - t * a.per_token.d : 0;
     const bool is_v = kr >= a.kvh;
     const int head = is_v ? kr - a.kvh : kr;
     const int64_t slot = live ? a.slots[t] : -1;
@@ -65,8 +81,10 @@ struct ReadArgs {
   uint8_t* value;
   uint8_t* pool;
   const int64_t* slots;
-  int64_t num_tokens, num_slots;
+  int64_t num_slots;
+  int rows;  // tokens * 2 kvh
   int kvh, upb_log2;
+  Divisor per_token;  // 2 kvh
   float k_scale, v_scale;
   int* err;
 };
@@ -77,11 +95,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int g = threadIdx.x & 7;
-  const int64_t rows = a.num_tokens * 2 * a.kvh;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kRowsPerBlock;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 3); r < rows; r += stride) {
-    const int64_t t = r / (2 * a.kvh);
-    const int kr = static_cast<int>(r - t * 2 * a.kvh);
+  for (int r = blockIdx.x * kRowsPerBlock + (threadIdx.x >> 3); r < a.rows; r += gridDim.x * kRowsPerBlock) {
+    const int t = quotient(r, a.per_token);
+    const int kr = r - t * a.per_token.d;
     const bool is_v = kr >= a.kvh;
     const int head = is_v ? kr - a.kvh : kr;
     const int64_t slot = a.slots[t];
@@ -93,9 +109,12 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
       const uint8_t* unit = unit_of(a.pool, slot, head, a.kvh, a.upb_log2);
       if (is_v) {
         w = *reinterpret_cast<const uint2*>(unit + kOffV + 256 * (i >> 2) + 32 * g + 8 * (i & 3));
-        const uint8_t* s = unit + kOffVScale + 32 * (i >> 2) + (i & 3);
-        sw.x = s[0] | (s[4] << 8) | (s[8] << 16) | (static_cast<uint32_t>(s[12]) << 24);
-        sw.y = s[16] | (s[20] << 8) | (s[24] << 16) | (static_cast<uint32_t>(s[28]) << 24);
+        // byte i % 4 of the eight words of its quad
+        const uint4 s0 = *reinterpret_cast<const uint4*>(unit + kOffVScale + 32 * (i >> 2));
+        const uint4 s1 = *reinterpret_cast<const uint4*>(unit + kOffVScale + 32 * (i >> 2) + 16);
+        const uint32_t pick = (i & 3) | ((4 + (i & 3)) << 4);
+        sw.x = __byte_perm(__byte_perm(s0.x, s0.y, pick), __byte_perm(s0.z, s0.w, pick), 0x5410);
+        sw.y = __byte_perm(__byte_perm(s1.x, s1.y, pick), __byte_perm(s1.z, s1.w, pick), 0x5410);
       } else {
         w = *reinterpret_cast<const uint2*>(unit + 64 * i + 8 * g);
         sw = *reinterpret_cast<const uint2*>(unit + kOffKScale + 8 * i);
@@ -115,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&c[k]));
       return f32_to_pair<T>(f.x * sc, f.y * sc);
     };
-    uint8_t* dst = (is_v ? a.value : a.key) + (t * a.kvh + head) * (kD * 2);
+    uint8_t* dst = (is_v ? a.value : a.key) + (static_cast<int64_t>(t) * a.kvh + head) * (kD * 2);
     if (is_v) {  // byte j: dims 16 j + 2 g and + 1
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) *reinterpret_cast<uint32_t*>(dst + 32 * j + 4 * g) = value(j, scale_of(j));
@@ -184,13 +203,14 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a
   for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); w < items; w += nw) {
     const int64_t t = w / chunks;
     const int lo = static_cast<int>(w - t * chunks) * a.chunk, hi = min(lo + a.chunk, rounds);
-    // this lane's words of its row of round r
+    // where this lane's words of the first q, k and v row of its eight lanes lie
+    const uint8_t* qp = a.q + t * a.q_stride + sub * 256 + 4 * g;
+    const uint8_t* kp = a.k + t * a.k_stride + sub * 256 + 4 * g;
+    const uint8_t* vp = a.v + t * a.v_stride + sub * 256 + 4 * g;
     auto load = [&](int r, uint32_t (&x)[kGroups]) {
-      const bool is_q = r < rq, is_v = r >= rq + rk;
-      const int head = 4 * (r - (is_q ? 0 : is_v ? rq + rk : rq)) + sub;
-      const bool live = head < (is_q ? a.num_heads : a.kvh);
-      const uint8_t* src = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) +
-                           head * 256 + 4 * g;
+      const int i = r < rq ? r : r < rq + rk ? r - rq : r - rq - rk;
+      const uint8_t* src = (r < rq ? qp : r < rq + rk ? kp : vp) + i * 1024;
+      const bool live = 4 * i + sub < (r < rq ? a.num_heads : a.kvh);
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) x[j] = live ? *reinterpret_cast<const uint32_t*>(src + 32 * j) : 0u;
     };
@@ -199,6 +219,8 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a
     const int64_t slot = a.slots[t];
     const bool slot_ok = slot >= 0 && slot < a.num_slots;
     if (!slot_ok && lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrBadSlot);
+    uint8_t* unit = unit_of(a.pool, slot_ok ? slot : 0, sub, a.kvh, a.upb_log2);  // of KV head sub
+    const int token = static_cast<int>(slot & 15);
     uint64_t cs[kGroups], sn[kGroups], wt[kGroups];  // sn of the lower half negated
     if (lo < rq + rk) {
       int64_t p = a.positions[t];
@@ -206,23 +228,24 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a
         if (lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrContextTooLong);
         p = p < 0 ? 0 : a.max_pos - 1;
       }
+      const float* ct = a.cos_table + p * kD + 2 * g;
+      const float* st = a.sin_table + p * kD + 2 * g;
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) {
-        const float2 c = *reinterpret_cast<const float2*>(a.cos_table + p * kD + 16 * j + 2 * g);
-        const float2 s = *reinterpret_cast<const float2*>(a.sin_table + p * kD + 16 * j + 2 * g);
+        const float2 c = *reinterpret_cast<const float2*>(ct + 16 * j), s = *reinterpret_cast<const float2*>(st + 16 * j);
         cs[j] = bf16x2_to_f32x2(pack_bf16x2(c.x, c.y));
         sn[j] = bf16x2_to_f32x2(j < 4 ? pack_bf16x2(-s.x, -s.y) : pack_bf16x2(s.x, s.y));
       }
     }
     for (int r = lo; r < hi; ++r) {
       const bool is_q = r < rq, is_v = r >= rq + rk;
-      const int head = 4 * (r - (is_q ? 0 : is_v ? rq + rk : rq)) + sub;
-      const bool live = head < (is_q ? a.num_heads : a.kvh);
+      const int i = is_q ? r : is_v ? r - rq - rk : r - rq;
+      const bool live = 4 * i + sub < (is_q ? a.num_heads : a.kvh);
       if (r == lo || r == rq) {
-        const uint8_t* weight = is_q ? a.q_weight : a.k_weight;
+        const uint8_t* weight = (is_q ? a.q_weight : a.k_weight) + 4 * g;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
-          wt[j] = bf16x2_to_f32x2(*reinterpret_cast<const uint32_t*>(weight + 32 * j + 4 * g));
+          wt[j] = bf16x2_to_f32x2(*reinterpret_cast<const uint32_t*>(weight + 32 * j));
       }
       uint32_t x[kGroups];
 #pragma unroll
@@ -254,16 +277,16 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a
         }
       }
       if (is_q) {
-        uint8_t* dst = a.q_out + (t * a.num_heads + head) * 256 + 4 * g;
+        if (live) {
+          uint8_t* dst = a.q_out + (t * a.num_heads + 4 * i + sub) * 256 + 4 * g;
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j)
-          if (live) *reinterpret_cast<uint32_t*>(dst + 32 * j) = x[j];
+          for (int j = 0; j < kGroups; ++j) *reinterpret_cast<uint32_t*>(dst + 32 * j) = x[j];
+        }
       } else {
         uint32_t w0, w1, scale;
         quantise_row<__nv_bfloat16>(x, is_v ? a.v_inv : a.k_inv, g, w0, w1, scale);
-        const bool store = live && slot_ok;
-        store_row(store ? unit_of(a.pool, slot, head, a.kvh, a.upb_log2) : a.pool, static_cast<int>(slot & 15), is_v,
-                  store, g, w0, w1, scale);
+        store_row(unit + static_cast<int64_t>(i) * ((4 * kUnitBytes) << a.upb_log2), token, is_v, live && slot_ok, g,
+                  w0, w1, scale);
       }
     }
   }
@@ -273,6 +296,20 @@ int sm_count() {
   int sms = 148, dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms;
+}
+
+// Calls launch(first token, rows, grid) for the tokens, as many at a time as the kernels' row index takes.
+template <typename Launch>
+int in_launches(int64_t num_tokens, int kvh, Launch&& launch) {
+  const int64_t per_token = 2 * static_cast<int64_t>(kvh), most_tokens = kMostRows / per_token;
+  const int64_t most_blocks = int64_t(sm_count()) * 8;
+  for (int64_t first = 0; first < num_tokens; first += most_tokens) {
+    const int64_t rows = (num_tokens - first < most_tokens ? num_tokens - first : most_tokens) * per_token;
+    const int64_t want = (rows + kRowsPerBlock - 1) / kRowsPerBlock;
+    const int rc = launch(first, static_cast<int>(rows), dim3(static_cast<unsigned>(want < most_blocks ? want : most_blocks)));
+    if (rc != NVK_OK) return rc;
+  }
+  return NVK_OK;
 }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -307,20 +344,24 @@ extern "C" int nvk_fp4_append(const void* key, const void* value, int64_t key_to
   a.value_stride = value_token_stride * 2;
   a.pool = static_cast<uint8_t*>(kv_cache);
   a.slots = slot_mapping;
-  a.num_tokens = num_tokens;
   a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
   a.kvh = num_kv_heads;
   a.upb_log2 = units_log2(block_size);
+  a.per_token = divisor(2 * num_kv_heads);
   a.k_inv = 1.f / k_scale;
   a.v_inv = 1.f / v_scale;
   a.err = error_word;
-  const int64_t want = (num_tokens * 2 * num_kv_heads + kRowsPerBlock - 1) / kRowsPerBlock;
-  const int64_t most = int64_t(sm_count()) * 8;
-  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return check_cuda(dtype == NVK_DTYPE_BF16 ? launch_pdl(append_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, a)
-                                            : launch_pdl(append_kernel<__half>, grid, dim3(kThreads), 0, st, a),
-                    "fp4_append launch");
+  return in_launches(num_tokens, num_kv_heads, [&](int64_t first, int rows, dim3 grid) {
+    AppendArgs b = a;
+    b.rows = rows;
+    b.key += first * a.key_stride;
+    b.value += first * a.value_stride;
+    b.slots += first;
+    return check_cuda(dtype == NVK_DTYPE_BF16 ? launch_pdl(append_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, b)
+                                              : launch_pdl(append_kernel<__half>, grid, dim3(kThreads), 0, st, b),
+                      "fp4_append launch");
+  });
 }
 
 extern "C" int nvk_fp4_read(void* key, void* value, const void* kv_cache, const int64_t* slot_mapping,
@@ -343,20 +384,24 @@ extern "C" int nvk_fp4_read(void* key, void* value, const void* kv_cache, const 
   a.value = static_cast<uint8_t*>(value);
   a.pool = static_cast<uint8_t*>(const_cast<void*>(kv_cache));
   a.slots = slot_mapping;
-  a.num_tokens = num_tokens;
   a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
   a.kvh = num_kv_heads;
   a.upb_log2 = units_log2(block_size);
+  a.per_token = divisor(2 * num_kv_heads);
   a.k_scale = k_scale;
   a.v_scale = v_scale;
   a.err = error_word;
-  const int64_t want = (num_tokens * 2 * num_kv_heads + kRowsPerBlock - 1) / kRowsPerBlock;
-  const int64_t most = int64_t(sm_count()) * 8;
-  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return check_cuda(dtype == NVK_DTYPE_BF16 ? launch_pdl(read_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, a)
-                                            : launch_pdl(read_kernel<__half>, grid, dim3(kThreads), 0, st, a),
-                    "fp4_read launch");
+  return in_launches(num_tokens, num_kv_heads, [&](int64_t first, int rows, dim3 grid) {
+    ReadArgs b = a;
+    b.rows = rows;
+    b.key += first * num_kv_heads * (kD * 2);
+    b.value += first * num_kv_heads * (kD * 2);
+    b.slots += first;
+    return check_cuda(dtype == NVK_DTYPE_BF16 ? launch_pdl(read_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, b)
+                                              : launch_pdl(read_kernel<__half>, grid, dim3(kThreads), 0, st, b),
+                      "fp4_read launch");
+  });
 }
 
 extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, const void* value,
@@ -415,7 +460,7 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   a.chunk = num_tokens >= int64_t(sms) * 16 ? rounds : 1;
   const int64_t items = num_tokens * ((rounds + a.chunk - 1) / a.chunk);
   const int64_t want = (items + kThreads / 32 - 1) / (kThreads / 32);
-  const int64_t most = int64_t(sms) * 8;
+  const int64_t most = int64_t(sms) * 2;  // one resident wave: its warps stride over the items
   return check_cuda(launch_pdl(norm_rope_kernel, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kThreads),
                                0, reinterpret_cast<cudaStream_t>(stream), a),
                     "fp4_qk_norm_rope_append launch");

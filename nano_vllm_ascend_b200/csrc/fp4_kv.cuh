@@ -219,7 +219,7 @@ inline int check_pool(const void* kv_cache, int num_blocks, int block_size, int 
   if (head_dim != kD) return fail(NVK_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (128 only)", who, head_dim);
   if (units_log2(block_size) < 0)
     return fail(NVK_ERR_UNSUPPORTED, "%s: block_size %d unsupported (a power of two in [16, 256])", who, block_size);
-  if (num_blocks <= 0 || num_kv_heads <= 0)
+  if (num_blocks <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535)
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: bad pool (blocks=%d kv_heads=%d)", who, num_blocks, num_kv_heads);
   if (!kv_cache) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   if (!aligned16(kv_cache)) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: the pool must be 16-byte aligned", who);
