@@ -58,13 +58,13 @@ extern "C" int nvk_fp4_paged_prefill(void* out, const void* query, const void* k
   a.paged = 1;
   a.batch = batch;
   a.qtiles = (max_q_len + kRows - 1) / kRows;
-  a.scale_log2 = scale * 1.4426950408889634f * k_scale * kFp4TileScale;
+  a.scale_log2 = scale * 1.4426950408889634f * k_scale;
   a.pool = static_cast<const uint8_t*>(kv_cache);
   a.kvh = num_kv_heads;
   a.upb_log2 = fp4::units_log2(block_size);
   a.max_blocks = max_blocks_per_seq;
   a.total_q = total_q;
-  a.out_scale = v_scale * kFp4TileScale;
+  a.out_scale = v_scale;
   const size_t smem = sizeof(PrefillSmem) + 1024;
   if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&fp4_prefill_kernel), smem)) != NVK_OK) return rc;
   int dev = 0, sms = 148;

@@ -50,13 +50,13 @@
 //   4-bit pool, warps 12-15 (decoders; warps 10 and 11 idle): thread r owns
 //     token row r of each K and V tile. It loads the row's packed words
 //     straight into registers one tile ahead (in flight while the other of K
-//     and V is decoded), turns them into bf16 and stores them where the TMA
-//     copy of a bf16 tile would have put them. A code's bits, moved to bf16's
-//     sign, low exponent and top mantissa bit, are the value times 2^-126, so
-//     one bf16 multiplication by scale * 2^117 gives the value times 2^-9,
-//     exactly; the 2^9 goes into the softmax scale and the output's factor.
-//     The tiles being exact, the result is that of the bf16 kernel over the
-//     values that the codes stand for. 16 warps have 128 registers a thread at
+//     and V is decoded), turns them into fp16, which holds the values exactly,
+//     and stores them where the TMA copy of a tile would have put them. All
+//     operands are fp16 then: the decoders also turn the item's Q rows into
+//     fp16, each scaled by a power of two into its range (the softmax takes
+//     the factor back), and P is fp16, three bits more exact than bf16. Items
+//     are published one earlier, so that the next item's first tiles are
+//     decoded behind this one's last. 16 warps have 128 registers a thread at
 //     launch: the softmax warpgroups take 168, the other two give them up.
 // Every mbarrier wait is bounded; on a timeout the CTA records the error,
 // drains its in-flight copies and MMAs, frees TMEM and exits.
@@ -86,7 +86,6 @@ constexpr int kThreadsFp4 = 16 * 32;
 // Registers a thread after the split of the 4-bit kernel's 512 x 128 (softmax, softmax, producer and MMA, decoders)
 constexpr int kRegsSoftmax = 168, kRegsIssue = 72, kRegsDecode = 104;
 static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsDecode <= 4 * 128, "setmaxnreg shares exceed the launch's registers");
-constexpr float kFp4TileScale = 512.f;    // a decoded tile holds 2^-9 times the values
 constexpr uint32_t kTmemCols = 512;       // S_0 | S_1 | O_0 | O_1, 128 columns each
 constexpr uint32_t kColO = 256;
 constexpr float kRescaleThreshold = 8.0f;
@@ -128,6 +127,8 @@ struct PrefillSmem {
   Item items[kItemRing];
   uint64_t item_full[kItemRing];                 // items[i % ring] written (one phase per use)
   uint64_t q_full[kStreams], q_empty[kStreams];  // one phase per item
+  uint64_t q_ready[kStreams];                    // 4-bit pool: Q_s is fp16 (one phase per item)
+  int8_t q_exp[2][kStreams][kRows];              // and was scaled by 2^-this (even and odd items)
   uint64_t full_k[kStages], k_empty[kStages];
   uint64_t full_v[kStages], v_empty[kStages];
   uint64_t s_full[kStreams];   // S_s(j) in TMEM (and, in issue order, P V_s(j-1) done)
@@ -200,6 +201,18 @@ __device__ __forceinline__ void flag_error(const PrefillArgs& a, PrefillSmem& sm
   sm.abort = 1;
 }
 
+// The 4-bit kernel holds P as 2^7 p: p is at most 2^8 (see kRescaleThreshold),
+// so fp16 takes it, with 11 bits down to p = 2^-21.
+template <bool kFp4>
+constexpr float kPShift = kFp4 ? 7.f : 0.f;
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr uint32_t umma_idesc_ab_bf16 = (1u << 7) | (1u << 10);
+
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -236,42 +249,50 @@ __device__ __forceinline__ void load_row(VRow& v, const uint8_t* unit, int i) {
                   : make_uint4(0, 0, 0, 0);
 }
 
-__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
-// Scale bytes of groups 2 k and 2 k + 1 (low two bytes of w) times 2^117, each as a bf16 pair.
+// Scale bytes of groups 2 k and 2 k + 1 (low two bytes of w), each as a pair of fp16.
 __device__ __forceinline__ void scale_pairs(uint32_t w, uint32_t& s0, uint32_t& s1) {
   uint32_t lo, hi;
   fp4::e4m3_to_half2(w, lo, hi);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-  constexpr float kUp = 0x1p117f;
-  s0 = pack_bf16x2(f.x * kUp, f.x * kUp);
-  s1 = pack_bf16x2(f.y * kUp, f.y * kUp);
+  s0 = __byte_perm(lo, lo, 0x1010);
+  s1 = __byte_perm(lo, lo, 0x3232);
 }
 
 // Eight codes (dims ascending from the low nibble) of one group into chunk c
 // (dims 8 c .. 8 c + 7) of token row r of a tile in the 128-byte-swizzled layout.
-__device__ __forceinline__ void put_chunk(uint8_t* tile, int r, int c, uint32_t codes, uint32_t s) {
-  const uint32_t even = codes & 0x0f0f0f0fu, odd = (codes >> 4) & 0x0f0f0f0fu;
+__device__ __forceinline__ void put_chunk(uint32_t tile, int r, int c, uint32_t codes, uint32_t s) {
   uint32_t o[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    // code 2 k in the low half, 2 k + 1 in the high one (a selector with bit 3 set repeats
-    // a byte's top bit, here 0); times 2^6 + 2^12 puts one copy of the magnitude at bits
-    // 6-8 and one of the sign at bit 15
-    uint32_t y;
-    asm("prmt.b32 %0, %1, %2, %3;"
-        : "=r"(y)
-        : "r"(even), "r"(odd), "r"(k | ((8 | k) << 4) | ((4 + k) << 8) | ((12 + k) << 12)));
-    o[k] = bf16x2_mul((y * 0x1040u) & 0x81c081c0u, s);
-  }
-  st_shared_v4(smem_u32(tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4)), o[0], o[1], o[2], o[3]);
+  fp4::e2m1_to_half2(codes, o[0], o[1], o[2], o[3]);
+  st_shared_v4(tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), fp4::hmul2(o[0], s),
+               fp4::hmul2(o[1], s), fp4::hmul2(o[2], s), fp4::hmul2(o[3], s));
 }
 
-__device__ __forceinline__ void decode_row(const KRow& k, uint8_t* tile, int r) {
+// Row r of a Q tile from bf16 to fp16 in place, scaled by 2^-e such that its
+// largest entry lies in [1, 2) (entries 2^14 below it lose bits that a sum of
+// 128 terms does not show); returns e.
+__device__ __forceinline__ int q_row_to_half(uint32_t tile, int r) {
+  auto chunk = [&](int c) { return tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+  uint32_t big = 0;  // bf16 magnitudes order as integers
+#pragma unroll 4
+  for (int c = 0; c < 16; ++c) {
+    const uint4 v = ld_shared_v4(chunk(c));
+    big = __vmaxu2(__vmaxu2(big, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)),
+                   __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+  }
+  const int e = min(max(static_cast<int>(max(big & 0xffffu, big >> 16) >> 7), 27), 227) - 127;  // within 2^+-100
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  auto half = [&](uint32_t w) {
+    const __half2 h = __floats2half2_rn(bf16lo_to_f32(w) * down, bf16hi_to_f32(w) * down);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  };
+#pragma unroll 4
+  for (int c = 0; c < 16; ++c) {
+    const uint4 v = ld_shared_v4(chunk(c));
+    st_shared_v4(chunk(c), half(v.x), half(v.y), half(v.z), half(v.w));
+  }
+  return e;
+}
+
+__device__ __forceinline__ void decode_row(const KRow& k, uint32_t tile, int r) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(k.w);  // word 4 t + p: groups 2 p and 2 p + 1
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -284,7 +305,7 @@ __device__ __forceinline__ void decode_row(const KRow& k, uint8_t* tile, int r) 
         put_chunk(tile, r, 2 * (2 * p + e) + h, __byte_perm(w[8 * h + p], w[8 * h + 4 + p], e ? 0x7632 : 0x5410), s[e]);
   }
 }
-__device__ __forceinline__ void decode_row(const VRow& v, uint8_t* tile, int r) {
+__device__ __forceinline__ void decode_row(const VRow& v, uint32_t tile, int r) {
   const uint32_t* sw = reinterpret_cast<const uint32_t*>(v.s);  // word j: group j of the quad's tokens
   const int sh = 8 * (r & 3);
 #pragma unroll
@@ -331,6 +352,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     }
     for (int s = 0; s < kStreams; ++s) {
       mbar_init(&sm.q_full[s], 1);
+      mbar_init(&sm.q_ready[s], 128);
       mbar_init(&sm.q_empty[s], 1);
       mbar_init(&sm.s_full[s], 1);
       mbar_init(&sm.p_lo[s], kStreamThreads);
@@ -382,13 +404,20 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       if (lane == 0) {
         // The Q buffers, and with them the ring slot (read by every role
         // before the previous item's last S), are free once the previous
-        // item's last S of each stream has completed.
-        for (int s = 0; s < ns && ok && qi > 0; ++s)
-          if (!mbar_wait(&sm.q_empty[s], (qi - 1) & 1)) ok = false;
+        // item's last S of each stream has completed. The 4-bit kernel fills
+        // the slot before that wait: its last user, four items back, was done
+        // when the last S of the item before the previous one had completed,
+        // for which this loop has waited already.
+        auto q_free = [&] {
+          for (int s = 0; s < ns && ok && qi > 0; ++s)
+            if (!mbar_wait(&sm.q_empty[s], (qi - 1) & 1)) ok = false;
+        };
+        if (!kFp4) q_free();
         Item& slot = sm.items[qi % kItemRing];
         slot = it;
         if (!have || !ok) slot.n_kv = -1;
         mbar_arrive(&sm.item_full[qi % kItemRing]);
+        if (kFp4 && have) q_free();
         if (have && ok) {
           for (int s = 0; s < ns; ++s) {
             mbar_arrive_expect_tx(&sm.q_full[s], kTileBytes);
@@ -461,8 +490,10 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------- MMA ----
     if constexpr (kSplit) regs_dec<kRegsIssue>();
-    constexpr uint32_t idesc_qk = umma_idesc_bf16(kRows, kKeys, false);
-    constexpr uint32_t idesc_pv = umma_idesc_bf16(kRows, kD, true);
+    // the operands' type fields: 1 for bf16, 0 for fp16
+    constexpr uint32_t types = kFp4 ? umma_idesc_ab_bf16 : 0u;
+    constexpr uint32_t idesc_qk = umma_idesc_bf16(kRows, kKeys, false) & ~types;
+    constexpr uint32_t idesc_pv = umma_idesc_bf16(kRows, kD, true) & ~types;
     bool ok = true;
     auto wait_all = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
     auto commit = [](uint64_t* bar) {
@@ -504,7 +535,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         const int st = g % kStages;
         if (!wait_all(&sm.full_k[st], (g / kStages) & 1)) { ok = false; break; }
         for (int s = 0; s < ns && ok; ++s) {
-          if (!wait_all(&sm.q_full[s], qi & 1)) { ok = false; break; }
+          if (!wait_all(kFp4 ? &sm.q_ready[s] : &sm.q_full[s], qi & 1)) { ok = false; break; }
           tc_fence_after();
           issue_s(s, st);
           if (it.n_kv == 1) commit(&sm.q_empty[s]);
@@ -590,22 +621,32 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       const uint8_t* unit = unit_at(0);
       load_row(k, unit, i);
       load_row(v, unit, i);
+      auto q_to_half = [&] {
+        for (int s = 0; s < ns; ++s) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full[s], qi & 1))) return false;
+          sm.q_exp[qi & 1][s][r] = static_cast<int8_t>(q_row_to_half(smem_u32(sm.q[s]), r));
+          fence_proxy_async_smem();
+          mbar_arrive(&sm.q_ready[s]);
+        }
+        return true;
+      };
       for (int j = 0; j < it.n_kv; ++j, ++g) {
         const int st = g % kStages;
         unit = j + 1 < it.n_kv ? unit_at(j + 1) : nullptr;
         const uint32_t parity = ((g / kStages) - 1) & 1;
         if (sm.abort || (g >= kStages && !mbar_wait(&sm.k_empty[st], parity))) ok = false;
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        decode_row(k, sm.k[st], r);
+        decode_row(k, smem_u32(sm.k[st]), r);
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_k[st]);
         load_row(k, unit, i);
         if (g >= kStages && !mbar_wait(&sm.v_empty[st], parity)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        decode_row(v, sm.v[st], r);
+        decode_row(v, smem_u32(sm.v[st]), r);
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_v[st]);
         load_row(v, unit, i);
+        if (j == 0 && !q_to_half()) { ok = false; break; }
       }
       ++qi;
     }
@@ -618,7 +659,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tmem_s = tmem + s * kKeys + t_lane;
     const uint32_t tmem_o = tmem + kColO + s * kD + t_lane;
-    const float sc = a.scale_log2;
+    float sc = a.scale_log2;
     uint8_t* stage = sm.stage[s];
     int qi = 0, g = 0;
     bool ok = true;
@@ -636,6 +677,10 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         // warp-uniform outcome: the tcgen05.ld/st below need a converged warp
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[s], g & 1))) { ok = false; break; }
         tc_fence_after();
+        // S_s(0) came of Q_s, which was ready after its exponents were stored
+        // (q_ready itself may be two items on when this warp gets here)
+        if (kFp4 && j == 0)
+          sc = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + sm.q_exp[qi & 1][s][r]) << 23);
         const int kbase = j * kKeys;
         uint32_t sr[4][32];
 #pragma unroll
@@ -663,7 +708,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           l *= alpha;
           m = m_new;
         }
-        const float neg_mu = (m == -INFINITY) ? 0.f : -m;
+        const float neg_mu = (m == -INFINITY) ? 0.f : kPShift<kFp4> - m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};  // independent add chains
         // P over the first 64 columns of S_s (column k holds keys 2k and 2k+1
         // as a bf16 pair): word e of chunk c overwrites score e, already read.
@@ -676,7 +721,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
             const float p1 = fast_exp2(fmaf(__uint_as_float(sr[c][2 * e + 1]), sc, neg_mu));
             sum[(2 * e) & 3] += p0;
             sum[(2 * e + 1) & 3] += p1;
-            sr[c][e] = pack_bf16x2(p0, p1);
+            sr[c][e] = kFp4 ? pack_half2(p0, p1) : pack_bf16x2(p0, p1);
           }
           tmem_st16_first(tmem_s + c * 16, sr[c]);
         };

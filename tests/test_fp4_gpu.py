@@ -6,14 +6,18 @@ tolerance counts the roundings on the way (relative half steps: bf16 2^-8,
 fp16 2^-11):
 
 * the output's own, 2^-8 |o|;
-* the weights', which are held in fp16 in decode (rounded, multiplied by V's
-  scale and rounded again: two half steps) and in bf16 in prefill: of the
-  weighted mean of |v|, A;
+* the weights', which are held in fp16 (in decode rounded, multiplied by V's
+  scale and rounded again: two half steps; in prefill once), of the weighted
+  mean of |v|, A;
 * scores: sums of 128 products in fp32 (in the test's range below 2^7 in log2
   units, so within 2^-14 of them after 128 roundings of 2^-24 relative to the
   sum of magnitudes), the exponential's 2^-22, fp16's floor for entries of q
   far below the row's largest: together below 2^-12 of a weight, so 2^-11 A
-  with the denominator's share.
+  with the denominator's share;
+* fp16's smallest step, 2^-24: a weight far below the largest one (which is at
+  least 1 in the units of p) is off by half of it, over the power of two that
+  p is held with. In prefill that is 2^-25 / 2^7 of |v| a key; in decode
+  2^-25 / 2^4 of |v| and, for the product with the scale, of a code of up to 6.
 """
 
 import numpy as np
@@ -28,13 +32,15 @@ pytestmark = pytest.mark.gpu
 
 D = 128
 SCALE = D ** -0.5
-DECODE_A = 2 * 2.0 ** -11 + 2.0 ** -11
-PREFILL_A = 2.0 ** -8 + 2.0 ** -11
+DECODE = dict(per_a=2 * 2.0 ** -11 + 2.0 ** -11, step=2.0 ** -29, code=6.0)
+PREFILL = dict(per_a=2.0 ** -11 + 2.0 ** -11, step=2.0 ** -32, code=0.0)
 
 
-def check(got, want, a, per_a, what=""):
+def check(got, want, a, v, how, what=""):
+    """``want`` and ``a`` from the restatement, ``v`` the rows attended over, ``how`` DECODE or PREFILL."""
     err = (got.double() - want).abs()
-    tol = want.abs() * 2.0 ** -8 + a * per_a + 1e-30
+    far = v.shape[0] * how["step"] * (float(v.abs().max()) + how["code"]) if v.numel() else 0.0
+    tol = want.abs() * 2.0 ** -8 + a * how["per_a"] + far + 1e-30
     assert bool((err <= tol).all()), f"{what}: off by up to {float((err / tol).max()):.2f} tolerances"
     assert not torch.isnan(got).any()
 
@@ -243,7 +249,7 @@ def decode_case(dev, ctx, h, kvh, bs, seed=0, q_mul=1.0, num_ctas=0, ws=None, sp
     for b, n in enumerate(ctx):
         sl = seq_slots(tables[b], n, bs, dev)
         want, a = orc.attention(q[b:b + 1], kr[sl], vr[sl], SCALE)
-        check(out[b:b + 1], want, a, DECODE_A, f"sequence {b} of {n} tokens")
+        check(out[b:b + 1], want, a, vr[sl], DECODE, f"sequence {b} of {n} tokens")
     return pool, tables, q, out
 
 
@@ -335,13 +341,13 @@ def test_decode_flags_bad_blocks_and_long_contexts(cuda_device):
         k = torch.cat([kr[blk * bs:(blk + 1) * bs], torch.zeros(n, kvh, D, device=dev, dtype=torch.float64)])
         v = torch.cat([vr[blk * bs:(blk + 1) * bs], torch.zeros(n, kvh, D, device=dev, dtype=torch.float64)])
         want, a = orc.attention(q[b:b + 1], k, v, SCALE)
-        check(out[b:b + 1], want, a, DECODE_A)
+        check(out[b:b + 1], want, a, v, DECODE)
     ws.zero_()
     tables = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=dev)
     ops_fp4.paged_decode_fp4(out, q, pool, tables, torch.tensor([33, -5], dtype=torch.int32, device=dev), SCALE, ws)
     assert int(ws[:4].view(torch.int32).item()) == 8
     want, a = orc.attention(q[:1], kr[:32], vr[:32], SCALE)
-    check(out[:1], want, a, DECODE_A)
+    check(out[:1], want, a, vr[:32], DECODE)
     assert not out[1].any()
 
 
@@ -391,11 +397,11 @@ def test_decode_far_offsets(cuda_device):
     out = torch.empty_like(q)
     lens = torch.tensor([n], dtype=torch.int32, device=dev)
     ops_fp4.paged_decode_fp4(out, q, pool, table.to(dev), lens, SCALE, workspace(dev, h, kvh))
-    check(out, want, a, DECODE_A)
+    check(out, want, a, vr.double(), DECODE)
     out.fill_(0)
     cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
     ops_fp4.paged_prefill_fp4(out, q, pool, table.to(dev), cu, lens, 1, SCALE)
-    check(out, want, a, PREFILL_A)
+    check(out, want, a, vr.double(), PREFILL)
 
 
 # ---------------------------------------------------------------- prefill ---
@@ -416,7 +422,7 @@ def prefill_case(dev, q_lens, cached, h, kvh, bs, seed=0, q_mul=1.0, spread=Fals
     for b, (m, n) in enumerate(zip(q_lens, kv)):
         sl = seq_slots(tables[b], n, bs, dev)
         want, a = orc.attention(q[at:at + m], kr[sl], vr[sl], SCALE)
-        check(out[at:at + m], want, a, PREFILL_A, f"sequence {b}: {m} over {n}")
+        check(out[at:at + m], want, a, vr[sl], PREFILL, f"sequence {b}: {m} over {n}")
         at += m
     return pool, tables, q, cu, lens, out
 
@@ -451,15 +457,17 @@ def test_prefill_many_items_per_cta(cuda_device):
     prefill_case(cuda_device, q, c, 8, 2, 32, seed=8)
 
 
-def test_prefill_matches_the_bf16_kernel_over_the_same_values(cuda_device):
-    """The tiles are exact, so the result is that of ops.paged_prefill over the pool that the codes stand for."""
+def test_prefill_is_near_the_bf16_kernel_over_the_same_values(cuda_device):
+    """The tiles are exact: ops.paged_prefill over the pool that the codes stand for differs by the weights' roundings
+    (bf16 there, fp16 here) and the outputs'."""
     dev = cuda_device
     pool, tables, q, cu, lens, out = prefill_case(dev, [130, 50], [200, 0], 8, 4, 128, seed=2)
     nb = pool.shape[0]
     kr, vr = ops_fp4.kv_read_fp4(pool, torch.arange(nb * 128, device=dev))
     got = torch.empty_like(out)
     ops.paged_prefill(got, q, kr.view(nb, 128, 4, D), vr.view(nb, 128, 4, D), tables.to(dev), cu, lens, 130, SCALE)
-    assert torch.equal(got, out)
+    a = vr.abs().max().double()
+    assert bool(((got.double() - out.double()).abs() <= 2 * 2.0 ** -8 * out.double().abs() + a * 2 * 2.0 ** -8).all())
 
 
 def test_prefill_rows_that_see_no_key_and_hidden_rows(cuda_device):
@@ -479,7 +487,7 @@ def test_prefill_rows_that_see_no_key_and_hidden_rows(cuda_device):
     assert int(err.item()) == 0
     for lo, hi, k, v in ((0, 30, kr[:20], vr[:20]), (40, 50, kr[32:48], vr[32:48])):
         want, a = orc.attention(q[lo:hi], k, v, SCALE)
-        check(out[lo:hi], want, a, PREFILL_A)
+        check(out[lo:hi], want, a, v, PREFILL)
     assert not out[:10].any() and not out[30:40].any()
 
 
@@ -524,7 +532,7 @@ def test_append_decode_prefill_together_in_a_graph(cuda_device):
                                   torch.tensor([n0], dtype=torch.int32, device=dev), n0, SCALE)
         kr, vr = ops_fp4.kv_read_fp4(pool, slots[:n0])
         want, a = orc.attention(q, kr.double(), vr.double(), SCALE)
-        check(out, want, a, PREFILL_A, "prefill")
+        check(out, want, a, vr.double(), PREFILL, "prefill")
         ws = workspace(dev, h, kvh)
         x, p, sl = new[n0:n0 + 1].clone(), pos[n0:n0 + 1].clone(), slots[n0:n0 + 1].clone()
         ctx = torch.tensor([n0 + 1], dtype=torch.int32, device=dev)
@@ -549,7 +557,7 @@ def test_append_decode_prefill_together_in_a_graph(cuda_device):
             graph.replay()
             kr, vr = ops_fp4.kv_read_fp4(pool, slots[:n0 + i + 1])
             want, a = orc.attention(qd, kr.double(), vr.double(), SCALE)
-            check(od, want, a, DECODE_A, f"decode step {i}")
+            check(od, want, a, vr.double(), DECODE, f"decode step {i}")
     torch.cuda.current_stream(dev).wait_stream(stream)
 
 
