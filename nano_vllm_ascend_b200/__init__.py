@@ -4,6 +4,7 @@ Drop-in host classes (same names and contracts as the reference's):
 
 * ``PagedKVCache`` -- pool + CUDA append          (npu/paged_kv_cache.py)
 * ``BlockManager`` / ``PagedKVCacheMetadata``     (npu/block_manager.py)
+* ``PagedKVCacheFp4`` -- the pool held in 4 bits   (same interface, ops_fp4)
 * ``PagedAttention``  -- decode attention          (layers/npu_paged_attention.py)
 * ``BatchPrefillAttention`` -- causal prefill     (layers/npu_prefill_attention.py)
 * ``DecodeGraphRunner`` -- CUDA-graph decode       (npu/acl_graph.py)
@@ -18,6 +19,7 @@ built for sm_100a by ``nano_vllm_ascend_b200._build``.
 from . import device_errors
 from .block_manager import BlockManager, BlockState, PagedKVCacheMetadata
 from .cuda_graph import DecodeGraphRunner, DecodeGraphStats, copy_block_tables
+from .fp4_kv_cache import Fp4Layer, PagedKVCacheFp4
 from .paged_attention import PagedAttention
 from .paged_kv_cache import PagedKVCache
 from .device_errors import KVCacheDeviceError, check_errors
@@ -33,11 +35,13 @@ __all__ = [
     "BlockState",
     "DecodeGraphRunner",
     "DecodeGraphStats",
+    "Fp4Layer",
     "KVCacheDeviceError",
     "NpuBatchPrefillAttention",
     "NpuPagedAttention",
     "PagedAttention",
     "PagedKVCache",
+    "PagedKVCacheFp4",
     "PagedKVCacheMetadata",
     "check_errors",
     "copy_block_tables",

@@ -53,16 +53,17 @@ from .block_manager import PagedKVCacheMetadata
 _recording: "GraphSlot | None" = None
 
 
-def graph_workspace(attn, batch_size: int) -> torch.Tensor | None:
+def graph_workspace(attn, batch_size: int, kind: str = "") -> torch.Tensor | None:
     """Called by an attention layer: the split-K workspace of the decode graph
-    being recorded, or None outside a runner's warm-up and capture."""
+    being recorded, or None outside a runner's warm-up and capture. Kernels
+    that lay their workspace out differently name different ``kind``s."""
     slot = _recording
     if slot is None:
         return None
     if batch_size != slot.batch_size:
         raise RuntimeError(f"attention over {batch_size} sequences inside the batch-{slot.batch_size} decode graph")
     slot.attention_calls += 1
-    return slot.workspace_for(attn.workspace_bytes(batch_size))
+    return slot.workspace_for(attn.workspace_bytes(batch_size), kind)
 
 
 def recording_slot() -> "GraphSlot | None":
@@ -116,18 +117,28 @@ class GraphSlot:
         self.context_lens = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
         self.slot_mapping = torch.zeros(attn_metadata.slot_mapping.shape, dtype=torch.int64, device=self.device)
         self._table_cols = width  # columns that may hold non-zero entries
-        self.workspace: torch.Tensor | None = None
+        self.workspaces: dict[str, torch.Tensor] = {}
         self.graph: Any = None
         self.logits: torch.Tensor | None = None
         self.attention_calls = 0
         self.error_name = f"decode graph batch {batch_size}"
 
-    def workspace_for(self, nbytes: int) -> torch.Tensor:
-        if self.workspace is None or self.workspace.numel() < nbytes:
+    @property
+    def workspace(self) -> torch.Tensor | None:
+        """The bf16 layers' workspace, once an attention call has sized it."""
+        return self.workspaces.get("")
+
+    def workspace_for(self, nbytes: int, kind: str = "") -> torch.Tensor:
+        workspace = self.workspaces.get(kind)
+        if workspace is None or workspace.numel() < nbytes:
             if self.backend.capturing():
                 raise RuntimeError("decode workspace must be sized by the warm-up run before capture")
-            self.workspace = torch.zeros(max(nbytes, 1), dtype=torch.uint8, device=self.device)
-        return self.workspace
+            workspace = self.workspaces[kind] = torch.zeros(max(nbytes, 1), dtype=torch.uint8, device=self.device)
+        return workspace
+
+    def error_names(self) -> dict[str, torch.Tensor]:
+        """The workspaces (their heads are the device error words) by the names of their errors."""
+        return {f"{self.error_name} {kind}".rstrip(): ws for kind, ws in self.workspaces.items()}
 
     def metadata(self, like=None):
         """The step metadata as the graph sees it (the static buffers), in the type of
@@ -242,14 +253,15 @@ class DecodeGraphRunner:
         self.backend.replay(slot.graph)
         self.stats.replays += 1
         if errors is not None:
-            errors.launched(slot.error_name, device_errors.SHARED)
+            errors.launched(*slot.error_names(), device_errors.SHARED)
         return slot.logits
 
     def _errors(self, slot: GraphSlot):
-        if slot.device.type != "cuda" or slot.workspace is None:
+        if slot.device.type != "cuda" or not slot.workspaces:
             return None
         errors = device_errors.state(slot.device)
-        errors.watch(slot.error_name, slot.workspace)
+        for name, workspace in slot.error_names().items():
+            errors.watch(name, workspace)
         return errors
 
     def _step(self, slot: GraphSlot, static_md):
@@ -294,7 +306,8 @@ class DecodeGraphRunner:
         """Drops every captured graph (call before tearing down the process group)."""
         for slot in self.slots.values():
             if slot.device.type == "cuda":
-                device_errors.state(slot.device).forget(slot.error_name)
+                for name in slot.error_names():
+                    device_errors.state(slot.device).forget(name)
         self.slots.clear()
 
 

@@ -18,15 +18,21 @@ outside the pool, a device ``context_lens`` too long, a fused-append slot
 that is not the sequence's last position) is reported through the decode
 workspace's error word and raised by ``device_errors`` on a following call
 or by ``device_errors.check_errors()``.
+
+Over a ``PagedKVCacheFp4`` both cache arguments are the layer's ``Fp4Layer``
+and the 4-bit decode kernel runs.
 """
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import torch
 from torch import nn
 
-from . import device_errors, ops
+from . import device_errors, ops, ops_fp4
 from .cuda_graph import graph_workspace
+from .fp4_kv_cache import Fp4Layer
 from .paged_kv_cache import take_deferred
 
 _NUM_SMS: dict[int, int] = {}
@@ -61,6 +67,25 @@ def shared_workspace(device: torch.device, nbytes: int, shape: tuple = ()) -> to
     return ws
 
 
+# Eager-mode workspaces of the 4-bit kernel, one per device and stream (calls
+# on two streams may overlap), grown on demand. Its layout does not hang on the
+# call's shape, so a workspace is zeroed once.
+_FP4_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _fp4_workspace(device: torch.device, nbytes: int) -> tuple[torch.Tensor, bool]:
+    """A zeroed workspace, and whether it is kept. A call that a caller's own
+    graph captures gets one of its own, zeroed by each replay, so that graphs
+    may be replayed in any order (and none is left to eager calls)."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device), False
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    ws = _FP4_WORKSPACES.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _FP4_WORKSPACES[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return ws, True
+
+
 class PagedAttention(nn.Module):
     def __init__(self, num_heads: int, num_key_value_heads: int, head_dim: int, num_ctas: int = 0):
         super().__init__()
@@ -69,6 +94,8 @@ class PagedAttention(nn.Module):
         self.head_dim = head_dim
         self.scale = head_dim ** -0.5
         self.num_ctas = num_ctas  # 0: one persistent CTA per SM
+        self._fp4 = SimpleNamespace(workspace_bytes=lambda batch: ops_fp4.decode_fp4_workspace_bytes(
+            num_heads, num_key_value_heads, head_dim, num_ctas))
 
     def workspace_bytes(self, batch: int) -> int:
         return ops.decode_workspace_bytes(batch, self.num_heads, self.num_key_value_heads, self.head_dim,
@@ -94,6 +121,8 @@ class PagedAttention(nn.Module):
             if longest > block_tables.shape[1] * key_cache.shape[1]:
                 raise RuntimeError(f"missing block: context length {longest} exceeds the "
                                    f"{block_tables.shape[1]}-block table")
+        if isinstance(key_cache, Fp4Layer):
+            return self._forward_fp4(output, q, key_cache, block_tables, context_lens)
         with torch.cuda.device(device):
             errors = device_errors.state(device)
             errors.raise_if_flagged()
@@ -118,6 +147,27 @@ class PagedAttention(nn.Module):
             ops.paged_decode(output, q.contiguous(), key_cache, value_cache, tables.to(torch.int32),
                              ctx.to(torch.int32), self.scale, workspace, self.num_ctas, new_key=new_key,
                              new_value=new_value, slot_mapping=slots)
+            if word is not None:
+                errors.launched(word)
+        return output
+
+    def _forward_fp4(self, output: torch.Tensor, q: torch.Tensor, layer: Fp4Layer, block_tables: torch.Tensor,
+                     context_lens: torch.Tensor) -> torch.Tensor:
+        device = q.device
+        with torch.cuda.device(device):
+            errors = device_errors.state(device)
+            errors.raise_if_flagged()
+            workspace = graph_workspace(self._fp4, q.shape[0], "(4-bit)")
+            word = None  # the graph runner reads its slot's word after each replay
+            if workspace is None:
+                workspace, kept = _fp4_workspace(device, self._fp4.workspace_bytes(q.shape[0]))
+                if kept:
+                    word = errors.watch(f"4-bit paged decode, stream {torch.cuda.current_stream().cuda_stream:#x}",
+                                        workspace)
+            tables = block_tables.to(device=device, dtype=torch.int32)
+            ctx = context_lens.to(device=device, dtype=torch.int32)
+            ops_fp4.paged_decode_fp4(output, q.contiguous(), layer.pool, tables, ctx, self.scale, workspace,
+                                     self.num_ctas, layer.k_scale, layer.v_scale)
             if word is not None:
                 errors.launched(word)
         return output

@@ -20,6 +20,10 @@ A paged-mode ``context_lens`` longer than its block-table row raises
 a block id outside the pool is reported through the device's error word and
 raised by ``device_errors`` on a following call or by
 ``device_errors.check_errors()``.
+
+Over a ``PagedKVCacheFp4`` both cache arguments are the layer's ``Fp4Layer``;
+paged mode then runs the 4-bit kernel over what the pool holds, dense mode
+still attends over this step's own ``k`` and ``v``.
 """
 
 from __future__ import annotations
@@ -27,7 +31,8 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import device_errors, ops
+from . import device_errors, ops, ops_fp4
+from .fp4_kv_cache import Fp4Layer
 
 
 def _cu(values: list[int], device: torch.device) -> torch.Tensor:
@@ -91,8 +96,13 @@ class BatchPrefillAttention(nn.Module):
                     if longest > tables.shape[1] * key_cache.shape[1]:
                         raise RuntimeError(f"missing block: context length {longest} exceeds the "
                                            f"{tables.shape[1]}-block table")
-                ops.paged_prefill(out, query, key_cache, value_cache, tables, cu_q, ctx, max_prompt_len,
-                                  self.scale, error_word=errors.word)
+                if isinstance(key_cache, Fp4Layer):
+                    ops_fp4.paged_prefill_fp4(out, query, key_cache.pool, tables, cu_q, ctx, max_prompt_len,
+                                              self.scale, key_cache.k_scale, key_cache.v_scale,
+                                              error_word=errors.word)
+                else:
+                    ops.paged_prefill(out, query, key_cache, value_cache, tables, cu_q, ctx, max_prompt_len,
+                                      self.scale, error_word=errors.word)
             else:
                 ops.dense_prefill(out, query, k.contiguous(), v.contiguous(), cu_q, cu_kv, max_prompt_len,
                                   self.scale, error_word=errors.word)

@@ -21,7 +21,9 @@ runs:
   (8 bytes a sequence) instead of one ``.item()`` per sequence
   (model_runner.py:284-286); the device error words are read with them;
 * prefill runs the same layers eagerly with prefix-aware paged prefill
-  attention over the pool (cached prefix + the rows just appended).
+  attention over the pool (cached prefix + the rows just appended);
+* with ``kv_cache_dtype="fp4"`` the pool is held in 4 bits
+  (``PagedKVCacheFp4``) and the same steps run on its kernels.
 
 The model is Qwen3-shaped with seeded random weights (``PathModel``; no
 checkpoint is loaded -- model loading, model_runner.py:85-111, is not part
@@ -39,13 +41,14 @@ from types import SimpleNamespace
 import torch
 import torch.nn.functional as F
 
-from . import device_errors, ops
+from . import device_errors, ops, ops_fp4
 from .block_manager import BlockManager
 from .cuda_graph import DecodeGraphRunner
 from .device_metadata import DeviceBlockTables
+from .fp4_kv_cache import Fp4Layer, PagedKVCacheFp4
 from .paged_attention import PagedAttention
 from .paged_kv_cache import PagedKVCache
-from .pool import num_blocks_from_memory
+from .pool import fp4_bytes_per_block, num_blocks_from_memory
 
 DEFAULT_DECODE_GRAPH_BATCH_SIZES = [1, 2, 4, 8, 16, 32]
 
@@ -139,14 +142,22 @@ class PathModel:
             h = _rms_norm(x, layer.in_norm, s.rms_norm_eps)
             qkv = F.linear(h, layer.qkv).view(t, h_all, s.head_dim)
             kc, vc = kv_cache.get_physical_cache(i)
-            q = ops.qk_norm_rope_append(qkv[:, :s.num_heads], qkv[:, s.num_heads:s.num_heads + kvh],
-                                        qkv[:, s.num_heads + kvh:], layer.q_norm, layer.k_norm, s.rms_norm_eps,
-                                        self.cos, self.sin, position_ids_flat, kc, vc, md.slot_mapping,
-                                        error_word=errors.word)
+            rows = (qkv[:, :s.num_heads], qkv[:, s.num_heads:s.num_heads + kvh], qkv[:, s.num_heads + kvh:],
+                    layer.q_norm, layer.k_norm, s.rms_norm_eps, self.cos, self.sin, position_ids_flat)
+            fp4 = isinstance(kc, Fp4Layer)
+            if fp4:
+                q = ops_fp4.qk_norm_rope_append_fp4(*rows, kc.pool, md.slot_mapping, kc.k_scale, kc.v_scale,
+                                                    error_word=errors.word)
+            else:
+                q = ops.qk_norm_rope_append(*rows, kc, vc, md.slot_mapping, error_word=errors.word)
             if is_prefill:
                 attn = torch.empty_like(q)
-                ops.paged_prefill(attn, q, kc, vc, tables, cu_q, kv_lens, max_q, s.head_dim ** -0.5,
-                                  error_word=errors.word)
+                if fp4:
+                    ops_fp4.paged_prefill_fp4(attn, q, kc.pool, tables, cu_q, kv_lens, max_q, s.head_dim ** -0.5,
+                                              kc.k_scale, kc.v_scale, error_word=errors.word)
+                else:
+                    ops.paged_prefill(attn, q, kc, vc, tables, cu_q, kv_lens, max_q, s.head_dim ** -0.5,
+                                      error_word=errors.word)
             else:
                 attn = self.paged_attn(q, kc, vc, md.block_tables, md.context_lens)
             x = x + F.linear(attn.view(t, -1), layer.o)
@@ -202,7 +213,10 @@ class StepRunner:
     def __init__(self, shape: ModelShape | None = None, device="cuda", max_model_len: int = 2048,
                  num_blocks: int | None = None, block_size: int = 128, memory_utilization: float = 0.8,
                  max_num_seqs: int = 32, enable_prefix_cache: bool = False, enable_decode_graph: bool = True,
-                 decode_graph_batch_sizes: list[int] | None = None, seed: int = 0):
+                 decode_graph_batch_sizes: list[int] | None = None, seed: int = 0, kv_cache_dtype: str = "bf16",
+                 k_scale=1.0, v_scale=1.0):
+        if kv_cache_dtype not in ("bf16", "fp4"):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is neither 'bf16' nor 'fp4'")
         self.shape = shape or ModelShape()
         self.device = torch.device(device)
         self.max_model_len = max_model_len
@@ -210,12 +224,18 @@ class StepRunner:
         self.enable_prefix_cache = enable_prefix_cache
         s = self.shape
         self.model = PathModel(self.shape, self.device, seed)
+        fp4 = kv_cache_dtype == "fp4"
+        block_bytes = fp4_bytes_per_block(s.num_layers, block_size, s.num_kv_heads) if fp4 else None
         self.num_blocks = num_blocks or num_blocks_from_memory(memory_utilization, s.num_layers, block_size,
                                                                s.num_kv_heads, s.head_dim, torch.bfloat16,
-                                                               self.device)
+                                                               self.device, block_bytes)
         self.block_manager = BlockManager(self.num_blocks, block_size, self.device)
-        self.kv_cache = PagedKVCache(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
-                                     torch.bfloat16, self.device)
+        if fp4:
+            self.kv_cache = PagedKVCacheFp4(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
+                                            self.device, k_scale, v_scale)
+        else:
+            self.kv_cache = PagedKVCache(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
+                                         torch.bfloat16, self.device)
         self.table_width = math.ceil(max_model_len / block_size)
         self.device_tables = DeviceBlockTables(self.block_manager, max_num_seqs, self.table_width, self.device)
         self.errors = device_errors.state(self.device)
