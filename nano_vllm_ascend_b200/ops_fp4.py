@@ -35,25 +35,37 @@ def pool_shape(num_blocks: int, block_size: int, num_kv_heads: int) -> tuple[int
 
 
 # A decode step makes a few of these calls a layer, so the checks are written
-# to cost little: tensors' properties are read once, and torch's raw stream
-# handle is asked for instead of a Stream object (3 us less a call).
+# to cost little: tensors' properties are read once, torch's raw stream handle
+# is asked for instead of a Stream object (3 us less a call), and entry points
+# are looked up once.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+class _EntryPoints(dict):
+    def __missing__(self, name: str):
+        fn = self[name] = getattr(_lib.load(), name)
+        return fn
+
+
+_entry_points = _EntryPoints()
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
     """Calls ``name`` on ``dev`` and its current stream (the last argument)."""
     index = dev.index
     if index == torch.cuda.current_device():
-        _lib.call(name, *args, _raw_stream(index))
+        rc = _entry_points[name](*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, _raw_stream(index))
+            rc = _entry_points[name](*args, _raw_stream(index))
+    if rc:
+        _lib.check(name, rc)
 
 
-def _check_devices(dev: torch.device, **tensors: torch.Tensor) -> None:
+def _wrong_device(dev: torch.device, **tensors: torch.Tensor) -> None:
+    """Raises for the first tensor that is not on the CUDA device ``dev``."""
     for name, t in tensors.items():
-        if t.device != dev or not t.is_cuda:
-            _require_cuda(name, t, dev)
+        _require_cuda(name, t, dev)
 
 
 def _check_pool(who: str, kv_cache: torch.Tensor) -> tuple[int, int, int]:
@@ -97,7 +109,8 @@ def kv_append_fp4(kv_cache: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     of ``error_word``."""
     who = "kv_append_fp4"
     dev = kv_cache.device
-    _check_devices(dev, kv_cache=kv_cache, key=key, value=value, slot_mapping=slot_mapping)
+    if not kv_cache.is_cuda or key.device != dev or value.device != dev or slot_mapping.device != dev:
+        _wrong_device(dev, kv_cache=kv_cache, key=key, value=value, slot_mapping=slot_mapping)
     nb, bs, kvh = _check_pool(who, kv_cache)
     dtype, shape = key.dtype, key.shape
     if dtype not in _DTYPES or value.dtype != dtype:
@@ -121,7 +134,8 @@ def kv_read_fp4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, k_scale: flo
     outside the pool gives zeros and sets bit 4 of ``error_word``."""
     who = "kv_read_fp4"
     dev = kv_cache.device
-    _check_devices(dev, kv_cache=kv_cache, slot_mapping=slot_mapping)
+    if not kv_cache.is_cuda or slot_mapping.device != dev:
+        _wrong_device(dev, kv_cache=kv_cache, slot_mapping=slot_mapping)
     nb, bs, kvh = _check_pool(who, kv_cache)
     if dtype not in _DTYPES:
         raise ValueError(f"{who}: dtype must be bfloat16 or float16, got {dtype}")
@@ -150,9 +164,12 @@ def qk_norm_rope_append_fp4(query: torch.Tensor, key: torch.Tensor, value: torch
     kernel. Returns the rotated query [tokens, heads, 128]."""
     who = "qk_norm_rope_append_fp4"
     dev = query.device
-    _check_devices(dev, query=query, key=key, value=value, q_weight=q_weight, k_weight=k_weight,
-                   cos_table=cos_table, sin_table=sin_table, positions=positions, kv_cache=kv_cache,
-                   slot_mapping=slot_mapping)
+    if not query.is_cuda or key.device != dev or value.device != dev or q_weight.device != dev \
+            or k_weight.device != dev or cos_table.device != dev or sin_table.device != dev \
+            or positions.device != dev or kv_cache.device != dev or slot_mapping.device != dev:
+        _wrong_device(dev, query=query, key=key, value=value, q_weight=q_weight, k_weight=k_weight,
+                      cos_table=cos_table, sin_table=sin_table, positions=positions, kv_cache=kv_cache,
+                      slot_mapping=slot_mapping)
     if query.dtype != _BF16 or key.dtype != _BF16 or value.dtype != _BF16:
         raise ValueError(f"{who}: query, key and value must be bfloat16")
     q_stride, k_stride, v_stride = _row_stride("query", query), _row_stride("key", key), _row_stride("value", value)
@@ -193,7 +210,9 @@ def decode_fp4_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int 
 def _check_attention(who: str, dev, out, query, kv_cache, block_tables, lens) -> tuple:
     """Checks what decode and prefill share; returns what their calls take: query's shape, the pool's blocks,
     block size and KV heads, and the table's rows, row stride and columns."""
-    _check_devices(dev, out=out, query=query, kv_cache=kv_cache, block_tables=block_tables, lens=lens)
+    if not query.is_cuda or out.device != dev or kv_cache.device != dev or block_tables.device != dev \
+            or lens.device != dev:
+        _wrong_device(dev, out=out, query=query, kv_cache=kv_cache, block_tables=block_tables, lens=lens)
     if query.dtype != _BF16 or out.dtype != _BF16:
         raise ValueError(f"{who}: query and out must be bfloat16")
     shape = query.shape
@@ -225,7 +244,8 @@ def paged_decode_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Ten
     dev = query.device
     shape, nb, bs, kvh, batch, stride, width = _check_attention(who, dev, out, query, kv_cache, block_tables,
                                                                 context_lens)
-    _check_devices(dev, workspace=workspace)
+    if workspace.device != dev:
+        _wrong_device(dev, workspace=workspace)
     if shape[0] != batch or not workspace.is_contiguous():
         raise ValueError(f"{who}: {shape[0]} queries for {batch} sequences, or a strided workspace")
     _call(dev, "nvk_fp4_paged_decode", out.data_ptr(), query.data_ptr(), kv_cache.data_ptr(), nb, bs,
@@ -242,7 +262,8 @@ def paged_prefill_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Te
     who = "paged_prefill_fp4"
     dev = query.device
     shape, nb, bs, kvh, batch, stride, width = _check_attention(who, dev, out, query, kv_cache, block_tables, kv_lens)
-    _check_devices(dev, cu_seqlens_q=cu_seqlens_q)
+    if cu_seqlens_q.device != dev:
+        _wrong_device(dev, cu_seqlens_q=cu_seqlens_q)
     cu = _check_index(who, "cu_seqlens_q", cu_seqlens_q, torch.int32, batch + 1)
     _call(dev, "nvk_fp4_paged_prefill", out.data_ptr(), query.data_ptr(), kv_cache.data_ptr(), nb, bs,
           block_tables.data_ptr(), stride, width, cu.data_ptr(), kv_lens.data_ptr(), batch, shape[0], max_q_len,
