@@ -206,6 +206,7 @@ __device__ __forceinline__ void scores(const State& st, uint32_t unit, int valid
   e4m3_to_half2(ksb.y, sb[2], sb[3]);
 #pragma unroll
   for (int c = 0; c < 4; ++c) x[c] = 0.f;
+  float y[4] = {0.f, 0.f, 0.f, 0.f};  // odd groups: two shorter chains of sums
 #pragma unroll
   for (int w = 0; w < 4; ++w) {  // a word holds groups 2 w and 2 w + 1
     uint32_t p[4], q[4];
@@ -219,9 +220,11 @@ __device__ __forceinline__ void scores(const State& st, uint32_t unit, int valid
     const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&sb[w]));
     x[0] = fmaf(d[0], fa.x, x[0]), x[1] = fmaf(d[1], fa.x, x[1]);
     x[2] = fmaf(d[2], fb.x, x[2]), x[3] = fmaf(d[3], fb.x, x[3]);
-    x[0] = fmaf(e[0], fa.y, x[0]), x[1] = fmaf(e[1], fa.y, x[1]);
-    x[2] = fmaf(e[2], fb.y, x[2]), x[3] = fmaf(e[3], fb.y, x[3]);
+    y[0] = fmaf(e[0], fa.y, y[0]), y[1] = fmaf(e[1], fa.y, y[1]);
+    y[2] = fmaf(e[2], fb.y, y[2]), y[3] = fmaf(e[3], fb.y, y[3]);
   }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) x[c] += y[c];
   if (kMask) {
     if (ta >= valid) x[0] = x[1] = -INFINITY;
     if (ta + 2 >= valid) x[2] = x[3] = -INFINITY;
@@ -294,6 +297,12 @@ __device__ __forceinline__ void attend(State& st, uint32_t tile, uint32_t vscale
   __syncwarp();  // vscale is written
   weigh(st, tile, vscale, g, t, b[0][0], b[0][1]);
   weigh(st, tile + kUnitBytes, vscale + kVScaleBytes, g, t, b[1][0], b[1][1]);
+}
+
+__device__ __forceinline__ int ticket(int* p) {
+  int v;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // Orders this thread's shared-memory writes before later copies into them.
@@ -600,17 +609,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
   __syncthreads();
   if (tid < 2 && sm.end[tid].pair >= 0) {
     const End e = sm.end[tid];
-    __threadfence();  // the CTA's pieces, which the barrier put before this, are out before the ticket
-    if (atomicAdd(a.tickets + e.c0, 1) == e.c1 - e.c0) {
+    // the CTA's pieces, which the barrier put before this, are out before the ticket; whoever takes
+    // the last one sees all of them
+    if (ticket(a.tickets + e.c0) == e.c1 - e.c0) {
       a.tickets[e.c0] = 0;  // every piece is in: nobody else touches it in this call
-      __threadfence();
       sm.end[tid].last = 1;
     }
   }
   __syncthreads();
   // A task is a share of the pieces of one end and head: part, part + parts, ...,
   // kAhead loads in flight. Several parts meet in shared memory (the rings are done).
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 4;
   const int most = max(1, kWarps / (2 * a.group));
   auto parts_of = [&](const End& e) { return min(most, (e.c1 - e.c0 + kAhead) / kAhead); };
   float4* sum_o = reinterpret_cast<float4*>(sm.ring);
