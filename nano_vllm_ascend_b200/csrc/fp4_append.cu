@@ -8,6 +8,8 @@
 // maximum is three shuffles, each 4-byte load of the eight lanes is one whole
 // 32-byte sector, a lane's eight code bytes are what it stores, and the
 // rotation pairs (i, i + 64) sit in one lane.
+#include <type_traits>
+
 #include "fp4_kv.cuh"
 
 namespace nvk {
@@ -24,7 +26,7 @@ struct Divisor {
   uint32_t m, shift;
   int d;
 };
-inline Divisor divisor(int d) {
+inline Divisor divisor(int d) {  // d of 1 is for the caller
   uint32_t l = 1;
   while ((int64_t(1) << l) < d) ++l;
   return Divisor{static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + d - 1) / d), l - 1, d};
@@ -168,9 +170,11 @@ struct NormArgs {
   const int64_t* slots;
   uint8_t* q_out;  // [T, H, 128] contiguous
   uint8_t* pool;
-  int64_t num_tokens, num_slots;
+  int64_t num_slots;
   int num_heads, kvh, upb_log2;
-  int chunk;  // rounds of four head rows per warp item
+  int items;            // num_tokens * chunks
+  int chunk, chunks;    // rounds of four head rows per warp item, items per token
+  Divisor per_token;    // chunks, where it is not 1
   float eps, k_inv, v_inv;
   int* err;
 };
@@ -195,77 +199,153 @@ __device__ __forceinline__ uint32_t f32x2_to_bf16x2(uint64_t v) {
 // The mean square is summed in 64 bits and its root is correctly rounded, so
 // the bf16 row does not hang on the order of the sum: a row that differed in
 // one bf16 bit could be stored one whole e2m1 step away.
-// Issue-bound where it is not HBM-bound: two values an instruction (f32x2)
-// throughout, and the next round's row is loaded before this one's arithmetic.
+// HBM-bound once enough is in flight: each warp copies its rounds ahead, kDepth
+// at a time, into a ring in shared memory (cp.async; with the cos and sin rows
+// of a new token), across the borders of its items: 64 KB an SM. One round
+// ahead in registers, 16 KB an SM, took 37.5 us for 8192 tokens of 16 + 2 * 8
+// heads.
+constexpr int kDepth = 4;
+constexpr int kRowPitch = 256 + 32;  // the four rows of a round lie eight banks apart
+struct NormSmem {
+  alignas(16) uint8_t rows[kWarps][kDepth][4 * kRowPitch];
+  alignas(16) float table[kWarps][kDepth + 1][2][kD];  // cos and sin of the items that have rounds in the ring
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// kWide: rows and tables are 16-byte aligned; else they are copied 4 bytes at a time.
+template <bool kWide>
 __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  NormSmem& sm = *reinterpret_cast<NormSmem*>(smem_raw);
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, g = lane & 7, sub = lane >> 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane & 7, sub = lane >> 3;
   const int rq = (a.num_heads + 3) / 4, rk = (a.kvh + 3) / 4, rounds = rq + 2 * rk;
-  const int chunks = (rounds + a.chunk - 1) / a.chunk;
-  const int64_t items = a.num_tokens * chunks;
-  const int64_t nw = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < items; w += nw) {
-    const int64_t t = w / chunks;
-    const int lo = static_cast<int>(w - t * chunks) * a.chunk, hi = min(lo + a.chunk, rounds);
-    // where this lane's words of the first q, k and v row of its eight lanes lie
-    const uint8_t* qp = a.q + t * a.q_stride + sub * 256 + 4 * g;
-    const uint8_t* kp = a.k + t * a.k_stride + sub * 256 + 4 * g;
-    const uint8_t* vp = a.v + t * a.v_stride + sub * 256 + 4 * g;
-    auto load = [&](int r, uint32_t (&x)[kGroups]) {
-      const int i = r < rq ? r : r < rq + rk ? r - rq : r - rq - rk;
-      const uint8_t* src = (r < rq ? qp : r < rq + rk ? kp : vp) + i * 1024;
-      const bool live = 4 * i + sub < (r < rq ? a.num_heads : a.kvh);
+  const int nw = gridDim.x * kWarps;
+  const int64_t unit_step = static_cast<int64_t>(4 * kUnitBytes) << a.upb_log2;  // to the unit of four heads on
+  const uint32_t ring = smem_u32(sm.rows[warp]), tables = smem_u32(sm.table[warp]);
+  auto token_of = [&](int w) { return a.chunks == 1 ? w : quotient(w, a.per_token); };
+
+  // ---- copies ahead: the next round to copy, its item, and the one after that one's position ----
+  int cw = blockIdx.x * kWarps + warp, cr = 0, chi = 0, citem = -1, cstage = 0;
+  int64_t cpos = cw < a.items ? a.positions[token_of(cw)] : 0;
+  int ct = 0, crows = 0;  // rows from the round's first one to the end of its q, k or v heads
+  const uint8_t* csrc = nullptr;  // where this lane's first copy of the round starts
+  bool cnew = true;  // at an item's first round
+  const int crow = kWide ? lane >> 4 : sub, ccol = kWide ? 16 * (lane & 15) : 4 * g;  // of that copy
+  auto at_round = [&] {  // csrc and crows of round cr
+    const bool q = cr < rq, k = cr < rq + rk;
+    const int i = q ? cr : k ? cr - rq : cr - rq - rk;
+    csrc = (q ? a.q + ct * a.q_stride : k ? a.k + ct * a.k_stride : a.v + ct * a.v_stride) + (4 * i + crow) * 256 + ccol;
+    crows = (q ? a.num_heads : a.kvh) - 4 * i;
+  };
+  auto copy_round = [&] {
+    if (cw < a.items) {
+      if (cnew) {
+        ct = token_of(cw);
+        cr = (cw - ct * a.chunks) * a.chunk;
+        chi = min(cr + a.chunk, rounds);
+        ++citem;
+        at_round();
+        if (cr < rq + rk) {
+          int64_t p = cpos;
+          if (p < 0 || p >= a.max_pos) {
+            if (lane == 0 && cr == 0 && a.err) atomicOr(a.err, kErrContextTooLong);
+            p = p < 0 ? 0 : a.max_pos - 1;
+          }
+          const uint32_t to = tables + (citem % (kDepth + 1)) * (2 * kD * 4);
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) x[j] = live ? *reinterpret_cast<const uint32_t*>(src + 32 * j) : 0u;
-    };
-    uint32_t next[kGroups];
-    load(lo, next);
-    const int64_t slot = a.slots[t];
+          for (int h = 0; h < 2; ++h) {
+            const float* row = (h ? a.sin_table : a.cos_table) + p * kD;
+            if (kWide) {
+              cp_async16(to + h * kD * 4 + 16 * lane, row + 4 * lane);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) cp_async4(to + h * kD * 4 + 4 * (lane + 32 * k), row + lane + 32 * k);
+            }
+          }
+        }
+        if (cw + nw < a.items) cpos = a.positions[token_of(cw + nw)];
+      }
+      const uint32_t to = ring + cstage * (4 * kRowPitch) + crow * kRowPitch + ccol;
+      if (kWide) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (crow + 2 * h < crows) cp_async16(to + 2 * h * kRowPitch, csrc + 512 * h);
+      } else if (crow < crows) {
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) cp_async4(to + 32 * j, csrc + 32 * j);
+      }
+      csrc += 1024;
+      crows -= 4;
+      cnew = ++cr == chi;
+      if (cnew) cw += nw;
+      else if (cr == rq || cr == rq + rk) at_round();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");  // empty behind the last round: the waits count groups
+    cstage = cstage + 1 == kDepth ? 0 : cstage + 1;
+  };
+  for (int k = 0; k < kDepth; ++k) copy_round();
+
+  int stage = 0, item = 0;
+  int64_t next_slot = blockIdx.x * kWarps + warp < a.items ? a.slots[token_of(blockIdx.x * kWarps + warp)] : 0;
+  for (int w = blockIdx.x * kWarps + warp; w < a.items; w += nw, ++item) {
+    const int64_t t = token_of(w);
+    const int lo = (w - static_cast<int>(t) * a.chunks) * a.chunk, hi = min(lo + a.chunk, rounds);
+    const int64_t slot = next_slot;
+    if (w + nw < a.items) next_slot = a.slots[token_of(w + nw)];
     const bool slot_ok = slot >= 0 && slot < a.num_slots;
     if (!slot_ok && lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrBadSlot);
     uint8_t* unit = unit_of(a.pool, slot_ok ? slot : 0, sub, a.kvh, a.upb_log2);  // of KV head sub
     const int token = static_cast<int>(slot & 15);
+    uint8_t* q_dst = a.q_out + (t * a.num_heads + sub) * 256 + 4 * g;
     uint64_t cs[kGroups], sn[kGroups], wt[kGroups];  // sn of the lower half negated
-    if (lo < rq + rk) {
-      int64_t p = a.positions[t];
-      if (p < 0 || p >= a.max_pos) {
-        if (lane == 0 && lo == 0 && a.err) atomicOr(a.err, kErrContextTooLong);
-        p = p < 0 ? 0 : a.max_pos - 1;
-      }
-      const float* ct = a.cos_table + p * kD + 2 * g;
-      const float* st = a.sin_table + p * kD + 2 * g;
-#pragma unroll
-      for (int j = 0; j < kGroups; ++j) {
-        const float2 c = *reinterpret_cast<const float2*>(ct + 16 * j), s = *reinterpret_cast<const float2*>(st + 16 * j);
-        cs[j] = bf16x2_to_f32x2(pack_bf16x2(c.x, c.y));
-        sn[j] = bf16x2_to_f32x2(j < 4 ? pack_bf16x2(-s.x, -s.y) : pack_bf16x2(s.x, s.y));
-      }
-    }
-    for (int r = lo; r < hi; ++r) {
-      const bool is_q = r < rq, is_v = r >= rq + rk;
-      const int i = is_q ? r : is_v ? r - rq - rk : r - rq;
-      const bool live = 4 * i + sub < (is_q ? a.num_heads : a.kvh);
-      if (r == lo || r == rq) {
-        const uint8_t* weight = (is_q ? a.q_weight : a.k_weight) + 4 * g;
+    // Round i of the q (kind 0), k (1) or v heads (2).
+    auto round = [&](auto kind, int i, bool first) {
+      constexpr int kKind = decltype(kind)::value;
+      const bool live = 4 * i + sub < (kKind == 0 ? a.num_heads : a.kvh);
+      if (kKind < 2 && (first || i == 0)) {
+        const uint8_t* weight = (kKind == 0 ? a.q_weight : a.k_weight) + 4 * g;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
           wt[j] = bf16x2_to_f32x2(*reinterpret_cast<const uint32_t*>(weight + 32 * j));
       }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      __syncwarp();  // the round's rows, copied by all lanes
       uint32_t x[kGroups];
+      const uint32_t from = ring + stage * (4 * kRowPitch) + sub * kRowPitch + 4 * g;
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) x[j] = next[j];
-      if (r + 1 < hi) load(r + 1, next);
-      if (!is_v) {
-        double ss = 0.0;
+      for (int j = 0; j < kGroups; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[j]) : "r"(from + 32 * j));
+      if (kKind < 2 && first) {
+        const float* row = &sm.table[warp][item % (kDepth + 1)][0][2 * g];
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          const float2 c = *reinterpret_cast<const float2*>(row + 16 * j);
+          const float2 s = *reinterpret_cast<const float2*>(row + kD + 16 * j);
+          cs[j] = bf16x2_to_f32x2(pack_bf16x2(c.x, c.y));
+          sn[j] = bf16x2_to_f32x2(j < 4 ? pack_bf16x2(-s.x, -s.y) : pack_bf16x2(s.x, s.y));
+        }
+      }
+      __syncwarp();  // read by all lanes: the stage may be filled again
+      copy_round();
+      stage = stage + 1 == kDepth ? 0 : stage + 1;
+      if constexpr (kKind < 2) {
+        double part[4] = {0.0, 0.0, 0.0, 0.0};  // four chains
         uint64_t f[kGroups];
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
           const float2 v = pair_to_f32<__nv_bfloat16>(x[j]);
           f[j] = f32x2_pack(v.x, v.y);
           const double d0 = v.x, d1 = v.y;
-          ss = fma(d1, d1, fma(d0, d0, ss));
+          part[j & 3] = fma(d1, d1, fma(d0, d0, part[j & 3]));
         }
+        double ss = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
         for (int off = 1; off < 8; off <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         const float rinv = __frsqrt_rn(static_cast<float>(ss * (1.0 / kD) + static_cast<double>(a.eps)));
@@ -273,27 +353,30 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)  // the norm's bf16 result
           f[j] = bf16x2_to_f32x2(f32x2_to_bf16x2(f32x2_mul(f32x2_mul(f[j], rr), wt[j])));
-          // out[i] = y[i] cos[i] - y[i+64] sin[i];  out[i+64] = y[i+64] cos[i+64] + y[i] sin[i+64]
-          // (products of bf16 are exact in fp32: one rounding each)
+        // out[i] = y[i] cos[i] - y[i+64] sin[i];  out[i+64] = y[i+64] cos[i+64] + y[i] sin[i+64]
+        // (products of bf16 are exact in fp32: one rounding each)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           x[j] = f32x2_to_bf16x2(f32x2_fma(f[j], cs[j], f32x2_mul(f[j + 4], sn[j])));
           x[j + 4] = f32x2_to_bf16x2(f32x2_fma(f[j + 4], cs[j + 4], f32x2_mul(f[j], sn[j + 4])));
         }
       }
-      if (is_q) {
+      if constexpr (kKind == 0) {
+        uint8_t* dst = q_dst + i * 1024;
         if (live) {
-          uint8_t* dst = a.q_out + (t * a.num_heads + 4 * i + sub) * 256 + 4 * g;
 #pragma unroll
           for (int j = 0; j < kGroups; ++j) *reinterpret_cast<uint32_t*>(dst + 32 * j) = x[j];
         }
       } else {
         uint32_t w0, w1, scale;
-        quantise_row<__nv_bfloat16>(x, is_v ? a.v_inv : a.k_inv, g, w0, w1, scale);
-        store_row(unit + static_cast<int64_t>(i) * ((4 * kUnitBytes) << a.upb_log2), token, is_v, live && slot_ok, g,
-                  w0, w1, scale);
+        quantise_row<__nv_bfloat16>(x, kKind == 2 ? a.v_inv : a.k_inv, g, w0, w1, scale);
+        store_row(unit + i * unit_step, token, kKind == 2, live && slot_ok, g, w0, w1, scale);
       }
-    }
+    };
+    int r = lo;
+    for (; r < min(hi, rq); ++r) round(std::integral_constant<int, 0>{}, r, r == lo);
+    for (; r < min(hi, rq + rk); ++r) round(std::integral_constant<int, 1>{}, r - rq, r == lo);
+    for (; r < hi; ++r) round(std::integral_constant<int, 2>{}, r - rq - rk, false);
   }
 }
 
@@ -429,6 +512,8 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   int rc = check_pool(kv_cache, num_blocks, block_size, num_kv_heads, head_dim, k_scale, v_scale, who);
   if (rc != NVK_OK) return rc;
   if (num_tokens == 0) return NVK_OK;
+  if (num_tokens > (int64_t(1) << 30))
+    return fail(NVK_ERR_UNSUPPORTED, "%s: %lld tokens are above the kernel's range", who, (long long)num_tokens);
   if (!query || !key || !value || !q_weight || !k_weight || !cos_table || !sin_table || !positions || !query_out ||
       !slot_mapping)
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
@@ -453,7 +538,6 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   a.slots = slot_mapping;
   a.q_out = static_cast<uint8_t*>(query_out);
   a.pool = static_cast<uint8_t*>(kv_cache);
-  a.num_tokens = num_tokens;
   a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
   a.num_heads = num_heads;
   a.kvh = num_kv_heads;
@@ -466,10 +550,19 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   const int rounds = (num_heads + 3) / 4 + 2 * ((num_kv_heads + 3) / 4);
   // a whole token per warp (cos and sin loaded once) when the tokens alone give every SM 16 warps
   a.chunk = num_tokens >= int64_t(sms) * 16 ? rounds : 1;
-  const int64_t items = num_tokens * ((rounds + a.chunk - 1) / a.chunk);
-  const int64_t want = (items + kWarps - 1) / kWarps;
-  const int64_t most = int64_t(sms) * 2;  // one resident wave: its warps stride over the items
-  return check_cuda(launch_pdl(norm_rope_kernel, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kThreads),
-                               0, reinterpret_cast<cudaStream_t>(stream), a),
+  a.chunks = (rounds + a.chunk - 1) / a.chunk;
+  a.items = static_cast<int>(num_tokens) * a.chunks;
+  a.per_token = divisor(a.chunks);
+  // 16-byte copies where every row and table allows them
+  const bool wide = aligned16(query) && aligned16(key) && aligned16(value) && aligned16(cos_table) &&
+                    aligned16(sin_table) && query_stride % 8 == 0 && key_stride % 8 == 0 && value_stride % 8 == 0;
+  const void* kernel = wide ? reinterpret_cast<const void*>(&norm_rope_kernel<true>)
+                            : reinterpret_cast<const void*>(&norm_rope_kernel<false>);
+  if ((rc = ensure_dynamic_smem(kernel, sizeof(NormSmem))) != NVK_OK) return rc;
+  const int want = (a.items + kWarps - 1) / kWarps, most = sms * 2;  // one resident wave
+  const dim3 grid(want < most ? want : most);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return check_cuda(wide ? launch_pdl(norm_rope_kernel<true>, grid, dim3(kThreads), sizeof(NormSmem), st, a)
+                         : launch_pdl(norm_rope_kernel<false>, grid, dim3(kThreads), sizeof(NormSmem), st, a),
                     "fp4_qk_norm_rope_append launch");
 }
