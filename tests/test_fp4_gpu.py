@@ -192,7 +192,7 @@ def rope_tables(max_pos, theta=1e6):
 
 
 @pytest.mark.parametrize("tokens,h,kvh,bs", [(1, 16, 8, 128), (33, 5, 1, 16), (7, 9, 3, 64), (2500, 4, 2, 32),
-                                              (3000, 7, 1, 128)])
+                                              (3000, 7, 1, 128), (2367, 16, 8, 64), (2368, 4, 1, 16)])
 def test_norm_rope_append_is_exact(cuda_device, tokens, h, kvh, bs):
     dev = cuda_device
     g = torch.Generator().manual_seed(tokens)
@@ -231,6 +231,65 @@ def test_norm_rope_append_bad_slot_and_position(cuda_device):
     assert int(err.item()) == 4 + 8
     _, vr = ops_fp4.kv_read_fp4(pool, torch.arange(32, device=dev))
     assert vr[5].any() and not vr[torch.arange(32) != 5].any()
+
+
+def norm_inputs(dev, tokens, h, kvh, seed):
+    g = torch.Generator().manual_seed(seed)
+    qkv = (torch.randn(tokens, h + 2 * kvh, D, generator=g) * 3).to(torch.bfloat16).to(dev)
+    wq, wk = ((1 + 0.1 * torch.randn(D, generator=g)).to(torch.bfloat16).to(dev) for _ in range(2))
+    pos = torch.randint(0, 512, (tokens,), generator=g).to(dev)
+    slots = torch.randperm(tokens + 7, generator=g)[:tokens].to(dev)
+    pool = torch.zeros(ops_fp4.pool_shape(-(-(tokens + 7) // 32), 32, kvh), dtype=torch.uint8, device=dev)
+    return qkv, wq, wk, pos, slots, pool
+
+
+@pytest.mark.parametrize("tokens", [5, 3001])
+@pytest.mark.parametrize("how", ["rows", "tables", "odd pitch"])
+def test_norm_rope_append_of_rows_with_4_byte_alignment(cuda_device, tokens, how):
+    """Rows, tables or token strides that only 4-byte accesses may take give the same bits."""
+    dev, h, kvh = cuda_device, 6, 3
+    qkv, wq, wk, pos, slots, pool = norm_inputs(dev, tokens, h, kvh, tokens)
+    cos, sin = (t.to(dev) for t in rope_tables(512))
+    split = lambda t: (t[:, :h], t[:, h:h + kvh], t[:, h + kvh:])
+    want = ops_fp4.qk_norm_rope_append_fp4(*split(qkv), wq, wk, 1e-6, cos, sin, pos, pool, slots)
+    width = (h + 2 * kvh) * D
+    if how == "tables":
+        cos, sin = (torch.cat((t.new_zeros(1), t.flatten()))[1:].view(512, D) for t in (cos, sin))
+        assert cos.data_ptr() % 16 == 4
+        rows = qkv
+    else:
+        pitch, first = (width, 2) if how == "rows" else (width + 2, 0)
+        flat = torch.zeros(first + tokens * pitch, dtype=torch.bfloat16, device=dev)
+        rows = flat[first:].as_strided((tokens, h + 2 * kvh, D), (pitch, D, 1), first)
+        rows.copy_(qkv)
+    again = torch.zeros_like(pool)
+    got = ops_fp4.qk_norm_rope_append_fp4(*split(rows), wq, wk, 1e-6, cos, sin, pos, again, slots)
+    assert torch.equal(got.view(torch.int16), want.view(torch.int16)) and torch.equal(again, pool)
+
+
+def test_norm_rope_append_of_special_rows_and_in_place(cuda_device):
+    """A NaN makes its whole row NaN, an infinity its own place (the others are 0), a row of zeros stays one; other
+    rows are not touched by them. The query may be normalised in place."""
+    dev, h, kvh, tokens = cuda_device, 4, 2, 40
+    qkv, wq, wk, pos, slots, pool = norm_inputs(dev, tokens, h, kvh, 3)
+    cos, sin = torch.ones(512, D, device=dev), torch.zeros(512, D, device=dev)  # no rotation: 0 * inf is not asked for
+    qkv[4, 1, 77] = float("nan")
+    qkv[9, h, 3] = float("nan")
+    qkv[11, 0] = 0
+    qkv[12, h + 1] = 0
+    want = orc.norm_rope(qkv[:, :h].float().cpu().numpy(), wq.float().cpu().numpy(), 1e-6, cos[pos].cpu().numpy(),
+                         sin[pos].cpu().numpy())
+    q = qkv[:, :h].contiguous()
+    got = ops_fp4.qk_norm_rope_append_fp4(q, qkv[:, h:h + kvh], qkv[:, h + kvh:], wq, wk, 1e-6, cos, sin, pos, pool,
+                                          slots, query_out=q)
+    assert got.data_ptr() == q.data_ptr()
+    bad = torch.isnan(want)
+    assert bad[4, 1].all() and int(bad.sum()) == D
+    got = got.cpu()
+    assert torch.equal(torch.isnan(got), bad) and torch.equal(got[~bad], want[~bad])
+    kr, vr = ops_fp4.kv_read_fp4(pool, slots)
+    assert torch.isnan(kr[9, 0]).all() and int(torch.isnan(kr).sum()) == D and not torch.isnan(vr).any()
+    assert not kr[12, 1].any() and kr[12, 0].any()
 
 
 # ----------------------------------------------------------------- decode ---
@@ -571,3 +630,47 @@ def test_decode_repeats_bit_for_bit(cuda_device):
         again = torch.empty_like(out)
         ops_fp4.paged_decode_fp4(again, q, pool, tables.to(dev), lens, SCALE, ws)
         assert torch.equal(again, out)
+
+
+def test_two_calls_at_once(cuda_device):
+    """Calls on two streams over one pool, each with a workspace of its own, give what each gives alone."""
+    dev = cuda_device
+    h, kvh, bs, ctx = 8, 2, 64, [5000, 33, 0, 700]
+    nb = sum(-(-n // bs) for n in ctx)
+    pool, _, _ = make_pool(dev, nb, bs, kvh, 11)
+    tables = seeded_tables(ctx, bs, nb, 11).to(dev)
+    lens = torch.tensor(ctx, dtype=torch.int32, device=dev)
+    cu = torch.arange(len(ctx) + 1, dtype=torch.int32, device=dev)
+    g = torch.Generator(device=dev).manual_seed(2)
+    qs = [torch.randn(len(ctx), h, D, generator=g, device=dev).to(torch.bfloat16) for _ in range(2)]
+    streams, spaces = [torch.cuda.Stream(dev) for _ in range(2)], [workspace(dev, h, kvh) for _ in range(2)]
+
+    def calls(i, n):
+        outs = []
+        for _ in range(n):
+            o, p = torch.empty_like(qs[i]), torch.empty_like(qs[i])
+            ops_fp4.paged_decode_fp4(o, qs[i], pool, tables, lens, SCALE, spaces[i])
+            ops_fp4.paged_prefill_fp4(p, qs[i], pool, tables, cu, lens, 1, SCALE)
+            outs += [o, p]
+        return outs
+
+    alone = [calls(i, 1) for i in range(2)]
+    torch.cuda.synchronize(dev)
+    both = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                both[i] += calls(i, 1)
+    torch.cuda.synchronize(dev)
+    for i in range(2):
+        for k, o in enumerate(both[i]):
+            assert torch.equal(o, alone[i][k % 2])
+
+
+def test_query_may_be_overwritten(cuda_device):
+    """out may be the query itself in decode: a row is read before any warp writes it."""
+    dev = cuda_device
+    pool, tables, q, out = decode_case(dev, [3000, 0, 17], 8, 4, 32, seed=9)
+    ops_fp4.paged_decode_fp4(q, q, pool, tables.to(dev), torch.tensor([3000, 0, 17], dtype=torch.int32, device=dev),
+                             SCALE, workspace(dev, 8, 4))
+    assert torch.equal(q, out)
