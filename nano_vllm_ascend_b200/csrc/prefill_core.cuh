@@ -266,30 +266,51 @@ __device__ __forceinline__ void put_chunk(uint32_t tile, int r, int c, uint32_t 
                fp4::hmul2(o[1], s), fp4::hmul2(o[2], s), fp4::hmul2(o[3], s));
 }
 
-// Row r of a Q tile from bf16 to fp16 in place, scaled by 2^-e such that its
-// largest entry lies in [1, 2) (entries 2^14 below it lose bits that a sum of
-// 128 terms does not show); returns e.
+__device__ __forceinline__ uint32_t bf16x2_abs_max(uint32_t a, uint32_t b) {  // (signs mixed; NaN wins)
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Row r of a Q tile from bf16 to fp16 in place, scaled by a power of two:
+// fp16's exponent field is bf16's less f, such that the row's largest entry
+// gets 30, and 10 fraction bits hold bf16's 7. Entries 2^29 below the largest
+// become 0 or a wrong subnormal, which a sum of 128 terms does not show.
+// Returns the log2 of what the row's scores have to be multiplied by, f - 112.
 __device__ __forceinline__ int q_row_to_half(uint32_t tile, int r) {
   auto chunk = [&](int c) { return tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
-  uint32_t big = 0;  // bf16 magnitudes order as integers
+  uint32_t big = 0;
 #pragma unroll 4
   for (int c = 0; c < 16; ++c) {
     const uint4 v = ld_shared_v4(chunk(c));
-    big = __vmaxu2(__vmaxu2(big, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)),
-                   __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    big = bf16x2_abs_max(bf16x2_abs_max(big, bf16x2_abs_max(v.x, v.y)), bf16x2_abs_max(v.z, v.w));
   }
-  const int e = min(max(static_cast<int>(max(big & 0xffffu, big >> 16) >> 7), 27), 227) - 127;  // within 2^+-100
-  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  auto half = [&](uint32_t w) {
-    const __half2 h = __floats2half2_rn(bf16lo_to_f32(w) * down, bf16hi_to_f32(w) * down);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  };
-#pragma unroll 4
-  for (int c = 0; c < 16; ++c) {
-    const uint4 v = ld_shared_v4(chunk(c));
-    st_shared_v4(chunk(c), half(v.x), half(v.y), half(v.z), half(v.w));
+  const int top = static_cast<int>(max(big & 0x7fffu, (big >> 16) & 0x7fffu) >> 7);
+  const int f = min(max(top, 30), 254) - 30;
+  if (top == 255) {  // an infinity or a NaN: it has to stay one
+    const float down = __uint_as_float(static_cast<uint32_t>(127 + 112 - f) << 23);
+    auto half = [&](uint32_t w) { return pack_half2(bf16lo_to_f32(w) * down, bf16hi_to_f32(w) * down); };
+#pragma unroll 1
+    for (int c = 0; c < 16; ++c) {
+      const uint4 v = ld_shared_v4(chunk(c));
+      st_shared_v4(chunk(c), half(v.x), half(v.y), half(v.z), half(v.w));
+    }
+  } else {
+    const uint32_t base = static_cast<uint32_t>(f) * 0x00800080u;
+    auto half = [&](uint32_t w) {
+      return ((__vmaxu2(w & 0x7fff7fffu, base) - base) << 3) | (w & 0x80008000u);
+    };
+#pragma unroll 1
+    for (int c0 = 0; c0 < 16; c0 += 4) {
+      uint4 v[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = ld_shared_v4(chunk(c0 + c));
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        st_shared_v4(chunk(c0 + c), half(v[c].x), half(v[c].y), half(v[c].z), half(v[c].w));
+    }
   }
-  return e;
+  return f - 112;
 }
 
 __device__ __forceinline__ void decode_row(const KRow& k, uint32_t tile, int r) {
@@ -397,6 +418,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         }
     };
     int w = blockIdx.x, qi = 0, g = 0, k_issued = 0, v_issued = 0;
+    int q_extra = 0;  // streams that have a load of item qi, where that is not all of them
     bool ok = true;
     while (true) {
       Item it;
@@ -408,18 +430,20 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         // the slot before that wait: its last user, four items back, was done
         // when the last S of the item before the previous one had completed,
         // for which this loop has waited already.
-        auto q_free = [&] {
+        if (!kFp4)
           for (int s = 0; s < ns && ok && qi > 0; ++s)
             if (!mbar_wait(&sm.q_empty[s], (qi - 1) & 1)) ok = false;
-        };
-        if (!kFp4) q_free();
         Item& slot = sm.items[qi % kItemRing];
         slot = it;
         if (!have || !ok) slot.n_kv = -1;
         mbar_arrive(&sm.item_full[qi % kItemRing]);
-        if (kFp4 && have) q_free();
         if (have && ok) {
           for (int s = 0; s < ns; ++s) {
+            if (kFp4 && qi > 0 && !mbar_wait(&sm.q_empty[s], (qi - 1) & 1)) {
+              ok = false;
+              q_extra = s;
+              break;
+            }
             mbar_arrive_expect_tx(&sm.q_full[s], kTileBytes);
             tma_load_3d(sm.q[s], &qmap, &sm.q_full[s], 0, it.h0 + s, it.q0 + it.qt * kRows);
             tma_load_3d(sm.q[s] + kHalfBytes, &qmap, &sm.q_full[s], 64, it.h0 + s, it.q0 + it.qt * kRows);
@@ -481,7 +505,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       // reloaded only after its previous load was consumed, so only the last
       // load of each stream can be in flight).
       for (int s = 0; s < ns; ++s)
-        if (qi > 0) (void)mbar_wait(&sm.q_full[s], (qi - 1) & 1);
+        if (const int loads = qi + (s < q_extra ? 1 : 0); loads > 0) (void)mbar_wait(&sm.q_full[s], (loads - 1) & 1);
       for (int j = max(0, k_issued - kStages); j < k_issued; ++j)
         (void)mbar_wait(&sm.full_k[j % kStages], (j / kStages) & 1);
       for (int j = max(0, v_issued - kStages); j < v_issued; ++j)
@@ -500,29 +524,32 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       if (elect_one_sync()) umma_commit(bar);
       __syncwarp();
     };
+    // One elected thread issues a whole product (electing for every step makes
+    // the code several times as long). Steps move the descriptors' address
+    // field, in units of 16 bytes.
     auto issue_s = [&](int s, int st) {  // S_s = Q_s K(stage st)^T
-      const uint32_t q_addr = smem_u32(sm.q[s]);
-      const uint32_t k_addr = smem_u32(sm.k[st]);
+      if (elect_one_sync()) {
+        const uint64_t qa = smem_desc_sw128(smem_u32(sm.q[s]), 16, 1024);
+        const uint64_t kb = smem_desc_sw128(smem_u32(sm.k[st]), 16, 1024);
 #pragma unroll
-      for (int kk = 0; kk < kD / 16; ++kk) {
-        const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-        const uint64_t qa = smem_desc_sw128(q_addr + off, 16, 1024);
-        const uint64_t kb = smem_desc_sw128(k_addr + off, 16, 1024);
-        if (elect_one_sync()) umma_f16_ss(tmem + s * kKeys, qa, kb, idesc_qk, kk > 0);
-        __syncwarp();
+        for (int kk = 0; kk < kD / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
+          umma_f16_ss(tmem + s * kKeys, qa + off, kb + off, idesc_qk, kk > 0);
+        }
+        umma_commit(&sm.s_full[s]);
       }
-      commit(&sm.s_full[s]);
+      __syncwarp();
     };
     // O_s (+)= P_s V(stage st) over the keys of 16-key steps kk0 .. kk0 + 3
     auto issue_pv = [&](int s, int st, int kk0, bool first) {
-      const uint32_t v_addr = smem_u32(sm.v[st]);
+      if (elect_one_sync()) {
+        const uint64_t vb = smem_desc_sw128(smem_u32(sm.v[st]), kHalfBytes, 1024);
 #pragma unroll
-      for (int kk = kk0; kk < kk0 + 4; ++kk) {
-        const uint64_t vb = smem_desc_sw128(v_addr + kk * 16 * 128, kHalfBytes, 1024);
-        if (elect_one_sync())
-          umma_f16_ts(tmem + kColO + s * kD, tmem + s * kKeys + kk * 8, vb, idesc_pv, (!first || kk > 0) ? 1u : 0u);
-        __syncwarp();
+        for (int kk = kk0; kk < kk0 + 4; ++kk)
+          umma_f16_ts(tmem + kColO + s * kD, tmem + s * kKeys + kk * 8, vb + kk * (16 * 128 >> 4), idesc_pv,
+                      (!first || kk > 0) ? 1u : 0u);
       }
+      __syncwarp();
     };
     int qi = 0, g = 0;
     while (ok) {
@@ -621,13 +648,11 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       const uint8_t* unit = unit_at(0);
       load_row(k, unit, i);
       load_row(v, unit, i);
-      auto q_to_half = [&] {
-        for (int s = 0; s < ns; ++s) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full[s], qi & 1))) return false;
-          sm.q_exp[qi & 1][s][r] = static_cast<int8_t>(q_row_to_half(smem_u32(sm.q[s]), r));
-          fence_proxy_async_smem();
-          mbar_arrive(&sm.q_ready[s]);
-        }
+      auto q_to_half = [&](int s) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full[s], qi & 1))) return false;
+        sm.q_exp[qi & 1][s][r] = static_cast<int8_t>(q_row_to_half(smem_u32(sm.q[s]), r));
+        fence_proxy_async_smem();
+        mbar_arrive(&sm.q_ready[s]);
         return true;
       };
       for (int j = 0; j < it.n_kv; ++j, ++g) {
@@ -640,13 +665,15 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_k[st]);
         load_row(k, unit, i);
+        // Q_0 before V: with K it is what the item's first scores wait for; Q_1 arrives half a tile later
+        if (j == 0 && !q_to_half(0)) { ok = false; break; }
         if (g >= kStages && !mbar_wait(&sm.v_empty[st], parity)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         decode_row(v, smem_u32(sm.v[st]), r);
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_v[st]);
         load_row(v, unit, i);
-        if (j == 0 && !q_to_half()) { ok = false; break; }
+        if (j == 0 && ns > 1 && !q_to_half(1)) { ok = false; break; }
       }
       ++qi;
     }
@@ -683,10 +710,25 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           sc = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + sm.q_exp[qi & 1][s][r]) << 23);
         const int kbase = j * kKeys;
         uint32_t sr[4][32];
+        // The 4-bit kernel masks in tensor memory, in a loop: masking all of the row's registers at once is code that
+        // runs once an item, and fetching it took longer (the instruction caches are full of the decoders' code).
+        if (kFp4 && __any_sync(0xffffffffu, kbase + kKeys - 1 > lim)) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int seen = lim - kbase - c * 32;  // the chunk's columns up to this one are seen
+            tmem_ld32(tmem_s + c * 32, sr[0]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e > seen) sr[0][e] = __float_as_uint(-INFINITY);
+            tmem_st32(tmem_s + c * 32, sr[0]);
+          }
+          tmem_st_wait();
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + c * 32, sr[c]);
         tmem_ld_wait();
-        if (kbase + kKeys - 1 > lim) {
+        if (!kFp4 && kbase + kKeys - 1 > lim) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -764,11 +806,13 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       const int row0 = (warp & 3) * 32;
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-#pragma unroll 1
+        uint32_t both[2][32];
+        tmem_ld32(tmem_o + h * 64, both[0]);
+        tmem_ld32(tmem_o + h * 64 + 32, both[1]);
+        tmem_ld_wait();
+#pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t o[32];
-          tmem_ld32(tmem_o + h * 64 + c * 32, o);
-          tmem_ld_wait();
+          const uint32_t(&o)[32] = both[c];
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
             const uint32_t x = pack_bf16x2(__uint_as_float(o[q4 * 8 + 0]) * inv, __uint_as_float(o[q4 * 8 + 1]) * inv);
@@ -784,15 +828,20 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           mbar_arrive(&sm.o_free[s]);
         }
         __syncwarp();  // this warp's 32 row halves are in stage[s]
-#pragma unroll 4
+        uint4 out[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int row = row0 + k * 4 + (lane >> 3), c16 = lane & 7;
+          out[k] = ld_shared_v4(smem_u32(stage + row * 128 + ((c16 ^ (row & 7)) << 4)));
+        }
+#pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int row = row0 + k * 4 + (lane >> 3), c16 = lane & 7;
           if (row < rows) {
-            const uint4 v4 = ld_shared_v4(smem_u32(stage + row * 128 + ((c16 ^ (row & 7)) << 4)));
             __nv_bfloat16* dst = a.out +
                                  (static_cast<int64_t>(it.q0 + it.qt * kRows + row) * a.num_heads + it.h0 + s) * kD +
                                  h * 64 + c16 * 8;
-            *reinterpret_cast<uint4*>(dst) = v4;
+            *reinterpret_cast<uint4*>(dst) = out[k];
           }
         }
         __syncwarp();  // read out before the next half overwrites the rows
