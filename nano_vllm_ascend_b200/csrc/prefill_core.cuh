@@ -128,7 +128,6 @@ struct PrefillSmem {
   uint64_t item_full[kItemRing];                 // items[i % ring] written (one phase per use)
   uint64_t q_full[kStreams], q_empty[kStreams];  // one phase per item
   uint64_t q_ready[kStreams];                    // 4-bit pool: Q_s is fp16 (one phase per item)
-  int8_t q_exp[2][kStreams][kRows];              // and was scaled by 2^-this (even and odd items)
   uint64_t full_k[kStages], k_empty[kStages];
   uint64_t full_v[kStages], v_empty[kStages];
   uint64_t s_full[kStreams];   // S_s(j) in TMEM (and, in issue order, P V_s(j-1) done)
@@ -276,41 +275,36 @@ __device__ __forceinline__ uint32_t bf16x2_abs_max(uint32_t a, uint32_t b) {  //
 // fp16's exponent field is bf16's less f, such that the row's largest entry
 // gets 30, and 10 fraction bits hold bf16's 7. Entries 2^29 below the largest
 // become 0 or a wrong subnormal, which a sum of 128 terms does not show.
-// Returns the log2 of what the row's scores have to be multiplied by, f - 112.
-__device__ __forceinline__ int q_row_to_half(uint32_t tile, int r) {
+// Returns what the row's scores have to be multiplied by, 2^(f - 112), or NaN
+// for a row with a NaN or an infinity (whose softmax is NaN everywhere). Short
+// loops: fetching this code, once an item, costs as much as running it.
+__device__ __forceinline__ float q_row_to_half(uint32_t tile, int r) {
   auto chunk = [&](int c) { return tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+  constexpr int kN = 4;  // chunks a step
   uint32_t big = 0;
-#pragma unroll 4
-  for (int c = 0; c < 16; ++c) {
-    const uint4 v = ld_shared_v4(chunk(c));
-    big = bf16x2_abs_max(bf16x2_abs_max(big, bf16x2_abs_max(v.x, v.y)), bf16x2_abs_max(v.z, v.w));
-  }
+#pragma unroll 1
+  for (int c0 = 0; c0 < 16; c0 += kN)
+#pragma unroll
+    for (int c = 0; c < kN; ++c) {
+      const uint4 v = ld_shared_v4(chunk(c0 + c));
+      big = bf16x2_abs_max(bf16x2_abs_max(big, bf16x2_abs_max(v.x, v.y)), bf16x2_abs_max(v.z, v.w));
+    }
   const int top = static_cast<int>(max(big & 0x7fffu, (big >> 16) & 0x7fffu) >> 7);
-  const int f = min(max(top, 30), 254) - 30;
-  if (top == 255) {  // an infinity or a NaN: it has to stay one
-    const float down = __uint_as_float(static_cast<uint32_t>(127 + 112 - f) << 23);
-    auto half = [&](uint32_t w) { return pack_half2(bf16lo_to_f32(w) * down, bf16hi_to_f32(w) * down); };
+  const int f = max(top, 30) - 30;
+  const uint32_t base = static_cast<uint32_t>(f) * 0x00800080u;
+  auto half = [&](uint32_t w) {
+    uint32_t m;  // of bf16 magnitudes
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w & 0x7fff7fffu), "r"(base));
+    return ((m - base) << 3) | (w & 0x80008000u);
+  };
 #pragma unroll 1
-    for (int c = 0; c < 16; ++c) {
-      const uint4 v = ld_shared_v4(chunk(c));
-      st_shared_v4(chunk(c), half(v.x), half(v.y), half(v.z), half(v.w));
-    }
-  } else {
-    const uint32_t base = static_cast<uint32_t>(f) * 0x00800080u;
-    auto half = [&](uint32_t w) {
-      return ((__vmaxu2(w & 0x7fff7fffu, base) - base) << 3) | (w & 0x80008000u);
-    };
-#pragma unroll 1
-    for (int c0 = 0; c0 < 16; c0 += 4) {
-      uint4 v[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = ld_shared_v4(chunk(c0 + c));
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        st_shared_v4(chunk(c0 + c), half(v[c].x), half(v[c].y), half(v[c].z), half(v[c].w));
-    }
+  for (int c0 = 0; c0 < 16; c0 += 2) {
+    const uint32_t at0 = chunk(c0), at1 = chunk(c0 + 1);
+    const uint4 u = ld_shared_v4(at0), v = ld_shared_v4(at1);
+    st_shared_v4(at0, half(u.x), half(u.y), half(u.z), half(u.w));
+    st_shared_v4(at1, half(v.x), half(v.y), half(v.z), half(v.w));
   }
-  return f - 112;
+  return __uint_as_float(top == 255 ? 0x7fffffffu : static_cast<uint32_t>(127 - 112 + f) << 23);
 }
 
 __device__ __forceinline__ void decode_row(const KRow& k, uint32_t tile, int r) {
@@ -373,7 +367,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     }
     for (int s = 0; s < kStreams; ++s) {
       mbar_init(&sm.q_full[s], 1);
-      mbar_init(&sm.q_ready[s], 128);
+      mbar_init(&sm.q_ready[s], kStreamThreads);
       mbar_init(&sm.q_empty[s], 1);
       mbar_init(&sm.s_full[s], 1);
       mbar_init(&sm.p_lo[s], kStreamThreads);
@@ -648,13 +642,6 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       const uint8_t* unit = unit_at(0);
       load_row(k, unit, i);
       load_row(v, unit, i);
-      auto q_to_half = [&](int s) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full[s], qi & 1))) return false;
-        sm.q_exp[qi & 1][s][r] = static_cast<int8_t>(q_row_to_half(smem_u32(sm.q[s]), r));
-        fence_proxy_async_smem();
-        mbar_arrive(&sm.q_ready[s]);
-        return true;
-      };
       for (int j = 0; j < it.n_kv; ++j, ++g) {
         const int st = g % kStages;
         unit = j + 1 < it.n_kv ? unit_at(j + 1) : nullptr;
@@ -665,15 +652,12 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_k[st]);
         load_row(k, unit, i);
-        // Q_0 before V: with K it is what the item's first scores wait for; Q_1 arrives half a tile later
-        if (j == 0 && !q_to_half(0)) { ok = false; break; }
         if (g >= kStages && !mbar_wait(&sm.v_empty[st], parity)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         decode_row(v, smem_u32(sm.v[st]), r);
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_v[st]);
         load_row(v, unit, i);
-        if (j == 0 && ns > 1 && !q_to_half(1)) { ok = false; break; }
       }
       ++qi;
     }
@@ -690,12 +674,27 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     uint8_t* stage = sm.stage[s];
     int qi = 0, g = 0;
     bool ok = true;
+    Item it;
+    // Item n's descriptor and, in the 4-bit kernel, this thread's row of its
+    // Q, which becomes fp16 here, between an item's last P and its O: these
+    // warps are eight, and have nothing to do while the last P V runs.
+    auto begin_item = [&](int n) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&sm.item_full[n % kItemRing], (n / kItemRing) & 1))) return false;
+      it = sm.items[n % kItemRing];
+      if (kFp4 && it.n_kv > 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full[s], n & 1))) return false;
+        sc = a.scale_log2 * q_row_to_half(smem_u32(sm.q[s]), r);
+        fence_proxy_async_smem();
+        mbar_arrive(&sm.q_ready[s]);
+      }
+      return true;
+    };
+    if (kFp4) ok = begin_item(0);
     while (ok) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&sm.item_full[qi % kItemRing], (qi / kItemRing) & 1))) {
+      if (!kFp4 && !begin_item(qi)) {
         ok = false;
         break;
       }
-      const Item it = sm.items[qi % kItemRing];
       if (it.n_kv < 0) break;
       const int i = it.qt * kRows + r;
       const int lim = (i < it.lq) ? (it.lk - it.lq + i) : (it.lk - 1);
@@ -704,10 +703,6 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         // warp-uniform outcome: the tcgen05.ld/st below need a converged warp
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[s], g & 1))) { ok = false; break; }
         tc_fence_after();
-        // S_s(0) came of Q_s, which was ready after its exponents were stored
-        // (q_ready itself may be two items on when this warp gets here)
-        if (kFp4 && j == 0)
-          sc = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + sm.q_exp[qi & 1][s][r]) << 23);
         const int kbase = j * kKeys;
         uint32_t sr[4][32];
         // The 4-bit kernel masks in tensor memory, in a loop: masking all of the row's registers at once is code that
@@ -793,58 +788,50 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         mbar_arrive(&sm.p_hi[s]);
       }
       if (!ok) break;
+      const int rows = min(kRows, it.lq - it.qt * kRows);
+      __nv_bfloat16* out = a.out + (static_cast<int64_t>(it.q0 + it.qt * kRows) * a.num_heads + it.h0 + s) * kD;
+      if (kFp4 && !begin_item(qi + 1)) {
+        ok = false;
+        break;
+      }
       // The item's last P V_s complete: normalise the O_s rows and store them
-      // through stage[s], one 64-dim half at a time: thread r writes its row
-      // half there (16-byte chunk c of row r at chunk c ^ (r % 8): conflict
-      // free), then its warp stores the 32 row halves its lanes wrote, four
-      // whole 128-byte row halves per instruction, so the global writes are
+      // through stage[s], 32 dims at a time (its two halves in turn): thread r
+      // writes its row's 64 bytes there (16-byte chunk c of row r at chunk
+      // c ^ (r / 2 % 4): conflict free), then its warp stores the 32 pieces
+      // that its lanes wrote, eight per instruction, so the global writes are
       // coalesced and no warp waits for another.
       if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_ready[s], qi & 1))) { ok = false; break; }
       tc_fence_after();
       const float inv = kFp4 ? (l == 0.f ? 0.f : a.out_scale / l) : (l > 0.f ? 1.f / l : 0.f);
-      const int rows = min(kRows, it.lq - it.qt * kRows);
-      const int row0 = (warp & 3) * 32;
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        uint32_t both[2][32];
-        tmem_ld32(tmem_o + h * 64, both[0]);
-        tmem_ld32(tmem_o + h * 64 + 32, both[1]);
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tmem_o + c * 32, o);
         tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t(&o)[32] = both[c];
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const uint32_t x = pack_bf16x2(__uint_as_float(o[q4 * 8 + 0]) * inv, __uint_as_float(o[q4 * 8 + 1]) * inv);
-            const uint32_t y = pack_bf16x2(__uint_as_float(o[q4 * 8 + 2]) * inv, __uint_as_float(o[q4 * 8 + 3]) * inv);
-            const uint32_t z = pack_bf16x2(__uint_as_float(o[q4 * 8 + 4]) * inv, __uint_as_float(o[q4 * 8 + 5]) * inv);
-            const uint32_t u = pack_bf16x2(__uint_as_float(o[q4 * 8 + 6]) * inv, __uint_as_float(o[q4 * 8 + 7]) * inv);
-            const int chunk = c * 4 + q4;
-            st_shared_v4(smem_u32(stage + r * 128 + ((chunk ^ (r & 7)) << 4)), x, y, z, u);
-          }
-        }
-        if (h == 1) {  // O_s is read out: the next item's first P V_s may overwrite it
+        if (c == 3) {  // O_s is read out: the next item's first P V_s may overwrite it
           tc_fence_before();
           mbar_arrive(&sm.o_free[s]);
         }
-        __syncwarp();  // this warp's 32 row halves are in stage[s]
-        uint4 out[8];
+        const uint32_t half = smem_u32(stage + (c & 1) * (kRows * 64));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int row = row0 + k * 4 + (lane >> 3), c16 = lane & 7;
-          out[k] = ld_shared_v4(smem_u32(stage + row * 128 + ((c16 ^ (row & 7)) << 4)));
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const uint32_t x = pack_bf16x2(__uint_as_float(o[q4 * 8 + 0]) * inv, __uint_as_float(o[q4 * 8 + 1]) * inv);
+          const uint32_t y = pack_bf16x2(__uint_as_float(o[q4 * 8 + 2]) * inv, __uint_as_float(o[q4 * 8 + 3]) * inv);
+          const uint32_t z = pack_bf16x2(__uint_as_float(o[q4 * 8 + 4]) * inv, __uint_as_float(o[q4 * 8 + 5]) * inv);
+          const uint32_t u = pack_bf16x2(__uint_as_float(o[q4 * 8 + 6]) * inv, __uint_as_float(o[q4 * 8 + 7]) * inv);
+          st_shared_v4(half + r * 64 + ((q4 ^ ((r >> 1) & 3)) << 4), x, y, z, u);
         }
+        __syncwarp();  // this warp's pieces are in this half, and the ones before them out of the other
+        uint4 v[4];
+        const int row0 = (warp & 3) * 32 + (lane >> 2), c16 = lane & 3;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int row = row0 + k * 4 + (lane >> 3), c16 = lane & 7;
-          if (row < rows) {
-            __nv_bfloat16* dst = a.out +
-                                 (static_cast<int64_t>(it.q0 + it.qt * kRows + row) * a.num_heads + it.h0 + s) * kD +
-                                 h * 64 + c16 * 8;
-            *reinterpret_cast<uint4*>(dst) = out[k];
-          }
-        }
-        __syncwarp();  // read out before the next half overwrites the rows
+        for (int k = 0; k < 4; ++k)
+          v[k] = ld_shared_v4(half + (row0 + 8 * k) * 64 + ((c16 ^ ((row0 >> 1) & 3)) << 4));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (row0 + 8 * k < rows)
+            *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + 8 * k) * a.num_heads * kD + c * 32 + c16 * 8) =
+                v[k];
       }
       if (!ok) break;
       ++qi;
