@@ -291,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_kernel(const NormArgs a
     asm volatile("cp.async.commit_group;" ::: "memory");  // empty behind the last round: the waits count groups
     cstage = cstage + 1 == kDepth ? 0 : cstage + 1;
   };
+#pragma unroll 1  // (one copy of the code: 0.3 us of 36, 0.13 of 2.8)
   for (int k = 0; k < kDepth; ++k) copy_round();
 
   int stage = 0, item = 0;
