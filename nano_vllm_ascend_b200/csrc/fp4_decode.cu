@@ -12,9 +12,11 @@
 // K and V enter as e2m1 -> fp16 (one conversion for two values): exact. K's
 // scales multiply the fp32 sums of their groups, V's the weights: P s is
 // rounded to fp16 twice (P, then the product: 2^-10 of a weight), with 2^4 p s
-// normal down to 2^-18. Q is scaled by a power of two into fp16's range
-// (entries 2^14 below the row's largest lose bits that a sum of 128 terms does
-// not show). Scores, maxima, sums and O are fp32.
+// normal down to 2^-18. Q is scaled by a power of two into fp16's range, which
+// holds its 8 bits exactly. Scores, maxima, sums and O are fp32; the last
+// division is a product with an approximate reciprocal (2^-21, below bf16's
+// half step of 2^-8; the exact one is 2 KB of code, and code that runs once
+// costs its fetch).
 //
 // Data: every warp streams its tiles (two units, 32 tokens) through a ring of
 // its own in shared memory, one bulk copy of 4608 contiguous bytes a tile (two
@@ -145,25 +147,18 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
 #pragma unroll
   for (int j = 0; j < kGroups; ++j)
     raw[j] = live ? *reinterpret_cast<const uint2*>(row + 16 * j) : make_uint2(0, 0);
-  // the row's largest exponent: bf16 magnitudes order as integers
   uint32_t big = 0;
 #pragma unroll
-  for (int j = 0; j < kGroups; ++j) {
-    big = max(big, max(raw[j].x & 0x7fffu, (raw[j].x >> 16) & 0x7fffu));
-    big = max(big, max(raw[j].y & 0x7fffu, (raw[j].y >> 16) & 0x7fffu));
-  }
-  big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-  big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-  const int e = min(max(static_cast<int>(big >> 7), 27), 227) - 127;  // within 2^+-100
-  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+  for (int j = 0; j < kGroups; ++j) big = bf16x2_abs_max(big, bf16x2_abs_max(raw[j].x, raw[j].y));
+  big = bf16x2_abs_max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+  big = bf16x2_abs_max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+  const HalfRow half = half_row(big);
 #pragma unroll
-  for (int j = 0; j < kGroups; ++j) {
-    st_shared_v2(st.q + 512 * (j >> 1) + 8 * (j & 1), half2_of(bf16lo_to_f32(raw[j].x) * down, bf16hi_to_f32(raw[j].x) * down),
-                 half2_of(bf16lo_to_f32(raw[j].y) * down, bf16hi_to_f32(raw[j].y) * down));
-  }
-  st.sc[0] = __shfl_sync(0xffffffffu, up, 8 * t) * a.scale_log2;
-  st.sc[1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * a.scale_log2;
+  for (int j = 0; j < kGroups; ++j)
+    st_shared_v2(st.q + 512 * (j >> 1) + 8 * (j & 1), bf16x2_to_half2(raw[j].x, half.base),
+                 bf16x2_to_half2(raw[j].y, half.base));
+  st.sc[0] = __shfl_sync(0xffffffffu, half.up, 8 * t) * a.scale_log2;
+  st.sc[1] = __shfl_sync(0xffffffffu, half.up, 8 * t + 4) * a.scale_log2;
   st.ref[0] = st.ref[1] = 0.f;
   st.thr[0] = st.thr[1] = -INFINITY;
   st.l[0] = st.l[1] = 0.f;
@@ -431,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
       const int head = 2 * t + e;
       if (head >= a.group) continue;
       if (whole) {
-        const float inv = st.l[e] == 0.f ? 0.f : a.v_scale / st.l[e];
+        const float inv = st.l[e] == 0.f ? 0.f : __fdividef(a.v_scale, st.l[e]);
         __nv_bfloat16* row = a.out + (static_cast<int64_t>(b) * a.heads + h * a.group + head) * kD + 2 * g;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
@@ -556,7 +551,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
   // it had), piece 2 w + 1 of one that goes on behind it. A run of pieces of
   // one pair is its first one and then pieces 2 w of the warps after that.
   auto write_out = [&](int pair, int head, float l, const float4& o) {
-    const float inv = l == 0.f ? 0.f : a.v_scale / l;
+    const float inv = l == 0.f ? 0.f : __fdividef(a.v_scale, l);
     const int pb = pair / a.kvh, ph = pair - pb * a.kvh;
     *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
         make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));

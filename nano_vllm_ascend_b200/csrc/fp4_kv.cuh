@@ -94,6 +94,31 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   return r;
 }
 
+// Q for the tensor cores: a row from bf16 to fp16, scaled by a power of two.
+// fp16's exponent field is bf16's less f, such that the row's largest entry
+// gets 30, and 10 fraction bits hold bf16's 7. Entries 2^29 below the largest
+// become 0 or a wrong subnormal, which a sum of 128 terms does not show.
+__device__ __forceinline__ uint32_t bf16x2_abs_max(uint32_t a, uint32_t b) {  // (signs mixed; NaN wins)
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+struct HalfRow {
+  uint32_t base;  // f in both exponent fields
+  float up;       // what the row's scores have to be multiplied by: 2^(f - 112), or NaN for a row with a
+                  // NaN or an infinity (whose softmax is NaN everywhere)
+};
+__device__ __forceinline__ HalfRow half_row(uint32_t largest) {  // the bf16x2_abs_max of the row's pairs
+  const uint32_t top = max(largest & 0x7fffu, (largest >> 16) & 0x7fffu) >> 7;
+  const uint32_t f = max(top, 30u) - 30u;
+  return HalfRow{f * 0x00800080u, __uint_as_float(top == 255u ? 0x7fffffffu : (127u - 112u + f) << 23)};
+}
+__device__ __forceinline__ uint32_t bf16x2_to_half2(uint32_t w, uint32_t base) {
+  uint32_t m;  // of magnitudes
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w & 0x7fff7fffu), "r"(base));
+  return ((m - base) << 3) | (w & 0x80008000u);
+}
+
 // A pair of 16-bit floats to fp32, and back.
 template <typename T>
 __device__ __forceinline__ float2 pair_to_f32(uint32_t w);

@@ -265,38 +265,22 @@ __device__ __forceinline__ void put_chunk(uint32_t tile, int r, int c, uint32_t 
                fp4::hmul2(o[1], s), fp4::hmul2(o[2], s), fp4::hmul2(o[3], s));
 }
 
-__device__ __forceinline__ uint32_t bf16x2_abs_max(uint32_t a, uint32_t b) {  // (signs mixed; NaN wins)
-  uint32_t r;
-  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
-// Row r of a Q tile from bf16 to fp16 in place, scaled by a power of two:
-// fp16's exponent field is bf16's less f, such that the row's largest entry
-// gets 30, and 10 fraction bits hold bf16's 7. Entries 2^29 below the largest
-// become 0 or a wrong subnormal, which a sum of 128 terms does not show.
-// Returns what the row's scores have to be multiplied by, 2^(f - 112), or NaN
-// for a row with a NaN or an infinity (whose softmax is NaN everywhere). Short
-// loops: fetching this code, once an item, costs as much as running it.
+// Row r of a Q tile from bf16 to fp16 in place (see fp4_kv.cuh); returns what
+// its scores have to be multiplied by. Short loops: fetching this code, once an
+// item, costs as much as running it.
 __device__ __forceinline__ float q_row_to_half(uint32_t tile, int r) {
   auto chunk = [&](int c) { return tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
-  constexpr int kN = 4;  // chunks a step
   uint32_t big = 0;
 #pragma unroll 1
-  for (int c0 = 0; c0 < 16; c0 += kN)
+  for (int c0 = 0; c0 < 16; c0 += 4)
 #pragma unroll
-    for (int c = 0; c < kN; ++c) {
+    for (int c = 0; c < 4; ++c) {
       const uint4 v = ld_shared_v4(chunk(c0 + c));
-      big = bf16x2_abs_max(bf16x2_abs_max(big, bf16x2_abs_max(v.x, v.y)), bf16x2_abs_max(v.z, v.w));
+      big = fp4::bf16x2_abs_max(fp4::bf16x2_abs_max(big, fp4::bf16x2_abs_max(v.x, v.y)),
+                                fp4::bf16x2_abs_max(v.z, v.w));
     }
-  const int top = static_cast<int>(max(big & 0x7fffu, (big >> 16) & 0x7fffu) >> 7);
-  const int f = max(top, 30) - 30;
-  const uint32_t base = static_cast<uint32_t>(f) * 0x00800080u;
-  auto half = [&](uint32_t w) {
-    uint32_t m;  // of bf16 magnitudes
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w & 0x7fff7fffu), "r"(base));
-    return ((m - base) << 3) | (w & 0x80008000u);
-  };
+  const fp4::HalfRow row = fp4::half_row(big);
+  auto half = [&](uint32_t w) { return fp4::bf16x2_to_half2(w, row.base); };
 #pragma unroll 1
   for (int c0 = 0; c0 < 16; c0 += 2) {
     const uint32_t at0 = chunk(c0), at1 = chunk(c0 + 1);
@@ -304,7 +288,7 @@ __device__ __forceinline__ float q_row_to_half(uint32_t tile, int r) {
     st_shared_v4(at0, half(u.x), half(u.y), half(u.z), half(u.w));
     st_shared_v4(at1, half(v.x), half(v.y), half(v.z), half(v.w));
   }
-  return __uint_as_float(top == 255 ? 0x7fffffffu : static_cast<uint32_t>(127 - 112 + f) << 23);
+  return row.up;
 }
 
 __device__ __forceinline__ void decode_row(const KRow& k, uint32_t tile, int r) {

@@ -674,3 +674,37 @@ def test_query_may_be_overwritten(cuda_device):
     ops_fp4.paged_decode_fp4(q, q, pool, tables.to(dev), torch.tensor([3000, 0, 17], dtype=torch.int32, device=dev),
                              SCALE, workspace(dev, 8, 4))
     assert torch.equal(q, out)
+
+
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+def test_queries_of_any_magnitude(cuda_device, which):
+    """Queries far from 1 (the scale undoes it), rows whose entries span 2^24, rows of zeros, and rows with a NaN or an
+    infinity, which come out as NaN and leave the others alone. Heads are rows of one tile, so a neighbour shows."""
+    dev, h, kvh, bs, n = cuda_device, 4, 2, 32, 150
+    pool, kr, vr = make_pool(dev, 6, bs, kvh, 21)
+    table = torch.tensor([[4, 0, 3, 1, 5]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    sl = seq_slots(table[0], n, bs, dev)
+    m = 1 if which == "decode" else 40
+    g = torch.Generator().manual_seed(5)
+    base = torch.randn(m, h, D, generator=g)
+    spread = base * torch.exp2(torch.randint(-24, 1, (m, h, D), generator=g).float())
+    for q_mul, x in ((2.0 ** 60, base), (2.0 ** -100, base), (2.0 ** -120, base), (1.0, spread), (0.0, base)):
+        q = (x * q_mul).to(torch.bfloat16).to(dev)
+        q[0, 1, 7], q[0, 2, 100] = float("nan"), float("inf")
+        scale = SCALE / q_mul if 0 < q_mul else SCALE
+        if q_mul < 2.0 ** -100:
+            scale = SCALE * 2.0 ** 100  # as far as fp32 holds scale * log2(e) * 2^-112 apart: scores near 2^-20
+        out = torch.empty_like(q)
+        if which == "decode":
+            ops_fp4.paged_decode_fp4(out, q, pool, table, lens, scale, workspace(dev, h, kvh))
+        else:
+            ops_fp4.paged_prefill_fp4(out, q, pool, table, torch.tensor([0, m], dtype=torch.int32, device=dev), lens,
+                                      m, scale)
+        bad = torch.zeros(m, h, dtype=torch.bool, device=dev)
+        bad[0, 1] = bad[0, 2] = True
+        assert torch.equal(torch.isnan(out).all(-1), bad) and torch.equal(torch.isnan(out).any(-1), bad)
+        clean = torch.where(bad[..., None], torch.zeros_like(q), q)
+        want, a = orc.attention(clean, kr[sl], vr[sl], scale)
+        keep = ~bad[..., None].expand_as(want)
+        check(out[keep], want[keep], a[keep], vr[sl], DECODE if which == "decode" else PREFILL, f"times {q_mul}")
