@@ -48,6 +48,8 @@
  *                         device, src/nanovllm_ascend/model_runner.py:31): KV-head
  *                         sharded decode whose output all-gather across GPUs
  *                         happens inside the attention kernel
+ *   nvk_fp4_*          <- no reference counterpart: the pool held in 4 bits, with
+ *                         the calls above that write and read it
  */
 #ifndef NVK_PAGED_KV_H_
 #define NVK_PAGED_KV_H_
@@ -324,8 +326,8 @@ NVK_API int nvk_lm_head_argmax(const void* hidden, int64_t hidden_stride, const 
  *   together. Slot numbers are those of the bf16 pool. The order of the bytes
  *   in a unit (16 tokens of one KV head) is described in csrc/fp4_kv.cuh; read
  *   rows with nvk_fp4_read. Zero-fill the pool once when it is allocated (a
- *   zero byte is a zero value). Rows past a sequence's context are not used,
- *   whatever they hold.
+ *   zero byte is a zero value; a value that rounds to 0 loses its sign). Rows
+ *   past a sequence's context are not used, whatever they hold.
  * Supported: head_dim 128; block_size a power of two in [16, 256]; any number
  *   of KV heads.
  */
@@ -382,6 +384,10 @@ NVK_API int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, cons
  * heads and CTAs or with others, as long as it is large enough. Calls that
  * share one must be ordered on one stream. Its first int is the error word
  * (bits as for nvk_paged_decode; blocks outside the pool read as zeros).
+ * block_tables and context_lens are step metadata, read while the kernel
+ * before this one in the stream drains: what writes them on the stream must be
+ * a copy, nvk_decode_metadata or a kernel that is not launched with
+ * programmatic stream serialisation.
  */
 NVK_API int nvk_fp4_paged_decode_workspace_size(int num_heads, int num_kv_heads, int head_dim, int num_ctas,
                                                 size_t* bytes);

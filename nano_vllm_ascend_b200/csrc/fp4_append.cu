@@ -403,6 +403,7 @@ int in_launches(int64_t num_tokens, int kvh, Launch&& launch) {
 }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
 }  // namespace
 }  // namespace fp4
@@ -423,6 +424,7 @@ extern "C" int nvk_fp4_append(const void* key, const void* value, int64_t key_to
   if (num_tokens == 0) return NVK_OK;
   if (!key || !value || !slot_mapping) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   const int64_t row = static_cast<int64_t>(num_kv_heads) * kD;
+  if (!aligned8(slot_mapping)) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: slots must be 8-byte aligned", who);
   if (!aligned4(key) || !aligned4(value) || key_token_stride % 2 || value_token_stride % 2 ||
       (num_tokens > 1 && (key_token_stride < row || value_token_stride < row)))
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: rows must be 4-byte aligned and token strides (%lld, %lld) cover a row",
@@ -468,8 +470,8 @@ extern "C" int nvk_fp4_read(void* key, void* value, const void* kv_cache, const 
     return fail(NVK_ERR_UNSUPPORTED, "%s: dtype %d (bf16 or fp16 rows only)", who, dtype);
   if (num_tokens == 0) return NVK_OK;
   if (!key || !value || !slot_mapping) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  if (!aligned16(key) || !aligned16(value))
-    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: the rows must be 16-byte aligned", who);
+  if (!aligned16(key) || !aligned16(value) || !aligned8(slot_mapping))
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: the rows must be 16-byte aligned, the slots 8-byte aligned", who);
   ReadArgs a;
   a.key = static_cast<uint8_t*>(key);
   a.value = static_cast<uint8_t*>(value);
@@ -513,16 +515,19 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   int rc = check_pool(kv_cache, num_blocks, block_size, num_kv_heads, head_dim, k_scale, v_scale, who);
   if (rc != NVK_OK) return rc;
   if (num_tokens == 0) return NVK_OK;
-  if (num_tokens > (int64_t(1) << 30))
-    return fail(NVK_ERR_UNSUPPORTED, "%s: %lld tokens are above the kernel's range", who, (long long)num_tokens);
+  if (num_tokens > (int64_t(1) << 30) || num_heads > (1 << 20))  // the item index: 32 bits
+    return fail(NVK_ERR_UNSUPPORTED, "%s: %lld tokens or %d heads are above the kernel's range", who,
+                (long long)num_tokens, num_heads);
   if (!query || !key || !value || !q_weight || !k_weight || !cos_table || !sin_table || !positions || !query_out ||
       !slot_mapping)
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   if (!aligned4(query) || !aligned4(key) || !aligned4(value) || !aligned4(q_weight) || !aligned4(k_weight) ||
-      !aligned4(query_out) || query_stride % 2 || key_stride % 2 || value_stride % 2 ||
+      !aligned4(query_out) || !aligned4(cos_table) || !aligned4(sin_table) || !aligned8(positions) ||
+      !aligned8(slot_mapping) || query_stride % 2 || key_stride % 2 || value_stride % 2 ||
       (num_tokens > 1 && (query_stride < int64_t(num_heads) * kD || key_stride < int64_t(num_kv_heads) * kD ||
                           value_stride < int64_t(num_kv_heads) * kD)))
-    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: rows must be 4-byte aligned and strides cover a row", who);
+    return fail(NVK_ERR_INVALID_ARGUMENT, "%s: rows and tables must be 4-byte aligned, positions and slots 8-byte aligned, and strides cover a row",
+                who);
   NormArgs a;
   a.q = static_cast<const uint8_t*>(query);
   a.k = static_cast<const uint8_t*>(key);

@@ -42,9 +42,10 @@
 //     signalled once stored; lazy rescaling of O_s (only when the running
 //     max grew by more than 2^8; S_s(j) having landed means P V_s(j-1),
 //     issued before it, is complete). Per item, once its last P V_s has
-//     completed, the normalised O_s rows go out through a staging buffer:
-//     each warp stores the 32 rows its own lanes staged as whole 128-byte
-//     row halves (coalesced), and O_s is released to the next item.
+//     completed, the normalised O_s rows go out through a staging buffer, 32
+//     dims at a time: each warp stores the 64-byte pieces of the 32 rows that
+//     its own lanes staged, eight per instruction (coalesced), and O_s is
+//     released to the next item.
 // Ten warps put three on one SM sub-partition, whose register file holds
 // 3 x 32 x 168 registers: the kernel is held to 168 registers a thread.
 //   4-bit pool, warps 12-15 (decoders; warps 10 and 11 idle): thread r owns
@@ -52,12 +53,27 @@
 //     straight into registers one tile ahead (in flight while the other of K
 //     and V is decoded), turns them into fp16, which holds the values exactly,
 //     and stores them where the TMA copy of a tile would have put them. All
-//     operands are fp16 then: the decoders also turn the item's Q rows into
-//     fp16, each scaled by a power of two into its range (the softmax takes
-//     the factor back), and P is fp16, three bits more exact than bf16. Items
-//     are published one earlier, so that the next item's first tiles are
-//     decoded behind this one's last. 16 warps have 128 registers a thread at
-//     launch: the softmax warpgroups take 168, the other two give them up.
+//     operands are fp16 then: the softmax warps turn the next item's Q rows
+//     into fp16, each scaled by a power of two into its range, between an
+//     item's last P and its output, and P is fp16, three bits more exact than
+//     bf16. Items are published one earlier, so that the next item's first
+//     tiles are decoded behind this one's last. 16 warps have 128 registers a
+//     thread at launch: the softmax warpgroups take 168, the other two give
+//     them up.
+// What bounds it: the chain softmax -> P V + S -> softmax of a stream, of which
+// two overlap (tensor pipe 42 % of active cycles, exp unit 42 %, issue 50 % with
+// 4-bit K and V), and instruction fetch: 70 KB of code (4-bit), of which warps
+// wait for what they run once an item. That is why the rare parts are short
+// loops and one elected thread issues a whole product. Code that the roles ran
+// in line before (masks over all registers, an election for every step, Q in
+// the decoders): 89.8 us against 82.5 for 32 x 256 queries over 1024 keys, 16
+// heads on 8 (60.2 GFLOP; with bf16 K and V 75.1 against 73.6).
+// Measured and not taken for the 4-bit kernel, same work: scores read twice in
+// a loop instead of held in registers 91.4 us; each thread storing its output
+// row directly 98.2; Q by the two idle warps 86.2 or by the decoders 83.2 to
+// 85.4; one loop over the tiles of all items 95.5; the upper half of the next S
+// issued before the end of P 89.4 (products of 64 columns take as long as of
+// 128).
 // Every mbarrier wait is bounded; on a timeout the CTA records the error,
 // drains its in-flight copies and MMAs, frees TMEM and exits.
 #pragma once

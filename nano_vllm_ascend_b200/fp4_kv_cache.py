@@ -47,6 +47,11 @@ class Fp4Layer:
     def device(self) -> torch.device:
         return self.pool.device
 
+    def check_pair(self, value_cache) -> None:
+        """Raises unless ``value_cache`` is this layer too (it holds K and V together)."""
+        if not isinstance(value_cache, Fp4Layer) or value_cache.pool is not self.pool:
+            raise ValueError("key_cache and value_cache must be the same layer of a PagedKVCacheFp4")
+
 
 def _constants(name: str, value: float | Sequence[float], layers: int) -> list[float]:
     values = [float(value)] * layers if isinstance(value, (int, float)) else [float(v) for v in value]

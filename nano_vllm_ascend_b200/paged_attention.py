@@ -122,6 +122,7 @@ class PagedAttention(nn.Module):
                 raise RuntimeError(f"missing block: context length {longest} exceeds the "
                                    f"{block_tables.shape[1]}-block table")
         if isinstance(key_cache, Fp4Layer):
+            key_cache.check_pair(value_cache)
             return self._forward_fp4(output, q, key_cache, block_tables, context_lens)
         with torch.cuda.device(device):
             errors = device_errors.state(device)

@@ -97,6 +97,7 @@ class BatchPrefillAttention(nn.Module):
                         raise RuntimeError(f"missing block: context length {longest} exceeds the "
                                            f"{tables.shape[1]}-block table")
                 if isinstance(key_cache, Fp4Layer):
+                    key_cache.check_pair(value_cache)
                     ops_fp4.paged_prefill_fp4(out, query, key_cache.pool, tables, cu_q, ctx, max_prompt_len,
                                               self.scale, key_cache.k_scale, key_cache.v_scale,
                                               error_word=errors.word)

@@ -68,7 +68,9 @@ def norm_args(**kw):
 @pytest.mark.parametrize("kw,code,text", BAD_POOL + [
     (dict(tokens=-1), INVALID, "bad sizes"), (dict(h=0), INVALID, "bad sizes"), (dict(max_pos=0), INVALID, "bad sizes"),
     (dict(q=0), INVALID, "null"), (dict(out=0), INVALID, "null"), (dict(cos=0), INVALID, "null"),
-    (dict(qs=2046), INVALID, "strides"), (dict(vs=1025), INVALID, "strides"), (dict(v=P + 1), INVALID, "aligned")])
+    (dict(qs=2046), INVALID, "strides"), (dict(vs=1025), INVALID, "strides"), (dict(v=P + 1), INVALID, "aligned"),
+    (dict(sin=P + 2), INVALID, "aligned"), (dict(pos=P + 4), INVALID, "aligned"), (dict(slots=P + 4), INVALID, "aligned"),
+    (dict(tokens=(1 << 30) + 1), UNSUPPORTED, "range"), (dict(h=(1 << 20) + 1, qs=1 << 28), UNSUPPORTED, "range")])
 def test_norm_rope_append_refuses(kw, code, text):
     refused("nvk_fp4_qk_norm_rope_append", norm_args(**kw), code, text)
 
@@ -186,6 +188,11 @@ def test_attention_over_a_4_bit_layer_checks_like_the_bf16_one():
     with pytest.raises(RuntimeError, match="missing block: context length 33"):
         attn(torch.zeros(2, 16, 128, dtype=torch.bfloat16), key, value, torch.zeros(2, 2, dtype=torch.int32),
              torch.tensor([5, 33], dtype=torch.int32))
+    other = PagedKVCacheFp4(2, 4, 16, 8, 128, "cpu").get_physical_cache(1)[0]
+    for wrong in (other, torch.zeros(4, 16, 8, 128, dtype=torch.bfloat16), None):
+        with pytest.raises(ValueError, match="must be the same layer"):
+            attn(torch.zeros(2, 16, 128, dtype=torch.bfloat16), key, wrong, torch.zeros(2, 2, dtype=torch.int32),
+                 torch.tensor([5, 31], dtype=torch.int32))
 
 
 class Backend:
