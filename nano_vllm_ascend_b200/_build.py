@@ -1,4 +1,5 @@
-"""Builds the in-tree C-ABI library ``libnvk_paged.so`` for sm_100a with nvcc.
+"""Builds the in-tree C-ABI library ``libnvk_paged.so`` for sm_100a with nvcc,
+and the CPython module ``_fp4_calls.so`` (``csrc/fp4_calls.cpp``) with g++.
 
 Every ``csrc/*.cu`` file is compiled separately (``-gencode
 arch=compute_100a,code=sm_100a -lineinfo -O3``) and linked into one shared
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -21,6 +23,8 @@ INCLUDE = PKG_DIR.parent / "include"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_NAME = "libnvk_paged.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+CALLS_SRC = CSRC / "fp4_calls.cpp"
+CALLS_PATH = PKG_DIR / "_fp4_calls.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -84,7 +88,29 @@ def build(verbose_ptxas: bool = False, force: bool = False) -> Path:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("linking libnvk_paged.so failed")
         os.replace(tmp, LIB_PATH)
+    _build_calls(force)
     return LIB_PATH
+
+
+def _build_calls(force: bool) -> None:
+    """The binding uses torch's tensors, so it is built against the installed torch."""
+    import torch
+
+    torch_dir = Path(torch.__file__).parent
+    newest = max(p.stat().st_mtime for p in (CALLS_SRC, INCLUDE / "nvk_paged_kv.h", torch_dir / "version.py"))
+    if not force and CALLS_PATH.exists() and CALLS_PATH.stat().st_mtime >= newest:
+        return
+    includes = [INCLUDE, torch_dir / "include", torch_dir / "include/torch/csrc/api/include",
+                sysconfig.get_paths()["include"], Path(nvcc_path()).resolve().parent.parent / "include"]
+    tmp = CALLS_PATH.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           *(f"-I{path}" for path in includes), str(CALLS_SRC), "-o", str(tmp), f"-L{torch_dir / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"g++ failed on {CALLS_SRC.name}")
+    os.replace(tmp, CALLS_PATH)
 
 
 if __name__ == "__main__":

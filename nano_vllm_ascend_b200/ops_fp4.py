@@ -2,7 +2,10 @@
 
 As in ``ops``, each function validates devices, dtypes, shapes and strides,
 then calls the matching ``nvk_fp4_*`` entry point (include/nvk_paged_kv.h) on
-the tensors' current CUDA stream, and there is no non-CUDA path.
+the tensors' current CUDA stream, and there is no non-CUDA path. Calls whose
+arguments need no repair go through ``csrc/fp4_calls.cpp``, which makes the
+same checks in a third of the time; what it does not take, the code here checks
+again, calls or refuses.
 
 ``kv_cache`` is ONE layer of the pool, K and V together: contiguous uint8
 [num_blocks, kv_heads, block_size / 16, 2304] (``pool_shape``), zero-filled
@@ -22,6 +25,11 @@ import torch
 from . import _lib
 from .ops import _require_cuda, _require_rows
 
+try:
+    from . import _fp4_calls as _calls
+except ImportError:  # not built yet, or for another torch: every call is checked and made here
+    _calls = None
+
 _BF16 = torch.bfloat16
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 HEAD_DIM = 128
@@ -39,15 +47,30 @@ def pool_shape(num_blocks: int, block_size: int, num_kv_heads: int) -> tuple[int
 # is asked for instead of a Stream object (3 us less a call), and entry points
 # are looked up once.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_NOT_TAKEN = 1
+_BOUND = ("nvk_fp4_append", "nvk_fp4_read", "nvk_fp4_qk_norm_rope_append", "nvk_fp4_paged_decode",
+          "nvk_fp4_paged_prefill")
 
 
 class _EntryPoints(dict):
     def __missing__(self, name: str):
-        fn = self[name] = getattr(_lib.load(), name)
+        lib = _lib.load()
+        if _calls is not None:  # from the first call on
+            _calls.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _BOUND))
+        fn = self[name] = getattr(lib, name)
         return fn
 
 
 _entry_points = _EntryPoints()
+
+
+def _leave(*args) -> int:
+    return _NOT_TAKEN
+
+
+_append, _read, _norm_rope_append, _decode, _prefill = (
+    (_leave,) * 5 if _calls is None else
+    (_calls.append, _calls.read, _calls.norm_rope_append, _calls.decode, _calls.prefill))
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
@@ -107,6 +130,11 @@ def kv_append_fp4(kv_cache: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     fp16; the token stride may be larger) into the pool at ``slot_mapping``
     (int64). Slots must differ; one outside the pool is skipped and sets bit 4
     of ``error_word``."""
+    rc = _append(kv_cache, key, value, slot_mapping, k_scale, v_scale, error_word)
+    if rc == 0:
+        return
+    if rc != _NOT_TAKEN:
+        _lib.check("nvk_fp4_append", rc)
     who = "kv_append_fp4"
     dev = kv_cache.device
     if not kv_cache.is_cuda or key.device != dev or value.device != dev or slot_mapping.device != dev:
@@ -132,6 +160,12 @@ def kv_read_fp4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, k_scale: flo
     """The K and V rows [tokens, kv_heads, 128] that the pool holds at
     ``slot_mapping`` (int64; any order, repeats allowed), as ``dtype``; a slot
     outside the pool gives zeros and sets bit 4 of ``error_word``."""
+    if key_out is None and value_out is None and dtype in _DTYPES:
+        rows = _read(kv_cache, slot_mapping, k_scale, v_scale, dtype is torch.float16, error_word)
+        if rows.__class__ is tuple:
+            return rows
+        if rows != _NOT_TAKEN:
+            _lib.check("nvk_fp4_read", rows)
     who = "kv_read_fp4"
     dev = kv_cache.device
     if not kv_cache.is_cuda or slot_mapping.device != dev:
@@ -162,6 +196,12 @@ def qk_norm_rope_append_fp4(query: torch.Tensor, key: torch.Tensor, value: torch
     """``ops.qk_norm_rope_append`` into a 4-bit pool: per-head RMSNorm of q and
     k, rotary embedding, and the append of the rotated k and of v, in one
     kernel. Returns the rotated query [tokens, heads, 128]."""
+    rotated = _norm_rope_append(query, key, value, q_weight, k_weight, eps, cos_table, sin_table, positions, kv_cache,
+                                slot_mapping, k_scale, v_scale, query_out, error_word)
+    if rotated.__class__ is not int:
+        return rotated
+    if rotated != _NOT_TAKEN:
+        _lib.check("nvk_fp4_qk_norm_rope_append", rotated)
     who = "qk_norm_rope_append_fp4"
     dev = query.device
     if not query.is_cuda or key.device != dev or value.device != dev or q_weight.device != dev \
@@ -240,6 +280,11 @@ def paged_decode_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Ten
     hold decode_fp4_workspace_bytes(heads, kv_heads); calls sharing it must be
     ordered on one stream. Its first int32 is the device error word.
     """
+    rc = _decode(out, query, kv_cache, block_tables, context_lens, scale, workspace, num_ctas, k_scale, v_scale)
+    if rc == 0:
+        return out
+    if rc != _NOT_TAKEN:
+        _lib.check("nvk_fp4_paged_decode", rc)
     who = "paged_decode_fp4"
     dev = query.device
     shape, nb, bs, kvh, batch, stride, width = _check_attention(who, dev, out, query, kv_cache, block_tables,
@@ -259,6 +304,12 @@ def paged_prefill_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Te
                       k_scale: float = 1.0, v_scale: float = 1.0,
                       error_word: torch.Tensor | None = None) -> torch.Tensor:
     """Causal (bottom-right) prefill attention over a 4-bit pool into ``out``."""
+    rc = _prefill(out, query, kv_cache, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale, k_scale, v_scale,
+                  error_word)
+    if rc == 0:
+        return out
+    if rc != _NOT_TAKEN:
+        _lib.check("nvk_fp4_paged_prefill", rc)
     who = "paged_prefill_fp4"
     dev = query.device
     shape, nb, bs, kvh, batch, stride, width = _check_attention(who, dev, out, query, kv_cache, block_tables, kv_lens)
