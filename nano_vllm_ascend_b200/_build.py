@@ -1,5 +1,5 @@
 """Builds the in-tree C-ABI library ``libnvk_paged.so`` for sm_100a with nvcc,
-and the CPython module ``_fp4_calls.so`` (``csrc/fp4_calls.cpp``) with g++.
+and the CPython module ``_fp4_calls`` (``csrc/fp4_calls.cpp``) with g++.
 
 Every ``csrc/*.cu`` file is compiled separately (``-gencode
 arch=compute_100a,code=sm_100a -lineinfo -O3``) and linked into one shared
@@ -24,7 +24,7 @@ BUILD_DIR = PKG_DIR / "_build"
 LIB_NAME = "libnvk_paged.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 CALLS_SRC = CSRC / "fp4_calls.cpp"
-CALLS_PATH = PKG_DIR / "_fp4_calls.so"
+CALLS_PATH = PKG_DIR / ("_fp4_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [

@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <climits>
 
@@ -294,5 +295,6 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp4_calls", nullptr, -1, methods}
 PyMODINIT_FUNC PyInit__fp4_calls() {
   PyObject* m = PyModule_Create(&module);
   if (m) PyModule_AddIntConstant(m, "NOT_TAKEN", kNotTaken);
+  if (m) PyModule_AddStringConstant(m, "TORCH_VERSION", TORCH_VERSION);  // that it was built for
   return m;
 }

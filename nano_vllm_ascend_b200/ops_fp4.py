@@ -27,8 +27,10 @@ from .ops import _require_cuda, _require_rows
 
 try:
     from . import _fp4_calls as _calls
-except ImportError:  # not built yet, or for another torch: every call is checked and made here
+except ImportError:
     _calls = None
+if _calls is not None and not torch.__version__.startswith(_calls.TORCH_VERSION):
+    _calls = None  # built for another torch; as without it, every call is checked and made here
 
 _BF16 = torch.bfloat16
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
