@@ -54,7 +54,7 @@ struct AppendArgs {
   int* err;
 };
 
-// 32 registers: eight blocks an SM, one resident wave (8192 tokens: 12.2 us against 14.2 with six).
+// 32 registers: eight blocks an SM (8192 tokens: 12.2 us against 14.2 with six).
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 8) append_kernel(const AppendArgs a) {
   pdl_launch_dependents();
@@ -387,11 +387,15 @@ int sm_count() {
   return sms;
 }
 
-// Calls launch(first token, tokens, items, grid) for the tokens, as many at a time as the kernels' index takes.
+// Calls launch(first token, tokens, items, grid) for the tokens, as many at a time as the kernels' index takes, with
+// at most `per_sm` blocks an SM. Eight are resident: the append takes two waves, whose second one evens out what
+// does not divide (8192 tokens 11.4 us against 12.3 in one, 16384 21.2 against 22.3), the read, which waits for
+// memory, one (10.0 and 18.0 against 10.3 and 18.3).
+constexpr int kAppendBlocks = 16, kReadBlocks = 8;
 template <typename Launch>
-int in_launches(int64_t num_tokens, int kvh, Launch&& launch) {
+int in_launches(int64_t num_tokens, int kvh, int per_sm, Launch&& launch) {
   const int64_t per_group = 2 * static_cast<int64_t>(kvh), most_tokens = kMostItems / per_group * 4;
-  const int64_t most_blocks = int64_t(sm_count()) * 8;
+  const int64_t most_blocks = int64_t(sm_count()) * per_sm;
   for (int64_t first = 0; first < num_tokens; first += most_tokens) {
     const int64_t tokens = num_tokens - first < most_tokens ? num_tokens - first : most_tokens;
     const int64_t items = (tokens + 3) / 4 * per_group, want = (items + kWarps - 1) / kWarps;
@@ -444,7 +448,7 @@ extern "C" int nvk_fp4_append(const void* key, const void* value, int64_t key_to
   a.v_inv = 1.f / v_scale;
   a.err = error_word;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return in_launches(num_tokens, num_kv_heads, [&](int64_t first, int tokens, int items, dim3 grid) {
+  return in_launches(num_tokens, num_kv_heads, kAppendBlocks, [&](int64_t first, int tokens, int items, dim3 grid) {
     AppendArgs b = a;
     b.num_tokens = tokens;
     b.items = items;
@@ -485,7 +489,7 @@ extern "C" int nvk_fp4_read(void* key, void* value, const void* kv_cache, const 
   a.v_scale = v_scale;
   a.err = error_word;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return in_launches(num_tokens, num_kv_heads, [&](int64_t first, int tokens, int items, dim3 grid) {
+  return in_launches(num_tokens, num_kv_heads, kReadBlocks, [&](int64_t first, int tokens, int items, dim3 grid) {
     ReadArgs b = a;
     b.num_tokens = tokens;
     b.items = items;
