@@ -558,9 +558,17 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   a.err = error_word;
   const int sms = sm_count();
   const int rounds = (num_heads + 3) / 4 + 2 * ((num_kv_heads + 3) / 4);
-  // a whole token per warp (cos and sin loaded once) when the tokens alone give every SM 16 warps
-  a.chunk = num_tokens >= int64_t(sms) * 16 ? rounds : 1;
-  a.chunks = (rounds + a.chunk - 1) / a.chunk;
+  // A token's rounds in `chunks` items of `chunk`: the split for which the warps of one resident wave end first, an
+  // item's start (position, slot, the cos and sin rows) weighing a little more than a round. With 8 rounds a token:
+  // 2048 tokens whole 10.5 us, in eighths 15.5; 2400 whole 15.8, in halves 14.1; 8192 whole 35.6, in halves 34.2;
+  // 32768 whole 116.5, in halves 125.7.
+  const int64_t warps = int64_t(sms) * 2 * kWarps;
+  int64_t best = INT64_MAX;
+  for (int n = 1; n <= rounds; n = n < 8 ? n + 1 : n < rounds && 2 * n > rounds ? rounds : 2 * n) {
+    const int chunk = (rounds + n - 1) / n, chunks = (rounds + chunk - 1) / chunk;
+    const int64_t cost = (num_tokens * chunks + warps - 1) / warps * (6 * chunk + 7);
+    if (cost < best && (chunks == 1 || num_tokens * chunks <= kMostItems)) best = cost, a.chunk = chunk, a.chunks = chunks;
+  }
   a.items = static_cast<int>(num_tokens) * a.chunks;
   a.per_token = divisor(a.chunks);
   // 16-byte copies where every row and table allows them

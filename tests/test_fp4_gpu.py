@@ -192,7 +192,8 @@ def rope_tables(max_pos, theta=1e6):
 
 
 @pytest.mark.parametrize("tokens,h,kvh,bs", [(1, 16, 8, 128), (33, 5, 1, 16), (7, 9, 3, 64), (2500, 4, 2, 32),
-                                              (3000, 7, 1, 128), (2367, 16, 8, 64), (2368, 4, 1, 16)])
+                                              (3000, 7, 1, 128), (2367, 16, 8, 64), (2368, 4, 1, 16),
+                                              (300, 16, 8, 32), (2500, 16, 8, 128), (700, 35, 5, 64)])
 def test_norm_rope_append_is_exact(cuda_device, tokens, h, kvh, bs):
     dev = cuda_device
     g = torch.Generator().manual_seed(tokens)
