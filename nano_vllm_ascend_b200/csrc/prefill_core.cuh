@@ -58,7 +58,7 @@
 //     item's last P and its output, and P is fp16, three bits more exact than
 //     bf16. Items are published one earlier, so that the next item's first
 //     tiles are decoded behind this one's last. 16 warps have 128 registers a
-//     thread at launch: the softmax warpgroups take 168, the other two give
+//     thread at launch: the softmax warpgroups take 176, the other two give
 //     them up.
 // What bounds it: the chain softmax -> P V + S -> softmax of a stream, of which
 // two overlap (tensor pipe 42 % of active cycles, exp unit 42 %, issue 50 % with
@@ -67,7 +67,9 @@
 // loops and one elected thread issues a whole product. Code that the roles ran
 // in line before (masks over all registers, an election for every step, Q in
 // the decoders): 89.8 us against 82.5 for 32 x 256 queries over 1024 keys, 16
-// heads on 8 (60.2 GFLOP; with bf16 K and V 75.1 against 73.6).
+// heads on 8 (60.2 GFLOP; with bf16 K and V 75.1 against 73.6). Exponents and
+// sums two values an instruction: 80 us (with eight registers more for the
+// softmax; 85 with spills of one), bf16 71.5, the same bits.
 // Measured and not taken for the 4-bit kernel, same work: scores read twice in
 // a loop instead of held in registers 91.4 us; each thread storing its output
 // row directly 98.2; Q by the two idle warps 86.2 or by the decoders 83.2 to
@@ -100,7 +102,7 @@ constexpr int kThreads = 10 * 32;
 constexpr int kDecodeWarp0 = 12;          // 4-bit pool: warps 12-15
 constexpr int kThreadsFp4 = 16 * 32;
 // Registers a thread after the split of the 4-bit kernel's 512 x 128 (softmax, softmax, producer and MMA, decoders)
-constexpr int kRegsSoftmax = 168, kRegsIssue = 72, kRegsDecode = 104;
+constexpr int kRegsSoftmax = 176, kRegsIssue = 64, kRegsDecode = 96;
 static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsDecode <= 4 * 128, "setmaxnreg shares exceed the launch's registers");
 constexpr uint32_t kTmemCols = 512;       // S_0 | S_1 | O_0 | O_1, 128 columns each
 constexpr uint32_t kColO = 256;
@@ -746,7 +748,8 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           m = m_new;
         }
         const float neg_mu = (m == -INFINITY) ? 0.f : kPShift<kFp4> - m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};  // independent add chains
+        uint64_t sum[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};  // independent add chains
+        const uint64_t sc2 = f32x2_pack(sc, sc), mu2 = f32x2_pack(neg_mu, neg_mu);
         // P over the first 64 columns of S_s (column k holds keys 2k and 2k+1
         // as a bf16 pair): word e of chunk c overwrites score e, already read.
         // Keys 0-63 are signalled first, so that their P V starts while the
@@ -754,10 +757,12 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         auto exps = [&](int c) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = fast_exp2(fmaf(__uint_as_float(sr[c][2 * e]), sc, neg_mu));
-            const float p1 = fast_exp2(fmaf(__uint_as_float(sr[c][2 * e + 1]), sc, neg_mu));
-            sum[(2 * e) & 3] += p0;
-            sum[(2 * e + 1) & 3] += p1;
+            float p0, p1;
+            f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), sc2, mu2),
+                         p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            sum[e & 1] = f32x2_add(sum[e & 1], f32x2_pack(p0, p1));
             sr[c][e] = kFp4 ? pack_half2(p0, p1) : pack_bf16x2(p0, p1);
           }
           tmem_st16_first(tmem_s + c * 16, sr[c]);
@@ -782,7 +787,10 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         mbar_arrive(&sm.p_lo[s]);
         exps(2);
         exps(3);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float s0, s1, s2, s3;
+        f32x2_unpack(sum[0], s0, s1);
+        f32x2_unpack(sum[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&sm.p_hi[s]);
