@@ -560,14 +560,16 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   const int rounds = (num_heads + 3) / 4 + 2 * ((num_kv_heads + 3) / 4);
   // A token's rounds in `chunks` items of `chunk`: the split for which the warps of one resident wave end first, an
   // item's start (position, slot, the cos and sin rows) weighing a little more than a round. With 8 rounds a token:
-  // 2048 tokens whole 10.5 us, in eighths 15.5; 2400 whole 15.8, in halves 14.1; 8192 whole 35.6, in halves 34.2;
-  // 32768 whole 116.5, in halves 125.7.
+  // 2048 tokens whole 10.5 us, in eighths 15.5; 2400 whole 15.8, in halves 14.1; 32768 whole 116.5, in halves 125.7.
+  // A finer split has to win a tenth: where all blocks end at once, the next kernel's are not there to follow (8192
+  // tokens alone whole 35.6, in halves 34.2; each followed by a read 43.5 and 44.7).
   const int64_t warps = int64_t(sms) * 2 * kWarps;
-  int64_t best = INT64_MAX;
+  int64_t best = 0;
   for (int n = 1; n <= rounds; n = n < 8 ? n + 1 : n < rounds && 2 * n > rounds ? rounds : 2 * n) {
     const int chunk = (rounds + n - 1) / n, chunks = (rounds + chunk - 1) / chunk;
     const int64_t cost = (num_tokens * chunks + warps - 1) / warps * (6 * chunk + 7);
-    if (cost < best && (chunks == 1 || num_tokens * chunks <= kMostItems)) best = cost, a.chunk = chunk, a.chunks = chunks;
+    if (chunks > 1 && (cost >= best - best / 10 || num_tokens * chunks > kMostItems)) continue;
+    best = cost, a.chunk = chunk, a.chunks = chunks;
   }
   a.items = static_cast<int>(num_tokens) * a.chunks;
   a.per_token = divisor(a.chunks);
