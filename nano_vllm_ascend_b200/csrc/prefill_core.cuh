@@ -75,7 +75,9 @@
 // row directly 98.2; Q by the two idle warps 86.2 or by the decoders 83.2 to
 // 85.4; one loop over the tiles of all items 95.5; the upper half of the next S
 // issued before the end of P 89.4 (products of 64 columns take as long as of
-// 128).
+// 128); against 80: Q's largest exponents by the idle warps 82; a quarter of
+// the exponentials as a polynomial, two values an instruction, 83 (left out
+// altogether 79.6: the exponential unit is not what it waits for).
 // Every mbarrier wait is bounded; on a timeout the CTA records the error,
 // drains its in-flight copies and MMAs, frees TMEM and exits.
 #pragma once
