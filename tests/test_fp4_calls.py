@@ -184,3 +184,29 @@ def test_host_tensors_are_left_to_the_wrapper():
         c.append(1, 2, 3)
     with pytest.raises(ValueError, match="must be a CUDA tensor|CUDA"):
         run("append", st)
+
+
+@pytest.mark.gpu
+def test_captured_calls_allocate_in_the_graph(cuda_device):
+    """Outputs that a captured call allocates belong to the graph; a replay on new inputs writes them again."""
+    st = state(cuda_device)
+    st["err"] = None
+    want = []
+    for seed in (0, 1):
+        st["q"].copy_(torch.randn(T, H, D, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16))
+        st["k"].copy_(torch.randn(T, KVH, D, generator=torch.Generator().manual_seed(seed + 9)).to(torch.bfloat16))
+        q, _, _ = [*run("norm", st), None][:3]
+        k, v, _ = run("read", st)
+        want.append([t.clone() for t in (q, k, v)])
+    stream = torch.cuda.Stream(cuda_device)
+    stream.wait_stream(torch.cuda.current_stream(cuda_device))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        q = run("norm", st)[0]
+        k, v, _ = run("read", st)
+    for seed in (0, 1, 0):
+        st["q"].copy_(torch.randn(T, H, D, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16))
+        st["k"].copy_(torch.randn(T, KVH, D, generator=torch.Generator().manual_seed(seed + 9)).to(torch.bfloat16))
+        graph.replay()
+        for got, expected in zip((q, k, v), want[seed]):
+            assert torch.equal(got, expected)
