@@ -165,8 +165,8 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
   for (int j = 0; j < kGroups; ++j)
     st_shared_v2(st.q + 512 * (j >> 1) + 8 * (j & 1), bf16x2_to_half2(raw[j].x, half.base),
                  bf16x2_to_half2(raw[j].y, half.base));
-  st.sc[0] = __shfl_sync(0xffffffffu, half.up, 8 * t) * a.scale_log2;
-  st.sc[1] = __shfl_sync(0xffffffffu, half.up, 8 * t + 4) * a.scale_log2;
+  st.sc[0] = score_factor(__shfl_sync(0xffffffffu, half.up, 8 * t), a.scale_log2);
+  st.sc[1] = score_factor(__shfl_sync(0xffffffffu, half.up, 8 * t + 4), a.scale_log2);
   st.ref[0] = st.ref[1] = 0.f;
   st.thr[0] = st.thr[1] = -INFINITY;
   st.l[0] = st.l[1] = 0.f;

@@ -113,6 +113,14 @@ __device__ __forceinline__ HalfRow half_row(uint32_t largest) {  // the bf16x2_a
   const uint32_t f = max(top, 30u) - 30u;
   return HalfRow{f * 0x00800080u, __uint_as_float(top == 255u ? 0x7fffffffu : (127u - 112u + f) << 23)};
 }
+// The factor from a row's products to its scores in log2 units. At least the
+// smallest normal number, so that a masked product, -inf, stays -inf under it
+// (a row of zeros has the smallest `up`, and times a small scale and constant
+// it would be 0): products are below 2^35, so such scores are 0 to fp32 anyway.
+__device__ __forceinline__ float score_factor(float up, float scale_log2) {
+  const float f = up * scale_log2;
+  return f < 1.17549435e-38f ? 1.17549435e-38f : f;  // NaN stays
+}
 __device__ __forceinline__ uint32_t bf16x2_to_half2(uint32_t w, uint32_t base) {
   uint32_t m;  // of magnitudes
   asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w & 0x7fff7fffu), "r"(base));

@@ -687,7 +687,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       it = sm.items[n % kItemRing];
       if (kFp4 && it.n_kv > 0) {
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full[s], n & 1))) return false;
-        sc = a.scale_log2 * q_row_to_half(smem_u32(sm.q[s]), r);
+        sc = fp4::score_factor(q_row_to_half(smem_u32(sm.q[s]), r), a.scale_log2);
         fence_proxy_async_smem();
         mbar_arrive(&sm.q_ready[s]);
       }

@@ -1,0 +1,56 @@
+"""4-bit attention at the ends of its ranges: constants, scales, queries, scores and V rows of any magnitude.
+
+Compared with 64-bit arithmetic over the values that the codes stand for; tolerances as in tests/test_fp4_gpu.py.
+"""
+
+import pytest
+import torch
+
+from nano_vllm_ascend_b200 import ops_fp4
+from oracle import fp4_oracle as orc
+from tests.test_fp4_gpu import D, DECODE, PREFILL, SCALE, check, random_rows, seq_slots, workspace
+
+pytestmark = pytest.mark.gpu
+
+
+def pool_of(dev, k, v, bs, ks=1.0, vs=1.0):
+    """A pool that holds rows k and v (times the constants), and what it reads back, in float64."""
+    nb = -(-k.shape[0] // bs)
+    pool = torch.zeros(ops_fp4.pool_shape(nb, bs, k.shape[1]), dtype=torch.uint8, device=dev)
+    slots = torch.arange(k.shape[0], device=dev)
+    ops_fp4.kv_append_fp4(pool, (k.to(dev) * ks).contiguous(), (v.to(dev) * vs).contiguous(), slots, ks, vs)
+    kr, vr = ops_fp4.kv_read_fp4(pool, slots, ks, vs)
+    return pool, kr.double(), vr.double()
+
+
+def attend(which, q, pool, n, scale, ks=1.0, vs=1.0, num_ctas=0):
+    """q [m, heads, 128] over the pool's first n slots: m tokens of one sequence, or one of m == 1 in decode."""
+    dev, (nb, kvh) = q.device, pool.shape[:2]
+    table = torch.arange(nb, dtype=torch.int32, device=dev)[None]
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    out = torch.full_like(q, float("nan"))
+    if which == "decode":
+        ws = workspace(dev, q.shape[1], kvh, num_ctas)
+        ops_fp4.paged_decode_fp4(out, q, pool, table, lens, scale, ws, num_ctas, ks, vs)
+        assert int(ws[:4].view(torch.int32).item()) == 0
+    else:
+        cu = torch.tensor([0, q.shape[0]], dtype=torch.int32, device=dev)
+        ops_fp4.paged_prefill_fp4(out, q, pool, table, cu, lens, q.shape[0], scale, ks, vs)
+    return out
+
+
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("ks,scale", [(2.0 ** -60, SCALE), (2.0 ** -36, SCALE), (1.0, 1e-38), (1.0, 1e-45),
+                                      (2.0 ** -60, 1e-38), (2.0 ** 60, 1e-38)])
+def test_zero_and_tiny_queries_with_any_constant(cuda_device, which, ks, scale):
+    """Rows of zeros and of next to nothing weigh all keys the same, whatever the constant and the scale, with a tile
+    that ends inside (150 tokens) and, in prefill, masked rows."""
+    dev, h, n = cuda_device, 4, 150
+    m = 1 if which == "decode" else 40
+    k, v = random_rows(n, 2, 31, spread=False)
+    pool, kr, vr = pool_of(dev, k, v, 32, ks)
+    q = torch.randn(m, h, D, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16)
+    q = (q * torch.tensor([0.0, 2.0 ** -126, 2.0 ** -133, 1.0], dtype=torch.bfloat16)[None, :, None]).to(dev)
+    out = attend(which, q, pool, n, scale, ks)
+    want, a = orc.attention(q, kr, vr, scale)
+    check(out, want, a, vr, DECODE if which == "decode" else PREFILL)
