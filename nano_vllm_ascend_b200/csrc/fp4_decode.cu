@@ -58,8 +58,9 @@ constexpr int kMinTiles = 8;
 // heads: 18.3 us with 32, 21.2 with 48, 42 with 148; 2 heads: 12.9, 12.9, 15.1).
 constexpr int kMostPieces = 32;
 constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
-constexpr float kRescale = 3.f;  // log2 by which a score may pass the running maximum before O is rescaled
-constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and scales up to 448, P s fits fp16
+constexpr float kRescale = 3.f;  // log2 by which a score may pass the reference before that moves and O is rescaled
+constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and scales up to 448, P s fits fp16 (p goes
+                                 // by differences of products, so that this holds for scores of any magnitude)
 constexpr size_t kTicketOffset = 256;
 constexpr size_t kMlOffset = kTicketOffset + kMaxCtas * sizeof(int);
 
@@ -71,7 +72,7 @@ struct DecodeArgs {
   const int32_t* ctx;
   int* err;
   int* tickets;  // [CTAs], at zero between calls
-  float2* ws_ml; // [CTAs][2][group] (maximum, sum) of a split pair's piece
+  float4* ws_ml; // [CTAs][2][group] of a split pair's piece: see Smem's piece_ml
   float* ws_o;   // [CTAs][2][group][128]
   int batch, heads, kvh, group;
   int bt_stride, max_blocks, num_blocks, upb_log2;
@@ -121,9 +122,9 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
 
 struct State {
   uint32_t q;              // shared address of this lane's B fragments of Q^T (see load_q)
-  float sc[2];             // log2 factor of the scores of heads 2 t and 2 t + 1
-  float ref[2];            // p = 2^(score - ref): their running maximum - kPShift
-  float thr[2];            // the score above which it moves: their running maximum + kRescale (-inf at first)
+  float sc[2];             // factor from products to scores in log2 units, of heads 2 t and 2 t + 1
+  float ref[2];            // p = 2^((product - ref) * sc + kPShift): their running largest product
+  float thr[2];            // the product above which it moves: by kRescale in log2 units (-inf at first)
   float l[2];              // this lane's part of the sum of p
   float o[kGroups][4];     // O^T: dims 16 j + 2 g (heads 2 t, 2 t + 1), then 16 j + 2 g + 1 (the same)
 };
@@ -269,19 +270,19 @@ __device__ __forceinline__ void attend(State& st, uint32_t tile, uint32_t vscale
   float x[2][4];
   scores<kMask>(st, tile, valid, g, t, x[0]);
   scores<kMask>(st, tile + kUnitBytes, valid - kUnitTokens, g, t, x[1]);
-  const float hi0 = fmaxf(fmax3(x[0][0], x[0][2], x[1][0]), x[1][2]) * st.sc[0];
-  const float hi1 = fmaxf(fmax3(x[0][1], x[0][3], x[1][1]), x[1][3]) * st.sc[1];
+  const float hi0 = fmaxf(fmax3(x[0][0], x[0][2], x[1][0]), x[1][2]);
+  const float hi1 = fmaxf(fmax3(x[0][1], x[0][3], x[1][1]), x[1][3]);
   if (__any_sync(0xffffffffu, hi0 > st.thr[0] || hi1 > st.thr[1])) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float m = e ? hi1 : hi0;
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-      m = fmaxf(m, st.thr[e] - kRescale);
-      const float ref = m == -INFINITY ? 0.f : m - kPShift;
-      const float f = st.thr[e] == -INFINITY ? 0.f : fast_exp2(st.ref[e] - ref);
-      st.ref[e] = ref;
-      st.thr[e] = m + kRescale;
+      const bool first = st.thr[e] == -INFINITY;
+      m = first ? m : fmaxf(m, st.ref[e]);
+      const float f = first ? 0.f : fast_exp2((st.ref[e] - m) * st.sc[e]);
+      st.ref[e] = m == -INFINITY ? 0.f : m;
+      st.thr[e] = __fadd_rd(m, __fdividef(kRescale, st.sc[e]));  // down: p stays within its bound
       st.l[e] *= f;
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) st.o[j][e] *= f, st.o[j][2 + e] *= f;
@@ -290,8 +291,8 @@ __device__ __forceinline__ void attend(State& st, uint32_t tile, uint32_t vscale
   uint32_t b[2][2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const float p0 = fast_exp2(fmaf(x[u][0], st.sc[0], -st.ref[0])), p1 = fast_exp2(fmaf(x[u][1], st.sc[1], -st.ref[1]));
-    const float p2 = fast_exp2(fmaf(x[u][2], st.sc[0], -st.ref[0])), p3 = fast_exp2(fmaf(x[u][3], st.sc[1], -st.ref[1]));
+    auto weight = [&](int c) { return fast_exp2(fmaf(x[u][c] - st.ref[c & 1], st.sc[c & 1], kPShift)); };
+    const float p0 = weight(0), p1 = weight(1), p2 = weight(2), p3 = weight(3);
     st.l[0] += p0 + p2;
     st.l[1] += p1 + p3;
     b[u][0] = movmatrix(half2_of(p0, p1));
@@ -334,10 +335,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
   extern __shared__ __align__(128) uint8_t smem_raw[];
   using Sm = Smem<kWarps>;
   Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
-  // Pieces of pairs that are not one warp's: [2 * kWarps][group] (m, l), and
-  // [group][128] each: a warp's first one in its own place, its last one in
-  // the warp's ring.
-  float2* piece_ml = reinterpret_cast<float2*>(smem_raw + sizeof(Sm));
+  // Pieces of pairs that are not one warp's: [2 * kWarps][group] (largest
+  // product, or -inf; sum; sc, the pair's; unused), and [group][128] each: a
+  // warp's first one in its own place, its last one in the warp's ring.
+  float4* piece_ml = reinterpret_cast<float4*>(smem_raw + sizeof(Sm));
   float* piece_first = reinterpret_cast<float*>(piece_ml + 2 * kWarps * a.group);
   auto piece_o = [&](int p) {
     return (p & 1) ? reinterpret_cast<float*>(sm.ring[p >> 1]) : piece_first + (p >> 1) * a.group * kD;
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
           *reinterpret_cast<uint32_t*>(row + 16 * j) = pack_bf16x2(st.o[j][e] * inv, st.o[j][2 + e] * inv);
       } else {
         const int at = (2 * warp + slot) * a.group + head;
-        if (g == 0) piece_ml[at] = make_float2(st.thr[e] - kRescale, st.l[e]);
+        if (g == 0) piece_ml[at] = make_float4(st.thr[e] == -INFINITY ? -INFINITY : st.ref[e], st.l[e], st.sc[e], 0.f);
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
           *reinterpret_cast<float2*>(piece_o(2 * warp + slot) + head * kD + 16 * j + 2 * g) = make_float2(st.o[j][e], st.o[j][2 + e]);
@@ -564,8 +565,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
     *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(pb) * a.heads + ph * a.group + head) * kD + 4 * lane) =
         make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
   };
-  auto weight = [](float2 ml, float m) {  // a piece whose scores were all -inf or NaN has the latter's NaN in its sum
-    return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - m);
+  // a piece whose products were all -inf or NaN has the latter's NaN in its sum
+  auto weight = [](float ref, float l, float m, float sc) {
+    return ref == -INFINITY ? (l == 0.f ? 0.f : 1.f) : fast_exp2((ref - m) * sc);
   };
   auto warp_max = [](float m) {
 #pragma unroll
@@ -587,9 +589,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
       const int head = k - at, first = __ffs(starts) - 1;
       const int pair = __shfl_sync(0xffffffffu, mine, first);
       const int count = __popc(__ballot_sync(0xffffffffu, mine == pair));
-      const float2 ml = mine == pair ? piece_ml[lane * a.group + head] : make_float2(-INFINITY, 0.f);
+      const float4 ml = mine == pair ? piece_ml[lane * a.group + head] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
       const float m = warp_max(ml.x);
-      const float w = weight(ml, m), l = warp_sum(ml.y * w);
+      const float w = weight(ml.x, ml.y, m, ml.z), l = warp_sum(ml.y * w);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int i = 0; i < count; ++i) {
@@ -603,7 +605,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
         write_out(pair, head, l, o);
       } else {
         const int64_t to = (static_cast<int64_t>(c) * 2 + end) * a.group + head;
-        if (lane == 0) a.ws_ml[to] = make_float2(m, l);
+        if (lane == first) a.ws_ml[to] = make_float4(m, l, ml.z, 0.f);
         *reinterpret_cast<float4*>(a.ws_o + to * kD + 4 * lane) = o;
       }
     }
@@ -634,6 +636,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
     // the pair's piece in CTA i: its end 1 where it begins, its end 0 after that
     const int count = e.c1 - e.c0 + 1, parts = parts_of(e);
     auto at = [&](int i) { return (static_cast<int64_t>(e.c0 + i) * 2 + (i == 0 ? 1 : 0)) * a.group + head; };
+    const float sc = __ldcg(&a.ws_ml[at(0)].z);
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = lane; i < count; i += 32) m = fmaxf(m, __ldcg(&a.ws_ml[at(i)].x));
@@ -643,14 +646,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int i = i0 + j * parts;
-        ml[j] = i < count ? __ldcg(&a.ws_ml[at(i)]) : make_float2(-INFINITY, 0.f);
+        ml[j] = i < count ? __ldcg(reinterpret_cast<const float2*>(a.ws_ml + at(i))) : make_float2(-INFINITY, 0.f);
         v[j] = i < count ? __ldcg(reinterpret_cast<const float4*>(a.ws_o + at(i) * kD + 4 * lane))
                          : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       if (i0 == part) m = warp_max(m);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const float w = weight(ml[j], m);
+        const float w = weight(ml[j].x, ml[j].y, m, sc);
         l += w * ml[j].y;
         o.x += w * v[j].x, o.y += w * v[j].y, o.z += w * v[j].z, o.w += w * v[j].w;
       }
@@ -680,7 +683,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
 
 template <int kWarps>
 constexpr size_t smem_bytes(int group) {
-  return sizeof(Smem<kWarps>) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float2) + kD * sizeof(float));
+  return sizeof(Smem<kWarps>) + static_cast<size_t>(kWarps) * group * (2 * sizeof(float4) + kD * sizeof(float));
 }
 // 16 warps where shared memory has room for the pieces of the group's heads
 // beside their rings, else 12 (16 against 12 at two heads, 256 contexts of
@@ -711,7 +714,7 @@ int launch(DecodeArgs a, int batch, int ctas, cudaStream_t stream) {
 }
 
 size_t workspace_bytes(int group, int ctas) {
-  return kMlOffset + static_cast<size_t>(ctas) * 2 * group * (sizeof(float2) + kD * sizeof(float));
+  return kMlOffset + static_cast<size_t>(ctas) * 2 * group * (sizeof(float4) + kD * sizeof(float));
 }
 
 int resolve_ctas(int num_ctas, int* out) {
@@ -793,8 +796,8 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   a.pool = static_cast<const uint8_t*>(kv_cache);
   a.err = reinterpret_cast<int*>(ws);
   a.tickets = reinterpret_cast<int*>(ws + kTicketOffset);
-  a.ws_ml = reinterpret_cast<float2*>(ws + kMlOffset);
-  a.ws_o = reinterpret_cast<float*>(ws + kMlOffset + static_cast<size_t>(ctas) * 2 * group * sizeof(float2));
+  a.ws_ml = reinterpret_cast<float4*>(ws + kMlOffset);
+  a.ws_o = reinterpret_cast<float*>(ws + kMlOffset + static_cast<size_t>(ctas) * 2 * group * sizeof(float4));
   a.heads = num_heads;
   a.kvh = num_kv_heads;
   a.group = group;

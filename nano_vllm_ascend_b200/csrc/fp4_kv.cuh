@@ -113,13 +113,16 @@ __device__ __forceinline__ HalfRow half_row(uint32_t largest) {  // the bf16x2_a
   const uint32_t f = max(top, 30u) - 30u;
   return HalfRow{f * 0x00800080u, __uint_as_float(top == 255u ? 0x7fffffffu : (127u - 112u + f) << 23)};
 }
-// The factor from a row's products to its scores in log2 units. At least the
-// smallest normal number, so that a masked product, -inf, stays -inf under it
-// (a row of zeros has the smallest `up`, and times a small scale and constant
-// it would be 0): products are below 2^35, so such scores are 0 to fp32 anyway.
+// The factor from a row's products, which are below 2^35, to its scores in log2
+// units, kept where both ends stay numbers. At least the smallest normal, so
+// that a masked product, -inf, stays -inf under it (a row of zeros has the
+// smallest `up`, and times a small scale and constant it would be 0): such
+// scores are 0 to fp32 anyway. At most 2^90, so that scores stay finite:
+// products that differ do so by 2^-34 or more, whose weights are 1 and 0 anyway.
 __device__ __forceinline__ float score_factor(float up, float scale_log2) {
+  constexpr float kLeast = 1.17549435e-38f, kMost = 1.2379400392853803e27f;
   const float f = up * scale_log2;
-  return f < 1.17549435e-38f ? 1.17549435e-38f : f;  // NaN stays
+  return f < kLeast ? kLeast : f > kMost ? kMost : f;  // NaN stays
 }
 __device__ __forceinline__ uint32_t bf16x2_to_half2(uint32_t w, uint32_t base) {
   uint32_t m;  // of magnitudes

@@ -109,6 +109,7 @@ static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsDecode <= 4 * 128, "setmaxnre
 constexpr uint32_t kTmemCols = 512;       // S_0 | S_1 | O_0 | O_1, 128 columns each
 constexpr uint32_t kColO = 256;
 constexpr float kRescaleThreshold = 8.0f;
+constexpr float kFarScore = 1024.f;       // 4-bit kernel: scores whose rounding in fp32, 2^-14, would show in a weight
 constexpr int kItemRing = 4;              // item descriptors published ahead by the producer
 
 struct PrefillArgs {
@@ -702,7 +703,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       if (it.n_kv < 0) break;
       const int i = it.qt * kRows + r;
       const int lim = (i < it.lq) ? (it.lk - it.lq + i) : (it.lk - 1);
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // m: the reference score in log2 units; in the 4-bit kernel its product q . k
       for (int j = 0; j < it.n_kv; ++j, ++g) {
         // warp-uniform outcome: the tcgen05.ld/st below need a converged warp
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[s], g & 1))) { ok = false; break; }
@@ -741,15 +742,46 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) mx[c] = fmax3(mx[c], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-        const float m_new = fmaxf(m, mt);
-        const bool resc = m_new > m + kRescaleThreshold;
-        const float alpha = resc ? fast_exp2(m - m_new) : 1.f;
-        if (resc) {
-          l *= alpha;
-          m = m_new;
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        bool resc;
+        float alpha, neg_mu;
+        if constexpr (kFp4) {
+          resc = (top - m) * sc > kRescaleThreshold;
+          alpha = resc ? fast_exp2((m - top) * sc) : 1.f;
+          if (resc) {
+            l *= alpha;
+            m = top;
+          }
+          neg_mu = (m == -INFINITY) ? 0.f : fmaf(-m, sc, kPShift<true>);
+          // Far from 0 the rounding of neg_mu would reach the weights (and from
+          // 2^22 on lead P out of fp16): the reference is subtracted from the
+          // products instead, which is exact where it matters.
+          if (__any_sync(0xffffffffu, fabsf(neg_mu) > kFarScore)) {
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld32(tmem_s + c * 32, sr[0]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) sr[0][e] = __float_as_uint(__uint_as_float(sr[0][e]) - ref);
+              tmem_st32(tmem_s + c * 32, sr[0]);
+            }
+            tmem_st_wait();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + c * 32, sr[c]);
+            tmem_ld_wait();
+            neg_mu = kPShift<true>;
+          }
+        } else {
+          const float m_new = fmaxf(m, top * sc);
+          resc = m_new > m + kRescaleThreshold;
+          alpha = resc ? fast_exp2(m - m_new) : 1.f;
+          if (resc) {
+            l *= alpha;
+            m = m_new;
+          }
+          neg_mu = (m == -INFINITY) ? 0.f : kPShift<false> - m;
         }
-        const float neg_mu = (m == -INFINITY) ? 0.f : kPShift<kFp4> - m;
         uint64_t sum[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};  // independent add chains
         const uint64_t sc2 = f32x2_pack(sc, sc), mu2 = f32x2_pack(neg_mu, neg_mu);
         // P over the first 64 columns of S_s (column k holds keys 2k and 2k+1

@@ -54,3 +54,32 @@ def test_zero_and_tiny_queries_with_any_constant(cuda_device, which, ks, scale):
     out = attend(which, q, pool, n, scale, ks)
     want, a = orc.attention(q, kr, vr, scale)
     check(out, want, a, vr, DECODE if which == "decode" else PREFILL)
+
+
+def exact_scores_case(dev, n, kvh, m, h):
+    """K rows and queries whose products q . k are multiples of 1/2 below 2^21, so exact in fp32, about +-2^20.2 and 0
+    with differences of a few units; V random."""
+    g = torch.Generator().manual_seed(n + m)
+    levels = torch.tensor([0.0, 0.5, 1, 1.5, 2, 3, 4, 6])
+    k = levels[torch.randint(0, 8, (n, kvh, D), generator=g)] * (torch.randint(0, 2, (n, kvh, D), generator=g) * 2 - 1)
+    k[:, :, 16::16] = 6.0  # every group's scale is 1
+    k[:, :, :16] = 0.0
+    k[:, :, 0] = 2304.0  # 6 * 384
+    q = torch.randint(-3, 4, (m, h, D), generator=g).float()
+    q[:, :, :16] = 0.0
+    q[:, :, 0] = torch.tensor([512.0, -512.0, 0.0, 512.0]).repeat(h // 4)
+    _, v = random_rows(n, kvh, n, spread=False)
+    return q.to(torch.bfloat16).to(dev), k.to(torch.bfloat16), v
+
+
+@pytest.mark.parametrize("which,n,num_ctas", [("decode", 150, 1), ("decode", 3000, 7), ("decode", 5000, 148),
+                                              ("prefill", 300, 0)])
+@pytest.mark.parametrize("e", [-12, -6, 0, 4, 8, 12, 40, 90, 120])
+def test_scores_of_any_magnitude(cuda_device, which, n, num_ctas, e):
+    """Scores of 2^8 to past fp32's largest, whose differences are exact: the weights go by the differences alone."""
+    m = 1 if which == "decode" else 40
+    q, k, v = exact_scores_case(cuda_device, n, 2, m, 8)
+    pool, kr, vr = pool_of(cuda_device, k, v, 32)
+    out = attend(which, q, pool, n, 2.0 ** e, num_ctas=num_ctas)
+    want, a = orc.attention(q, kr, vr, 2.0 ** e)
+    check(out, want, a, vr, DECODE if which == "decode" else PREFILL, f"scale 2^{e}")
