@@ -378,7 +378,9 @@ NVK_API int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, cons
  * values that the first context_lens[b] tokens' codes stand for. out, query:
  * bf16 [batch, num_heads, head_dim], contiguous; num_heads / num_kv_heads any
  * of 1 to 8; scale > 0. block_tables and context_lens (device memory) as in
- * nvk_paged_decode; a length of 0 (or below) yields zeros.
+ * nvk_paged_decode; a length of 0 (or below) yields zeros. A weight is rounded
+ * to fp16, twice, and to 2^-28 of the largest one: what a token far below that
+ * one gives is off by at most 2^-29 of the largest |v| of the KV head.
  * workspace: nvk_fp4_paged_decode_workspace_size bytes, zeroed once; every
  * call leaves it ready for the next one of any batch, with as many heads, KV
  * heads and CTAs or with others, as long as it is large enough. Calls that

@@ -11,12 +11,14 @@
 //   O^T[16 dims x 8 heads] (8 tiles) += V^T[16 dims x 16 tokens] . P^T
 // K and V enter as e2m1 -> fp16 (one conversion for two values): exact. K's
 // scales multiply the fp32 sums of their groups, V's the weights: P s is
-// rounded to fp16 twice (P, then the product: 2^-10 of a weight), with 2^4 p s
-// normal down to 2^-18. Q is scaled by a power of two into fp16's range, which
-// holds its 8 bits exactly. Scores, maxima, sums and O are fp32; the last
-// division is a product with an approximate reciprocal (2^-21, below bf16's
-// half step of 2^-8; the exact one is 2 KB of code, and code that runs once
-// costs its fetch).
+// rounded to fp16 twice (P, then the product: 2^-10 of a weight). 2^4 p is
+// normal down to p = 2^-18, and the scales are held times a power of two that
+// brings the largest one so far near 448, so that however small V is, the
+// product loses nothing beside that. Q is scaled by a power of two into fp16's
+// range, which holds its 8 bits exactly. Scores, maxima, sums and O are fp32;
+// the last division is a product with an approximate reciprocal (2^-21, below
+// bf16's half step of 2^-8; the exact one is 2 KB of code, and code that runs
+// once costs its fetch).
 //
 // Data: every warp streams its tiles (two units, 32 tokens) through a ring of
 // its own in shared memory, one bulk copy of 4608 contiguous bytes a tile (two
@@ -59,7 +61,7 @@ constexpr int kMinTiles = 8;
 constexpr int kMostPieces = 32;
 constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
 constexpr float kRescale = 3.f;  // log2 by which a score may pass the reference before that moves and O is rescaled
-constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and scales up to 448, P s fits fp16 (p goes
+constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and scales up to 480, P s fits fp16 (p goes
                                  // by differences of products, so that this holds for scores of any magnitude)
 constexpr size_t kTicketOffset = 256;
 constexpr size_t kMlOffset = kTicketOffset + kMaxCtas * sizeof(int);
@@ -127,6 +129,8 @@ struct State {
   float thr[2];            // the product above which it moves: by kRescale in log2 units (-inf at first)
   float l[2];              // this lane's part of the sum of p
   float o[kGroups][4];     // O^T: dims 16 j + 2 g (heads 2 t, 2 t + 1), then 16 j + 2 g + 1 (the same)
+  uint32_t room;           // V's scales, and so O, are held times 2^e (e of 0 to 15), such that the largest scale so
+                           // far stays below 512; 8 e in every byte
 };
 
 __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
@@ -171,26 +175,48 @@ __device__ __forceinline__ void load_q(const DecodeArgs& a, int b, int h, int g,
   st.ref[0] = st.ref[1] = 0.f;
   st.thr[0] = st.thr[1] = -INFINITY;
   st.l[0] = st.l[1] = 0.f;
+  st.room = 15 * 0x08080808u;
 #pragma unroll
   for (int j = 0; j < kGroups; ++j)
 #pragma unroll
     for (int c = 0; c < 4; ++c) st.o[j][c] = 0.f;
 }
 
-// A unit's V scales to fp16, once for the whole warp: lane i converts word i.
-// Tokens from `valid` on get scales of 0, so that nothing that their bytes
-// hold (a NaN) meets their weights of 0.
+// A unit's V scales, word `lane`: group lane % 8 of the quad lane / 8. Tokens
+// from `valid` on get scales of 0, so that nothing that their bytes hold (a NaN)
+// meets their weights of 0.
 template <bool kMask>
-__device__ __forceinline__ void convert_vscales(uint32_t unit, uint32_t to, int valid, int lane) {
+__device__ __forceinline__ uint32_t vscale_word(uint32_t unit, int valid, int lane) {
   uint32_t w = ld_shared(unit + kOffVScale + 4 * lane);
-  const int quad = lane >> 3, j = lane & 7;
   if (kMask) {
-    const int n = min(max(valid - 4 * quad, 0), 4);
+    const int n = min(max(valid - 4 * (lane >> 3), 0), 4);
     w &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1;
   }
+  return w;
+}
+// A scale byte's exponent field, its bits 3 to 6, has to be at most 15 - e.
+__device__ __forceinline__ bool above(uint32_t w, uint32_t room) { return (w + room) & 0x80808080u; }
+// Lowers the power of two to what the tile's scales allow, and O with it.
+__device__ __forceinline__ void make_room(State& st, uint32_t w0, uint32_t w1) {
+  uint32_t m = __vmaxu4(w0, w1) & 0x78787878u;
+  m = __vmaxu4(m, m >> 16);
+  m = __reduce_max_sync(0xffffffffu, max(m & 0xffu, (m >> 8) & 0xffu));
+  const uint32_t old = st.room & 0xffu, now = min(old, 15u * 8 - m);
+  st.room = now * 0x01010101u;
+  if (!__any_sync(0xffffffffu, st.thr[0] != -INFINITY || st.thr[1] != -INFINITY)) return;  // O is 0 yet (or NaN)
+  const float f = __uint_as_float((127u << 23) - ((old - now) << 20));
+#pragma unroll
+  for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) st.o[j][c] *= f;
+}
+// The words to fp16, once for the whole warp, times the power of two (exact).
+__device__ __forceinline__ void convert_vscales(const State& st, uint32_t w, uint32_t to, int lane) {
+  const int quad = lane >> 3, j = lane & 7;
+  const uint32_t up = 0x3c003c00u + ((st.room & 0x00ff00ffu) << 7);
   uint32_t lo, hi;
   e4m3_to_half2(w, lo, hi);
-  st_shared_v2(to + 64 * (j >> 1) + 16 * quad + 8 * (j & 1), lo, hi);
+  st_shared_v2(to + 64 * (j >> 1) + 16 * quad + 8 * (j & 1), hmul2(lo, up), hmul2(hi, up));
 }
 
 // Scores of one unit (without the factor sc): x[0], x[1] of token ta's heads
@@ -265,8 +291,11 @@ __device__ __forceinline__ void weigh(State& st, uint32_t unit, uint32_t vscale,
 template <bool kMask>
 __device__ __forceinline__ void attend(State& st, uint32_t tile, uint32_t vscale, int valid, int g, int t, int lane) {
   __syncwarp();  // the tile before this one is done with vscale
-  convert_vscales<kMask>(tile, vscale, valid, lane);
-  convert_vscales<kMask>(tile + kUnitBytes, vscale + kVScaleBytes, valid - kUnitTokens, lane);
+  const uint32_t w0 = vscale_word<kMask>(tile, valid, lane);
+  const uint32_t w1 = vscale_word<kMask>(tile + kUnitBytes, valid - kUnitTokens, lane);
+  if (__any_sync(0xffffffffu, above(w0, st.room) || above(w1, st.room))) make_room(st, w0, w1);
+  convert_vscales(st, w0, vscale, lane);
+  convert_vscales(st, w1, vscale + kVScaleBytes, lane);
   float x[2][4];
   scores<kMask>(st, tile, valid, g, t, x[0]);
   scores<kMask>(st, tile + kUnitBytes, valid - kUnitTokens, g, t, x[1]);
@@ -430,12 +459,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
       st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], off);
       st.l[1] += __shfl_xor_sync(0xffffffffu, st.l[1], off);
     }
+    const float down = __uint_as_float((127u << 23) - ((st.room & 0xffu) << 20));
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int head = 2 * t + e;
       if (head >= a.group) continue;
       if (whole) {
-        const float inv = st.l[e] == 0.f ? 0.f : __fdividef(a.v_scale, st.l[e]);
+        const float inv = st.l[e] == 0.f ? 0.f : __fdividef(a.v_scale, st.l[e]) * down;
         __nv_bfloat16* row = a.out + (static_cast<int64_t>(b) * a.heads + h * a.group + head) * kD + 2 * g;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
@@ -445,7 +475,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
         if (g == 0) piece_ml[at] = make_float4(st.thr[e] == -INFINITY ? -INFINITY : st.ref[e], st.l[e], st.sc[e], 0.f);
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
-          *reinterpret_cast<float2*>(piece_o(2 * warp + slot) + head * kD + 16 * j + 2 * g) = make_float2(st.o[j][e], st.o[j][2 + e]);
+          *reinterpret_cast<float2*>(piece_o(2 * warp + slot) + head * kD + 16 * j + 2 * g) =
+              make_float2(st.o[j][e] * down, st.o[j][2 + e] * down);
       }
     }
     if (!whole && lane == 0) sm.piece_pair[2 * warp + slot] = b * a.kvh + h;

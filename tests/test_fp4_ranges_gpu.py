@@ -83,3 +83,57 @@ def test_scores_of_any_magnitude(cuda_device, which, n, num_ctas, e):
     out = attend(which, q, pool, n, 2.0 ** e, num_ctas=num_ctas)
     want, a = orc.attention(q, kr, vr, 2.0 ** e)
     check(out, want, a, vr, DECODE if which == "decode" else PREFILL, f"scale 2^{e}")
+
+
+def check_relative(got, want, a, v, how):
+    """As ``check``, with what small weights lose counted against the largest |v| of the same KV head: half of fp16's
+    smallest step over the power of two that p is held with, and 2^-36 for the products with the scales, which are
+    held with the largest of them near fp16's end (half of 2^-24 of a code of 6, over 2^4 p and 2^8 of the scale)."""
+    n, kvh, _ = v.shape
+    top = v.abs().amax((0, 2)).repeat_interleave(got.shape[1] // kvh)[None, :, None]
+    tol = want.abs() * 2.0 ** -8 + a * how["per_a"] + n * (how["step"] + 2.0 ** -36) * top + 1e-30
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), f"off by up to {float((err / tol).max()):.2f} tolerances"
+
+
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+@pytest.mark.parametrize("far", [8, 16, 20, 23])
+@pytest.mark.parametrize("at", [0, 7000, 20479])
+@pytest.mark.parametrize("s", [2.0 ** -9, 3 * 2.0 ** -9, 2.0 ** -6, 1.0, 448.0])
+def test_a_long_tail_of_small_rows_behind_one_dominant_token(cuda_device, which, far, at, s):
+    """20479 tokens of weight 2^-far beside one whose V is zero: the output is the tail's share, for V of every
+    magnitude that the format holds. One CTA, so that a warp has hundreds of the tail beside the dominant token."""
+    dev, n, kvh, h = cuda_device, 20480, 1, 4
+    g = torch.Generator().manual_seed(far)
+    v = s * torch.tensor([3.0, 4.0, 6.0])[torch.randint(0, 3, (n, kvh, D), generator=g)]
+    v[:, :, ::16] = 6.0 * s  # every group of the tail has its scale
+    k = torch.zeros(n, kvh, D)
+    v[at], k[at, :, 5] = 0.0, 6.0
+    pool, kr, vr = pool_of(dev, k.to(torch.bfloat16), v.to(torch.bfloat16), 256)
+    assert torch.equal(vr.cpu(), v.double())
+    q = torch.zeros(1, h, D, dtype=torch.bfloat16, device=dev)
+    q[:, :, 5] = 1.0
+    scale = far / 6 / 1.4426950408889634
+    out = attend(which, q, pool, n, scale, num_ctas=1)
+    want, a = orc.attention(q, kr, vr, scale)
+    check_relative(out, want, a, vr, DECODE if which == "decode" else PREFILL)
+
+
+@pytest.mark.parametrize("num_ctas", [1, 5, 148])
+@pytest.mark.parametrize("h", [3, 8])
+def test_v_groups_whose_scales_grow(cuda_device, num_ctas, h):
+    """Groups of random magnitude, larger from token to token here and smaller there, some of zeros, over all splits."""
+    n, kvh = 3000, 1
+    g = torch.Generator().manual_seed(h)
+    k, v = random_rows(n, kvh, 77, spread=False)
+    e = torch.randint(-9, 9, (n, kvh, 8, 1), generator=g).float()
+    e[:, :, 0] = torch.linspace(-9, 8, n)[:, None, None]  # grows
+    e[:, :, 1] = torch.linspace(8, -9, n)[:, None, None]
+    e[:, :, 2] = -8.0
+    v = (v.float().view(n, kvh, 8, 16) * torch.exp2(e)).view(n, kvh, D)
+    v[:, :, 48:64] = 0.0
+    pool, kr, vr = pool_of(cuda_device, k, v.to(torch.bfloat16), 32)
+    q = torch.randn(1, h, D, generator=g).to(torch.bfloat16).to(cuda_device)
+    out = attend("decode", q, pool, n, SCALE, num_ctas=num_ctas)
+    want, a = orc.attention(q, kr, vr, SCALE)
+    check_relative(out, want, a, vr, DECODE)
