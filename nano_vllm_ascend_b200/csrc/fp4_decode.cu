@@ -293,11 +293,11 @@ __device__ __forceinline__ void attend(State& st, uint32_t tile, uint32_t vscale
   __syncwarp();  // the tile before this one is done with vscale
   const uint32_t w0 = vscale_word<kMask>(tile, valid, lane);
   const uint32_t w1 = vscale_word<kMask>(tile + kUnitBytes, valid - kUnitTokens, lane);
+  float x[2][4];
+  scores<kMask>(st, tile, valid, g, t, x[0]);
   if (__any_sync(0xffffffffu, above(w0, st.room) || above(w1, st.room))) make_room(st, w0, w1);
   convert_vscales(st, w0, vscale, lane);
   convert_vscales(st, w1, vscale + kVScaleBytes, lane);
-  float x[2][4];
-  scores<kMask>(st, tile, valid, g, t, x[0]);
   scores<kMask>(st, tile + kUnitBytes, valid - kUnitTokens, g, t, x[1]);
   const float hi0 = fmaxf(fmax3(x[0][0], x[0][2], x[1][0]), x[1][2]);
   const float hi1 = fmaxf(fmax3(x[0][1], x[0][3], x[1][1]), x[1][3]);
