@@ -384,13 +384,17 @@ NVK_API int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, cons
  * workspace: nvk_fp4_paged_decode_workspace_size bytes, zeroed once; every
  * call leaves it ready for the next one of any batch, with as many heads, KV
  * heads and CTAs or with others, as long as it is large enough. Calls that
- * share one must be ordered on one stream. Its first int is the error word
- * (bits as for nvk_paged_decode; blocks outside the pool read as zeros).
+ * share one must be ordered on one stream. Only its first
+ * NVK_FP4_DECODE_ZEROED_BYTES have to be zero. Its first int is the error word
+ * (bits as for nvk_paged_decode; blocks outside the pool read as zeros);
+ * nvk_fp4_paged_decode_reporting sets those bits in error_word instead (NULL: as
+ * nvk_fp4_paged_decode), which may be one for the calls of many workspaces.
  * block_tables and context_lens are step metadata, read while the kernel
  * before this one in the stream drains: what writes them on the stream must be
  * a copy, nvk_decode_metadata or a kernel that is not launched with
  * programmatic stream serialisation.
  */
+#define NVK_FP4_DECODE_ZEROED_BYTES 4352
 NVK_API int nvk_fp4_paged_decode_workspace_size(int num_heads, int num_kv_heads, int head_dim, int num_ctas,
                                                 size_t* bytes);
 NVK_API int nvk_fp4_paged_decode(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
@@ -398,6 +402,12 @@ NVK_API int nvk_fp4_paged_decode(void* out, const void* query, const void* kv_ca
                                  const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,
                                  int head_dim, float scale, float k_scale, float v_scale, int num_ctas,
                                  void* workspace, size_t workspace_bytes, nvk_stream_t stream);
+NVK_API int nvk_fp4_paged_decode_reporting(void* out, const void* query, const void* kv_cache, int num_blocks,
+                                           int block_size, const int32_t* block_tables, int block_table_stride,
+                                           int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                                           int num_heads, int num_kv_heads, int head_dim, float scale, float k_scale,
+                                           float v_scale, int num_ctas, void* workspace, size_t workspace_bytes,
+                                           int* error_word, nvk_stream_t stream);
 
 /*
  * nvk_paged_prefill over a 4-bit pool (same masking; num_heads any multiple

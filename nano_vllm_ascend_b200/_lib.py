@@ -118,6 +118,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _i32, _i32, _f32,
          _f32, _f32, _i32, _c_void_p, _size_t, _c_void_p],
     ),
+    "nvk_fp4_paged_decode_reporting": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _i32, _i32, _f32,
+         _f32, _f32, _i32, _c_void_p, _size_t, _c_void_p, _c_void_p],
+    ),
     "nvk_fp4_paged_prefill": (
         _i32,
         [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32,
@@ -127,6 +132,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
 
 FP4_UNIT_TOKENS = 16
 FP4_UNIT_BYTES = 2304
+FP4_DECODE_ZEROED_BYTES = 4352
 
 MAX_PEERS = 8
 PEER_HANDLE_BYTES = 64

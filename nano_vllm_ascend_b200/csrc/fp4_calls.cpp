@@ -30,7 +30,7 @@ constexpr int64_t kHeadDim = 128;
 decltype(&nvk_fp4_append) entry_append = nullptr;
 decltype(&nvk_fp4_read) entry_read = nullptr;
 decltype(&nvk_fp4_qk_norm_rope_append) entry_norm = nullptr;
-decltype(&nvk_fp4_paged_decode) entry_decode = nullptr;
+decltype(&nvk_fp4_paged_decode_reporting) entry_decode = nullptr;
 decltype(&nvk_fp4_paged_prefill) entry_prefill = nullptr;
 
 struct Leave {};  // thrown where a call is left to the wrapper
@@ -234,9 +234,9 @@ Attention attention(PyObject* const* a, PyObject* lens_object, c10::Device dev) 
                    to_int(query.size(1))};
 }
 
-// decode(out, query, kv_cache, block_tables, context_lens, scale, workspace, num_ctas, k_scale, v_scale)
+// decode(out, query, kv_cache, block_tables, context_lens, scale, workspace, num_ctas, k_scale, v_scale, error_word)
 PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return call(n, 10, [&] {
+  return call(n, 11, [&] {
     need(entry_decode);
     const c10::Device dev = call_device(tensor(a[1]));
     const Attention t = attention(a, a[4], dev);
@@ -246,7 +246,8 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return PyLong_FromLong(entry_decode(t.out.data_ptr(), t.query.data_ptr(), t.pool.data, t.pool.blocks,
                                         t.pool.block_size, t.tables, t.table_stride, t.table_columns, t.lens, t.batch,
                                         t.heads, t.pool.kv_heads, kHeadDim, number(a[5]), number(a[8]), number(a[9]),
-                                        integer(a[7]), ws.data_ptr(), ws.nbytes(), stream_on(dev)));
+                                        integer(a[7]), ws.data_ptr(), ws.nbytes(), error_ptr(a[10], dev),
+                                        stream_on(dev)));
   });
 }
 

@@ -65,6 +65,7 @@ constexpr float kPShift = 4.f;   // P is held as 2^4 p: with p up to 2^3 and sca
                                  // by differences of products, so that this holds for scores of any magnitude)
 constexpr size_t kTicketOffset = 256;
 constexpr size_t kMlOffset = kTicketOffset + kMaxCtas * sizeof(int);
+static_assert(kMlOffset == NVK_FP4_DECODE_ZEROED_BYTES, "what has to be zero is the error word and the tickets");
 
 struct DecodeArgs {
   __nv_bfloat16* out;
@@ -791,8 +792,19 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
                                     int block_size, const int32_t* block_tables, int block_table_stride,
                                     int max_blocks_per_seq, const int32_t* context_lens, int batch, int num_heads,
                                     int num_kv_heads, int head_dim, float scale, float k_scale, float v_scale,
-                                    int num_ctas, void* workspace, size_t workspace_bytes_given,
-                                    nvk_stream_t stream) {
+                                    int num_ctas, void* workspace, size_t workspace_bytes, nvk_stream_t stream) {
+  return nvk_fp4_paged_decode_reporting(out, query, kv_cache, num_blocks, block_size, block_tables,
+                                        block_table_stride, max_blocks_per_seq, context_lens, batch, num_heads,
+                                        num_kv_heads, head_dim, scale, k_scale, v_scale, num_ctas, workspace,
+                                        workspace_bytes, nullptr, stream);
+}
+
+extern "C" int nvk_fp4_paged_decode_reporting(void* out, const void* query, const void* kv_cache, int num_blocks,
+                                              int block_size, const int32_t* block_tables, int block_table_stride,
+                                              int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                                              int num_heads, int num_kv_heads, int head_dim, float scale,
+                                              float k_scale, float v_scale, int num_ctas, void* workspace,
+                                              size_t workspace_bytes_given, int* error_word, nvk_stream_t stream) {
   using namespace nvk;
   using namespace nvk::fp4;
   const char* who = "fp4_paged_decode";
@@ -825,7 +837,7 @@ extern "C" int nvk_fp4_paged_decode(void* out, const void* query, const void* kv
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeArgs a;
   a.pool = static_cast<const uint8_t*>(kv_cache);
-  a.err = reinterpret_cast<int*>(ws);
+  a.err = error_word ? error_word : reinterpret_cast<int*>(ws);
   a.tickets = reinterpret_cast<int*>(ws + kTicketOffset);
   a.ws_ml = reinterpret_cast<float4*>(ws + kMlOffset);
   a.ws_o = reinterpret_cast<float*>(ws + kMlOffset + static_cast<size_t>(ctas) * 2 * group * sizeof(float4));

@@ -17,9 +17,9 @@ the exceptions the reference raises for the same inputs:
 All of them are ``KVCacheDeviceError`` (a ``RuntimeError``; the slot case is
 also an ``IndexError``), carrying the raw ``bits``.
 
-Each device has one error word shared by the append and prefill launches of
-the drop-in classes; decode launches report into the head of their split-K
-workspace, which is registered here. Reading a word needs the stream, so the
+Each device has one error word shared by the append, prefill and 4-bit decode
+launches of the drop-in classes; bf16 decode and decode graphs report into the
+head of their split-K workspace, which is registered here. Reading a word needs the stream, so the
 drop-ins do it without blocking: after a launch, if no read is in flight, the
 words launched since the last read are copied into pinned host memory behind
 an event; the next call raises once that copy has landed and shows a bit.
@@ -74,14 +74,14 @@ def error_for(bits: int, where: str) -> KVCacheDeviceError:
     return cls(msg, bits)
 
 
-SHARED = "kv append / prefill"
+SHARED = "kv append / prefill / 4-bit decode"
 
 
 class DeviceErrorState:
     """The error words of one device and the read in flight (see the module docstring).
 
     Words are keyed by a name that also appears in the raised message; the
-    shared append/prefill word is ``SHARED``.
+    shared word is ``SHARED``.
     """
 
     def __init__(self, device: torch.device):

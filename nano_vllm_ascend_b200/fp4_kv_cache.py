@@ -87,6 +87,8 @@ class PagedKVCacheFp4:
         shape = (num_layers, *ops_fp4.pool_shape(num_blocks, block_size, num_kv_heads))
         constants = zip(_constants("k_scale", k_scale, num_layers), _constants("v_scale", v_scale, num_layers))
         self.kv_cache = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+        if self.device.type == "cuda":
+            device_errors.state(self.device)  # its word exists before any call over this cache is captured
         self.layers = [Fp4Layer(self.kv_cache[i], ks, vs) for i, (ks, vs) in enumerate(constants)]
 
     @property

@@ -50,7 +50,7 @@ def pool_shape(num_blocks: int, block_size: int, num_kv_heads: int) -> tuple[int
 # are looked up once.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _NOT_TAKEN = 1
-_BOUND = ("nvk_fp4_append", "nvk_fp4_read", "nvk_fp4_qk_norm_rope_append", "nvk_fp4_paged_decode",
+_BOUND = ("nvk_fp4_append", "nvk_fp4_read", "nvk_fp4_qk_norm_rope_append", "nvk_fp4_paged_decode_reporting",
           "nvk_fp4_paged_prefill")
 
 
@@ -275,18 +275,21 @@ def _check_attention(who: str, dev, out, query, kv_cache, block_tables, lens) ->
 
 def paged_decode_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
                      context_lens: torch.Tensor, scale: float, workspace: torch.Tensor, num_ctas: int = 0,
-                     k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
+                     k_scale: float = 1.0, v_scale: float = 1.0,
+                     error_word: torch.Tensor | None = None) -> torch.Tensor:
     """Paged GQA decode attention over a 4-bit pool into ``out`` ([batch, heads, 128] bf16).
 
     1 to 8 query heads per KV head. ``workspace`` (uint8, zeroed once) must
     hold decode_fp4_workspace_bytes(heads, kv_heads); calls sharing it must be
-    ordered on one stream. Its first int32 is the device error word.
+    ordered on one stream. Device errors are bits of ``error_word``, or of the
+    workspace's first int32.
     """
-    rc = _decode(out, query, kv_cache, block_tables, context_lens, scale, workspace, num_ctas, k_scale, v_scale)
+    rc = _decode(out, query, kv_cache, block_tables, context_lens, scale, workspace, num_ctas, k_scale, v_scale,
+                 error_word)
     if rc == 0:
         return out
     if rc != _NOT_TAKEN:
-        _lib.check("nvk_fp4_paged_decode", rc)
+        _lib.check("nvk_fp4_paged_decode_reporting", rc)
     who = "paged_decode_fp4"
     dev = query.device
     shape, nb, bs, kvh, batch, stride, width = _check_attention(who, dev, out, query, kv_cache, block_tables,
@@ -295,9 +298,9 @@ def paged_decode_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Ten
         _wrong_device(dev, workspace=workspace)
     if shape[0] != batch or not workspace.is_contiguous():
         raise ValueError(f"{who}: {shape[0]} queries for {batch} sequences, or a strided workspace")
-    _call(dev, "nvk_fp4_paged_decode", out.data_ptr(), query.data_ptr(), kv_cache.data_ptr(), nb, bs,
+    _call(dev, "nvk_fp4_paged_decode_reporting", out.data_ptr(), query.data_ptr(), kv_cache.data_ptr(), nb, bs,
           block_tables.data_ptr(), stride, width, context_lens.data_ptr(), batch, shape[1], kvh, HEAD_DIM, scale,
-          k_scale, v_scale, num_ctas, workspace.data_ptr(), workspace.nbytes)
+          k_scale, v_scale, num_ctas, workspace.data_ptr(), workspace.nbytes, _error_ptr(who, error_word, dev))
     return out
 
 

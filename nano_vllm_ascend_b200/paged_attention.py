@@ -20,7 +20,9 @@ workspace's error word and raised by ``device_errors`` on a following call
 or by ``device_errors.check_errors()``.
 
 Over a ``PagedKVCacheFp4`` both cache arguments are the layer's ``Fp4Layer``
-and the 4-bit decode kernel runs.
+and the 4-bit decode kernel runs. It reports into the device's shared error
+word, also from graphs that the caller captures (``check_errors()`` raises what
+their replays found), and from a ``DecodeGraphRunner`` into its workspace's.
 """
 
 from __future__ import annotations
@@ -31,6 +33,7 @@ import torch
 from torch import nn
 
 from . import device_errors, ops, ops_fp4
+from ._lib import FP4_DECODE_ZEROED_BYTES
 from .cuda_graph import graph_workspace
 from .fp4_kv_cache import Fp4Layer
 from .paged_kv_cache import take_deferred
@@ -73,17 +76,19 @@ def shared_workspace(device: torch.device, nbytes: int, shape: tuple = ()) -> to
 _FP4_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _fp4_workspace(device: torch.device, nbytes: int) -> tuple[torch.Tensor, bool]:
-    """A zeroed workspace, and whether it is kept. A call that a caller's own
-    graph captures gets one of its own, zeroed by each replay, so that graphs
-    may be replayed in any order (and none is left to eager calls)."""
+def _fp4_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """A workspace whose head is zero. A call that a caller's own graph
+    captures gets one of its own, its head zeroed by each replay, so that
+    graphs may be replayed in any order (and none is left to eager calls)."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device), False
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:FP4_DECODE_ZEROED_BYTES].zero_()
+        return ws
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
     ws = _FP4_WORKSPACES.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = _FP4_WORKSPACES[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return ws, True
+    return ws
 
 
 class PagedAttention(nn.Module):
@@ -161,14 +166,12 @@ class PagedAttention(nn.Module):
             workspace = graph_workspace(self._fp4, q.shape[0], "(4-bit)")
             word = None  # the graph runner reads its slot's word after each replay
             if workspace is None:
-                workspace, kept = _fp4_workspace(device, self._fp4.workspace_bytes(q.shape[0]))
-                if kept:
-                    word = errors.watch(f"4-bit paged decode, stream {torch.cuda.current_stream().cuda_stream:#x}",
-                                        workspace)
+                workspace = _fp4_workspace(device, self._fp4.workspace_bytes(q.shape[0]))
+                word = errors.word
             tables = block_tables.to(device=device, dtype=torch.int32)
             ctx = context_lens.to(device=device, dtype=torch.int32)
             ops_fp4.paged_decode_fp4(output, q.contiguous(), layer.pool, tables, ctx, self.scale, workspace,
-                                     self.num_ctas, layer.k_scale, layer.v_scale)
+                                     self.num_ctas, layer.k_scale, layer.v_scale, word)
             if word is not None:
-                errors.launched(word)
+                errors.launched()
         return output
