@@ -23,10 +23,13 @@ head of their split-K workspace, which is registered here. Reading a word needs 
 drop-ins do it without blocking: after a launch, if no read is in flight, the
 words launched since the last read are copied into pinned host memory behind
 an event; the next call raises once that copy has landed and shows a bit.
-Bits are sticky until raised (the word is then cleared on the stream), so
-nothing is lost between reads. ``check_errors()`` reads every word now
-(synchronising the current stream) and raises; a step driver calls it once
-per step, and ``DecodeGraphRunner`` reads its entry's words after each replay.
+Bits are sticky until raised (the words are then read again and cleared with
+the device idle, whichever stream set them), so nothing is lost between reads.
+``check_errors()`` reads every word now, behind the launches of all streams
+(waiting for the current stream), and raises; a step driver calls it once per
+step, and ``DecodeGraphRunner`` reads its entry's words after each replay. What
+replays of a caller's own graph found is in the words too; such a replay is
+behind ``check_errors()`` if it was on the current stream or has been waited for.
 Nothing here runs while a stream is capturing.
 """
 
@@ -90,6 +93,9 @@ class DeviceErrorState:
         self._words: dict[str, torch.Tensor] = {SHARED: self.word}
         self._dirty: set[str] = set()
         self._inflight: tuple[torch.cuda.Event | None, torch.Tensor, list[str]] | None = None
+        # Streams with launches since the last check, by their handles: an event behind the latest one (the default
+        # stream, 0, is always there to ask and needs none).
+        self._launches: dict[int, torch.cuda.Event | None] = {}
 
     def watch(self, name: str, word: torch.Tensor) -> str:
         """Registers (or replaces) the device word called ``name``: the first int32 of
@@ -112,6 +118,13 @@ class DeviceErrorState:
         if torch.cuda.is_current_stream_capturing():
             return
         self._dirty.update(names or (SHARED,))
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        if stream and self._launches.get(stream) is None:
+            self._launches[stream] = torch.cuda.Event()
+        if stream:
+            self._launches[stream].record(torch.cuda.current_stream(self.device))
+        else:
+            self._launches[0] = None
         self._poll()
 
     def _poll(self) -> None:
@@ -136,15 +149,25 @@ class DeviceErrorState:
     def _raise_from(self, inflight) -> None:
         _, host, names = inflight
         self._inflight = None
-        flagged = [(n, int(v)) for n, v in zip(names, host.tolist()) if v]
+        flagged = {n: v for n, v in zip(names, host.tolist()) if v}
         if not flagged:
             return
+        # What other streams' kernels set until here is raised with it, and none runs while the words are cleared.
+        torch.cuda.synchronize(self.device)
+        names = list(self._words)
+        host = self._copy_out(names)
+        torch.cuda.current_stream(self.device).synchronize()
+        for n, v in zip(names, host.tolist()):
+            if v:
+                flagged[n] = flagged.get(n, 0) | v
+                self._words[n].zero_()
+        torch.cuda.current_stream(self.device).synchronize()
+        self._dirty.clear()
+        self._launches.clear()
         bits = 0
-        for n, v in flagged:
+        for v in flagged.values():
             bits |= v
-            if n in self._words:
-                self._words[n].zero_()  # stream-ordered: later launches start clean
-        raise error_for(bits, ", ".join(sorted(n for n, _ in flagged)))
+        raise error_for(bits, ", ".join(sorted(flagged)))
 
     def raise_if_flagged(self) -> None:
         """Raises if a completed read shows an error bit (does not wait)."""
@@ -154,14 +177,20 @@ class DeviceErrorState:
             self._raise_from(self._inflight)
 
     def check(self) -> None:
-        """Reads every registered word now (waits for the current stream) and raises on any bit."""
+        """Reads every registered word now, behind the launches of all streams (waits for the current stream), and
+        raises on any bit."""
         if self._inflight is not None:
             self._inflight[0].synchronize()
             self._raise_from(self._inflight)
         names = list(self._words)
         self._dirty.clear()
+        current = torch.cuda.current_stream(self.device)
+        for stream, event in self._launches.items():
+            if stream != current.cuda_stream:
+                current.wait_event(event or torch.cuda.default_stream(self.device).record_event())
+        self._launches.clear()
         host = self._copy_out(names)
-        torch.cuda.current_stream(self.device).synchronize()
+        current.synchronize()
         self._raise_from((None, host, names))
 
 

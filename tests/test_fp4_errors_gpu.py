@@ -66,3 +66,62 @@ def test_decode_reports_where_it_is_told_to(cuda_device):
     for wrong in (word.long(), word.cpu(), word[:0]):
         with pytest.raises(ValueError, match="error_word"):
             ops_fp4.paged_decode_fp4(out, q, layer.pool, table, ctx, 0.1, ws, error_word=wrong)
+
+
+def test_check_errors_waits_for_other_streams(cuda_device):
+    """A call on a stream that is still busy when another stream asks for errors."""
+    dev = cuda_device
+    attn, layer, q, table, ctx = setup(dev)
+    attn(q, *layer, table, ctx)
+    check_errors(dev)
+    bad = table + 9
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(SLEEP)
+        attn(q, *layer, table, ctx)  # its read of the word is in flight for a while ...
+        torch.cuda._sleep(SLEEP)
+        attn(q, *layer, bad, ctx)    # ... so this call's waits for the next one
+    with pytest.raises(KVCacheDeviceError, match="outside the KV pool"):
+        check_errors(dev)
+    check_errors(dev)
+
+
+def test_clearing_a_word_loses_nothing_of_another_stream(cuda_device):
+    """One stream's error is raised there and cleared late, behind other work; a replay on another stream sets
+    another one meanwhile."""
+    dev = cuda_device
+    attn, layer, q, table, ctx = setup(dev)
+    bad, far = table + 9, ctx + BS
+    side = torch.cuda.Stream(dev)
+    with torch.cuda.stream(side):
+        attn(q, *layer, table, ctx)
+    torch.cuda.synchronize(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attn(q, *layer, table, far)
+    attn(q, *layer, bad, ctx)
+    torch.cuda.synchronize(dev)  # the read of the word has landed
+    torch.cuda._sleep(SLEEP)
+    with pytest.raises(KVCacheDeviceError, match="outside the KV pool"):
+        attn(q, *layer, table, ctx)  # raises before it launches; the word is cleared behind the sleep
+    with torch.cuda.stream(side):
+        graph.replay()
+    torch.cuda.synchronize(dev)
+    with pytest.raises(RuntimeError, match="missing block"):
+        check_errors(dev)
+    check_errors(dev)
+
+
+def test_an_error_is_not_raised_twice(cuda_device):
+    dev = cuda_device
+    attn, layer, q, table, ctx = setup(dev)
+    streams = [torch.cuda.Stream(dev) for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(s):
+            attn(q, *layer, table + 9, ctx)
+            s.synchronize()
+        with pytest.raises(KVCacheDeviceError):
+            check_errors(dev)
+        check_errors(dev)
