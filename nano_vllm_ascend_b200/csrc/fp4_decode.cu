@@ -55,9 +55,11 @@ constexpr int kMaxCtas = 1024;
 // give its joins more pieces (one sequence of 100 / 1000 tokens, 8 KV heads:
 // 4.8 / 7.1 us with 8, 6.0 / 8.3 with 16).
 constexpr int kMinTiles = 8;
-// CTAs per pair above which no more are used: the join reads the pieces of a
+// CTAs that the longest pair may be cut over: the join reads the pieces of a
 // pair one after another (one sequence of 40000 tokens, one KV head, 8 query
 // heads: 18.3 us with 32, 21.2 with 48, 42 with 148; 2 heads: 12.9, 12.9, 15.1).
+// The longest one's tiles count, not the number of pairs: short and empty
+// sequences beside it take no share of its pieces.
 constexpr int kMostPieces = 32;
 constexpr int kMaxGroup = 8;     // query heads per KV head: the columns of a fragment
 constexpr float kRescale = 3.f;  // log2 by which a score may pass the reference before that moves and O is rescaled
@@ -98,7 +100,7 @@ struct Smem {
   uint2 vscale[kWarps][2][kGroups / 2][4][2];  // [unit][j / 2][quad][j % 2]: V's scales of the quad's four tokens, fp16
   uint64_t full[kWarps][kStages];
   int pre[2 * kWarps * 32 + 1];  // tiles before each sequence (of one KV head)
-  int scan[kWarps];
+  int scan[kWarps], most[kWarps];
   int piece_pair[32];
   End end[2];
 };
@@ -394,7 +396,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
       const int v = __shfl_up_sync(0xffffffffu, sum, off);
       if (lane >= off) sum += v;
     }
-    if (lane == 31) sm.scan[warp] = sum;
+    const int most = __reduce_max_sync(0xffffffffu, max(u0, u1));
+    if (lane == 31) sm.scan[warp] = sum, sm.most[warp] = most;
     __syncthreads();
     int before = 0;
     for (int w = 0; w < warp; ++w) before += sm.scan[w];
@@ -413,9 +416,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) decode_kernel(const DecodeArgs
     }
   };
   const int total = sm.pre[a.batch] * a.kvh;  // the entry point keeps it below 2^31
-  const int64_t useful = static_cast<int64_t>(kMostPieces) * a.batch * a.kvh;
-  const int ctas = static_cast<int>(min(useful, static_cast<int64_t>(min(static_cast<int>(gridDim.x),
-                                                                       (total + kMinTiles - 1) / kMinTiles))));
+  int longest = 0;  // tiles of a pair
+  for (int w = 0; w < (a.batch + 63) / 64; ++w) longest = max(longest, sm.most[w]);
+  int ctas = min(static_cast<int>(gridDim.x), (total + kMinTiles - 1) / kMinTiles);
+  if (static_cast<int64_t>(longest) * ctas > static_cast<int64_t>(total) * kMostPieces)
+    ctas = static_cast<int>(static_cast<int64_t>(total) * kMostPieces / longest);
   const int c = blockIdx.x;
   if (c >= ctas) {
     pdl_wait();

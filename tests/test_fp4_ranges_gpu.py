@@ -8,7 +8,7 @@ import torch
 
 from nano_vllm_ascend_b200 import ops_fp4
 from oracle import fp4_oracle as orc
-from tests.test_fp4_gpu import D, DECODE, PREFILL, SCALE, check, random_rows, seq_slots, workspace
+from tests.test_fp4_gpu import D, DECODE, PREFILL, SCALE, check, decode_case, random_rows, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,15 @@ def test_v_groups_whose_scales_grow(cuda_device, num_ctas, h):
     out = attend("decode", q, pool, n, SCALE, num_ctas=num_ctas)
     want, a = orc.attention(q, kr, vr, SCALE)
     check_relative(out, want, a, vr, DECODE)
+
+
+@pytest.mark.parametrize("ctx,kvh,most", [([40000, 0, 1, 10, 0], 1, 33), ([3, 9, 0, 20000] + [1] * 60, 2, 2 * 33),
+                                          ([20000, 20000, 5], 1, 2 * 33 + 1)])
+def test_a_long_sequence_among_short_ones_has_few_pieces(cuda_device, ctx, kvh, most):
+    """A pair's pieces are read one after another by the CTA that joins them: about 32 at most, however many short and
+    empty sequences come with it. Pieces (csrc/fp4_decode.cu): float4 (product, sum, factor) by CTA, end and head."""
+    h, ctas = 2 * kvh, 148
+    ws = workspace(cuda_device, h, kvh, ctas)
+    decode_case(cuda_device, ctx, h, kvh, 64, seed=len(ctx), num_ctas=ctas, ws=ws)
+    sums = ws[4352:4352 + ctas * 2 * 2 * 16].view(torch.float32).view(ctas, 2, 2, 4)[..., 1]
+    assert 2 < int((sums[:, :, 0] > 0).sum()) <= most
