@@ -359,7 +359,7 @@ __device__ __forceinline__ int seq_tiles(const DecodeArgs& a, int b, bool report
     if (report) atomicOr(a.err, kErrContextTooLong);
     n = static_cast<int>(most);
   }
-  return n <= 0 ? 0 : (n + kTileTokens - 1) / kTileTokens;
+  return n <= 0 ? 0 : (n - 1) / kTileTokens + 1;
 }
 
 template <int kWarps>

@@ -149,3 +149,24 @@ def test_a_long_sequence_among_short_ones_has_few_pieces(cuda_device, ctx, kvh, 
     decode_case(cuda_device, ctx, h, kvh, 64, seed=len(ctx), num_ctas=ctas, ws=ws)
     sums = ws[4352:4352 + ctas * 2 * 2 * 16].view(torch.float32).view(ctas, 2, 2, 4)[..., 1]
     assert 2 < int((sums[:, :, 0] > 0).sum()) <= most
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 17, 2 ** 31 - 33])
+def test_the_longest_context_that_the_range_takes(cuda_device, n):
+    """A table of the most columns that the entry point takes (2^31 - 16 tokens), all of them one block: the mean of
+    that block's V (keys of zeros), for the longest contexts and one beyond, which is cut to the table's length."""
+    dev, width = cuda_device, (2 ** 31 - 16) // 16
+    _, v = random_rows(16, 1, 3, spread=False)
+    pool, _, vr = pool_of(dev, torch.zeros_like(v), v, 16)
+    q = torch.randn(1, 1, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+    out = torch.full_like(q, float("nan"))
+    ws = workspace(dev, 1, 1)
+    ops_fp4.paged_decode_fp4(out, q, pool, torch.zeros(1, width, dtype=torch.int32, device=dev),
+                             torch.tensor([n], dtype=torch.int32, device=dev), SCALE, ws)
+    assert int(ws[:4].view(torch.int32).item()) == (8 if n > 16 * width else 0)
+    # The weights are all the same: what rounds are fp32's sums over a warp's 2^26 / (148 * 16) tiles, and the output. A
+    # tile adds two products to O, each off by up to 2^-23 of it (matrix sums may be cut off, not rounded), and twice
+    # to the sum of weights, each off by up to 2^-24 of it.
+    want, mean = vr.mean(0, keepdim=True), vr.abs().mean(0, keepdim=True)
+    tol = want.abs() * 2.0 ** -8 + mean * (2 ** 26 / (148 * 16) * 2 * (2.0 ** -23 + 2.0 ** -24))
+    assert bool(((out.double() - want).abs() <= tol).all())
