@@ -412,9 +412,10 @@ NVK_API int nvk_fp4_paged_decode_reporting(void* out, const void* query, const v
 /*
  * nvk_paged_prefill over a 4-bit pool (same masking; num_heads any multiple
  * of num_kv_heads; scale > 0). A sequence longer than max_blocks_per_seq
- * blocks sets bit 8 of error_word (may be NULL), a block id outside the pool
- * bit 2; the keys that they would lead to count as rows of zeros. A sequence
- * whose query rows do not lie in [0, total_q) is skipped and sets bit 8.
+ * blocks sets bit 8 of error_word (may be NULL) and is taken as long as those;
+ * a block id outside the pool sets bit 2, and its keys count as rows of zeros. A
+ * length below 0 is one of 0. A sequence whose query rows do not lie in
+ * [0, total_q) is skipped and sets bit 8.
  */
 NVK_API int nvk_fp4_paged_prefill(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
                                   const int32_t* block_tables, int block_table_stride, int max_blocks_per_seq,

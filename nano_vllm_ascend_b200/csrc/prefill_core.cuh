@@ -185,6 +185,14 @@ __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it)
   }
   if (it.qt * kRows >= it.lq) return false;
   it.lk = a.paged ? a.kv_lens[it.b] : (a.cu_kv[it.b + 1] - a.cu_kv[it.b]);
+  if (a.pool) {  // a length is held to [0, what the table reaches]: it bounds the item's work and the sums below
+    const int64_t room = static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4);
+    if (it.lk > room) {
+      if (a.err) atomicOr(a.err, kErrContextTooLong);
+      it.lk = static_cast<int>(room);
+    }
+    it.lk = max(it.lk, 0);
+  }
   it.kv_row0 = a.paged ? 0 : a.cu_kv[it.b];
   const int i_last = min(it.qt * kRows + kRows - 1, it.lq - 1);
   const int lim_last = min(it.lk - it.lq + i_last, it.lk - 1);
@@ -629,12 +637,8 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       auto unit_at = [&](int j) -> const uint8_t* {
         const int tok = j * kKeys + r;
         if (tok >= it.lk) return nullptr;
-        const int u = tok >> 4, col = u >> a.upb_log2;
-        if (col >= a.max_blocks) {
-          if (a.err) atomicOr(a.err, kErrContextTooLong);
-          return nullptr;
-        }
-        const int blk = bt[col];
+        const int u = tok >> 4;
+        const int blk = bt[u >> a.upb_log2];
         if (blk < 0 || blk >= a.num_blocks) {
           if (a.err) atomicOr(a.err, kErrBadBlockId);
           return nullptr;

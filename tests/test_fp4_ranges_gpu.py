@@ -170,3 +170,22 @@ def test_the_longest_context_that_the_range_takes(cuda_device, n):
     want, mean = vr.mean(0, keepdim=True), vr.abs().mean(0, keepdim=True)
     tol = want.abs() * 2.0 ** -8 + mean * (2 ** 26 / (148 * 16) * 2 * (2.0 ** -23 + 2.0 ** -24))
     assert bool(((out.double() - want).abs() <= tol).all())
+
+
+def test_prefill_lengths_beyond_the_table(cuda_device):
+    """A length past the table's is cut to it, whatever it is, so that the work is bounded; one below 0 sees nothing."""
+    dev, h, m, bs = cuda_device, 4, 40, 32
+    k, v = random_rows(3 * bs, 2, 5, spread=False)
+    pool, kr, vr = pool_of(dev, k, v, bs)
+    q = torch.randn(2 * m, h, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+    table = torch.arange(3, dtype=torch.int32, device=dev).expand(2, 3).contiguous()
+    cu = torch.tensor([0, m, 2 * m], dtype=torch.int32, device=dev)
+    for long, negative in ((2 ** 31 - 1, -2 ** 31), (3 * bs + 1, -1)):
+        out = torch.full_like(q, float("nan"))
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        ops_fp4.paged_prefill_fp4(out, q, pool, table, cu, torch.tensor([long, negative], dtype=torch.int32, device=dev),
+                                  m, SCALE, error_word=err)
+        assert int(err.item()) == 8
+        want, a = orc.attention(q[:m], kr, vr, SCALE)
+        check(out[:m], want, a, vr, PREFILL)
+        assert not out[m:].any()
