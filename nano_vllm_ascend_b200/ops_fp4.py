@@ -19,18 +19,12 @@ and lengths are those of the bf16 pool.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
 from .ops import _require_cuda, _require_rows
-
-try:
-    from . import _fp4_calls as _calls
-except ImportError:
-    _calls = None
-if _calls is not None and not torch.__version__.startswith(_calls.TORCH_VERSION):
-    _calls = None  # built for another torch; as without it, every call is checked and made here
 
 _BF16 = torch.bfloat16
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
@@ -57,8 +51,9 @@ _BOUND = ("nvk_fp4_append", "nvk_fp4_read", "nvk_fp4_qk_norm_rope_append", "nvk_
 class _EntryPoints(dict):
     def __missing__(self, name: str):
         lib = _lib.load()
-        if _calls is not None:  # from the first call on
-            _calls.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _BOUND))
+        calls = _binding()
+        if calls is not None:  # from the first call on
+            calls.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _BOUND))
         fn = self[name] = getattr(lib, name)
         return fn
 
@@ -70,9 +65,36 @@ def _leave(*args) -> int:
     return _NOT_TAKEN
 
 
-_append, _read, _norm_rope_append, _decode, _prefill = (
-    (_leave,) * 5 if _calls is None else
-    (_calls.append, _calls.read, _calls.norm_rope_append, _calls.decode, _calls.prefill))
+@functools.cache
+def _binding():
+    """The compiled binding, loaded with the first call (importing the package maps no native code); None where it is
+    not built, or for another torch: then every call is checked and made here."""
+    try:
+        from . import _fp4_calls as calls
+    except ImportError:
+        return None
+    return calls if torch.__version__.startswith(calls.TORCH_VERSION) else None
+
+
+def __getattr__(name: str):
+    if name == "_calls":
+        return _binding()
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def _first(name: str):
+    """Stands for the binding's function until its first call, which puts that in its place."""
+    def call(*args):
+        calls = _binding()
+        fn = _leave if calls is None else getattr(calls, name)
+        if globals()[f"_{name}"] is call:
+            globals()[f"_{name}"] = fn
+        return fn(*args)
+    return call
+
+
+_append, _read, _norm_rope_append, _decode, _prefill = map(
+    _first, ("append", "read", "norm_rope_append", "decode", "prefill"))
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
