@@ -561,14 +561,18 @@ extern "C" int nvk_fp4_qk_norm_rope_append(const void* query, const void* key, c
   // A token's rounds in `chunks` items of `chunk`: the split for which the warps of one resident wave end first, an
   // item's start (position, slot, the cos and sin rows) weighing a little more than a round. With 8 rounds a token:
   // 2048 tokens whole 10.5 us, in eighths 15.5; 2400 whole 15.8, in halves 14.1; 32768 whole 116.5, in halves 125.7.
-  // A finer split has to win a tenth: where all blocks end at once, the next kernel's are not there to follow (8192
-  // tokens alone whole 35.6, in halves 34.2; each followed by a read 43.5 and 44.7).
+  // A finer split has to win a thirty-second, which is as far as this estimate goes. Followed by the prefill attention
+  // of a step (sequences of 256 over 768 cached tokens), coarser and finer, with the share that the estimate says:
+  // 16 + 2 * 8 heads, 1500 tokens 35.3 and 34.0 (9 %), 5000 110.9 and 109.2 (6 %), 8192 116.3 and 115.6 (1 %; alone
+  // 35.5 and 34.3, followed by a read of the rows 43.5 and 44.7); 32 + 2 * 8, 2400 tokens 83.8 and 81.9 (4 %), 10000
+  // 236.6 and 238.1 (2 %; alone 54 and 61); 5 + 2 * 1, 2400 tokens 32.8 and 30.4 (8 %); 40 + 2 * 8, 8192 tokens 338.5
+  // and 338.9 (6 %).
   const int64_t warps = int64_t(sms) * 2 * kWarps;
   int64_t best = 0;
   for (int n = 1; n <= rounds; n = n < 8 ? n + 1 : n < rounds && 2 * n > rounds ? rounds : 2 * n) {
     const int chunk = (rounds + n - 1) / n, chunks = (rounds + chunk - 1) / chunk;
     const int64_t cost = (num_tokens * chunks + warps - 1) / warps * (6 * chunk + 7);
-    if (chunks > 1 && (cost >= best - best / 10 || num_tokens * chunks > kMostItems)) continue;
+    if (chunks > 1 && (cost >= best - best / 32 || num_tokens * chunks > kMostItems)) continue;
     best = cost, a.chunk = chunk, a.chunks = chunks;
   }
   a.items = static_cast<int>(num_tokens) * a.chunks;
