@@ -28,19 +28,23 @@
 //
 // Schedule: the tiles of all (sequence, KV head) pairs, sequence
 // major, are cut into equal contiguous ranges, one per CTA, each cut into
-// equal ranges of its warps. A warp keeps its own running maximum, sum and O;
+// equal ranges of its warps, wherever the cuts fall. A warp keeps its own
+// running maximum (as a product of q and k: weights go by differences of
+// products, so that they are right however large the scores are), sum and O;
 // pairs that lie in one warp are written by it, the others' pieces meet in
 // shared memory at the end, and pairs split over CTAs in the workspace, where
 // the CTA that arrives last (a ticket) joins them. Nothing waits for another
 // CTA.
 //
 // What bounds it: with much to read, instruction issue (about 300 a unit and
-// warp, 66 % of the slots; the ALU pipe at 60 % with 64 conversions of 2 values
+// warp, 67 % of the slots; the ALU pipe at 59 % with 64 conversions of 2 values
 // a unit, which run at half rate) and the power limit behind it (256 contexts
-// of about 4096 tokens, 8 KV heads, 1.2 GB: 215 us = 5.6 TB/s alone, 236 us in
-// a long run at 1710 MHz); with little, fixed latencies: launch, schedule and
+// of about 4096 tokens, 8 KV heads, 1.2 GB: 215 us = 5.6 TB/s alone, 240 to 253
+// us in a long run at 1710 MHz); with little, latencies: launch, schedule and
 // first bytes about 4 us, the pieces' meeting 1 to 2, a split pair's ticket and
-// join 2 (one context of 100 tokens 4.8 us, 32 of 256 to 2304 15.05).
+// join 2 (one context of 100 tokens 4.9 us, 32 of 256 to 2304 16.9). The last
+// comes from cuts inside pairs, which most are: 38 of 42 with 4 contexts up to
+// 513 tokens, 141 of 147 with those 32.
 #include "fp4_kv.cuh"
 
 namespace nvk {
@@ -53,11 +57,12 @@ constexpr int kStages = 2;       // tiles in flight a warp
 constexpr int kMaxCtas = 1024;
 // Tiles below which a CTA is not used. Fewer spread short work over more SMs but
 // give its joins more pieces (one sequence of 100 / 1000 tokens, 8 KV heads:
-// 4.8 / 7.1 us with 8, 6.0 / 8.3 with 16).
+// 4.9 / 6.8 us with 8; when it was chosen 4.8 / 7.1, and 6.0 / 8.3 with 16).
 constexpr int kMinTiles = 8;
 // CTAs that the longest pair may be cut over: the join reads the pieces of a
 // pair one after another (one sequence of 40000 tokens, one KV head, 8 query
-// heads: 18.3 us with 32, 21.2 with 48, 42 with 148; 2 heads: 12.9, 12.9, 15.1).
+// heads: 18.3 us with 32, 21.2 with 48, 42 with 148; 2 heads: 12.9, 12.9, 15.1;
+// beside four of 10 tokens, 8 heads, 19.7 against 47.2 over all 148).
 // The longest one's tiles count, not the number of pairs: short and empty
 // sequences beside it take no share of its pieces.
 constexpr int kMostPieces = 32;
@@ -201,7 +206,7 @@ __device__ __forceinline__ uint32_t vscale_word(uint32_t unit, int valid, int la
 __device__ __forceinline__ bool above(uint32_t w, uint32_t room) { return (w + room) & 0x80808080u; }
 // Lowers the power of two to what the tile's scales allow, and O with it.
 __device__ __forceinline__ void make_room(State& st, uint32_t w0, uint32_t w1) {
-  uint32_t m = __vmaxu4(w0, w1) & 0x78787878u;
+  uint32_t m = __vmaxu4(w0 & 0x78787878u, w1 & 0x78787878u);
   m = __vmaxu4(m, m >> 16);
   m = __reduce_max_sync(0xffffffffu, max(m & 0xffu, (m >> 8) & 0xffu));
   const uint32_t old = st.room & 0xffu, now = min(old, 15u * 8 - m);
