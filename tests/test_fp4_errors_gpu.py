@@ -125,3 +125,20 @@ def test_an_error_is_not_raised_twice(cuda_device):
         with pytest.raises(KVCacheDeviceError):
             check_errors(dev)
         check_errors(dev)
+
+
+def test_a_larger_workspace_keeps_the_error_of_the_smaller_one(cuda_device):
+    """A call with more heads, which needs a larger workspace, comes before the error of an earlier call was read."""
+    dev = cuda_device
+    attn, layer, q, table, ctx = setup(dev)
+    big, big_layer, big_q, _, _ = setup(dev, 64, 8)
+    stream = torch.cuda.Stream(dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(SLEEP)
+        attn(q, *layer, table, ctx)      # its read of the word is in flight for a while ...
+        attn(q, *layer, table + 9, ctx)  # ... so this call's waits for the next one
+        big(big_q, *big_layer, table, ctx)
+        with pytest.raises(KVCacheDeviceError, match="outside the KV pool"):
+            check_errors(dev)
+        check_errors(dev)
