@@ -167,6 +167,7 @@ static_assert(sizeof(PrefillSmem) + 1024 <= 232448, "prefill shared memory excee
 // hands the ones whose rows see no key to `zero_rows`.
 __device__ __forceinline__ int item_streams(const PrefillArgs& a) { return a.paired ? kStreams : 1; }
 
+template <bool kFp4>
 __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it) {
   const int ns = item_streams(a);
   const int groups = a.num_heads / ns;  // head groups per sequence
@@ -179,13 +180,14 @@ __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it)
   it.b = rem / groups;
   it.q0 = a.cu_q[it.b];
   it.lq = a.cu_q[it.b + 1] - it.q0;
+  // (asked at run time: without the question the bf16 kernel, which never gets in, takes 0.4 us of 74 longer)
   if (a.pool && it.lq > 0 && (it.q0 < 0 || it.lq > a.total_q - it.q0)) {  // rows that the query does not have
     if (a.err) atomicOr(a.err, kErrContextTooLong);
     return false;
   }
   if (it.qt * kRows >= it.lq) return false;
   it.lk = a.paged ? a.kv_lens[it.b] : (a.cu_kv[it.b + 1] - a.cu_kv[it.b]);
-  if (a.pool) {  // a length is held to [0, what the table reaches]: it bounds the item's work and the sums below
+  if constexpr (kFp4) {  // a length is held to [0, what the table reaches]: it bounds the item's work and the sums below
     const int64_t room = static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4);
     if (it.lk > room) {
       if (a.err) atomicOr(a.err, kErrContextTooLong);
@@ -200,10 +202,10 @@ __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it)
   return true;
 }
 
-template <typename ZeroRows>
+template <bool kFp4, typename ZeroRows>
 __device__ __forceinline__ bool next_item(const PrefillArgs& a, int& w, int total, Item& it, ZeroRows&& zero_rows) {
   for (; w < total; w += gridDim.x) {
-    if (!load_item(a, w, it)) continue;
+    if (!load_item<kFp4>(a, w, it)) continue;
     if (it.n_kv == 0) {
       zero_rows(it);
       continue;
@@ -429,7 +431,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     bool ok = true;
     while (true) {
       Item it;
-      const bool have = next_item(a, w, total, it, zero_rows);
+      const bool have = next_item<kFp4>(a, w, total, it, zero_rows);
       if (lane == 0) {
         // The Q buffers, and with them the ring slot (read by every role
         // before the previous item's last S), are free once the previous
@@ -746,45 +748,32 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) mx[c] = fmax3(mx[c], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        bool resc;
-        float alpha, neg_mu;
-        if constexpr (kFp4) {
-          resc = (top - m) * sc > kRescaleThreshold;
-          alpha = resc ? fast_exp2((m - top) * sc) : 1.f;
-          if (resc) {
-            l *= alpha;
-            m = top;
-          }
-          neg_mu = (m == -INFINITY) ? 0.f : fmaf(-m, sc, kPShift<true>);
-          // Far from 0 the rounding of neg_mu would reach the weights (and from
-          // 2^22 on lead P out of fp16): the reference is subtracted from the
-          // products instead, which is exact where it matters.
-          if (__any_sync(0xffffffffu, fabsf(neg_mu) > kFarScore)) {
-            const float ref = m == -INFINITY ? 0.f : m;
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (kFp4 ? 1.f : sc);
+        const float m_new = fmaxf(m, mt);
+        const bool resc = kFp4 ? (m_new - m) * sc > kRescaleThreshold : m_new > m + kRescaleThreshold;
+        const float alpha = resc ? fast_exp2(kFp4 ? (m - m_new) * sc : m - m_new) : 1.f;
+        if (resc) {
+          l *= alpha;
+          m = m_new;
+        }
+        float neg_mu = (m == -INFINITY) ? 0.f : kFp4 ? fmaf(-m, sc, kPShift<kFp4>) : kPShift<kFp4> - m;
+        // The 4-bit kernel far from 0, where the rounding of neg_mu would reach the weights (and from 2^22 on lead P
+        // out of fp16): the reference is subtracted from the products instead, which is exact where it matters.
+        if (kFp4 && __any_sync(0xffffffffu, fabsf(neg_mu) > kFarScore)) {
+          const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              tmem_ld32(tmem_s + c * 32, sr[0]);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) sr[0][e] = __float_as_uint(__uint_as_float(sr[0][e]) - ref);
-              tmem_st32(tmem_s + c * 32, sr[0]);
-            }
-            tmem_st_wait();
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + c * 32, sr[c]);
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld32(tmem_s + c * 32, sr[0]);
             tmem_ld_wait();
-            neg_mu = kPShift<true>;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sr[0][e] = __float_as_uint(__uint_as_float(sr[0][e]) - ref);
+            tmem_st32(tmem_s + c * 32, sr[0]);
           }
-        } else {
-          const float m_new = fmaxf(m, top * sc);
-          resc = m_new > m + kRescaleThreshold;
-          alpha = resc ? fast_exp2(m - m_new) : 1.f;
-          if (resc) {
-            l *= alpha;
-            m = m_new;
-          }
-          neg_mu = (m == -INFINITY) ? 0.f : kPShift<false> - m;
+          tmem_st_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + c * 32, sr[c]);
+          tmem_ld_wait();
+          neg_mu = kPShift<kFp4>;
         }
         uint64_t sum[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};  // independent add chains
         const uint64_t sc2 = f32x2_pack(sc, sc), mu2 = f32x2_pack(neg_mu, neg_mu);
