@@ -415,9 +415,8 @@ NVK_API int nvk_fp4_paged_decode_reporting(void* out, const void* query, const v
  * blocks sets bit 8 of error_word (may be NULL) and is taken as long as those;
  * a block id outside the pool sets bit 2, and its keys count as rows of zeros. A
  * length below 0 is one of 0. A sequence whose query rows do not lie in
- * [0, total_q) is skipped and sets bit 8. A key that a query does not see takes
- * part in its sums of V with weight 0: a NaN that V holds there (not behind the
- * sequence's end) can make it NaN, as in nvk_paged_prefill.
+ * [0, total_q) is skipped and sets bit 8. What the rows of keys that a query
+ * does not see hold, a NaN of V among it, does not reach it.
  */
 NVK_API int nvk_fp4_paged_prefill(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
                                   const int32_t* block_tables, int block_table_stride, int max_blocks_per_seq,

@@ -82,6 +82,8 @@
 // drains its in-flight copies and MMAs, frees TMEM and exits.
 #pragma once
 
+#include <climits>
+
 #include "fp4_kv.cuh"
 #include "host_common.h"
 #include "nvk_common.cuh"
@@ -146,6 +148,7 @@ struct PrefillSmem {
   alignas(1024) uint8_t v[kStages][kTileBytes];
   alignas(1024) uint8_t stage[kStreams][kHalfBytes];  // epilogue: 64 dims of 128 output rows per stream
   Item items[kItemRing];
+  alignas(16) int nan_from[kItemRing][fp4::kGroups];       // 4-bit pool: the first token that has a NaN in V's group
   uint64_t item_full[kItemRing];                 // items[i % ring] written (one phase per use)
   uint64_t q_full[kStreams], q_empty[kStreams];  // one phase per item
   uint64_t q_ready[kStreams];                    // 4-bit pool: Q_s is fp16 (one phase per item)
@@ -279,10 +282,12 @@ __device__ __forceinline__ void load_row(VRow& v, const uint8_t* unit, int i) {
                   : make_uint4(0, 0, 0, 0);
 }
 
-// Scale bytes of groups 2 k and 2 k + 1 (low two bytes of w), each as a pair of fp16.
+// Scale bytes of groups 2 k and 2 k + 1 (low two bytes of w), each as a pair of fp16; a NaN as 0 with kNoNan.
+template <bool kNoNan = false>
 __device__ __forceinline__ void scale_pairs(uint32_t w, uint32_t& s0, uint32_t& s1) {
   uint32_t lo, hi;
   fp4::e4m3_to_half2(w, lo, hi);
+  if (kNoNan) asm("max.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0u));
   s0 = __byte_perm(lo, lo, 0x1010);
   s1 = __byte_perm(lo, lo, 0x3232);
 }
@@ -335,16 +340,33 @@ __device__ __forceinline__ void decode_row(const KRow& k, uint32_t tile, int r) 
         put_chunk(tile, r, 2 * (2 * p + e) + h, __byte_perm(w[8 * h + p], w[8 * h + 4 + p], e ? 0x7632 : 0x5410), s[e]);
   }
 }
-__device__ __forceinline__ void decode_row(const VRow& v, uint32_t tile, int r) {
-  const uint32_t* sw = reinterpret_cast<const uint32_t*>(v.s);  // word j: group j of the quad's tokens
-  const int sh = 8 * (r & 3);
+// The row's own scale bytes, of groups 0 to 3 and 4 to 7.
+__device__ __forceinline__ uint2 scale_bytes(const VRow& v, int r) {
+  const uint32_t pick = (r & 3) | ((4 + (r & 3)) << 4);  // v.s: word j holds group j of the quad's four tokens
+  auto four = [&](const uint4& w) {
+    return __byte_perm(__byte_perm(w.x, w.y, pick), __byte_perm(w.z, w.w, pick), 0x5410);
+  };
+  return make_uint2(four(v.s[0]), four(v.s[1]));
+}
+// A group of V whose scale is NaN is decoded as zeros: a weight of 0 times NaN
+// would reach the queries that do not see the row. Its token is noted for the
+// output, which turns to NaN where a query sees it.
+__device__ __forceinline__ void note_nan(uint2 bytes, int token, int* nan_from) {
+  if (((bytes.x + 0x01010101u) | (bytes.y + 0x01010101u)) & 0x80808080u) {  // from 0x7f alone
+#pragma unroll 1
+    for (int j = 0; j < fp4::kGroups; ++j) {
+      if ((bytes.x & 0x7fu) == 0x7fu) atomicMin(nan_from + j, token);
+      bytes.x = __funnelshift_r(bytes.x, bytes.y, 8);
+      bytes.y >>= 8;
+    }
+  }
+}
+__device__ __forceinline__ void decode_row(const VRow& v, uint2 bytes, uint32_t tile, int r) {
 #pragma unroll
   for (int q = 0; q < 2; ++q) {  // groups 4 q .. 4 q + 3
     uint32_t s[4];
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-      scale_pairs(((sw[4 * q + 2 * p] >> sh) & 0xffu) | (((sw[4 * q + 2 * p + 1] >> sh) & 0xffu) << 8), s[2 * p],
-                  s[2 * p + 1]);
+    scale_pairs<true>(q ? bytes.y : bytes.x, s[0], s[1]);
+    scale_pairs<true>((q ? bytes.y : bytes.x) >> 16, s[2], s[3]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // dims 8 h .. 8 h + 7 of each group: a 4 x 4 transpose of bytes
       uint32_t x[4];
@@ -445,6 +467,10 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         Item& slot = sm.items[qi % kItemRing];
         slot = it;
         if (!have || !ok) slot.n_kv = -1;
+        if constexpr (kFp4) {
+          int4* from = reinterpret_cast<int4*>(sm.nan_from[qi % kItemRing]);
+          from[0] = from[1] = make_int4(INT_MAX, INT_MAX, INT_MAX, INT_MAX);
+        }
         mbar_arrive(&sm.item_full[qi % kItemRing]);
         if (have && ok) {
           for (int s = 0; s < ns; ++s) {
@@ -665,7 +691,9 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         load_row(k, unit, i);
         if (g >= kStages && !mbar_wait(&sm.v_empty[st], parity)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        decode_row(v, smem_u32(sm.v[st]), r);
+        const uint2 bytes = scale_bytes(v, r);
+        note_nan(bytes, j * kKeys + r, sm.nan_from[qi % kItemRing]);
+        decode_row(v, bytes, smem_u32(sm.v[st]), r);
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_v[st]);
         load_row(v, unit, i);
@@ -838,6 +866,9 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_ready[s], qi & 1))) { ok = false; break; }
       tc_fence_after();
       const float inv = kFp4 ? (l == 0.f ? 0.f : a.out_scale / l) : (l > 0.f ? 1.f / l : 0.f);
+      // (`it` is the next item by now; this one's slot is filled again only behind its output)
+      const Item& done = sm.items[qi % kItemRing];
+      const int seen = kFp4 ? done.lk - done.lq + done.qt * kRows + r : 0;  // this row's last key
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -848,12 +879,18 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           mbar_arrive(&sm.o_free[s]);
         }
         const uint32_t half = smem_u32(stage + (c & 1) * (kRows * 64));
+        float by[2] = {inv, inv};  // groups 2 c and 2 c + 1: NaN where the row sees one that V holds
+        if constexpr (kFp4)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (seen >= sm.nan_from[qi % kItemRing][2 * c + e]) by[e] = __uint_as_float(0x7fffffffu);
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          const uint32_t x = pack_bf16x2(__uint_as_float(o[q4 * 8 + 0]) * inv, __uint_as_float(o[q4 * 8 + 1]) * inv);
-          const uint32_t y = pack_bf16x2(__uint_as_float(o[q4 * 8 + 2]) * inv, __uint_as_float(o[q4 * 8 + 3]) * inv);
-          const uint32_t z = pack_bf16x2(__uint_as_float(o[q4 * 8 + 4]) * inv, __uint_as_float(o[q4 * 8 + 5]) * inv);
-          const uint32_t u = pack_bf16x2(__uint_as_float(o[q4 * 8 + 6]) * inv, __uint_as_float(o[q4 * 8 + 7]) * inv);
+          const float f = by[q4 >> 1];
+          const uint32_t x = pack_bf16x2(__uint_as_float(o[q4 * 8 + 0]) * f, __uint_as_float(o[q4 * 8 + 1]) * f);
+          const uint32_t y = pack_bf16x2(__uint_as_float(o[q4 * 8 + 2]) * f, __uint_as_float(o[q4 * 8 + 3]) * f);
+          const uint32_t z = pack_bf16x2(__uint_as_float(o[q4 * 8 + 4]) * f, __uint_as_float(o[q4 * 8 + 5]) * f);
+          const uint32_t u = pack_bf16x2(__uint_as_float(o[q4 * 8 + 6]) * f, __uint_as_float(o[q4 * 8 + 7]) * f);
           st_shared_v4(half + r * 64 + ((q4 ^ ((r >> 1) & 3)) << 4), x, y, z, u);
         }
         __syncwarp();  // this warp's pieces are in this half, and the ones before them out of the other

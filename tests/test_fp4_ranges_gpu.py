@@ -189,3 +189,36 @@ def test_prefill_lengths_beyond_the_table(cuda_device):
         want, a = orc.attention(q[:m], kr, vr, SCALE)
         check(out[:m], want, a, vr, PREFILL)
         assert not out[m:].any()
+
+
+@pytest.mark.parametrize("m,cached,h", [(300, 100, 4), (40, 0, 3), (257, 0, 2), (1, 90, 4)])
+def test_prefill_nan_rows_reach_only_the_queries_that_see_them(cuda_device, m, cached, h):
+    """Rows of NaN in V (some groups of them) and in K: a query before such a row comes out as without it, one that
+    sees it is NaN in the row's groups, or everywhere for K."""
+    dev, kvh, bs = cuda_device, 1, 32
+    n = m + cached
+    k, v = random_rows(n, kvh, 41, spread=False)
+    pool, kr, vr = pool_of(dev, k, v, bs)
+    q = torch.randn(m, h, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(dev)
+    want, a = orc.attention(q, kr, vr, SCALE)
+    spoilt = sorted({n - 1, cached + m // 2, cached + m // 3, min(cached + m // 2 + 1, n - 1), cached // 2})
+    for i, j in enumerate(spoilt):  # V: groups i and i + 2
+        row, rest = v[j:j + 1].clone(), vr[j].clone()
+        for grp in (i, i + 2):
+            row[:, :, 16 * grp + 3 * i] = float("nan")
+        ops_fp4.kv_append_fp4(pool, k[j:j + 1].to(dev), row.to(dev), torch.tensor([j], device=dev))
+    out = attend("prefill", q, pool, n, SCALE)
+    bad = torch.zeros(m, h, 8, 16, dtype=torch.bool, device=dev)
+    seen = cached + torch.arange(m, device=dev)  # the last key of each query
+    for i, j in enumerate(spoilt):
+        bad[seen >= j, :, i] = bad[seen >= j, :, i + 2] = True
+    bad = bad.view(m, h, D)
+    assert torch.equal(torch.isnan(out), bad)
+    fine = torch.where(bad, torch.zeros_like(want), want)
+    check(torch.where(bad, torch.zeros_like(out), out), fine, a, vr, PREFILL)
+    j = cached + m // 2
+    row = k[j:j + 1].clone()
+    row[:, :, 77] = float("nan")
+    ops_fp4.kv_append_fp4(pool, row.to(dev), v[j:j + 1].to(dev), torch.tensor([j], device=dev))
+    out = attend("prefill", q, pool, n, SCALE)
+    assert bool(torch.isnan(out[seen >= j]).all()) and not torch.isnan(out[(seen < j) & (seen < min(spoilt))]).any()
