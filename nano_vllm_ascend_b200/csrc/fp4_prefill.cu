@@ -2,9 +2,9 @@
 // appended this step). The kernel body, with its design, is in
 // prefill_core.cuh; the pool's format is in fp4_kv.cuh.
 //
-// Tensor-bound by its operations (4 * 128 a visible pair and head); 80 us
+// Tensor-bound by its operations (4 * 128 a visible pair and head); 82.4 us
 // for 32 requests of 256 tokens over 768 cached ones (16 heads on 8, blocks of
-// 128; 60.2 GFLOP, 755 TF/s), where the bf16 kernel over 3.6 times the bytes
+// 128; 60.2 GFLOP, 730 TF/s), where the bf16 kernel over 3.6 times the bytes
 // takes 71.5: the decoders' instructions and the fetch of the longer code are
 // the difference.
 #include "prefill_core.cuh"
