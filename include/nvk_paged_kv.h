@@ -50,6 +50,13 @@
  *                         happens inside the attention kernel
  *   nvk_fp4_*          <- no reference counterpart: the pool held in 4 bits, with
  *                         the calls above that write and read it
+ *   nvk_fp8_*          <- no reference counterpart: the pool held in 8 bits
+ *   nvk_rotary         <- apply_rotary_pos_emb_tnd, src/nanovllm_ascend/layers/
+ *                         rotary_embedding.py:58-99, in other layouts too, with
+ *                         q_norm and k_norm where weights are given
+ *   nvk_copy_blocks, nvk_remap_blocks
+ *                      <- no reference counterpart: pages of any pool copied,
+ *                         cleared and renumbered
  */
 #ifndef NVK_PAGED_KV_H_
 #define NVK_PAGED_KV_H_
@@ -423,6 +430,124 @@ NVK_API int nvk_fp4_paged_prefill(void* out, const void* query, const void* kv_c
                                   const int32_t* cu_seqlens_q, const int32_t* kv_lens, int batch, int total_q,
                                   int max_q_len, int num_heads, int num_kv_heads, int head_dim, float scale,
                                   float k_scale, float v_scale, int* error_word, nvk_stream_t stream);
+
+/*
+ * ---- The KV cache held in 8 bits ----
+ * No counterpart in the reference: 258 bytes instead of 512 per token and KV
+ * head, for K and V together.
+ *
+ * 16 tokens of one (block, KV head) make a unit with one exponent for K and
+ * one for V; a value is an e4m3 code times 2^exponent, which bf16 holds
+ * exactly. An append raises a unit's exponent to the least e with amax <= 448 *
+ * 2^e over the finite values that it writes there, e from -40 to 40 (smaller
+ * values lose precision below 2^-46, larger ones saturate at 448 * 2^40), and
+ * brings the unit's other rows to it (rounding what becomes subnormal once
+ * more). An append that writes a unit's first token starts the unit anew: the
+ * exponent comes from its rows alone and the unit's other rows become zeros, so
+ * that nothing of a block's earlier sequence stays. A sequence's tokens are
+ * therefore appended in order (any number a call, in any order within it). A
+ * row with a NaN reads as NaN throughout, infinities saturate.
+ *
+ * kv_cache: ONE layer of the pool, uint8 [num_blocks, num_kv_heads,
+ *   block_size / 16, NVK_FP8_UNIT_BYTES], contiguous, 16-byte aligned; K and V
+ *   together. Slot numbers are those of the bf16 pool. The order of the bytes
+ *   in a unit is described in csrc/fp8_kv.cuh; read rows with nvk_fp8_read.
+ *   Zero-fill the pool once when it is allocated. Rows past a sequence's
+ *   context are not used, whatever they hold.
+ * Supported: head_dim 128; block_size a power of two in [16, 256]; any number
+ *   of KV heads.
+ */
+#define NVK_FP8_UNIT_TOKENS 16
+#define NVK_FP8_UNIT_BYTES 4128
+
+/*
+ * nvk_kv_append into an 8-bit pool: rows of `dtype` [num_tokens, num_kv_heads,
+ * head_dim], 2-byte aligned (fastest with 16-byte aligned rows),
+ * key_token_stride / value_token_stride ELEMENTS between tokens. A slot
+ * outside the pool is skipped and sets bit 4 of error_word (may be NULL). Slots
+ * of one call must differ (of two rows for one slot, one is written). Calls
+ * that write the same unit must be ordered on one stream.
+ * workspace: nvk_fp8_append_workspace_size bytes (0 for short calls), 4-byte
+ * aligned, of any content, for this call alone.
+ */
+NVK_API int nvk_fp8_append_workspace_size(int64_t num_tokens, int64_t num_slots, size_t* bytes);
+NVK_API int nvk_fp8_append(const void* key, const void* value, int64_t key_token_stride, int64_t value_token_stride,
+                           void* kv_cache, const int64_t* slot_mapping, int64_t num_tokens, int num_blocks,
+                           int block_size, int num_kv_heads, int head_dim, int dtype, void* workspace,
+                           size_t workspace_bytes, int* error_word, nvk_stream_t stream);
+
+/*
+ * The rows that an 8-bit pool holds at slot_mapping, as `dtype` rows key /
+ * value [num_tokens, num_kv_heads, head_dim], contiguous, 16-byte aligned
+ * (exact in bf16). A slot outside the pool gives zeros and sets bit 4 of
+ * error_word (may be NULL).
+ */
+NVK_API int nvk_fp8_read(void* key, void* value, const void* kv_cache, const int64_t* slot_mapping,
+                         int64_t num_tokens, int num_blocks, int block_size, int num_kv_heads, int head_dim,
+                         int dtype, int* error_word, nvk_stream_t stream);
+
+/*
+ * nvk_paged_decode over an 8-bit pool, with the conditions of
+ * nvk_fp4_paged_decode_reporting (heads, lengths, metadata read early, the
+ * workspace and its first int as the error word where error_word is NULL).
+ */
+#define NVK_FP8_DECODE_ZEROED_BYTES NVK_FP4_DECODE_ZEROED_BYTES
+NVK_API int nvk_fp8_paged_decode_workspace_size(int num_heads, int num_kv_heads, int head_dim, int num_ctas,
+                                                size_t* bytes);
+NVK_API int nvk_fp8_paged_decode(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
+                                 const int32_t* block_tables, int block_table_stride, int max_blocks_per_seq,
+                                 const int32_t* context_lens, int batch, int num_heads, int num_kv_heads,
+                                 int head_dim, float scale, int num_ctas, void* workspace, size_t workspace_bytes,
+                                 int* error_word, nvk_stream_t stream);
+
+/* nvk_paged_prefill over an 8-bit pool, with the conditions of nvk_fp4_paged_prefill. */
+NVK_API int nvk_fp8_paged_prefill(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
+                                  const int32_t* block_tables, int block_table_stride, int max_blocks_per_seq,
+                                  const int32_t* cu_seqlens_q, const int32_t* kv_lens, int batch, int total_q,
+                                  int max_q_len, int num_heads, int num_kv_heads, int head_dim, float scale,
+                                  int* error_word, nvk_stream_t stream);
+
+/*
+ * ---- Rotary positions ----
+ * The heads of q and k, `dtype` rows [num_tokens, heads, head_dim] (strides in
+ * ELEMENTS between tokens, heads and dims packed), turned by their positions
+ * over the first rotary_dim dims in pairs: dims (i, i + rotary_dim / 2), or (2 i,
+ * 2 i + 1) where `interleaved`; pair i turns by position * inv_freq[i] radians
+ * (double, rotary_dim / 2 of them), in 64 bits, so that no position loses
+ * precision; the turned pair is multiplied by attention_scale. Dims from
+ * rotary_dim on pass. With q_weight and k_weight (`dtype` [head_dim], both or
+ * neither) each head is first divided by its root mean square (eps added to
+ * the mean square) and multiplied by the weight. Rounded once, at the end. An
+ * output may be its input (same pointer and stride). head_dim even, up to 512;
+ * num_heads or num_kv_heads may be 0, whose pointers are then not used.
+ */
+NVK_API int nvk_rotary(void* query_out, void* key_out, const void* query, const void* key, int64_t query_out_stride,
+                       int64_t key_out_stride, int64_t query_stride, int64_t key_stride, const void* q_weight,
+                       const void* k_weight, float eps, const double* inv_freq, const int64_t* positions,
+                       float attention_scale, int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                       int rotary_dim, int interleaved, int dtype, nvk_stream_t stream);
+
+/*
+ * ---- Pages of a pool ----
+ * pool (and pool2, may be NULL: K and V of a bf16 pool): [num_layers,
+ * num_blocks, block_bytes], contiguous, 16-byte aligned, of any type;
+ * block_bytes a multiple of 16. pairs: int32 [num_pairs][2] in device memory,
+ * 8-byte aligned. Pair (src, dst) copies block src to block dst in every layer
+ * of both; src -1 fills dst with zeros; dst -1 does nothing (padding). Another
+ * number outside [0, num_blocks) is skipped and sets bit 2 of error_word (may
+ * be NULL). No dst may be another pair's src or dst: the pairs are not ordered.
+ */
+NVK_API int nvk_copy_blocks(void* pool, void* pool2, int num_layers, int num_blocks, int64_t block_bytes,
+                            const int32_t* pairs, int num_pairs, int* error_word, nvk_stream_t stream);
+
+/*
+ * block_tables[r][c] = map[block_tables[r][c]], in place, for int32 rows
+ * row_stride entries apart. A block id or its map outside [0, num_blocks) stays
+ * as it was and sets bit 2 of error_word (may be NULL). The decode kernels may
+ * read the tables behind it in the stream like any other metadata.
+ */
+NVK_API int nvk_remap_blocks(int32_t* block_tables, int64_t row_stride, int64_t num_rows, int width,
+                             const int32_t* map, int num_blocks, int* error_word, nvk_stream_t stream);
 
 /*
  * ---- Prefix-cache index (host code) ----

@@ -128,11 +128,43 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32,
          _i32, _i32, _i32, _f32, _f32, _f32, _c_void_p, _c_void_p],
     ),
+    "nvk_fp8_append_workspace_size": (_i32, [_i64, _i64, ctypes.POINTER(_size_t)]),
+    "nvk_fp8_append": (
+        _i32,
+        [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _c_void_p,
+         _size_t, _c_void_p, _c_void_p],
+    ),
+    "nvk_fp8_read": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p],
+    ),
+    "nvk_fp8_paged_decode_workspace_size": (_i32, [_i32, _i32, _i32, _i32, ctypes.POINTER(_size_t)]),
+    "nvk_fp8_paged_decode": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _i32, _i32, _f32,
+         _i32, _c_void_p, _size_t, _c_void_p, _c_void_p],
+    ),
+    "nvk_fp8_paged_prefill": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _i32, _i32, _i32,
+         _i32, _i32, _i32, _f32, _c_void_p, _c_void_p],
+    ),
+    "nvk_rotary": (
+        _i32,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p, _f32, _c_void_p,
+         _c_void_p, _f32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _c_void_p],
+    ),
+    "nvk_copy_blocks": (_i32, [_c_void_p, _c_void_p, _i32, _i32, _i64, _c_void_p, _i32, _c_void_p, _c_void_p]),
+    "nvk_remap_blocks": (_i32, [_c_void_p, _i64, _i64, _i32, _c_void_p, _i32, _c_void_p, _c_void_p]),
 }
 
 FP4_UNIT_TOKENS = 16
 FP4_UNIT_BYTES = 2304
 FP4_DECODE_ZEROED_BYTES = 4352
+
+FP8_UNIT_TOKENS = 16
+FP8_UNIT_BYTES = 4128
+FP8_DECODE_ZEROED_BYTES = FP4_DECODE_ZEROED_BYTES
 
 MAX_PEERS = 8
 PEER_HANDLE_BYTES = 64

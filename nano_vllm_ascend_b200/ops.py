@@ -138,6 +138,134 @@ def qk_norm_rope_append(
     return query_out
 
 
+# ------------------------------------------------------ rotary positions ---
+_ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def rotary(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    inv_freq: torch.Tensor,
+    positions: torch.Tensor,
+    interleaved: bool = False,
+    attention_scale: float = 1.0,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    query_out: torch.Tensor | None = None,
+    key_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions of the heads ``query`` [T, H, D] and ``key`` [T, KVH, D]
+    (bf16 or fp16; the token stride may be larger), in one kernel.
+
+    The first 2 * len(inv_freq) dims of each head turn, in pairs (i, i + half) or,
+    ``interleaved``, (2i, 2i + 1), by ``positions`` (int64 [T]) times ``inv_freq``
+    (float64, radians; see ``rotary_frequencies``), times ``attention_scale``; the
+    rest passes. With ``q_weight`` and ``k_weight`` ([D]) each head is RMS-normed
+    first. fp32 inside, rounded once. Returns new tensors, or ``query_out`` and
+    ``key_out``, which may be the inputs themselves.
+    """
+    dev = query.device
+    for name, t in (("query", query), ("key", key), ("inv_freq", inv_freq), ("positions", positions)):
+        _require_cuda(name, t, dev)
+    _require_rows("query", query)
+    _require_rows("key", key)
+    tokens, heads, dim = query.shape
+    if query.dtype not in _ROW_DTYPES or key.dtype != query.dtype:
+        raise ValueError(f"rotary: query and key must both be bfloat16 or float16, got {query.dtype} and {key.dtype}")
+    if key.shape[0] != tokens or key.shape[2] != dim:
+        raise ValueError(f"rotary: query {tuple(query.shape)} and key {tuple(key.shape)} do not match")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= dim:
+        raise ValueError(f"rotary: inv_freq must be float64 with 1 to {dim // 2} entries, got {inv_freq.dtype} "
+                         f"{tuple(inv_freq.shape)}")
+    if positions.dtype != torch.int64 or positions.numel() != tokens:
+        raise ValueError("rotary: positions must be int64 [tokens]")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("rotary: norm weights for only one of query and key")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        _require_cuda(name, w, dev)
+        if w.dtype != query.dtype or w.numel() != dim:
+            raise ValueError(f"rotary: {name} must be {query.dtype} [{dim}]")
+    outs = []
+    for name, t, out in (("query_out", query, query_out), ("key_out", key, key_out)):
+        if out is None:
+            out = torch.empty(t.shape, dtype=t.dtype, device=dev)
+        else:
+            _require_cuda(name, out, dev)
+            _require_rows(name, out)
+            if out.shape != t.shape or out.dtype != t.dtype:
+                raise ValueError(f"rotary: {name} must be {t.dtype} {tuple(t.shape)}")
+        outs.append(out)
+    args = (_ptr(outs[0]), _ptr(outs[1]), _ptr(query), _ptr(key), outs[0].stride(0), outs[1].stride(0),
+            query.stride(0), key.stride(0), _ptr(None if q_weight is None else q_weight.contiguous()),
+            _ptr(None if k_weight is None else k_weight.contiguous()), float(eps), _ptr(inv_freq.contiguous()),
+            _ptr(positions.contiguous()), float(attention_scale), tokens, heads, key.shape[1], dim,
+            2 * inv_freq.numel(), int(bool(interleaved)), _ROW_DTYPES[query.dtype])
+    with torch.cuda.device(dev):
+        _lib.call("nvk_rotary", *args, _stream(dev))
+    return outs[0], outs[1]
+
+
+# ----------------------------------------------------------------- pages ---
+def copy_blocks(pools, pairs: torch.Tensor, error_word: torch.Tensor | None = None) -> None:
+    """Copies blocks of a pool in every layer, in place, in one kernel.
+
+    ``pools``: the pool's one or two tensors [layers, blocks, ...] (contiguous, any
+    dtype, equal shapes): a ``PagedKVCache``'s key_cache and value_cache, or the
+    kv_cache of a 4- or 8-bit one. ``pairs``: int32 [n, 2] on the device, (source,
+    destination) each: source -1 clears the destination, destination -1 is
+    padding; another block outside the pool is skipped and sets bit 2 of
+    ``error_word``. No destination may be another pair's source or destination.
+    """
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    if len(pools) not in (1, 2):
+        raise ValueError(f"copy_blocks: {len(pools)} tensors (a pool has one or two)")
+    dev = pools[0].device
+    for t in pools:
+        _require_cuda("pool", t, dev)
+        if t.dim() < 3 or not t.is_contiguous() or t.shape != pools[0].shape or t.dtype != pools[0].dtype:
+            raise ValueError("copy_blocks: pools must be contiguous [layers, blocks, ...] of equal shape and dtype")
+    _require_cuda("pairs", pairs, dev)
+    if pairs.dtype != torch.int32 or pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise ValueError(f"copy_blocks: pairs must be int32 [n, 2], got {pairs.dtype} {tuple(pairs.shape)}")
+    pairs = pairs.contiguous()
+    layers, blocks = pools[0].shape[:2]
+    _check_word("copy_blocks", error_word, dev)
+    if pairs.shape[0] == 0 or pools[0].numel() == 0:
+        return
+    with torch.cuda.device(dev):
+        _lib.call("nvk_copy_blocks", _ptr(pools[0]), _ptr(pools[1] if len(pools) == 2 else None), layers, blocks,
+                  pools[0].nbytes // (layers * blocks), _ptr(pairs), pairs.shape[0], _ptr(error_word), _stream(dev))
+
+
+def remap_blocks(block_tables: torch.Tensor, block_map: torch.Tensor, error_word: torch.Tensor | None = None) -> None:
+    """block_tables[r, c] = block_map[block_tables[r, c]] in place: int32 tables
+    [rows, columns] (the row stride may be larger) of blocks that moved, and the
+    int32 map of every block of the pool. A block id or its map outside the pool
+    stays and sets bit 2 of ``error_word``."""
+    dev = block_tables.device
+    _require_cuda("block_tables", block_tables, dev)
+    _require_cuda("block_map", block_map, dev)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1:
+        raise ValueError("remap_blocks: block_tables must be int32 [rows, columns] with unit column stride")
+    if block_map.dtype != torch.int32 or block_map.dim() != 1 or block_map.numel() == 0:
+        raise ValueError("remap_blocks: block_map must be int32 [blocks]")
+    _check_word("remap_blocks", error_word, dev)
+    rows, width = block_tables.shape
+    block_map = block_map.contiguous()
+    with torch.cuda.device(dev):
+        _lib.call("nvk_remap_blocks", _ptr(block_tables), block_tables.stride(0) if rows > 1 else width, rows, width,
+                  _ptr(block_map), block_map.numel(), _ptr(error_word), _stream(dev))
+
+
+def _check_word(who: str, error_word: torch.Tensor | None, dev: torch.device) -> None:
+    if error_word is not None and (error_word.device != dev or error_word.dtype != torch.int32
+                                   or error_word.numel() < 1):
+        raise ValueError(f"{who}: error_word must be an int32 on {dev}")
+
+
 # ----------------------------------------------------- lm head + argmax ---
 def lm_head_argmax_workspace_bytes(batch: int) -> int:
     out = ctypes.c_size_t(0)

@@ -109,6 +109,9 @@ def _call(dev: torch.device, name: str, *args) -> None:
         _lib.check(name, rc)
 
 
+call_on = _call  # for the wrappers of the other quantised pool
+
+
 def _wrong_device(dev: torch.device, **tensors: torch.Tensor) -> None:
     """Raises for the first tensor that is not on the CUDA device ``dev``."""
     for name, t in tensors.items():
@@ -271,9 +274,9 @@ def decode_fp4_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int 
     return int(out.value)
 
 
-def _check_attention(who: str, dev, out, query, kv_cache, block_tables, lens) -> tuple:
-    """Checks what decode and prefill share; returns what their calls take: query's shape, the pool's blocks,
-    block size and KV heads, and the table's rows, row stride and columns."""
+def _check_sequences(who: str, dev, out, query, kv_cache, block_tables, lens) -> tuple:
+    """Checks what attention over the sequences of any quantised pool shares; returns query's shape and the table's
+    rows, row stride and columns."""
     if not query.is_cuda or out.device != dev or kv_cache.device != dev or block_tables.device != dev \
             or lens.device != dev:
         _wrong_device(dev, out=out, query=query, kv_cache=kv_cache, block_tables=block_tables, lens=lens)
@@ -284,7 +287,6 @@ def _check_attention(who: str, dev, out, query, kv_cache, block_tables, lens) ->
             or not (query.is_contiguous() and out.is_contiguous()):
         raise ValueError(f"{who}: query and out must be contiguous [tokens, heads, {HEAD_DIM}], got "
                          f"{tuple(shape)} and {tuple(out.shape)}")
-    nb, bs, kvh = _check_pool(who, kv_cache)
     stride = block_tables.stride()
     if block_tables.dtype != torch.int32 or len(stride) != 2 or stride[1] != 1:
         raise ValueError(f"{who}: block_tables must be int32 [batch, max_blocks] with unit column stride")
@@ -292,7 +294,15 @@ def _check_attention(who: str, dev, out, query, kv_cache, block_tables, lens) ->
     if lens.dtype != torch.int32 or lens.numel() != batch or not lens.is_contiguous():
         raise ValueError(f"{who}: the sequences' lengths must be a contiguous int32 [batch] device tensor")
     # a single row's stride may be anything
-    return shape, nb, bs, kvh, batch, stride[0] if batch > 1 else width, width
+    return shape, batch, stride[0] if batch > 1 else width, width
+
+
+def _check_attention(who: str, dev, out, query, kv_cache, block_tables, lens) -> tuple:
+    """Checks what decode and prefill share; returns what their calls take: query's shape, the pool's blocks,
+    block size and KV heads, and the table's rows, row stride and columns."""
+    shape, batch, stride, width = _check_sequences(who, dev, out, query, kv_cache, block_tables, lens)
+    nb, bs, kvh = _check_pool(who, kv_cache)
+    return shape, nb, bs, kvh, batch, stride, width
 
 
 def paged_decode_fp4(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
