@@ -13,9 +13,9 @@ namespace nvk {
 using namespace prefill;
 namespace {
 
-__global__ void __launch_bounds__(kThreadsFp4, 1) fp4_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
+__global__ void __launch_bounds__(kThreadsDecoding, 1) fp4_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                      const PrefillArgs a) {
-  prefill_body<true>(qmap, qmap, qmap, a);
+  prefill_body<kHeldFp4>(qmap, qmap, qmap, a);
 }
 
 }  // namespace
@@ -79,7 +79,7 @@ extern "C" int nvk_fp4_paged_prefill(void* out, const void* query, const void* k
   if (items > (int64_t(1) << 30))
     return fail(NVK_ERR_UNSUPPORTED, "%s: %lld work items above the kernel's range", who, (long long)items);
   const int grid = static_cast<int>(items < sms ? items : sms);
-  return check_cuda(launch_pdl(fp4_prefill_kernel, dim3(grid), dim3(kThreadsFp4), smem,
+  return check_cuda(launch_pdl(fp4_prefill_kernel, dim3(grid), dim3(kThreadsDecoding), smem,
                                reinterpret_cast<cudaStream_t>(stream), qm, a),
                     "fp4_paged_prefill launch");
 }

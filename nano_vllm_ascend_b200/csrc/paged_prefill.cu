@@ -16,7 +16,7 @@ namespace {
 __global__ void __maxnreg__(168) prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                                                 const __grid_constant__ CUtensorMap kmap,
                                                 const __grid_constant__ CUtensorMap vmap, const PrefillArgs a) {
-  prefill_body<false>(qmap, kmap, vmap, a);
+  prefill_body<kHeldBf16>(qmap, kmap, vmap, a);
 }
 
 int launch_prefill(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, PrefillArgs a,

@@ -84,14 +84,19 @@
 #pragma once
 
 #include <climits>
+#include <cstddef>
 
 #include "fp4_kv.cuh"
+#include "fp8_kv.cuh"
 #include "host_common.h"
 #include "nvk_common.cuh"
 #include "tcgen05.cuh"
 
 namespace nvk {
 namespace prefill {
+
+// What K and V are held in: bf16 rows, the 4-bit pool, the 8-bit pool. The latter two are decoded by warps of the kernel.
+enum Held { kHeldBf16, kHeldFp4, kHeldFp8 };
 
 constexpr int kD = 128;
 constexpr int kRows = 128;                // query rows per item (UMMA M)
@@ -104,15 +109,18 @@ constexpr int kStreamThreads = 128;       // softmax threads per stream
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kThreads = 10 * 32;
-constexpr int kDecodeWarp0 = 12;          // 4-bit pool: warps 12-15
-constexpr int kThreadsFp4 = 16 * 32;
-// Registers a thread after the split of the 4-bit kernel's 512 x 128 (softmax, softmax, producer and MMA, decoders)
+constexpr int kDecodeWarp0 = 12;          // quantised pools: warps 12-15
+constexpr int kThreadsDecoding = 16 * 32;
+// Registers a thread after the split of the decoding kernels' 512 x 128 (softmax, softmax, producer and MMA, decoders)
 constexpr int kRegsSoftmax = 176, kRegsIssue = 64, kRegsDecode = 96;
 static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsDecode <= 4 * 128, "setmaxnreg shares exceed the launch's registers");
 constexpr uint32_t kTmemCols = 512;       // S_0 | S_1 | O_0 | O_1, 128 columns each
 constexpr uint32_t kColO = 256;
 constexpr float kRescaleThreshold = 8.0f;
-constexpr float kFarScore = 1024.f;       // 4-bit kernel: scores whose rounding in fp32, 2^-14, would show in a weight
+// 8-bit kernel: bounds of the factor from products (of rows below 2^16 and codes, times 2^40 at most) to scores, such
+// that it stays normal times 2^-40 and that differences of products times it stay finite.
+constexpr float kLeastFactor = 0x1p-80f, kMostFactor = 0x1p53f;
+constexpr float kFarScore = 1024.f;       // decoding kernels: scores whose rounding in fp32, 2^-14, would show in a weight
 constexpr int kItemRing = 4;              // item descriptors published ahead by the producer
 
 struct PrefillArgs {
@@ -131,7 +139,7 @@ struct PrefillArgs {
   int batch;
   int qtiles;  // query tiles of the longest sequence
   float scale_log2;
-  // the 4-bit pool
+  // a quantised pool
   const uint8_t* pool;
   int kvh, upb_log2, max_blocks, total_q;
   float out_scale;
@@ -149,7 +157,9 @@ struct PrefillSmem {
   alignas(1024) uint8_t v[kStages][kTileBytes];
   alignas(1024) uint8_t stage[kStreams][kHalfBytes];  // epilogue: 64 dims of 128 output rows per stream
   Item items[kItemRing];
-  alignas(16) int nan_from[kItemRing][fp4::kGroups];       // 4-bit pool: the first token that has a NaN in V's group
+  alignas(16) uint8_t exps[4][2][kKeys / fp8::kUnitTokens];  // 8-bit pool, tile g at g % 4: K's and V's units, + 127
+  alignas(16) int nan_from[kItemRing][fp4::kGroups];       // quantised pools: the first token that has a NaN in V's
+                                                           // group (4 bits), or in V (8 bits: the first entry)
   uint64_t item_full[kItemRing];                 // items[i % ring] written (one phase per use)
   uint64_t q_full[kStreams], q_empty[kStreams];  // one phase per item
   uint64_t q_ready[kStreams];                    // 4-bit pool: Q_s is fp16 (one phase per item)
@@ -171,7 +181,7 @@ static_assert(sizeof(PrefillSmem) + 1024 <= 232448, "prefill shared memory excee
 // hands the ones whose rows see no key to `zero_rows`.
 __device__ __forceinline__ int item_streams(const PrefillArgs& a) { return a.paired ? kStreams : 1; }
 
-template <bool kFp4>
+template <bool kDecoding>
 __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it) {
   const int ns = item_streams(a);
   const int groups = a.num_heads / ns;  // head groups per sequence
@@ -191,7 +201,7 @@ __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it)
   }
   if (it.qt * kRows >= it.lq) return false;
   it.lk = a.paged ? a.kv_lens[it.b] : (a.cu_kv[it.b + 1] - a.cu_kv[it.b]);
-  if constexpr (kFp4) {  // a length is held to [0, what the table reaches]: it bounds the item's work and the sums below
+  if constexpr (kDecoding) {  // a length is held to [0, what the table reaches]: it bounds the item's work and the sums below
     const int64_t room = static_cast<int64_t>(a.max_blocks) << (a.upb_log2 + 4);
     if (it.lk > room) {
       if (a.err) atomicOr(a.err, kErrContextTooLong);
@@ -206,10 +216,10 @@ __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it)
   return true;
 }
 
-template <bool kFp4, typename ZeroRows>
+template <bool kDecoding, typename ZeroRows>
 __device__ __forceinline__ bool next_item(const PrefillArgs& a, int& w, int total, Item& it, ZeroRows&& zero_rows) {
   for (; w < total; w += gridDim.x) {
-    if (!load_item<kFp4>(a, w, it)) continue;
+    if (!load_item<kDecoding>(a, w, it)) continue;
     if (it.n_kv == 0) {
       zero_rows(it);
       continue;
@@ -235,10 +245,10 @@ __device__ __forceinline__ void flag_error(const PrefillArgs& a, PrefillSmem& sm
   sm.abort = 1;
 }
 
-// The 4-bit kernel holds P as 2^7 p: p is at most 2^8 (see kRescaleThreshold),
+// The decoding kernels hold P as 2^7 p: p is at most 2^8 (see kRescaleThreshold),
 // so fp16 takes it, with 11 bits down to p = 2^-21.
-template <bool kFp4>
-constexpr float kPShift = kFp4 ? 7.f : 0.f;
+template <bool kDecoding>
+constexpr float kPShift = kDecoding ? 7.f : 0.f;
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -383,10 +393,64 @@ __device__ __forceinline__ void decode_row(const VRow& v, uint2 bytes, uint32_t 
   }
 }
 
+// The 8-bit pool: a decoding warp has the tile's tokens 32 w .. 32 w + 31, two
+// units, in eight loads of 512 contiguous bytes: a lane takes a chunk of 16
+// codes of four tokens a unit, such that eight lanes write two rows of four
+// chunks each to the tile, without bank conflicts. The codes become fp16 as they
+// are (one conversion for two), and the units' exponents go to the softmax
+// warps, which take K's into the factor of the unit's 16 scores and V's into
+// the exponents of its weights.
+// A lane's token (of the four in 512 bytes) and chunk.
+__device__ __forceinline__ int chunk_row(int lane) { return 2 * (lane >> 4) + (lane >> 2 & 1); }
+__device__ __forceinline__ int chunk_of(int lane) { return 4 * (lane >> 3 & 1) + (lane & 3); }
+
+struct Chunks {
+  uint4 w[8];
+};
+// Load i of part 0 (K) or 1 (V) of two units: the tokens from `seen` on as zeros.
+__device__ __forceinline__ uint4 load_chunk(const uint8_t* const (&unit)[2], int i, int part, int seen, int lane) {
+  const uint8_t* from = unit[i >> 2];
+  const int row = chunk_row(lane);
+  return from && 4 * i + row < seen
+             ? *reinterpret_cast<const uint4*>(from + part * fp8::kOffV + fp8::chunk_at(4 * (i & 3) + row, chunk_of(lane)))
+             : make_uint4(0, 0, 0, 0);
+}
+
+// Chunks to the tile, from its token row r0 on, each followed by the load that
+// takes its registers: `next(i)`. A row with a NaN holds nothing else: V's
+// becomes zeros and its token is noted (see note_nan).
+template <bool kIsV, typename Next>
+__device__ __forceinline__ void decode_chunks(Chunks& x, uint32_t tile, int r0, int token, int* nan_from, int lane,
+                                              Next&& next) {
+  const int k = chunk_row(lane), l = chunk_of(lane);  // dims 16 l .. 16 l + 15
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint4 w = x.w[i];
+    x.w[i] = next(i);
+    if (kIsV && (w.x & 0x7fu) == 0x7fu) {
+      w = make_uint4(0, 0, 0, 0);
+      atomicMin(nan_from, token + 4 * i + k);
+    }
+    const int r = r0 + 4 * i + k;
+    const uint32_t at = tile + (l >> 2) * kHalfBytes + r * 128 + (((2 * (l & 3)) ^ (r & 7)) << 4);
+    auto eight = [&](uint32_t to, uint32_t a, uint32_t b) {
+      uint32_t h[4];
+      fp4::e4m3_to_half2(a, h[0], h[1]);
+      fp4::e4m3_to_half2(b, h[2], h[3]);
+      st_shared_v4(to, h[0], h[1], h[2], h[3]);
+    };
+    eight(at, w.x, w.y);
+    eight(at ^ 16, w.z, w.w);
+  }
+}
+
 // kmap and vmap are read by the bf16 kernel only.
-template <bool kFp4>
+template <Held kHeld>
 __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                              const PrefillArgs& a) {
+  constexpr bool kFp4 = kHeld == kHeldFp4;
+  constexpr bool kDecoding = kHeld != kHeldBf16;  // fp16 operands
+  constexpr bool kExps = kHeld == kHeldFp8;       // a tile's units have exponents
   pdl_launch_dependents();
   pdl_wait();
   const int ns = item_streams(a);
@@ -398,9 +462,9 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       *reinterpret_cast<PrefillSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm.full_k[s], kFp4 ? 128 : 1);
+      mbar_init(&sm.full_k[s], kDecoding ? 128 : 1);
       mbar_init(&sm.k_empty[s], 1);
-      mbar_init(&sm.full_v[s], kFp4 ? 128 : 1);
+      mbar_init(&sm.full_v[s], kDecoding ? 128 : 1);
       mbar_init(&sm.v_empty[s], 1);
     }
     for (int s = 0; s < kStreams; ++s) {
@@ -426,16 +490,16 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  // The 4-bit kernel's register split: each role's branch starts with its
+  // The decoding kernels' register split: each role's branch starts with its
   // share (all four warps of a warpgroup name the same one).
-  constexpr bool kSplit = kFp4;
+  constexpr bool kSplit = kDecoding;
 
   if (warp == kProducerWarp) {
     // -------------------------------------------------------- producer ----
     if constexpr (kSplit) regs_dec<kRegsIssue>();
     if (lane == 0) {
       tma_prefetch_desc(&qmap);
-      if constexpr (!kFp4) {
+      if constexpr (!kDecoding) {
         tma_prefetch_desc(&kmap);
         tma_prefetch_desc(&vmap);
       }
@@ -454,28 +518,28 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     bool ok = true;
     while (true) {
       Item it;
-      const bool have = next_item<kFp4>(a, w, total, it, zero_rows);
+      const bool have = next_item<kDecoding>(a, w, total, it, zero_rows);
       if (lane == 0) {
         // The Q buffers, and with them the ring slot (read by every role
         // before the previous item's last S), are free once the previous
-        // item's last S of each stream has completed. The 4-bit kernel fills
+        // item's last S of each stream has completed. A decoding kernel fills
         // the slot before that wait: its last user, four items back, was done
         // when the last S of the item before the previous one had completed,
         // for which this loop has waited already.
-        if (!kFp4)
+        if (!kDecoding)
           for (int s = 0; s < ns && ok && qi > 0; ++s)
             if (!mbar_wait(&sm.q_empty[s], (qi - 1) & 1)) ok = false;
         Item& slot = sm.items[qi % kItemRing];
         slot = it;
         if (!have || !ok) slot.n_kv = -1;
-        if constexpr (kFp4) {
+        if constexpr (kDecoding) {
           int4* from = reinterpret_cast<int4*>(sm.nan_from[qi % kItemRing]);
           from[0] = from[1] = make_int4(INT_MAX, INT_MAX, INT_MAX, INT_MAX);
         }
         mbar_arrive(&sm.item_full[qi % kItemRing]);
         if (have && ok) {
           for (int s = 0; s < ns; ++s) {
-            if (kFp4 && qi > 0 && !mbar_wait(&sm.q_empty[s], (qi - 1) & 1)) {
+            if (kDecoding && qi > 0 && !mbar_wait(&sm.q_empty[s], (qi - 1) & 1)) {
               ok = false;
               q_extra = s;
               break;
@@ -488,7 +552,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!have || !ok) break;
-      if constexpr (!kFp4) {
+      if constexpr (!kDecoding) {
         const int32_t* bt = a.block_tables + static_cast<int64_t>(it.b) * a.bt_stride;
         int ids = 0;
         for (int j = 0; ok && j < it.n_kv; ++j, ++g) {
@@ -551,7 +615,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     // ------------------------------------------------------------- MMA ----
     if constexpr (kSplit) regs_dec<kRegsIssue>();
     // the operands' type fields: 1 for bf16, 0 for fp16
-    constexpr uint32_t types = kFp4 ? umma_idesc_ab_bf16 : 0u;
+    constexpr uint32_t types = kDecoding ? umma_idesc_ab_bf16 : 0u;
     constexpr uint32_t idesc_qk = umma_idesc_bf16(kRows, kKeys, false) & ~types;
     constexpr uint32_t idesc_pv = umma_idesc_bf16(kRows, kD, true) & ~types;
     bool ok = true;
@@ -598,7 +662,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         const int st = g % kStages;
         if (!wait_all(&sm.full_k[st], (g / kStages) & 1)) { ok = false; break; }
         for (int s = 0; s < ns && ok; ++s) {
-          if (!wait_all(kFp4 ? &sm.q_ready[s] : &sm.q_full[s], qi & 1)) { ok = false; break; }
+          if (!wait_all(kDecoding ? &sm.q_ready[s] : &sm.q_full[s], qi & 1)) { ok = false; break; }
           tc_fence_after();
           issue_s(s, st);
           if (it.n_kv == 1) commit(&sm.q_empty[s]);
@@ -646,7 +710,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     // All MMAs of this CTA complete before TMEM is released.
     commit(&sm.fin);
     (void)mbar_wait(&sm.fin, 0);
-  } else if (kFp4 && warp >= kDecodeWarp0) {
+  } else if (kDecoding && warp >= kDecodeWarp0) {
     // -------------------------------------------------------- decoders ----
     if constexpr (kSplit) regs_dec<kRegsDecode>();
     const int r = tid - kDecodeWarp0 * 32;  // token row of the tile
@@ -661,10 +725,9 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       const Item it = sm.items[qi % kItemRing];
       if (it.n_kv < 0) break;
       const int32_t* bt = a.block_tables + static_cast<int64_t>(it.b) * a.bt_stride;
-      // The unit of this thread's row of tile j; nullptr (a row of zeros) past
-      // the sequence's end and where the table leads nowhere.
-      auto unit_at = [&](int j) -> const uint8_t* {
-        const int tok = j * kKeys + r;
+      // The unit of token `tok`; nullptr (rows of zeros) past the sequence's
+      // end and where the table leads nowhere.
+      auto unit_of = [&](int tok) -> const uint8_t* {
         if (tok >= it.lk) return nullptr;
         const int u = tok >> 4;
         const int blk = bt[u >> a.upb_log2];
@@ -673,31 +736,87 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           return nullptr;
         }
         return a.pool + (((static_cast<int64_t>(blk) * a.kvh + it.kvh) << a.upb_log2) + (u & ((1 << a.upb_log2) - 1))) *
-                            fp4::kUnitBytes;
+                            (kFp4 ? fp4::kUnitBytes : fp8::kUnitBytes);
       };
-      KRow k;
-      VRow v;
-      const uint8_t* unit = unit_at(0);
-      load_row(k, unit, i);
-      load_row(v, unit, i);
-      for (int j = 0; j < it.n_kv; ++j, ++g) {
+      // Tile j's K to `full_k` and V to `full_v`, once their stages are free, with the next tile's loads behind each.
+      auto tile_of = [&](int j, auto&& decode_k, auto&& load_k, auto&& decode_v, auto&& load_v) {
         const int st = g % kStages;
-        unit = j + 1 < it.n_kv ? unit_at(j + 1) : nullptr;
         const uint32_t parity = ((g / kStages) - 1) & 1;
         if (sm.abort || (g >= kStages && !mbar_wait(&sm.k_empty[st], parity))) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        decode_row(k, smem_u32(sm.k[st]), r);
+        if (!__all_sync(0xffffffffu, ok)) return ok = false;
+        decode_k(smem_u32(sm.k[st]));
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_k[st]);
-        load_row(k, unit, i);
+        load_k();
         if (g >= kStages && !mbar_wait(&sm.v_empty[st], parity)) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        const uint2 bytes = scale_bytes(v, r);
-        note_nan(bytes, j * kKeys + r, sm.nan_from[qi % kItemRing]);
-        decode_row(v, bytes, smem_u32(sm.v[st]), r);
+        if (!__all_sync(0xffffffffu, ok)) return ok = false;
+        decode_v(smem_u32(sm.v[st]));
         fence_proxy_async_smem();
         mbar_arrive(&sm.full_v[st]);
+        load_v();
+        return true;
+      };
+      int* nan_from = sm.nan_from[qi % kItemRing];
+      if constexpr (kFp4) {
+        KRow k;
+        VRow v;
+        const uint8_t* unit = unit_of(r);
+        load_row(k, unit, i);
         load_row(v, unit, i);
+        for (int j = 0; j < it.n_kv; ++j, ++g) {
+          unit = j + 1 < it.n_kv ? unit_of((j + 1) * kKeys + r) : nullptr;
+          if (!tile_of(
+                  j, [&](uint32_t tile) { decode_row(k, tile, r); }, [&] { load_row(k, unit, i); },
+                  [&](uint32_t tile) {
+                    const uint2 bytes = scale_bytes(v, r);
+                    note_nan(bytes, j * kKeys + r, nan_from);
+                    decode_row(v, bytes, tile, r);
+                  },
+                  [&] { load_row(v, unit, i); }))
+            break;
+        }
+      } else {
+        // One set of registers: K's chunks make room for V's of the same tile, those for K's of the next one.
+        const int r0 = r & ~31;  // the warp's first token row
+        Chunks x;
+        const uint8_t* unit[2] = {unit_of(r0), unit_of(r0 + 16)};
+        int2 exps;  // lanes 0 and 1: of their unit
+        auto load_exps = [&] {
+          exps = make_int2(0, 0);
+          const uint8_t* mine = lane == 0 ? unit[0] : unit[1];
+          if (lane < 2 && mine) exps = *reinterpret_cast<const int2*>(mine + fp8::kOffExp);
+        };
+        load_exps();
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x.w[n] = load_chunk(unit, n, 0, it.lk - r0, lane);
+        for (int j = 0; j < it.n_kv; ++j, ++g) {
+          if (!tile_of(
+                  j,
+                  [&](uint32_t tile) {
+                    // (The slot's last tile, four back, is done: the wait for this stage of K, whose last tile is two
+                    // back, means that both streams' S of that tile, and with it P of the one before, were complete.)
+                    if (lane < 2) {
+                      sm.exps[g % 4][0][r0 / 16 + lane] = static_cast<uint8_t>(127 + fp8::held_exp(exps.x));
+                      sm.exps[g % 4][1][r0 / 16 + lane] = static_cast<uint8_t>(127 + fp8::held_exp(exps.y));
+                    }
+                    const int seen = it.lk - j * kKeys - r0;
+                    decode_chunks<false>(x, tile, r0, 0, nullptr, lane,
+                                         [&](int n) { return load_chunk(unit, n, 1, seen, lane); });
+                  },
+                  [&] {
+                    const int next = j + 1 < it.n_kv ? (j + 1) * kKeys + r0 : INT_MAX - 16;
+                    unit[0] = unit_of(next);
+                    unit[1] = unit_of(next + 16);
+                    load_exps();
+                  },
+                  [&](uint32_t tile) {
+                    const int seen = it.lk - (j + 1) * kKeys - r0;
+                    decode_chunks<true>(x, tile, r0, j * kKeys + r0, nan_from, lane,
+                                        [&](int n) { return load_chunk(unit, n, 0, seen, lane); });
+                  },
+                  [] {}))
+            break;
+        }
       }
       ++qi;
     }
@@ -721,33 +840,37 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     auto begin_item = [&](int n) {
       if (!__all_sync(0xffffffffu, mbar_wait(&sm.item_full[n % kItemRing], (n / kItemRing) & 1))) return false;
       it = sm.items[n % kItemRing];
-      if (kFp4 && it.n_kv > 0) {
+      if (kDecoding && it.n_kv > 0) {
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.q_full[s], n & 1))) return false;
         sc = fp4::score_factor(q_row_to_half(smem_u32(sm.q[s]), r), a.scale_log2);
+        if constexpr (kExps) sc = sc < kLeastFactor ? kLeastFactor : sc > kMostFactor ? kMostFactor : sc;  // NaN stays
         fence_proxy_async_smem();
         mbar_arrive(&sm.q_ready[s]);
       }
       return true;
     };
-    if (kFp4) ok = begin_item(0);
+    if (kDecoding) ok = begin_item(0);
     while (ok) {
-      if (!kFp4 && !begin_item(qi)) {
+      if (!kDecoding && !begin_item(qi)) {
         ok = false;
         break;
       }
       if (it.n_kv < 0) break;
       const int i = it.qt * kRows + r;
       const int lim = (i < it.lq) ? (it.lk - it.lq + i) : (it.lk - 1);
-      float m = -INFINITY, l = 0.f;  // m: the reference score in log2 units; in the 4-bit kernel its product q . k
+      // 8-bit kernel: weights are relative to p 2^e, e the unit's exponent of V: to the exponent `exp` beside m, and
+      // the sum l takes 2^-e back (see fp8_decode.cu).
+      float exp = -INFINITY;
+      float m = kExps ? 0.f : -INFINITY, l = 0.f;  // m: the reference score in log2 units; in a decoding kernel its product q . k
       for (int j = 0; j < it.n_kv; ++j, ++g) {
         // warp-uniform outcome: the tcgen05.ld/st below need a converged warp
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[s], g & 1))) { ok = false; break; }
         tc_fence_after();
         const int kbase = j * kKeys;
         uint32_t sr[4][32];
-        // The 4-bit kernel masks in tensor memory, in a loop: masking all of the row's registers at once is code that
+        // A decoding kernel masks in tensor memory, in a loop: masking all of the row's registers at once is code that
         // runs once an item, and fetching it took longer (the instruction caches are full of the decoders' code).
-        if (kFp4 && __any_sync(0xffffffffu, kbase + kKeys - 1 > lim)) {
+        if (kDecoding && __any_sync(0xffffffffu, kbase + kKeys - 1 > lim)) {
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             const int seen = lim - kbase - c * 32;  // the chunk's columns up to this one are seen
@@ -760,52 +883,104 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           }
           tmem_st_wait();
         }
+        auto load_scores = [&] {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + c * 32, sr[c]);
-        tmem_ld_wait();
-        if (!kFp4 && kbase + kKeys - 1 > lim) {
+          for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + c * 32, sr[c]);
+          tmem_ld_wait();
+        };
+        load_scores();
+        if (!kDecoding && kbase + kKeys - 1 > lim) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (kbase + c * 32 + e > lim) sr[c][e] = __float_as_uint(-INFINITY);
         }
+        // 8-bit kernel: the exponents of the tile's units stay in four registers, a byte each.
+        uint4 te = make_uint4(0, 0, 0, 0);
+        if constexpr (kExps) te = ld_shared_v4(smem_u32(sm.exps[g % 4]));
+        auto k_pow2 = [&](int u) {  // 2^e of K
+          return __uint_as_float(__byte_perm(u < 4 ? te.x : te.y, 0, (u & 3) << 12 | 0x444) >> 1);
+        };
+        auto v_exp = [&](int u) {  // e of V: 2^23 + byte, less 2^23 + 127
+          return __uint_as_float(__byte_perm(u < 4 ? te.z : te.w, 0x4b000000, 0x7540 + (u & 3))) - 8388735.f;
+        };
+        auto v_pow2_inv = [&](int u) {  // 2^-e of V
+          return __uint_as_float(0x7f000000u - (__byte_perm(u < 4 ? te.z : te.w, 0, (u & 3) << 12 | 0x444) >> 1));
+        };
         // The max is taken over raw scores (scale > 0), the scale folded into
         // the exponent's FMA below; max is exact, so its order is free.
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        constexpr int kParts = kExps ? kKeys / fp8::kUnitTokens : 4;  // units, or chunks
+        float mx[kParts];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int u = 0; u < kParts; ++u) {
+          mx[u] = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) mx[c] = fmax3(mx[c], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (kFp4 ? 1.f : sc);
-        const float m_new = fmaxf(m, mt);
-        const bool resc = kFp4 ? (m_new - m) * sc > kRescaleThreshold : m_new > m + kRescaleThreshold;
-        const float alpha = resc ? fast_exp2(kFp4 ? (m - m_new) * sc : m - m_new) : 1.f;
-        if (resc) {
-          l *= alpha;
-          m = m_new;
+          for (int e = u * (kKeys / kParts); e < (u + 1) * (kKeys / kParts); e += 2)
+            mx[u] = fmax3(mx[u], __uint_as_float(sr[e / 32][e % 32]), __uint_as_float(sr[e / 32][e % 32 + 1]));
         }
-        float neg_mu = (m == -INFINITY) ? 0.f : kFp4 ? fmaf(-m, sc, kPShift<kFp4>) : kPShift<kFp4> - m;
-        // The 4-bit kernel far from 0, where the rounding of neg_mu would reach the weights (and from 2^22 on lead P
+        bool resc;
+        float alpha = 1.f, mu;
+        if constexpr (kExps) {
+          float mt = -INFINITY, most = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < kParts; ++u) {
+            mx[u] *= k_pow2(u);
+            mt = fmaxf(mt, mx[u]);
+            most = fmaxf(most, fmaf(mx[u] - m, sc, v_exp(u) - exp));
+          }
+          resc = most > kRescaleThreshold;
+          if (resc) {
+            const float to = exp == -INFINITY ? mt : fmaxf(m, mt), old = fmaf(m - to, sc, exp);
+            most = old;
+#pragma unroll
+            for (int u = 0; u < kParts; ++u) most = fmaxf(most, fmaf(mx[u] - to, sc, v_exp(u)));
+            alpha = fast_exp2(old - most);
+            l *= alpha;
+            m = to;
+            exp = most;
+          }
+          mu = -m * sc;
+        } else {
+          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (kDecoding ? 1.f : sc);
+          const float m_new = fmaxf(m, mt);
+          resc = kDecoding ? (m_new - m) * sc > kRescaleThreshold : m_new > m + kRescaleThreshold;
+          alpha = resc ? fast_exp2(kDecoding ? (m - m_new) * sc : m - m_new) : 1.f;
+          if (resc) {
+            l *= alpha;
+            m = m_new;
+          }
+          mu = (m == -INFINITY) ? 0.f : kDecoding ? fmaf(-m, sc, kPShift<kDecoding>) : kPShift<kDecoding> - m;
+        }
+        // The decoding kernels far from 0, where the rounding of mu would reach the weights (and from 2^22 on lead P
         // out of fp16): the reference is subtracted from the products instead, which is exact where it matters.
-        if (kFp4 && __any_sync(0xffffffffu, fabsf(neg_mu) > kFarScore)) {
+        bool far = false;
+        if (kDecoding && __any_sync(0xffffffffu, fabsf(mu) > kFarScore)) {
+          far = true;
           const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             tmem_ld32(tmem_s + c * 32, sr[0]);
             tmem_ld_wait();
+            float f[2] = {1.f, 1.f};
+            if constexpr (kExps) {
+              const uint32_t two = (c < 2 ? te.x : te.y) >> (16 * (c & 1));
+              f[0] = __uint_as_float((two & 0xffu) << 23), f[1] = __uint_as_float((two & 0xff00u) << 15);
+            }
 #pragma unroll
-            for (int e = 0; e < 32; ++e) sr[0][e] = __float_as_uint(__uint_as_float(sr[0][e]) - ref);
+            for (int e = 0; e < 32; ++e)
+              sr[0][e] = __float_as_uint(kExps ? fmaf(__uint_as_float(sr[0][e]), f[e / 16], -ref)
+                                               : __uint_as_float(sr[0][e]) - ref);
             tmem_st32(tmem_s + c * 32, sr[0]);
           }
           tmem_st_wait();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + c * 32, sr[c]);
-          tmem_ld_wait();
-          neg_mu = kPShift<kFp4>;
+          load_scores();
+          mu = kExps ? 0.f : kPShift<kDecoding>;
         }
+        // (the exponent's part of the reference behind the products', which may be large)
+        if constexpr (kExps) mu = exp == -INFINITY ? 0.f : mu + (kPShift<kDecoding> - exp);
         uint64_t sum[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};  // independent add chains
-        const uint64_t sc2 = f32x2_pack(sc, sc), mu2 = f32x2_pack(neg_mu, neg_mu);
+        uint64_t sc2 = f32x2_pack(sc, sc), mu2 = f32x2_pack(mu, mu);
         // P over the first 64 columns of S_s (column k holds keys 2k and 2k+1
         // as a bf16 pair): word e of chunk c overwrites score e, already read.
         // Keys 0-63 are signalled first, so that their P V starts while the
@@ -813,13 +988,24 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         auto exps = [&](int c) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
+            if (kExps && e % 8 == 0) {  // a unit begins
+              const int u = 2 * c + e / 8;
+              const float by = far ? sc : sc * k_pow2(u), add = mu + v_exp(u);
+              sc2 = f32x2_pack(by, by), mu2 = f32x2_pack(add, add);
+              sum[0] = sum[1] = f32x2_pack(0.f, 0.f);
+            }
             float p0, p1;
             f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), sc2, mu2),
                          p0, p1);
             p0 = fast_exp2(p0);
             p1 = fast_exp2(p1);
             sum[e & 1] = f32x2_add(sum[e & 1], f32x2_pack(p0, p1));
-            sr[c][e] = kFp4 ? pack_half2(p0, p1) : pack_bf16x2(p0, p1);
+            sr[c][e] = kDecoding ? pack_half2(p0, p1) : pack_bf16x2(p0, p1);
+            if (kExps && e % 8 == 7) {
+              float s0, s1;
+              f32x2_unpack(f32x2_add(sum[0], sum[1]), s0, s1);
+              l = fmaf(s0 + s1, v_pow2_inv(2 * c + e / 8), l);
+            }
           }
           tmem_st16_first(tmem_s + c * 16, sr[c]);
         };
@@ -843,10 +1029,12 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         mbar_arrive(&sm.p_lo[s]);
         exps(2);
         exps(3);
-        float s0, s1, s2, s3;
-        f32x2_unpack(sum[0], s0, s1);
-        f32x2_unpack(sum[1], s2, s3);
-        l += (s0 + s1) + (s2 + s3);
+        if constexpr (!kExps) {
+          float s0, s1, s2, s3;
+          f32x2_unpack(sum[0], s0, s1);
+          f32x2_unpack(sum[1], s2, s3);
+          l += (s0 + s1) + (s2 + s3);
+        }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&sm.p_hi[s]);
@@ -854,7 +1042,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       if (!ok) break;
       const int rows = min(kRows, it.lq - it.qt * kRows);
       __nv_bfloat16* out = a.out + (static_cast<int64_t>(it.q0 + it.qt * kRows) * a.num_heads + it.h0 + s) * kD;
-      if (kFp4 && !begin_item(qi + 1)) {
+      if (kDecoding && !begin_item(qi + 1)) {
         ok = false;
         break;
       }
@@ -866,10 +1054,10 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       // coalesced and no warp waits for another.
       if (!__all_sync(0xffffffffu, mbar_wait(&sm.o_ready[s], qi & 1))) { ok = false; break; }
       tc_fence_after();
-      const float inv = kFp4 ? (l == 0.f ? 0.f : a.out_scale / l) : (l > 0.f ? 1.f / l : 0.f);
+      const float inv = kDecoding ? (l == 0.f ? 0.f : a.out_scale / l) : (l > 0.f ? 1.f / l : 0.f);
       // (`it` is the next item by now; this one's slot is filled again only behind its output)
       const Item& done = sm.items[qi % kItemRing];
-      const int seen = kFp4 ? done.lk - done.lq + done.qt * kRows + r : 0;  // this row's last key
+      const int seen = kDecoding ? done.lk - done.lq + done.qt * kRows + r : 0;  // this row's last key
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -881,10 +1069,10 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         }
         const uint32_t half = smem_u32(stage + (c & 1) * (kRows * 64));
         float by[2] = {inv, inv};  // groups 2 c and 2 c + 1: NaN where the row sees one that V holds
-        if constexpr (kFp4)
+        if constexpr (kDecoding)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (seen >= sm.nan_from[qi % kItemRing][2 * c + e]) by[e] = __uint_as_float(0x7fffffffu);
+            if (seen >= sm.nan_from[qi % kItemRing][kFp4 ? 2 * c + e : 0]) by[e] = __uint_as_float(0x7fffffffu);
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
           const float f = by[q4 >> 1];
@@ -910,7 +1098,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       ++qi;
     }
     if (!ok) flag_error(a, sm, kErrWaitTimeout);
-  } else if (kSplit && warp >= kProducerWarp) {
+  } else if (kSplit && warp >= kProducerWarp && warp < kDecodeWarp0) {
     regs_dec<kRegsIssue>();  // the idle warps of the producer's warpgroup
   }
 
