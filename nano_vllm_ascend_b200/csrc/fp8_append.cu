@@ -28,8 +28,9 @@ constexpr int kScanTokens = 512;
 constexpr int kScanChunk = 4;
 
 struct AppendArgs {
-  const uint8_t* rows[2];  // K, V
-  int64_t stride[2];       // bytes between tokens
+  const uint8_t* key;
+  const uint8_t* value;
+  int64_t key_stride, value_stride;  // bytes between tokens
   uint8_t* pool;
   const int64_t* slots;
   const int32_t* index;    // null: look through the slots
@@ -133,13 +134,14 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
     uint8_t* unit = unit_at(a.pool, unit_of[c], head, a.kvh, a.upb_log2);
     int* exp_at = reinterpret_cast<int*>(unit + kOffExp) + kv;
     const int e_old = held_exp(*exp_at);
-    const uint8_t* rows = a.rows[kv] + static_cast<int64_t>(head) * kD * 2 + 16 * part;
+    const uint8_t* rows = (kv ? a.value : a.key) + static_cast<int64_t>(head) * kD * 2 + 16 * part;
+    const int64_t stride = kv ? a.value_stride : a.key_stride;
     uint4 x[8];
     uint32_t here = 0;  // bit p: row 2 p + half is written
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       const int j = member[c][2 * p + half];
-      x[p] = j >= 0 ? load8<kWide>(rows + j * a.stride[kv]) : make_uint4(0, 0, 0, 0);
+      x[p] = j >= 0 ? load8<kWide>(rows + j * stride) : make_uint4(0, 0, 0, 0);
       here |= (j >= 0) << p;
     }
     uint32_t big = 0;
@@ -190,7 +192,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
 }
 
 struct ReadArgs {
-  uint8_t* out[2];
+  uint8_t* key;
+  uint8_t* value;
   uint8_t* pool;
   const int64_t* slots;
   int64_t num_slots;
@@ -199,35 +202,70 @@ struct ReadArgs {
   int* err;
 };
 
-// A half-warp takes a row: eight codes a lane.
+// Eight lanes take a row, a chunk of 16 codes each, and a warp four rows at a
+// time, kReadRows of those in flight: slots, then codes and exponents, then the
+// rows out.
+constexpr int kReadRows = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int part = threadIdx.x & 15;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / 16);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4); i < 2 * a.rows; i += step) {
-    const int kv = i >= a.rows;
-    const int64_t row = i - kv * a.rows, t = row / a.kvh;
-    const int head = static_cast<int>(row - t * a.kvh);
-    const int64_t s = a.slots[t];
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (s >= 0 && s < a.num_slots) {
-      const uint8_t* unit = unit_at(a.pool, s >> 4, head, a.kvh, a.upb_log2);
-      const float by = pow2(held_exp(reinterpret_cast<const int*>(unit + kOffExp)[kv]));
-      const uint2 w = *reinterpret_cast<const uint2*>(unit + kv * kOffV + chunk_at(s & 15, part >> 1) + 8 * (part & 1));
-      auto two = [&](uint32_t h) {
-        const float2 f = pair_to_f32<__half>(h);
-        return f32_to_pair<T>(f.x * by, f.y * by);
-      };
-      uint32_t h[4];
-      e4m3_to_half2(w.x, h[0], h[1]);
-      e4m3_to_half2(w.y, h[2], h[3]);
-      v = make_uint4(two(h[0]), two(h[1]), two(h[2]), two(h[3]));
-    } else if (part == 0 && a.err) {
-      atomicOr(a.err, kErrBadSlot);
+  const int c = threadIdx.x & 7;
+  constexpr int kPerBlock = kThreads / 8 * kReadRows;
+  const int64_t all = 2 * a.rows;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kPerBlock + (threadIdx.x >> 3); first < all;
+       first += static_cast<int64_t>(gridDim.x) * kPerBlock) {
+    int64_t slot[kReadRows];
+    int head[kReadRows];
+#pragma unroll
+    for (int n = 0; n < kReadRows; ++n) {
+      const int64_t i = first + n * (kThreads / 8), row = i < a.rows ? i : i - a.rows;
+      slot[n] = -1;
+      head[n] = 0;
+      if (i < all) {
+        int64_t t;
+        if (a.rows <= 0x7fffffff) t = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.kvh);
+        else t = row / a.kvh;
+        head[n] = static_cast<int>(row - t * a.kvh);
+        slot[n] = a.slots[t];
+        if ((slot[n] < 0 || slot[n] >= a.num_slots) && c == 0 && a.err) atomicOr(a.err, kErrBadSlot);
+      }
     }
-    *reinterpret_cast<uint4*>(a.out[kv] + row * (kD * 2) + 16 * part) = v;
+    uint4 w[kReadRows];
+    int e[kReadRows];
+#pragma unroll
+    for (int n = 0; n < kReadRows; ++n) {
+      w[n] = make_uint4(0, 0, 0, 0);
+      e[n] = 0;
+      if (slot[n] >= 0 && slot[n] < a.num_slots) {
+        const int kv = first + n * (kThreads / 8) >= a.rows;
+        const uint8_t* unit = unit_at(a.pool, slot[n] >> 4, head[n], a.kvh, a.upb_log2);
+        e[n] = reinterpret_cast<const int*>(unit + kOffExp)[kv];
+        w[n] = *reinterpret_cast<const uint4*>(unit + kv * kOffV + chunk_at(slot[n] & 15, c));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kReadRows; ++n) {
+      const int64_t i = first + n * (kThreads / 8);
+      if (i >= all) continue;
+      const float by = pow2(held_exp(e[n]));
+      auto eight = [&](uint32_t lo, uint32_t hi) {
+        uint32_t h[4];
+        e4m3_to_half2(lo, h[0], h[1]);
+        e4m3_to_half2(hi, h[2], h[3]);
+        uint32_t r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = pair_to_f32<__half>(h[j]);
+          r[j] = f32_to_pair<T>(f.x * by, f.y * by);
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+      };
+      uint4* out = reinterpret_cast<uint4*>((i < a.rows ? a.key + i * (kD * 2) : a.value + (i - a.rows) * (kD * 2)) + 32 * c);
+      out[0] = eight(w[n].x, w[n].y);
+      out[1] = eight(w[n].z, w[n].w);
+    }
   }
 }
 
@@ -269,10 +307,10 @@ extern "C" int nvk_fp8_append(const void* key, const void* value, int64_t key_to
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: token strides (%lld, %lld) must cover a row", who,
                 (long long)key_token_stride, (long long)value_token_stride);
   AppendArgs a;
-  a.rows[0] = static_cast<const uint8_t*>(key);
-  a.rows[1] = static_cast<const uint8_t*>(value);
-  a.stride[0] = key_token_stride * 2;
-  a.stride[1] = value_token_stride * 2;
+  a.key = static_cast<const uint8_t*>(key);
+  a.value = static_cast<const uint8_t*>(value);
+  a.key_stride = key_token_stride * 2;
+  a.value_stride = value_token_stride * 2;
   a.pool = static_cast<uint8_t*>(kv_cache);
   a.slots = slot_mapping;
   a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
@@ -320,8 +358,8 @@ extern "C" int nvk_fp8_read(void* key, void* value, const void* kv_cache, const 
   if (!aligned16(key) || !aligned16(value) || !aligned(slot_mapping, 8))
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: the rows must be 16-byte aligned, the slots 8-byte aligned", who);
   ReadArgs a;
-  a.out[0] = static_cast<uint8_t*>(key);
-  a.out[1] = static_cast<uint8_t*>(value);
+  a.key = static_cast<uint8_t*>(key);
+  a.value = static_cast<uint8_t*>(value);
   a.pool = static_cast<uint8_t*>(const_cast<void*>(kv_cache));
   a.slots = slot_mapping;
   a.num_slots = static_cast<int64_t>(num_blocks) * block_size;
@@ -329,8 +367,11 @@ extern "C" int nvk_fp8_read(void* key, void* value, const void* kv_cache, const 
   a.kvh = num_kv_heads;
   a.upb_log2 = units_log2(block_size);
   a.err = error_word;
-  const int64_t want = (2 * a.rows + kThreads / 16 - 1) / (kThreads / 16);
-  const dim3 grid(static_cast<unsigned>(want < 148 * 8 ? want : 148 * 8));
+  int sms = 148, dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  constexpr int kPerBlock = kThreads / 8 * kReadRows;
+  const int64_t want = (2 * a.rows + kPerBlock - 1) / kPerBlock, most = int64_t(sms) * 8;
+  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return check_cuda(dtype == NVK_DTYPE_BF16 ? launch_pdl(read_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, st, a)
                                             : launch_pdl(read_kernel<__half>, grid, dim3(kThreads), 0, st, a),
