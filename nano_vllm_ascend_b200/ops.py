@@ -11,7 +11,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _calls, _lib
 
 _BF16 = torch.bfloat16
 _KV_DTYPES = (torch.bfloat16, torch.float16)
@@ -140,6 +140,8 @@ def qk_norm_rope_append(
 
 # ------------------------------------------------------ rotary positions ---
 _ROW_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_rotary, _copy_blocks, _remap_blocks = (_calls.first(name, globals()) for name in
+                                        ("rotary", "copy_blocks", "remap_blocks"))
 
 
 def rotary(
@@ -165,6 +167,12 @@ def rotary(
     first. fp32 inside, rounded once. Returns new tensors, or ``query_out`` and
     ``key_out``, which may be the inputs themselves.
     """
+    turned = _rotary(query, key, inv_freq, positions, interleaved, attention_scale, q_weight, k_weight, eps, query_out,
+                     key_out)
+    if turned.__class__ is tuple:
+        return turned[0] if query_out is None else query_out, turned[1] if key_out is None else key_out
+    if turned != _calls.NOT_TAKEN:
+        _lib.check("nvk_rotary", turned)
     dev = query.device
     for name, t in (("query", query), ("key", key), ("inv_freq", inv_freq), ("positions", positions)):
         _require_cuda(name, t, dev)
@@ -220,7 +228,13 @@ def copy_blocks(pools, pairs: torch.Tensor, error_word: torch.Tensor | None = No
     ``error_word``. No destination may be another pair's source or destination.
     """
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
-    if len(pools) not in (1, 2):
+    if len(pools) in (1, 2):
+        rc = _copy_blocks(pools[0], pools[1] if len(pools) == 2 else None, pairs, error_word)
+        if rc == 0:
+            return
+        if rc != _calls.NOT_TAKEN:
+            _lib.check("nvk_copy_blocks", rc)
+    else:
         raise ValueError(f"copy_blocks: {len(pools)} tensors (a pool has one or two)")
     dev = pools[0].device
     for t in pools:
@@ -245,6 +259,11 @@ def remap_blocks(block_tables: torch.Tensor, block_map: torch.Tensor, error_word
     [rows, columns] (the row stride may be larger) of blocks that moved, and the
     int32 map of every block of the pool. A block id or its map outside the pool
     stays and sets bit 2 of ``error_word``."""
+    rc = _remap_blocks(block_tables, block_map, error_word)
+    if rc == 0:
+        return
+    if rc != _calls.NOT_TAKEN:
+        _lib.check("nvk_remap_blocks", rc)
     dev = block_tables.device
     _require_cuda("block_tables", block_tables, dev)
     _require_cuda("block_map", block_map, dev)

@@ -18,11 +18,12 @@ import ctypes
 
 import torch
 
-from . import _lib
-from .ops import _require_cuda
+from . import _calls, _lib
 from .ops_fp4 import (_BF16, _DTYPES, HEAD_DIM, _check_index, _check_sequences, _error_ptr, _row_stride, _wrong_device,
                       call_on)
 
+_append8, _read8, _decode8, _prefill8 = (_calls.first(name, globals()) for name in
+                                         ("append8", "read8", "decode8", "prefill8"))
 SCAN_TOKENS = 512  # up to here an append needs no workspace
 
 
@@ -50,6 +51,11 @@ def kv_append_fp8(kv_cache: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     (int64). Slots must differ; one outside the pool is skipped and sets bit 4
     of ``error_word``. Writing a unit's first token starts the unit anew (its
     other rows become zeros), so a sequence's tokens are appended in order."""
+    rc = _append8(kv_cache, key, value, slot_mapping, error_word)
+    if rc == 0:
+        return
+    if rc != _calls.NOT_TAKEN:
+        _lib.check("nvk_fp8_append", rc)
     who = "kv_append_fp8"
     dev = kv_cache.device
     if not kv_cache.is_cuda or key.device != dev or value.device != dev or slot_mapping.device != dev:
@@ -76,6 +82,12 @@ def kv_read_fp8(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch
     """The K and V rows [tokens, kv_heads, 128] that the pool holds at
     ``slot_mapping`` (int64; any order, repeats allowed), as ``dtype``; a slot
     outside the pool gives zeros and sets bit 4 of ``error_word``."""
+    if key_out is None and value_out is None and dtype in _DTYPES:
+        rows = _read8(kv_cache, slot_mapping, dtype is torch.float16, error_word)
+        if rows.__class__ is tuple:
+            return rows
+        if rows != _calls.NOT_TAKEN:
+            _lib.check("nvk_fp8_read", rows)
     who = "kv_read_fp8"
     dev = kv_cache.device
     if not kv_cache.is_cuda or slot_mapping.device != dev:
@@ -115,6 +127,11 @@ def paged_decode_fp8(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Ten
     ordered on one stream. Device errors are bits of ``error_word``, or of the
     workspace's first int32.
     """
+    rc = _decode8(out, query, kv_cache, block_tables, context_lens, scale, workspace, num_ctas, error_word)
+    if rc == 0:
+        return out
+    if rc != _calls.NOT_TAKEN:
+        _lib.check("nvk_fp8_paged_decode", rc)
     who = "paged_decode_fp8"
     dev = query.device
     shape, batch, stride, width = _check_sequences(who, dev, out, query, kv_cache, block_tables, context_lens)
@@ -133,6 +150,11 @@ def paged_prefill_fp8(out: torch.Tensor, query: torch.Tensor, kv_cache: torch.Te
                       cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int, scale: float,
                       error_word: torch.Tensor | None = None) -> torch.Tensor:
     """Causal (bottom-right) prefill attention over an 8-bit pool into ``out``."""
+    rc = _prefill8(out, query, kv_cache, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale, error_word)
+    if rc == 0:
+        return out
+    if rc != _calls.NOT_TAKEN:
+        _lib.check("nvk_fp8_paged_prefill", rc)
     who = "paged_prefill_fp8"
     dev = query.device
     shape, batch, stride, width = _check_sequences(who, dev, out, query, kv_cache, block_tables, kv_lens)
