@@ -206,11 +206,13 @@ def rotary(
             if out.shape != t.shape or out.dtype != t.dtype:
                 raise ValueError(f"rotary: {name} must be {t.dtype} {tuple(t.shape)}")
         outs.append(out)
+    # copies, where these make some, live until the launch
+    inv_freq, positions = inv_freq.contiguous(), positions.contiguous()
+    q_weight, k_weight = (w if w is None else w.contiguous() for w in (q_weight, k_weight))
     args = (_ptr(outs[0]), _ptr(outs[1]), _ptr(query), _ptr(key), outs[0].stride(0), outs[1].stride(0),
-            query.stride(0), key.stride(0), _ptr(None if q_weight is None else q_weight.contiguous()),
-            _ptr(None if k_weight is None else k_weight.contiguous()), float(eps), _ptr(inv_freq.contiguous()),
-            _ptr(positions.contiguous()), float(attention_scale), tokens, heads, key.shape[1], dim,
-            2 * inv_freq.numel(), int(bool(interleaved)), _ROW_DTYPES[query.dtype])
+            query.stride(0), key.stride(0), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(inv_freq),
+            _ptr(positions), float(attention_scale), tokens, heads, key.shape[1], dim, 2 * inv_freq.numel(),
+            int(bool(interleaved)), _ROW_DTYPES[query.dtype])
     with torch.cuda.device(dev):
         _lib.call("nvk_rotary", *args, _stream(dev))
     return outs[0], outs[1]
