@@ -570,6 +570,9 @@ NVK_API int nvk_prefix_cache_blocks(nvk_prefix_index* index, const int32_t* tabl
                                     int num_cached_blocks, int num_full_blocks, const int64_t* token_ids,
                                     int64_t num_tokens);
 NVK_API int nvk_prefix_forget_block(nvk_prefix_index* index, int block_id);
+/* Block `from` became block `to` (nvk_copy_blocks): its key follows, in its place among the blocks cached under it, and
+ * `to` forgets the one it had. */
+NVK_API int nvk_prefix_move_block(nvk_prefix_index* index, int from, int to);
 /* The block's key (interned id), -1 when it is not cached. */
 NVK_API int64_t nvk_prefix_block_key(const nvk_prefix_index* index, int block_id);
 NVK_API int nvk_prefix_clear(nvk_prefix_index* index);

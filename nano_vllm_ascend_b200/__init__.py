@@ -5,6 +5,7 @@ Drop-in host classes (same names and contracts as the reference's):
 * ``PagedKVCache`` -- pool + CUDA append          (npu/paged_kv_cache.py)
 * ``BlockManager`` / ``PagedKVCacheMetadata``     (npu/block_manager.py)
 * ``PagedKVCacheFp4`` -- the pool held in 4 bits   (same interface, ops_fp4)
+* ``PagedKVCacheFp8`` -- the pool held in 8 bits   (same interface, ops_fp8)
 * ``PagedAttention``  -- decode attention          (layers/npu_paged_attention.py)
 * ``BatchPrefillAttention`` -- causal prefill     (layers/npu_prefill_attention.py)
 * ``DecodeGraphRunner`` -- CUDA-graph decode       (npu/acl_graph.py)
@@ -20,10 +21,12 @@ from . import device_errors
 from .block_manager import BlockManager, BlockState, PagedKVCacheMetadata
 from .cuda_graph import DecodeGraphRunner, DecodeGraphStats, copy_block_tables
 from .fp4_kv_cache import Fp4Layer, PagedKVCacheFp4
+from .fp8_kv_cache import Fp8Layer, PagedKVCacheFp8
 from .paged_attention import PagedAttention
 from .paged_kv_cache import PagedKVCache
 from .device_errors import KVCacheDeviceError, check_errors
 from .prefill_attention import BatchPrefillAttention
+from .rotary import rotary_frequencies
 
 # Names used by the reference's call sites.
 NpuPagedAttention = PagedAttention
@@ -36,13 +39,16 @@ __all__ = [
     "DecodeGraphRunner",
     "DecodeGraphStats",
     "Fp4Layer",
+    "Fp8Layer",
     "KVCacheDeviceError",
     "NpuBatchPrefillAttention",
     "NpuPagedAttention",
     "PagedAttention",
     "PagedKVCache",
     "PagedKVCacheFp4",
+    "PagedKVCacheFp8",
     "PagedKVCacheMetadata",
     "check_errors",
     "copy_block_tables",
+    "rotary_frequencies",
 ]

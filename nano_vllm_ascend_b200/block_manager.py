@@ -178,6 +178,9 @@ class _NativePrefixIndex:
     def forget(self, block_id: int) -> None:
         _lib.call("nvk_prefix_forget_block", self._h, block_id)
 
+    def move(self, src: int, dst: int) -> None:
+        _lib.call("nvk_prefix_move_block", self._h, src, dst)
+
     def key(self, block_id: int) -> int | None:
         k = int(self._lib.nvk_prefix_block_key(self._h, block_id))
         return None if k < 0 else k
@@ -212,6 +215,7 @@ class BlockManager:
         self._cached: dict[ChainKey, list[int]] = {}
         self.block_tables: dict[int, list[int]] = {}
         self.seq_lens: dict[int, int] = {}
+        self.moves = 0  # how often compact() has renumbered blocks
 
     # ------------------------------------------------------------ free queue --
     @property
@@ -299,6 +303,63 @@ class BlockManager:
         self.seq_lens.pop(slot, None)
         for block_id in reversed(table):
             self._release_block(block_id)
+
+    # ------------------------------------------- forks and compaction --
+    # (the reference has neither). Both return the (source, destination) blocks
+    # whose contents have to be copied, by the caches' copy_blocks(), before
+    # the next step reads or writes the destinations.
+    def fork(self, slot: int, new_slot: int) -> list[tuple[int, int]]:
+        """Starts ``new_slot`` as a copy of ``slot``: full blocks are shared,
+        a last one that is partly filled gets a block of its own."""
+        if new_slot in self.block_tables:
+            raise ValueError(f"slot {new_slot} is in use")
+        table, length = self.block_tables[slot], self.seq_lens[slot]
+        full = length // self.block_size
+        copies = []
+        if length % self.block_size:
+            copies.append((table[full], self._alloc_block()))
+        for block_id in table[:full]:
+            self._retain_block(block_id)
+        self.block_tables[new_slot] = table[:full] + [dst for _, dst in copies]
+        self.seq_lens[new_slot] = length
+        return copies
+
+    def compact(self, copy_blocks=None) -> list[tuple[int, int]]:
+        """Renumbers the blocks in use to the lowest ids, in every table, so that
+        all of them lie below their number; their prefix-cache keys move along,
+        those of unused blocks that are moved over are forgotten.
+
+        ``copy_blocks``, if given, is called with the copies before anything is
+        renumbered: where it raises, nothing has been. Block ids that were
+        looked up before (a prepared sequence's cached prefix) are void
+        afterwards; device mirrors follow by ``DeviceBlockTables.remap()``."""
+        live = sum(block.ref_count > 0 for block in self.blocks)
+        holes = [b for b in range(live) if self.blocks[b].ref_count == 0]
+        movers = [b for b in range(live, self.num_blocks) if self.blocks[b].ref_count > 0]
+        moved = dict(zip(movers, holes))
+        if not moved:
+            return []
+        if copy_blocks is not None:
+            copy_blocks(list(moved.items()))
+        for src, dst in moved.items():
+            self._move_block(src, dst)
+        for table in self.block_tables.values():
+            table[:] = [moved.get(b, b) for b in table]
+        self.moves += 1
+        return list(moved.items())
+
+    def _move_block(self, src: int, dst: int) -> None:
+        self._free.remove(dst)
+        self._forget_key(dst)
+        old, new = self.blocks[src], self.blocks[dst]
+        if self._native is not None:
+            self._native.move(src, dst)
+        elif old.block_hash is not None:
+            holders = self._cached[old.block_hash]
+            holders[holders.index(src)] = dst
+        new.block_hash, old.block_hash = old.block_hash, None
+        new.ref_count, old.ref_count = old.ref_count, 0
+        self._free.push_back(src)
 
     # ------------------------------------------------------- prefix cache --
     def find_longest_prefix_blocks(self, token_ids, max_cache_blocks: int) -> list[int]:

@@ -180,6 +180,22 @@ extern "C" int nvk_prefix_forget_block(nvk_prefix_index* idx, int block_id) {
   return NVK_OK;
 }
 
+extern "C" int nvk_prefix_move_block(nvk_prefix_index* idx, int from, int to) {
+  int rc = check_index(idx, "prefix_move_block");
+  if (rc != NVK_OK) return rc;
+  if (from < 0 || from >= idx->num_blocks || to < 0 || to >= idx->num_blocks)
+    return nvk::fail(NVK_ERR_INVALID_ARGUMENT, "prefix_move_block: block id %d or %d out of range", from, to);
+  if (from == to) return NVK_OK;
+  idx->forget(to);
+  const int64_t key = idx->block_key[from];
+  if (key < 0) return NVK_OK;
+  for (int32_t& holder : idx->entries[key].holders)  // the key's place among its holders stays
+    if (holder == from) holder = to;
+  idx->block_key[to] = key;
+  idx->block_key[from] = -1;
+  return NVK_OK;
+}
+
 extern "C" int64_t nvk_prefix_block_key(const nvk_prefix_index* idx, int block_id) {
   if (!idx || block_id < 0 || block_id >= idx->num_blocks) return -1;
   return idx->block_key[block_id];

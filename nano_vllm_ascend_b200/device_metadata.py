@@ -18,7 +18,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, ops
 from .block_manager import PagedKVCacheMetadata
 
 
@@ -39,10 +39,23 @@ class DeviceBlockTables:
         self._events = [torch.cuda.Event() for _ in range(_STAGING_BUFFERS)]
         self._next = 0
         self._fn = _lib.load().nvk_decode_metadata
+        self._moves = block_manager.moves
 
     def forget(self, slot: int) -> None:
         """Drops what was sent for ``slot`` (optional: a new table is detected anyway)."""
         self._synced.pop(slot, None)
+
+    def remap(self, moved: list[tuple[int, int]]) -> None:
+        """Follows ``BlockManager.compact()`` on the device: renumbers the mirror's
+        entries instead of sending every table again (which the next step does
+        by itself where this was not called)."""
+        if moved and self._moves + 1 == self.bm.moves:
+            block_map = torch.arange(self.bm.num_blocks, dtype=torch.int32)
+            src, dst = torch.tensor(moved, dtype=torch.int64).unbind(1)
+            block_map[src] = dst.to(torch.int32)
+            with torch.cuda.device(self.device):
+                ops.remap_blocks(self.mirror, block_map.to(self.device), error_word=self.error_word)
+            self._moves = self.bm.moves
 
     def _staging_buffer(self, words: int) -> tuple[torch.Tensor, np.ndarray, torch.cuda.Event]:
         """A pinned int64 buffer of at least ``words`` words whose previous copy has finished,
@@ -77,6 +90,9 @@ class DeviceBlockTables:
         bm = self.bm
         bs = bm.block_size
         tables, seq_lens, synced = bm.block_tables, bm.seq_lens, self._synced
+        if self._moves != bm.moves:  # blocks were renumbered
+            synced.clear()
+            self._moves = bm.moves
         rows, cols = self.mirror.shape
         # the allocator's bookkeeping (ensure_blocks, seq_lens) and the update lists, in one pass.
         # What is sent is recorded only after the launch, so an error leaves the record as it was.

@@ -25,7 +25,7 @@ from typing import Sequence
 import torch
 
 from . import device_errors, ops_fp4
-from .paged_kv_cache import _packed_rows
+from .paged_kv_cache import _packed_rows, copy_pool_blocks
 from .pool import fp4_bytes_per_block
 
 
@@ -47,6 +47,21 @@ class Fp4Layer:
     def device(self) -> torch.device:
         return self.pool.device
 
+    # The calls over this layer, as the attention classes and the cache make them.
+    def append(self, key, value, slots, error_word) -> None:
+        ops_fp4.kv_append_fp4(self.pool, key, value, slots, self.k_scale, self.v_scale, error_word=error_word)
+
+    def read(self, slots, dtype, error_word):
+        return ops_fp4.kv_read_fp4(self.pool, slots, self.k_scale, self.v_scale, dtype=dtype, error_word=error_word)
+
+    def decode(self, out, query, block_tables, context_lens, scale, workspace, num_ctas, error_word) -> None:
+        ops_fp4.paged_decode_fp4(out, query, self.pool, block_tables, context_lens, scale, workspace, num_ctas,
+                                 self.k_scale, self.v_scale, error_word)
+
+    def prefill(self, out, query, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale, error_word) -> None:
+        ops_fp4.paged_prefill_fp4(out, query, self.pool, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale,
+                                  self.k_scale, self.v_scale, error_word=error_word)
+
     def check_pair(self, value_cache) -> None:
         """Raises unless ``value_cache`` is this layer too (it holds K and V together)."""
         if not isinstance(value_cache, Fp4Layer) or value_cache.pool is not self.pool:
@@ -63,7 +78,62 @@ def _constants(name: str, value: float | Sequence[float], layers: int) -> list[f
     return values
 
 
-class PagedKVCacheFp4:
+class QuantisedKVCache:
+    """What the pools held in fewer bits share: their checks, and calls that report into the device's error word.
+    ``kv_cache`` is [num_layers, num_blocks, ...], ``layers`` the layers that attention takes."""
+
+    def _device_slots(self, slot_mapping: torch.Tensor) -> torch.Tensor:
+        if not slot_mapping.is_cuda and slot_mapping.numel():
+            lo, hi = int(slot_mapping.min()), int(slot_mapping.max())
+            if lo < 0 or hi >= self.num_blocks * self.block_size:
+                bad = lo if lo < 0 else hi
+                raise IndexError(f"index_copy_(): index {bad} is out of bounds for dimension 0 with size "
+                                 f"{self.num_blocks * self.block_size}")
+        return slot_mapping.to(device=self.device, dtype=torch.long)
+
+    def write(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor,
+              slot_mapping: torch.Tensor) -> None:
+        """Quantises the rows (bf16 or fp16) into ``layer_idx`` at ``slot_mapping``. Slots must differ."""
+        total_tokens, num_kv_heads, head_dim = key_states.shape
+        if num_kv_heads != self.num_kv_heads or head_dim != self.head_dim:
+            raise ValueError(f"kv shape mismatch: got {tuple(key_states.shape)}")
+        if slot_mapping.numel() != total_tokens:
+            raise ValueError(f"slot_mapping numel {slot_mapping.numel()} != total_tokens {total_tokens}")
+        if value_states.shape != key_states.shape:
+            raise ValueError(f"kv shape mismatch: got {tuple(value_states.shape)}")
+        if total_tokens == 0:
+            return
+        slots = self._device_slots(slot_mapping)
+        layer = self.layers[layer_idx]
+        with torch.cuda.device(self.device):
+            errors = device_errors.state(self.device)
+            errors.raise_if_flagged()
+            layer.append(_packed_rows(key_states.to(self.device)), _packed_rows(value_states.to(self.device)), slots,
+                         errors.word)
+            errors.launched()
+
+    def read(self, layer_idx: int, slot_mapping: torch.Tensor,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """The K and V rows [slots, kv_heads, head_dim] that ``layer_idx`` holds at ``slot_mapping``."""
+        slots = self._device_slots(slot_mapping)
+        layer = self.layers[layer_idx]
+        with torch.cuda.device(self.device):
+            errors = device_errors.state(self.device)
+            errors.raise_if_flagged()
+            rows = layer.read(slots, dtype, errors.word)
+            errors.launched()
+        return rows
+
+    def get_physical_cache(self, layer_idx: int):
+        return self.layers[layer_idx], self.layers[layer_idx]
+
+    def copy_blocks(self, pairs) -> None:
+        """Copies blocks, (source, destination) each, in every layer; source -1
+        clears the destination (see ``copy_pool_blocks``)."""
+        copy_pool_blocks([self.kv_cache], pairs)
+
+
+class PagedKVCacheFp4(QuantisedKVCache):
     def __init__(
         self,
         num_layers: int,
@@ -95,50 +165,3 @@ class PagedKVCacheFp4:
     def bytes_per_block(self) -> int:
         """K + V bytes of one block across all layers."""
         return fp4_bytes_per_block(self.num_layers, self.block_size, self.num_kv_heads)
-
-    def _device_slots(self, slot_mapping: torch.Tensor) -> torch.Tensor:
-        if not slot_mapping.is_cuda and slot_mapping.numel():
-            lo, hi = int(slot_mapping.min()), int(slot_mapping.max())
-            if lo < 0 or hi >= self.num_blocks * self.block_size:
-                bad = lo if lo < 0 else hi
-                raise IndexError(f"index_copy_(): index {bad} is out of bounds for dimension 0 with size "
-                                 f"{self.num_blocks * self.block_size}")
-        return slot_mapping.to(device=self.device, dtype=torch.long)
-
-    def write(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor,
-              slot_mapping: torch.Tensor) -> None:
-        """Quantises the rows (bf16 or fp16) into ``layer_idx`` at ``slot_mapping``. Slots must differ."""
-        total_tokens, num_kv_heads, head_dim = key_states.shape
-        if num_kv_heads != self.num_kv_heads or head_dim != self.head_dim:
-            raise ValueError(f"kv shape mismatch: got {tuple(key_states.shape)}")
-        if slot_mapping.numel() != total_tokens:
-            raise ValueError(f"slot_mapping numel {slot_mapping.numel()} != total_tokens {total_tokens}")
-        if value_states.shape != key_states.shape:
-            raise ValueError(f"kv shape mismatch: got {tuple(value_states.shape)}")
-        if total_tokens == 0:
-            return
-        slots = self._device_slots(slot_mapping)
-        layer = self.layers[layer_idx]
-        with torch.cuda.device(self.device):
-            errors = device_errors.state(self.device)
-            errors.raise_if_flagged()
-            ops_fp4.kv_append_fp4(layer.pool, _packed_rows(key_states.to(self.device)),
-                                  _packed_rows(value_states.to(self.device)), slots, layer.k_scale, layer.v_scale,
-                                  error_word=errors.word)
-            errors.launched()
-
-    def read(self, layer_idx: int, slot_mapping: torch.Tensor,
-             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
-        """The K and V rows [slots, kv_heads, head_dim] that ``layer_idx`` holds at ``slot_mapping``."""
-        slots = self._device_slots(slot_mapping)
-        layer = self.layers[layer_idx]
-        with torch.cuda.device(self.device):
-            errors = device_errors.state(self.device)
-            errors.raise_if_flagged()
-            rows = ops_fp4.kv_read_fp4(layer.pool, slots, layer.k_scale, layer.v_scale, dtype=dtype,
-                                       error_word=errors.word)
-            errors.launched()
-        return rows
-
-    def get_physical_cache(self, layer_idx: int) -> tuple[Fp4Layer, Fp4Layer]:
-        return self.layers[layer_idx], self.layers[layer_idx]

@@ -19,8 +19,8 @@ that is not the sequence's last position) is reported through the decode
 workspace's error word and raised by ``device_errors`` on a following call
 or by ``device_errors.check_errors()``.
 
-Over a ``PagedKVCacheFp4`` both cache arguments are the layer's ``Fp4Layer``
-and the 4-bit decode kernel runs. It reports into the device's shared error
+Over a ``PagedKVCacheFp4`` or ``PagedKVCacheFp8`` both cache arguments are the
+layer's ``Fp4Layer`` or ``Fp8Layer`` and its decode kernel runs. It reports into the device's shared error
 word, also from graphs that the caller captures (``check_errors()`` raises what
 their replays found), and from a ``DecodeGraphRunner`` into its workspace's.
 """
@@ -36,6 +36,7 @@ from . import device_errors, ops, ops_fp4
 from ._lib import FP4_DECODE_ZEROED_BYTES
 from .cuda_graph import graph_workspace
 from .fp4_kv_cache import Fp4Layer
+from .fp8_kv_cache import Fp8Layer
 from .paged_kv_cache import take_deferred
 
 _NUM_SMS: dict[int, int] = {}
@@ -70,9 +71,9 @@ def shared_workspace(device: torch.device, nbytes: int, shape: tuple = ()) -> to
     return ws
 
 
-# Eager-mode workspaces of the 4-bit kernel, one per device and stream (calls
-# on two streams may overlap), grown on demand. Its layout does not hang on the
-# call's shape, so a workspace is zeroed once.
+# Eager-mode workspaces of the 4- and 8-bit kernels, one per device and stream
+# (calls on two streams may overlap), grown on demand. Their layout is one and
+# does not hang on the call's shape, so a workspace is zeroed once.
 _FP4_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 
 
@@ -126,9 +127,9 @@ class PagedAttention(nn.Module):
             if longest > block_tables.shape[1] * key_cache.shape[1]:
                 raise RuntimeError(f"missing block: context length {longest} exceeds the "
                                    f"{block_tables.shape[1]}-block table")
-        if isinstance(key_cache, Fp4Layer):
+        if isinstance(key_cache, (Fp4Layer, Fp8Layer)):
             key_cache.check_pair(value_cache)
-            return self._forward_fp4(output, q, key_cache, block_tables, context_lens)
+            return self._forward_quantised(output, q, key_cache, block_tables, context_lens)
         with torch.cuda.device(device):
             errors = device_errors.state(device)
             errors.raise_if_flagged()
@@ -157,21 +158,20 @@ class PagedAttention(nn.Module):
                 errors.launched(word)
         return output
 
-    def _forward_fp4(self, output: torch.Tensor, q: torch.Tensor, layer: Fp4Layer, block_tables: torch.Tensor,
-                     context_lens: torch.Tensor) -> torch.Tensor:
+    def _forward_quantised(self, output: torch.Tensor, q: torch.Tensor, layer: Fp4Layer | Fp8Layer,
+                           block_tables: torch.Tensor, context_lens: torch.Tensor) -> torch.Tensor:
         device = q.device
         with torch.cuda.device(device):
             errors = device_errors.state(device)
             errors.raise_if_flagged()
-            workspace = graph_workspace(self._fp4, q.shape[0], "(4-bit)")
+            workspace = graph_workspace(self._fp4, q.shape[0], "(4-bit)" if isinstance(layer, Fp4Layer) else "(8-bit)")
             word = None  # the graph runner reads its slot's word after each replay
             if workspace is None:
                 workspace = _fp4_workspace(device, self._fp4.workspace_bytes(q.shape[0]))
                 word = errors.word
             tables = block_tables.to(device=device, dtype=torch.int32)
             ctx = context_lens.to(device=device, dtype=torch.int32)
-            ops_fp4.paged_decode_fp4(output, q.contiguous(), layer.pool, tables, ctx, self.scale, workspace,
-                                     self.num_ctas, layer.k_scale, layer.v_scale, word)
+            layer.decode(output, q.contiguous(), tables, ctx, self.scale, workspace, self.num_ctas, word)
             if word is not None:
                 errors.launched()
         return output

@@ -161,6 +161,41 @@ class PagedKVCache:
     def get_physical_cache(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor]:
         return self.key_cache[layer_idx], self.value_cache[layer_idx]
 
+    def copy_blocks(self, pairs) -> None:
+        """Copies blocks, (source, destination) each, in every layer; source -1
+        clears the destination (see ``copy_pool_blocks``)."""
+        if self._pending:
+            raise RuntimeError("copy_blocks inside deferred_appends(): rows are held back")
+        copy_pool_blocks([self.key_cache, self.value_cache], pairs)
+
+
+def copy_pool_blocks(pools: list[torch.Tensor], pairs) -> None:
+    """``ops.copy_blocks`` of a cache's tensors [layers, blocks, ...]. ``pairs`` on
+    the host (a sequence of (source, destination), or a CPU tensor [n, 2]) are
+    checked: IndexError for a block outside the pool, ValueError where a
+    destination is another pair's source or destination. An int32 device tensor
+    [n, 2] is taken as it is; what it names outside the pool is skipped and
+    raises through ``device_errors``."""
+    device, blocks = pools[0].device, pools[0].shape[1]
+    if not (isinstance(pairs, torch.Tensor) and pairs.is_cuda):
+        pairs = torch.as_tensor(pairs)
+        if pairs.numel() == 0:
+            return
+        if pairs.dim() != 2 or pairs.shape[1] != 2 or pairs.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"copies must be (source, destination) block ids, got {pairs.dtype} {tuple(pairs.shape)}")
+        for src, dst in pairs.tolist():
+            if not (-1 <= src < blocks and 0 <= dst < blocks):
+                raise IndexError(f"copy of block {src} to {dst} in a pool of {blocks} blocks")
+        sources, targets = pairs[:, 0].tolist(), pairs[:, 1].tolist()
+        if len(set(targets)) != len(targets) or set(targets) & set(sources):
+            raise ValueError("a block that is copied to is also another copy's destination, or a source")
+        pairs = pairs.to(torch.int32).to(device)
+    with torch.cuda.device(device):
+        errors = device_errors.state(device)
+        errors.raise_if_flagged()
+        ops.copy_blocks(pools, pairs, error_word=errors.word)
+        errors.launched()
+
 
 def _packed_rows(t: torch.Tensor) -> torch.Tensor:
     """Keeps strided token rows (e.g. a slice of a fused QKV output) as they are;

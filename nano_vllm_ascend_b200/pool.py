@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import FP4_UNIT_BYTES, FP4_UNIT_TOKENS
+from ._lib import FP4_UNIT_BYTES, FP4_UNIT_TOKENS, FP8_UNIT_BYTES, FP8_UNIT_TOKENS
 
 
 def bytes_per_block(num_layers: int, block_size: int, num_kv_heads: int, head_dim: int,
@@ -16,6 +16,11 @@ def bytes_per_block(num_layers: int, block_size: int, num_kv_heads: int, head_di
 def fp4_bytes_per_block(num_layers: int, block_size: int, num_kv_heads: int) -> int:
     """K and V bytes of one block of a 4-bit pool (head_dim 128) across all layers."""
     return num_layers * num_kv_heads * (block_size // FP4_UNIT_TOKENS) * FP4_UNIT_BYTES
+
+
+def fp8_bytes_per_block(num_layers: int, block_size: int, num_kv_heads: int) -> int:
+    """K and V bytes of one block of an 8-bit pool (head_dim 128) across all layers."""
+    return num_layers * num_kv_heads * (block_size // FP8_UNIT_TOKENS) * FP8_UNIT_BYTES
 
 
 def num_blocks_for_budget(free_bytes: int, total_bytes: int, memory_utilization: float, num_layers: int,

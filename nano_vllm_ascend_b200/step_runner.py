@@ -22,8 +22,11 @@ runs:
   (model_runner.py:284-286); the device error words are read with them;
 * prefill runs the same layers eagerly with prefix-aware paged prefill
   attention over the pool (cached prefix + the rows just appended);
-* with ``kv_cache_dtype="fp4"`` the pool is held in 4 bits
-  (``PagedKVCacheFp4``) and the same steps run on its kernels.
+* with ``kv_cache_dtype="fp4"`` or ``"fp8"`` the pool is held in 4 or 8 bits
+  (``PagedKVCacheFp4``, ``PagedKVCacheFp8``) and the same steps run on its
+  kernels; before the 8-bit append, norm and RoPE are ``ops.rotary``;
+* ``fork()`` starts a sequence as a copy of another one, and ``compact()``
+  moves the pool's blocks in use to its front.
 
 The model is Qwen3-shaped with seeded random weights (``PathModel``; no
 checkpoint is loaded -- model loading, model_runner.py:85-111, is not part
@@ -41,14 +44,16 @@ from types import SimpleNamespace
 import torch
 import torch.nn.functional as F
 
-from . import device_errors, ops, ops_fp4
+from . import device_errors, ops, ops_fp4, ops_fp8
 from .block_manager import BlockManager
 from .cuda_graph import DecodeGraphRunner
 from .device_metadata import DeviceBlockTables
 from .fp4_kv_cache import Fp4Layer, PagedKVCacheFp4
+from .fp8_kv_cache import Fp8Layer, PagedKVCacheFp8
 from .paged_attention import PagedAttention
 from .paged_kv_cache import PagedKVCache
-from .pool import fp4_bytes_per_block, num_blocks_from_memory
+from .pool import fp4_bytes_per_block, fp8_bytes_per_block, num_blocks_from_memory
+from .rotary import rotary_frequencies
 
 DEFAULT_DECODE_GRAPH_BATCH_SIZES = [1, 2, 4, 8, 16, 32]
 
@@ -114,6 +119,7 @@ class PathModel:
         freqs = torch.outer(torch.arange(s.max_position, dtype=torch.float32), inv)
         emb = torch.cat((freqs, freqs), dim=-1)  # RotaryEmbedding's tables, rotary_embedding.py:20-40
         self.cos, self.sin = emb.cos().to(self.device), emb.sin().to(self.device)
+        self.inv_freq, _ = rotary_frequencies(s.head_dim, s.rope_theta, device=self.device)
         self.paged_attn = PagedAttention(s.num_heads, s.num_kv_heads, s.head_dim)
         self._lm_workspaces: dict[int, torch.Tensor] = {}
 
@@ -144,17 +150,20 @@ class PathModel:
             kc, vc = kv_cache.get_physical_cache(i)
             rows = (qkv[:, :s.num_heads], qkv[:, s.num_heads:s.num_heads + kvh], qkv[:, s.num_heads + kvh:],
                     layer.q_norm, layer.k_norm, s.rms_norm_eps, self.cos, self.sin, position_ids_flat)
-            fp4 = isinstance(kc, Fp4Layer)
-            if fp4:
+            quantised = isinstance(kc, (Fp4Layer, Fp8Layer))
+            if isinstance(kc, Fp8Layer):
+                q, k = ops.rotary(rows[0], rows[1], self.inv_freq, position_ids_flat, q_weight=layer.q_norm,
+                                  k_weight=layer.k_norm, eps=s.rms_norm_eps)
+                ops_fp8.kv_append_fp8(kc.pool, k, rows[2], md.slot_mapping, error_word=errors.word)
+            elif quantised:
                 q = ops_fp4.qk_norm_rope_append_fp4(*rows, kc.pool, md.slot_mapping, kc.k_scale, kc.v_scale,
                                                     error_word=errors.word)
             else:
                 q = ops.qk_norm_rope_append(*rows, kc, vc, md.slot_mapping, error_word=errors.word)
             if is_prefill:
                 attn = torch.empty_like(q)
-                if fp4:
-                    ops_fp4.paged_prefill_fp4(attn, q, kc.pool, tables, cu_q, kv_lens, max_q, s.head_dim ** -0.5,
-                                              kc.k_scale, kc.v_scale, error_word=errors.word)
+                if quantised:
+                    kc.prefill(attn, q, tables, cu_q, kv_lens, max_q, s.head_dim ** -0.5, errors.word)
                 else:
                     ops.paged_prefill(attn, q, kc, vc, tables, cu_q, kv_lens, max_q, s.head_dim ** -0.5,
                                       error_word=errors.word)
@@ -215,8 +224,8 @@ class StepRunner:
                  max_num_seqs: int = 32, enable_prefix_cache: bool = False, enable_decode_graph: bool = True,
                  decode_graph_batch_sizes: list[int] | None = None, seed: int = 0, kv_cache_dtype: str = "bf16",
                  k_scale=1.0, v_scale=1.0):
-        if kv_cache_dtype not in ("bf16", "fp4"):
-            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is neither 'bf16' nor 'fp4'")
+        if kv_cache_dtype not in ("bf16", "fp8", "fp4"):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is neither 'bf16' nor 'fp8' nor 'fp4'")
         self.shape = shape or ModelShape()
         self.device = torch.device(device)
         self.max_model_len = max_model_len
@@ -224,15 +233,18 @@ class StepRunner:
         self.enable_prefix_cache = enable_prefix_cache
         s = self.shape
         self.model = PathModel(self.shape, self.device, seed)
-        fp4 = kv_cache_dtype == "fp4"
-        block_bytes = fp4_bytes_per_block(s.num_layers, block_size, s.num_kv_heads) if fp4 else None
+        per_block = {"fp4": fp4_bytes_per_block, "fp8": fp8_bytes_per_block}.get(kv_cache_dtype)
+        block_bytes = per_block(s.num_layers, block_size, s.num_kv_heads) if per_block else None
         self.num_blocks = num_blocks or num_blocks_from_memory(memory_utilization, s.num_layers, block_size,
                                                                s.num_kv_heads, s.head_dim, torch.bfloat16,
                                                                self.device, block_bytes)
         self.block_manager = BlockManager(self.num_blocks, block_size, self.device)
-        if fp4:
+        if kv_cache_dtype == "fp4":
             self.kv_cache = PagedKVCacheFp4(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
                                             self.device, k_scale, v_scale)
+        elif kv_cache_dtype == "fp8":
+            self.kv_cache = PagedKVCacheFp8(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
+                                            self.device)
         else:
             self.kv_cache = PagedKVCache(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
                                          torch.bfloat16, self.device)
@@ -261,6 +273,7 @@ class StepRunner:
                                  f"{self.max_model_len}")
             seq.cached_block_ids = []
             seq.cached_prefix_len = 0
+            seq.block_moves = self.block_manager.moves
             if self.enable_prefix_cache:
                 full = seq.estimated_prompt_len // self.block_size
                 limit = full - 1 if seq.estimated_prompt_len % self.block_size == 0 and full > 0 else full
@@ -305,6 +318,9 @@ class StepRunner:
         if not seqs:
             return
         self._check_greedy(seqs)
+        for seq in seqs:
+            if seq.cached_block_ids and getattr(seq, "block_moves", None) != self.block_manager.moves:
+                raise RuntimeError(f"seq {seq.seq_id} was prepared before compact() moved its cached prefix")
         rows = [self._row(seq) for seq in seqs]
         lens = [seq.runtime_prompt_len for seq in seqs]
         ids = torch.cat([seq.runtime_prompt_token_ids.to(torch.int64) for seq in seqs])
@@ -365,6 +381,32 @@ class StepRunner:
             tokens = self._read_tokens(next_ids)
         for seq, token in zip(seqs, tokens):
             seq.set_decode_result(token)
+
+    # ------------------------------------------------- forks and compaction ---
+    def fork(self, seq, new_seq, next_token_id: int | None = None) -> None:
+        """Starts ``new_seq`` (not in flight) where ``seq`` is, with its next token or another one: the cache's full
+        blocks are shared, a partly filled last one is copied in every layer."""
+        if new_seq.seq_id in self._rows:
+            raise ValueError(f"seq {new_seq.seq_id} is in flight")
+        source = self._rows[seq.seq_id]
+        row = self._row(new_seq)
+        try:
+            self.kv_cache.copy_blocks(self.block_manager.fork(source, row))
+        except Exception:  # no free block, or an earlier step's error
+            self.free_seq(new_seq)
+            raise
+        self.device_tables.forget(row)
+        if hasattr(seq, "generated_token_ids"):
+            new_seq.generated_token_ids = list(seq.generated_token_ids)
+        new_seq.set_prefill_result(next_token_id=seq.next_token_id if next_token_id is None else next_token_id,
+                                   prompt_len=seq.cache_position)
+
+    def compact(self) -> int:
+        """Moves the blocks in use to the front of the pool, between steps; returns how many moved. Sequences prepared
+        before it with a cached prefix have to be prepared again."""
+        moved = self.block_manager.compact(self.kv_cache.copy_blocks)
+        self.device_tables.remap(moved)
+        return len(moved)
 
     # ------------------------------------------------------------ the rest ---
     def free_seq(self, seq) -> None:
