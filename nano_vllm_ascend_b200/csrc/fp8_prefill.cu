@@ -3,6 +3,8 @@
 // prefill_core.cuh; the pool's format is in fp8_kv.cuh.
 #include "prefill_core.cuh"
 
+#include <atomic>
+
 namespace nvk {
 using namespace prefill;
 namespace {
@@ -10,6 +12,48 @@ namespace {
 __global__ void __launch_bounds__(kThreadsDecoding, 1) fp8_prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                           const PrefillArgs a) {
   prefill_body<kHeldFp8>(qmap, qmap, qmap, a);
+}
+
+__global__ void __launch_bounds__(kThreadsDecoding, 1) fp8_prefill_parts_kernel(const __grid_constant__ CUtensorMap qmap,
+                                                                                const PrefillArgs a) {
+  prefill_body<kHeldFp8, true>(qmap, qmap, qmap, a);
+}
+
+constexpr size_t kSmem = sizeof(PrefillSmem) + 1024;
+
+struct ClusterLaunch {
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg{};
+  ClusterLaunch(int clusters, int ranks, cudaStream_t stream) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};
+    cfg.gridDim = dim3(clusters * ranks);
+    cfg.blockDim = dim3(kThreadsDecoding);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+  }
+};
+
+// Clusters of `ranks` CTAs that run at once on device `dev`; asked once.
+int clusters_at_once(int dev, int ranks) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][kMostParts + 1];
+  if (dev < 0 || dev >= kDevices) return 0;
+  int n = known[dev][ranks].load(std::memory_order_relaxed);
+  if (n == 0) {
+    ClusterLaunch at(1, ranks, nullptr);
+    if (cudaOccupancyMaxActiveClusters(&n, fp8_prefill_parts_kernel, &at.cfg) != cudaSuccess) n = 0;
+    if (n <= 0) {
+      cudaGetLastError();
+      n = -1;
+    }
+    known[dev][ranks].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 }  // namespace
@@ -54,7 +98,6 @@ extern "C" int nvk_fp8_paged_prefill(void* out, const void* query, const void* k
   a.num_blocks = num_blocks;
   a.num_heads = num_heads;
   a.qpk = num_heads / num_kv_heads;
-  a.paired = (a.qpk % 2 == 0) ? 1 : 0;
   a.paged = 1;
   a.batch = batch;
   a.qtiles = (max_q_len + kRows - 1) / kRows;
@@ -65,15 +108,28 @@ extern "C" int nvk_fp8_paged_prefill(void* out, const void* query, const void* k
   a.max_blocks = max_blocks_per_seq;
   a.total_q = total_q;
   a.out_scale = 1.f;
-  const size_t smem = sizeof(PrefillSmem) + 1024;
-  if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&fp8_prefill_kernel), smem)) != NVK_OK) return rc;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t items = static_cast<int64_t>(a.qtiles) * (num_heads / (a.paired ? kStreams : 1)) * batch;
+  // Two heads an item share the tiles of a KV head; where that leaves SMs without an item, one head an item, whose
+  // chain is shorter; where that leaves half of them or more, its keys over a cluster's CTAs, as many as are at hand.
+  const int64_t alone = static_cast<int64_t>(a.qtiles) * num_heads * batch;
+  a.paired = a.qpk % 2 == 0 && alone > sms;
+  const int64_t items = a.paired ? alone / kStreams : alone;
   if (items > (int64_t(1) << 30))
     return fail(NVK_ERR_UNSUPPORTED, "%s: %lld work items above the kernel's range", who, (long long)items);
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t most_tiles = (static_cast<int64_t>(max_blocks_per_seq) * block_size + kKeys - 1) / kKeys;
+  if (2 * items <= sms && most_tiles >= 2 * kLeastTiles) {
+    rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&fp8_prefill_parts_kernel), kSmem);
+    if (rc != NVK_OK) return rc;
+    for (int ranks = kMostParts; ranks > 1; --ranks)
+      if (items * ranks <= sms && most_tiles > (ranks - 1) * kLeastTiles && items <= clusters_at_once(dev, ranks)) {
+        ClusterLaunch at(static_cast<int>(items), ranks, st);
+        return check_cuda(cudaLaunchKernelEx(&at.cfg, fp8_prefill_parts_kernel, qm, a), "fp8_paged_prefill launch");
+      }
+  }
+  if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&fp8_prefill_kernel), kSmem)) != NVK_OK) return rc;
   const int grid = static_cast<int>(items < sms ? items : sms);
-  return check_cuda(launch_pdl(fp8_prefill_kernel, dim3(grid), dim3(kThreadsDecoding), smem,
-                               reinterpret_cast<cudaStream_t>(stream), qm, a),
+  return check_cuda(launch_pdl(fp8_prefill_kernel, dim3(grid), dim3(kThreadsDecoding), kSmem, st, qm, a),
                     "fp8_paged_prefill launch");
 }

@@ -149,6 +149,7 @@ struct PrefillArgs {
 // (n_kv < 0: no further item).
 struct Item {
   int qt, h0, kvh, b, q0, lq, lk, kv_row0, n_kv;
+  int k0;  // split items: this CTA's first key, n_kv its tiles
 };
 
 struct PrefillSmem {
@@ -173,6 +174,8 @@ struct PrefillSmem {
   uint64_t fin;
   uint32_t tmem_base;
   volatile int abort;
+  Item whole;                  // split items: the cluster's item
+  int parts;                   // and how many CTAs hold a part of it
 };
 
 static_assert(sizeof(PrefillSmem) + 1024 <= 232448, "prefill shared memory exceeds one SM's 227 KB");
@@ -217,8 +220,9 @@ __device__ __forceinline__ bool load_item(const PrefillArgs& a, int w, Item& it)
 }
 
 template <bool kDecoding, typename ZeroRows>
-__device__ __forceinline__ bool next_item(const PrefillArgs& a, int& w, int total, Item& it, ZeroRows&& zero_rows) {
-  for (; w < total; w += gridDim.x) {
+__device__ __forceinline__ bool next_item(const PrefillArgs& a, int& w, int step, int total, Item& it,
+                                          ZeroRows&& zero_rows) {
+  for (; w < total; w += step) {
     if (!load_item<kDecoding>(a, w, it)) continue;
     if (it.n_kv == 0) {
       zero_rows(it);
@@ -444,8 +448,60 @@ __device__ __forceinline__ void decode_chunks(Chunks& x, uint32_t tile, int r0, 
   }
 }
 
-// kmap and vmap are read by the bf16 kernel only.
-template <Held kHeld>
+// Split items (8-bit pool): the CTAs of a cluster take an item's key tiles in
+// runs of at least kLeastTiles; each leaves its O and softmax statistics in its
+// shared memory, over the K and V tiles, and all of them put rows together.
+constexpr int kLeastTiles = 2, kMostParts = 8;
+struct Part {
+  float m, exp, l, sc;
+};
+__device__ __forceinline__ uint32_t part_chunk(int row, int c) {  // four dims of a row of O: offset in sm.k
+  return row * (kD * 4) + ((c ^ (row & 7)) << 4);
+}
+
+// The output rows of this CTA, a share of the item's, by warps 0 to 7: a lane
+// takes a part's statistics (of eight at most), then four dims of all parts.
+__device__ __forceinline__ void join_parts(const PrefillArgs& a, PrefillSmem& sm, int rank, int ranks) {
+  const Item& it = sm.whole;
+  const int rows = min(kRows, it.lq - it.qt * kRows), share = (kRows + ranks - 1) / ranks, parts = sm.parts;
+  const uint32_t o_at = smem_u32(sm.k), part_at = smem_u32(sm.v);
+  const int lane = threadIdx.x & 31, p = lane & 7;
+  const int end = min(rows, (rank + 1) * share);
+#pragma unroll 1
+  for (int row = rank * share + (threadIdx.x >> 5); row < end; row += 8) {
+    const float4 x =
+        p < parts ? ld_cluster_f4(part_at + row * sizeof(Part), p) : make_float4(0.f, -INFINITY, 0.f, 0.f);  // Part
+    float4 y[kMostParts];
+#pragma unroll
+    for (int k = 0; k < kMostParts; ++k)
+      y[k] = k < parts ? ld_cluster_f4(o_at + part_chunk(row, lane), k) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool any = x.y != -INFINITY;  // the row sees a key of the part
+    float to = any ? x.x : -INFINITY;
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, off));
+    const float ref = any ? fmaf(x.x - to, x.w, x.y) : -INFINITY;
+    float most = ref;
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+    const float by = any ? fast_exp2(ref - most) : 0.f;
+    float l = x.z * by;
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kMostParts; ++k) {
+      const float w = __shfl_sync(0xffffffffu, by, k);
+      o.x = fmaf(y[k].x, w, o.x), o.y = fmaf(y[k].y, w, o.y), o.z = fmaf(y[k].z, w, o.z), o.w = fmaf(y[k].w, w, o.w);
+    }
+    const float inv = l == 0.f ? 0.f : a.out_scale / l;
+    __nv_bfloat16* out = a.out + (static_cast<int64_t>(it.q0 + it.qt * kRows + row) * a.num_heads + it.h0) * kD + 4 * lane;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+}
+
+// kmap and vmap are read by the bf16 kernel only. kParts: launched in clusters,
+// each of which has at most one item, of one stream.
+template <Held kHeld, bool kParts = false>
 __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                              const PrefillArgs& a) {
   constexpr bool kFp4 = kHeld == kHeldFp4;
@@ -453,7 +509,8 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
   constexpr bool kExps = kHeld == kHeldFp8;       // a tile's units have exponents
   pdl_launch_dependents();
   pdl_wait();
-  const int ns = item_streams(a);
+  const int ns = kParts ? 1 : item_streams(a);
+  const int rank = kParts ? static_cast<int>(cluster_rank()) : 0, ranks = kParts ? static_cast<int>(cluster_size()) : 1;
   const int total = a.qtiles * (a.num_heads / ns) * a.batch;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -480,6 +537,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     for (int i = 0; i < kItemRing; ++i) mbar_init(&sm.item_full[i], 1);
     mbar_init(&sm.fin, 1);
     sm.abort = 0;
+    if constexpr (kParts) sm.parts = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -513,12 +571,25 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           *reinterpret_cast<uint4*>(row + (lane & 15) * 8) = make_uint4(0, 0, 0, 0);
         }
     };
-    int w = blockIdx.x, qi = 0, g = 0, k_issued = 0, v_issued = 0;
+    const int step = kParts ? gridDim.x / ranks : gridDim.x;
+    int w = kParts ? blockIdx.x / ranks : blockIdx.x, qi = 0, g = 0, k_issued = 0, v_issued = 0;
     int q_extra = 0;  // streams that have a load of item qi, where that is not all of them
     bool ok = true;
     while (true) {
       Item it;
-      const bool have = next_item<kDecoding>(a, w, total, it, zero_rows);
+      bool have = next_item<kDecoding>(a, w, step, total, it, zero_rows);
+      if constexpr (kParts) {
+        if (have) {
+          const int per = it.n_kv < 2 * kLeastTiles ? it.n_kv : max(kLeastTiles, (it.n_kv + ranks - 1) / ranks);
+          if (lane == 0) {
+            sm.whole = it;
+            sm.parts = (it.n_kv + per - 1) / per;
+          }
+          it.k0 = rank * per * kKeys;
+          it.n_kv = min(per, it.n_kv - rank * per);
+          have = it.n_kv > 0;
+        }
+      }
       if (lane == 0) {
         // The Q buffers, and with them the ring slot (read by every role
         // before the previous item's last S), are free once the previous
@@ -596,7 +667,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         ok = false;
       }
       ++qi;
-      w += gridDim.x;
+      w += step;
       if (!ok) break;
     }
     if (lane == 0) {
@@ -778,8 +849,9 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       } else {
         // One set of registers: K's chunks make room for V's of the same tile, those for K's of the next one.
         const int r0 = r & ~31;  // the warp's first token row
+        const int tok0 = kParts ? it.k0 + r0 : r0;
         Chunks x;
-        const uint8_t* unit[2] = {unit_of(r0), unit_of(r0 + 16)};
+        const uint8_t* unit[2] = {unit_of(tok0), unit_of(tok0 + 16)};
         int2 exps;  // lanes 0 and 1: of their unit
         auto load_exps = [&] {
           exps = make_int2(0, 0);
@@ -788,7 +860,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         };
         load_exps();
 #pragma unroll
-        for (int n = 0; n < 8; ++n) x.w[n] = load_chunk(unit, n, 0, it.lk - r0, lane);
+        for (int n = 0; n < 8; ++n) x.w[n] = load_chunk(unit, n, 0, it.lk - tok0, lane);
         for (int j = 0; j < it.n_kv; ++j, ++g) {
           if (!tile_of(
                   j,
@@ -799,19 +871,19 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
                       sm.exps[g % 4][0][r0 / 16 + lane] = static_cast<uint8_t>(127 + fp8::held_exp(exps.x));
                       sm.exps[g % 4][1][r0 / 16 + lane] = static_cast<uint8_t>(127 + fp8::held_exp(exps.y));
                     }
-                    const int seen = it.lk - j * kKeys - r0;
+                    const int seen = it.lk - j * kKeys - tok0;
                     decode_chunks<false>(x, tile, r0, 0, nullptr, lane,
                                          [&](int n) { return load_chunk(unit, n, 1, seen, lane); });
                   },
                   [&] {
-                    const int next = j + 1 < it.n_kv ? (j + 1) * kKeys + r0 : INT_MAX - 16;
+                    const int next = j + 1 < it.n_kv ? (j + 1) * kKeys + tok0 : INT_MAX - 16;
                     unit[0] = unit_of(next);
                     unit[1] = unit_of(next + 16);
                     load_exps();
                   },
                   [&](uint32_t tile) {
-                    const int seen = it.lk - (j + 1) * kKeys - r0;
-                    decode_chunks<true>(x, tile, r0, j * kKeys + r0, nan_from, lane,
+                    const int seen = it.lk - (j + 1) * kKeys - tok0;
+                    decode_chunks<true>(x, tile, r0, j * kKeys + tok0, nan_from, lane,
                                         [&](int n) { return load_chunk(unit, n, 0, seen, lane); });
                   },
                   [] {}))
@@ -866,7 +938,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         // warp-uniform outcome: the tcgen05.ld/st below need a converged warp
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[s], g & 1))) { ok = false; break; }
         tc_fence_after();
-        const int kbase = j * kKeys;
+        const int kbase = (kParts ? it.k0 : 0) + j * kKeys;
         uint32_t sr[4][32];
         // A decoding kernel masks in tensor memory, in a loop: masking all of the row's registers at once is code that
         // runs once an item, and fetching it took longer (the instruction caches are full of the decoders' code).
@@ -1042,6 +1114,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       if (!ok) break;
       const int rows = min(kRows, it.lq - it.qt * kRows);
       __nv_bfloat16* out = a.out + (static_cast<int64_t>(it.q0 + it.qt * kRows) * a.num_heads + it.h0 + s) * kD;
+      const float sc_done = sc;
       if (kDecoding && !begin_item(qi + 1)) {
         ok = false;
         break;
@@ -1058,6 +1131,24 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       // (`it` is the next item by now; this one's slot is filled again only behind its output)
       const Item& done = sm.items[qi % kItemRing];
       const int seen = kDecoding ? done.lk - done.lq + done.qt * kRows + r : 0;  // this row's last key
+      if constexpr (kParts) {
+        if (sm.parts > 1) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tmem_o + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              st_shared_v4(smem_u32(sm.k) + part_chunk(r, 8 * c + e), o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+          if (seen >= sm.nan_from[qi % kItemRing][0]) l = __uint_as_float(0x7fffffffu);
+          st_shared_v4(smem_u32(sm.v) + r * sizeof(Part), __float_as_uint(m), __float_as_uint(exp), __float_as_uint(l),
+                       __float_as_uint(sc_done));
+          ++qi;
+          continue;
+        }
+      }
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -1105,6 +1196,12 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if constexpr (kParts) {  // (every wait above ends, so all threads of the cluster come here)
+    cluster_sync();
+    if (warp < kProducerWarp && sm.parts > 1) join_parts(a, sm, rank, ranks);
+    __syncwarp();
+    cluster_sync();  // the others have read this CTA's part
+  }
   if (warp == kMmaWarp) {
     __syncwarp();
     tmem_dealloc(tmem, kTmemCols);

@@ -164,12 +164,13 @@ __device__ __forceinline__ void store_words(void* p, const Words<V>& r) {
   else *static_cast<uint32_t*>(p) = r.w[0];
 }
 
-constexpr int kRowWarps = 8;
+constexpr int kRowWarps = 4;
+constexpr int kRowBlocks = 8;  // an SM: 64 registers a thread, 32 warps
 constexpr int kRowMostDim = 256;
 
 // `share` rows of a token a warp; `group` lanes a row (a power of two).
 template <typename T, int V, bool kNorm, bool kInterleaved>
-__global__ void __launch_bounds__(32 * kRowWarps) row_kernel(const Args a, int share, int shares, int group) {
+__global__ void __launch_bounds__(32 * kRowWarps, kRowBlocks) row_kernel(const Args a, int share, int shares, int group) {
   __shared__ float2 turns[kRowWarps][kRowMostDim / 2];
   pdl_launch_dependents();
   pdl_wait();
