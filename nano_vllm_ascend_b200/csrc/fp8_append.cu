@@ -15,6 +15,8 @@
 //    blocks look their units' 16 entries up. The index needs no clearing: entry
 //    i of slot s counts only if slots[i] is s, whatever else the memory held.
 // Slots must differ; of two rows for one slot, one is written whole.
+#include <algorithm>
+
 #include "fp8_kv.cuh"
 
 namespace nvk {
@@ -25,7 +27,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMostChunk = 16;     // tokens of a block
 constexpr int kScanTokens = 512;
-constexpr int kScanChunk = 4;
+constexpr int kMostShares = 16;
 
 struct AppendArgs {
   const uint8_t* key;
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a)
   __syncthreads();
   const int per_unit = 2 * a.kvh, items = num_owners * per_unit;
   const int half = lane >> 4, part = lane & 15;  // this lane's dims: 8 part .. 8 part + 7 of every other row
-  for (int w = warp; w < items; w += kWarps) {
+  for (int w = blockIdx.y * kWarps + warp; w < items; w += gridDim.y * kWarps) {
     const int c = owners[w / per_unit], rest = w % per_unit, kv = rest >= a.kvh, head = rest - kv * a.kvh;
     uint8_t* unit = unit_at(a.pool, unit_of[c], head, a.kvh, a.upb_log2);
     int* exp_at = reinterpret_cast<int*>(unit + kOffExp) + kv;
@@ -324,9 +326,12 @@ extern "C" int nvk_fp8_append(const void* key, const void* value, int64_t key_to
     if (rc != NVK_OK) return rc;
     a.chunk = kMostChunk;
   } else {
-    a.chunk = num_tokens <= 256 ? 1 : kScanChunk;
+    a.chunk = 1;
   }
-  const dim3 grid((a.tokens + a.chunk - 1) / a.chunk);
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int blocks = (a.tokens + a.chunk - 1) / a.chunk, rounds = (2 * a.kvh * a.chunk + kWarps - 1) / kWarps;
+  const dim3 grid(blocks, std::clamp(4 * sms / blocks, 1, std::min(rounds, kMostShares)));
   const bool wide = aligned16(key) && aligned16(value) && key_token_stride % 8 == 0 && value_token_stride % 8 == 0;
   auto launch = [&](auto kernel) { return check_cuda(launch_pdl(kernel, grid, dim3(kThreads), 0, st, a), "fp8_append launch"); };
   if (dtype == NVK_DTYPE_BF16)

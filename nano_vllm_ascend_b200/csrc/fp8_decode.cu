@@ -212,7 +212,7 @@ struct Format {
   static constexpr int kWarps = kWarpsOfF, kTileUnits = kUnitsOfF, kStages = kStagesOfF;
   static constexpr int kUnitBytes = fp8::kUnitBytes, kTileTokens = kTileUnits * kUnitTokens;
   static constexpr int kTileBytes = kTileUnits * kUnitBytes;
-  static constexpr int kMinTiles = 16 / kTileUnits;
+  static constexpr int kMinTiles = 8 / kTileUnits;
   static constexpr bool kExps = true;  // a piece's reference is its largest product and an exponent
   using State = fp8::State;
   struct Scratch {};

@@ -684,6 +684,114 @@ def test_prefill_flags_bad_blocks_and_lengths(cuda_device):
     assert not out[10:].any()
 
 
+# Few items: a cluster of CTAs shares an item's keys, 8 down to 2 of them by how many items there are.
+@pytest.mark.parametrize("items", [1, 14, 20, 25, 30, 40, 60, 74])
+def test_prefill_keys_over_clusters(cuda_device, items):
+    """Ragged lengths of one to 20 tiles of keys, some sequences empty: parts of two tiles and more, and undivided ones."""
+    g = torch.Generator().manual_seed(items)
+    q = torch.randint(0, 129, (items,), generator=g).tolist()
+    c = (torch.rand(items, generator=g) ** 2 * 2400).int().tolist()
+    q[0], c[0] = 128, 2400
+    prefill_case(cuda_device, q, c, 1, 1, 64, seed=items)
+
+
+@pytest.mark.parametrize("cached", list(range(0, 1400, 128)) + [127, 383, 385, 511, 513, 900])
+def test_prefill_keys_over_clusters_at_borders(cuda_device, cached):
+    prefill_case(cuda_device, [128], [cached], 2, 1, 128, seed=cached)
+    prefill_case(cuda_device, [1, 200], [cached, 1000], 3, 3, 16, seed=cached)
+
+
+def test_prefill_parts_whose_scores_and_exponents_differ(cuda_device):
+    for seed, kw in ((5, dict(q_mul=8.0)), (6, dict(q_mul=2.0 ** -6, spread=16)), (7, dict(q_mul=2.0 ** 30, mul=2.0 ** -30)),
+                     (8, dict(q_mul=2.0 ** -30, mul=2.0 ** 30)), (9, dict(q_mul=16.0, spread=8))):
+        prefill_case(cuda_device, [150], [1700], 4, 1, 32, seed=seed, **kw)
+
+
+def test_prefill_parts_that_no_row_or_only_some_rows_see(cuda_device):
+    """Fewer keys than queries, so that the first rows see none of the item's keys; the last tiles only the last rows."""
+    dev, h, kvh, bs = cuda_device, 2, 1, 128
+    pool, kr, vr = make_pool(dev, 10, bs, kvh, 3)
+    q_lens, kv = [1100, 700], [1000, 700]
+    q = torch.randn(1800, h, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(dev)
+    out = torch.full_like(q, 5.0)
+    tables = torch.stack([torch.randperm(10, generator=torch.Generator().manual_seed(i))[:8] for i in range(2)]).int()
+    cu = torch.tensor([0, 1100, 1800], dtype=torch.int32, device=dev)
+    ops_fp8.paged_prefill_fp8(out, q, pool, tables.to(dev), cu, torch.tensor(kv, dtype=torch.int32, device=dev), 1100,
+                              SCALE)
+    for b, (at, m, n) in enumerate(((0, 1100, 1000), (1100, 700, 700))):
+        sl = seq_slots(tables[b], n, bs, dev)
+        want, a = fp4_oracle.attention(q[at:at + m], kr[sl], vr[sl], SCALE)
+        check(out[at:at + m], want, a, n, float(vr.abs().max()), PREFILL, f"sequence {b}")
+    assert not out[:100].any()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("token", [0, 129, 600, 1055, 1150])
+def test_prefill_nan_in_any_part(cuda_device, which, token):
+    dev, h, kvh, bs, m, n = cuda_device, 4, 2, 16, 160, 1160
+    pool, tables, q, cu, lens, out = prefill_case(dev, [m], [n - m], h, kvh, bs, seed=9)
+    before = out.clone()
+    slot = int(tables[0, token // bs]) * bs + token % bs
+    at = 2048 * which + 128 * (slot % 16)
+    pool[slot // bs, 1, slot % bs // 16, at:at + 128] = 0x7F
+    ops_fp8.paged_prefill_fp8(out, q, pool, tables.to(dev), cu, lens, m, SCALE)
+    nan, first = torch.isnan(out), max(0, token - (n - m))  # query i sees keys up to n - m + i
+    assert nan[first:, 2:].all() and int(nan.sum()) == (m - first) * 2 * D
+    assert torch.equal(out[:, :2], before[:, :2]) and torch.equal(out[:first], before[:first])
+
+
+def test_prefill_parts_repeat_in_graphs_and_on_two_streams(cuda_device):
+    """Bit for bit: eager calls on two streams at once, and captured ones over lengths that change."""
+    dev = cuda_device
+    pool, tables, q, cu, lens, out = prefill_case(dev, [100, 30], [1500, 2500], 4, 2, 64, seed=3)
+    tables = tables.to(dev)
+    other = lens - 700
+
+    def run(to, n):
+        ops_fp8.paged_prefill_fp8(to, q, pool, tables, cu, n, 100, SCALE)
+
+    want = {id(lens): out.clone(), id(other): torch.empty_like(out)}
+    run(want[id(other)], other)
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    outs = [[torch.empty_like(out) for _ in range(10)] for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(dev))
+    for i in range(10):
+        for s, o, n in zip(streams, outs, (lens, other)):
+            with torch.cuda.stream(s):
+                run(o[i], n)
+    torch.cuda.synchronize()
+    for o, n in zip(outs, (lens, other)):
+        assert all(torch.equal(x, want[id(n)]) for x in o)
+    graph, held = torch.cuda.CUDAGraph(), lens.clone()
+    with torch.cuda.graph(graph):
+        run(out, held)
+        run(outs[0][0], held)
+    for n in (other, lens, other):
+        held.copy_(n)
+        graph.replay()
+        assert torch.equal(out, want[id(n)]) and torch.equal(outs[0][0], want[id(n)])
+
+
+def test_prefill_parts_flag_bad_blocks(cuda_device):
+    dev, bs = cuda_device, 128
+    pool, kr, vr = make_pool(dev, 12, bs, 1, 3)
+    q = torch.randn(20, 1, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(dev)
+    out = torch.empty_like(q)
+    for bad in range(12):
+        table = torch.arange(12, dtype=torch.int32)[None]
+        table[0, bad] = 12 if bad % 2 else -1
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        ops_fp8.paged_prefill_fp8(out, q, pool, table.to(dev), torch.tensor([0, 20], dtype=torch.int32, device=dev),
+                                  torch.tensor([1500], dtype=torch.int32, device=dev), 20, SCALE, error_word=err)
+        assert int(err.item()) == 2
+        k, v = kr[:1500].clone(), vr[:1500].clone()
+        k[bad * bs:(bad + 1) * bs] = 0  # what a bad block holds: zeros
+        v[bad * bs:(bad + 1) * bs] = 0
+        want, a = fp4_oracle.attention(q, k, v, SCALE)
+        check(out, want, a, 1500, float(vr.abs().max()), PREFILL, f"block {bad}")
+
+
 def test_append_decode_and_prefill_together(cuda_device):
     """As they are used: a prompt appended and prefilled, then tokens appended and decoded one by one; each decode is
     the last row of a prefill over the same pool."""
