@@ -10,10 +10,24 @@
 // token is written, makes them zeros.
 // Which tokens share a unit:
 //  - up to kScanTokens: every block looks through the call's slots for those
-//    of its tokens' units;
+//    of its one token's unit;
 //  - above: index_kernel writes each token's number to index[slot], and the
-//    blocks look their units' 16 entries up. The index needs no clearing: entry
-//    i of slot s counts only if slots[i] is s, whatever else the memory held.
+//    blocks look the units' 16 entries of their 16 tokens up. The index needs no
+//    clearing: entry i of slot s counts only if slots[i] is s, whatever else the
+//    memory held.
+// (8 heads, bf16, rows of a prompt and rows of as many sequences: the scan takes
+// 6.1 and 7.5 us at 512 tokens, the index 4.9 and 8.3; 3.9 and 4.8 against 4.8
+// and 7.7 at 256; 9.1 and 13.4 against 6.1 and 13.0 at 1024. Up to 512 a caller
+// needs no workspace.)
+// A prompt's rows fill their units, so that one token of 16 owns work; a decode
+// step's all do. A block's units are therefore shared by up to kMostShares
+// blocks, as far as that keeps four on an SM busy: 1024 rows of as many
+// sequences 43.7 -> 13.0 us, of a prompt 6.1 either way; 32 rows 4.4 -> 3.3.
+// (Four tokens a block instead of 16 in the indexed form: 15.4 us for a prompt's
+// 8192 rows instead of 10.5.)
+// Bound by latency when short (3.3 us for a decode step's 32 rows, of which 2
+// are a launch in a graph) and by the loads of rows when long: 8192 rows of 8
+// heads in bf16, 50.5 MB, take 10.5 us, 7.7 at the copy rate.
 // Slots must differ; of two rows for one slot, one is written whole.
 #include <algorithm>
 
@@ -209,8 +223,12 @@ struct ReadArgs {
 // that both sides' lines and pages are used while they are open. (Row by row in
 // the order of the output, 128 bytes from a place of their own each, 28672 to
 // 35712 tokens of 8 heads ran at 3.9 to 4.4 TB/s however many were in flight.)
+// Sixteen tokens that are a unit in order share an address and an exponent.
+// HBM-bound: 32768 rows of 8 heads, 202 MB, in 34.4 us (5.9 TB/s, 0.90 of the
+// measured copy rate); with an exponent and an address a row 38.7. Five blocks
+// an SM: 44.9 us with the append of 8192 rows, four 45.9, six 46.7, eight 54.4.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) read_kernel(const ReadArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, half = lane >> 4, part = lane & 15;
@@ -232,16 +250,27 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
       }
     }
     uint2 w[8];
-    int e[8];
+    float by[8];
+    const int64_t begin = __shfl_sync(0xffffffffu, mine, 0);
+    if (__all_sync(0xffffffffu, begin >= 0 && mine == begin + part && (begin & 15) == 0)) {  // a unit, in order
+      const uint8_t* unit = unit_at(a.pool, begin >> 4, head, a.kvh, a.upb_log2);
+      const float one = pow2(held_exp(reinterpret_cast<const int*>(unit + kOffExp)[kv]));
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const int64_t slot = __shfl_sync(0xffffffffu, mine, 2 * n + half);
-      w[n] = make_uint2(0, 0);
-      e[n] = 0;
-      if (slot >= 0) {
-        const uint8_t* unit = unit_at(a.pool, slot >> 4, head, a.kvh, a.upb_log2);
-        e[n] = reinterpret_cast<const int*>(unit + kOffExp)[kv];
-        w[n] = *reinterpret_cast<const uint2*>(unit + kv * kOffV + chunk_at(slot & 15, part >> 1) + 8 * (part & 1));
+      for (int n = 0; n < 8; ++n) {
+        w[n] = *reinterpret_cast<const uint2*>(unit + kv * kOffV + chunk_at(2 * n + half, part >> 1) + 8 * (part & 1));
+        by[n] = one;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int64_t slot = __shfl_sync(0xffffffffu, mine, 2 * n + half);
+        w[n] = make_uint2(0, 0);
+        by[n] = 1.f;
+        if (slot >= 0) {
+          const uint8_t* unit = unit_at(a.pool, slot >> 4, head, a.kvh, a.upb_log2);
+          by[n] = pow2(held_exp(reinterpret_cast<const int*>(unit + kOffExp)[kv]));
+          w[n] = *reinterpret_cast<const uint2*>(unit + kv * kOffV + chunk_at(slot & 15, part >> 1) + 8 * (part & 1));
+        }
       }
     }
     uint8_t* out = (kv ? a.value : a.key) + ((first * a.kvh + head) * kD + 8 * part) * 2;
@@ -249,10 +278,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs a) {
     for (int n = 0; n < 8; ++n) {
       const int r = 2 * n + half;
       if (r >= count) continue;
-      const float by = pow2(held_exp(e[n]));
       auto two = [&](uint32_t h) {
         const float2 f = pair_to_f32<__half>(h);
-        return f32_to_pair<T>(f.x * by, f.y * by);
+        return f32_to_pair<T>(f.x * by[n], f.y * by[n]);
       };
       uint32_t h[4];
       e4m3_to_half2(w[n].x, h[0], h[1]);

@@ -23,6 +23,12 @@
 // 2^-37 of it, so that whatever the units' exponents are, what a token gives is
 // right beside what the others give. Exponents are within 40 of 0, so that a
 // weight times 2^-e stays in fp32's range.
+// Measured: 256 contexts of 2048 to 6144 tokens (16 heads on 8, 2.16 GB) in 323
+// to 341 us, 0.97 to 1.02 of the measured copy rate; two of 40960 tokens (32 on
+// 8, 169 MB) in 33.3, 0.77: start, ends and the join of pieces; 77 ragged ones of
+// up to 1499 tokens (10 on 2) in 15.3 where their 33 MB take 5: a CTA's share is
+// four units a warp. A kernel of one warp a unit and dot products by lanes took
+// 4900, 29200 and 1003 us.
 #include <type_traits>
 
 #include "decode_core.cuh"
@@ -212,6 +218,7 @@ struct Format {
   static constexpr int kWarps = kWarpsOfF, kTileUnits = kUnitsOfF, kStages = kStagesOfF;
   static constexpr int kUnitBytes = fp8::kUnitBytes, kTileTokens = kTileUnits * kUnitTokens;
   static constexpr int kTileBytes = kTileUnits * kUnitBytes;
+  // a CTA's least work: 8 units, four contexts of up to 513 tokens then take 6.6 us (16: 7.4; 32: 9.0; 6: 6.9; 4: 7.4)
   static constexpr int kMinTiles = 8 / kTileUnits;
   static constexpr bool kExps = true;  // a piece's reference is its largest product and an exponent
   using State = fp8::State;
@@ -231,6 +238,9 @@ struct Format {
   static __device__ __forceinline__ int dim(int j, int g) { return 16 * g + 2 * j; }
 };
 
+// Up to four heads a group 16 warps fit, above 12 (whose rings hold a stage more): 256 contexts of 2048 to 6144 tokens,
+// two heads a group, 331 us with 16 warps and 338 with 12; four short ones 7.4 and 8.1; two of 40960, four heads, 33.2
+// and 33.5.
 constexpr int kFewHeads = 4;
 using Few = Format<16, 1, 2>;
 using Many = Format<12, 1, 3>;

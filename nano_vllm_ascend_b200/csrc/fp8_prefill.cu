@@ -1,6 +1,22 @@
 // Causal prefill attention over the 8-bit KV pool (cached prefix and the rows
 // appended this step). The kernel body, with its design, is in
 // prefill_core.cuh; the pool's format is in fp8_kv.cuh.
+//
+// Tensor-bound by its operations (4 * 128 a visible pair and head), in practice
+// by the chains of a tile: 98 us for 32 requests of 256 tokens over 768 cached
+// ones (16 heads on 8, blocks of 128; 60.2 GFLOP, 614 TF/s, tensor pipe 37 % of
+// its cycles), where the 4-bit kernel takes 80 to 82 and the bf16 one 71.5. The
+// decoders turn two codes a conversion (2 cycles a warp instruction, measured)
+// and a tile's 32768 codes pass four warps, beside 8 of softmax that take an
+// exponent a unit. Ways that were built and measured for the same work: fp16 or
+// bf16 products of code and exponent by the decoders 106 to 158 us (spills, and
+// the wider range of bf16 costs P three bits); codes brought in by bulk copies, by
+// the decoding or a further warp, 96 to 107; eight decoding warps of 20 98 to
+// 105; both operands' registers double 98 to 115; each unit asked into L2 two to
+// five tiles ahead 98 to 101; with one stream, the idle softmax warpgroup as
+// second decoder 25.5 instead of 24.6 for five ragged requests. Those five (up to
+// 300 tokens over up to 1000, 9 heads on 3) are bound by latency: each walks up
+// to 10 tiles of 2.3 us, whatever their 1.7 us of operations.
 #include "prefill_core.cuh"
 
 #include <atomic>
@@ -110,8 +126,11 @@ extern "C" int nvk_fp8_paged_prefill(void* out, const void* query, const void* k
   a.out_scale = 1.f;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  // Two heads an item share the tiles of a KV head; where that leaves SMs without an item, one head an item, whose
-  // chain is shorter; where that leaves half of them or more, its keys over a cluster's CTAs, as many as are at hand.
+  // Two heads an item share the tiles of a KV head; where one head an item leaves none of the SMs a second one, that
+  // (512 queries over 1024 keys, 16 heads on 8: 25.1 us with two heads an item, 22 with one); where it leaves half of
+  // the SMs or more without an item, its keys over a cluster's CTAs, as many as run at once (the same 20; 128 queries
+  // over 8192 keys 146 and 36; one over 4097 78 and 22; 64 over 264, three tiles, 14.3 and 11.9 undivided, 17.7
+  // divided).
   const int64_t alone = static_cast<int64_t>(a.qtiles) * num_heads * batch;
   a.paired = a.qpk % 2 == 0 && alone > sms;
   const int64_t items = a.paired ? alone / kStreams : alone;

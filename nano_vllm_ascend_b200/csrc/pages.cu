@@ -4,6 +4,12 @@
 // A pool is one or two tensors [layers, num_blocks, block], of any type: a
 // block of a layer is block_bytes contiguous bytes. Bound by HBM: each byte is
 // read and written once.
+// 45 blocks of 128 tokens of a bf16 pool (28 layers of 8 heads) copied and three
+// cleared, 1.36 GB, with the tables of 32 sequences: 231 us (0.90 of the
+// measured copy rate); by loads and stores, 16 bytes a thread, 285. One block of
+// an 8-bit pool of 28 layers, 14.8 MB: 4.9 us with the tables, the kernels'
+// latency. Pieces of 4 to 32 KB, 1 to 12 warps and 2 to 4 pieces ahead all ran
+// in 230 to 233 us.
 #include "host_common.h"
 #include "nvk_common.cuh"
 

@@ -1,7 +1,7 @@
 // Causal prefill attention on the sm_100a tensor cores (tcgen05 + TMEM): the
 // kernel body of paged_prefill.cu (bf16 K and V, copied by TMA) and of
-// fp4_prefill.cu (the 4-bit pool, whose tiles a warpgroup of their own
-// decodes into the same shared-memory layout).
+// fp4_prefill.cu and fp8_prefill.cu (the 4- and 8-bit pools, whose tiles a
+// warpgroup of their own decodes into the same shared-memory layout).
 //
 // Replaces torch_npu.npu_fused_infer_attention_score as called from
 // src/nanovllm_ascend/layers/npu_prefill_attention.py:82-112 (TND layout,
@@ -60,6 +60,9 @@
 //     tiles are decoded behind this one's last. 16 warps have 128 registers a
 //     thread at launch: the softmax warpgroups take 176, the other two give
 //     them up.
+//   8-bit pool: the same, but that a decoding warp has 32 token rows, two
+//     units, and stores the codes as they are, as fp16; the softmax warps take
+//     the units' exponents (see decode_chunks).
 // What bounds it: the chain softmax -> P V + S -> softmax of a stream, of which
 // two overlap (tensor pipe 42 % of active cycles, exp unit 43 %, issue 46 % with
 // 4-bit K and V), and instruction fetch: 70 KB of code (4-bit), of which warps
@@ -448,9 +451,12 @@ __device__ __forceinline__ void decode_chunks(Chunks& x, uint32_t tile, int r0, 
   }
 }
 
-// Split items (8-bit pool): the CTAs of a cluster take an item's key tiles in
-// runs of at least kLeastTiles; each leaves its O and softmax statistics in its
-// shared memory, over the K and V tiles, and all of them put rows together.
+// Split items (8-bit pool): where there are few items, a cluster of CTAs takes
+// one, each a run of its key tiles. Each leaves its O and softmax statistics in
+// its shared memory, over the K and V tiles; then every CTA puts a share of the
+// rows together, from all of them over distributed shared memory, the largest
+// reference first as within a tile. A run has kLeastTiles or more, since a tile
+// takes about 2.3 us and the two barriers and the join 3.
 constexpr int kLeastTiles = 2, kMostParts = 8;
 struct Part {
   float m, exp, l, sc;

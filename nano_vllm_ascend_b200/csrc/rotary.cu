@@ -18,6 +18,12 @@
 // a lane, exchanged in shared memory. V is 8 where rows allow 16-byte loads,
 // else 2. any_kernel takes what is left: odd halves, rows at odd addresses,
 // heads above 256 dims.
+// Measured: 8191 tokens of 40 heads of 128, half of each turned, 168 MB, 29.6 us
+// (5.7 TB/s, 0.87 of the measured copy rate); by any_kernel's way, a row a warp
+// and elements one by one, 173. Blocks of four warps, 64 registers: of eight 34.7
+// (their last wave leaves SMs idle), of two 30.0; two rows ahead 29.8; ten
+// blocks an SM (48 registers, spills) 38. A decode step's 32 tokens: 2.5 us,
+// of which 2 are a launch in a graph.
 #include "host_common.h"
 #include "nvk_common.cuh"
 
