@@ -128,9 +128,7 @@ extern "C" int nvk_fp8_paged_prefill(void* out, const void* query, const void* k
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   // Two heads an item share the tiles of a KV head; where one head an item leaves none of the SMs a second one, that
   // (512 queries over 1024 keys, 16 heads on 8: 25.1 us with two heads an item, 22 with one); where it leaves half of
-  // the SMs or more without an item, its keys over a cluster's CTAs, as many as run at once (the same 20; 128 queries
-  // over 8192 keys 146 and 36; one over 4097 78 and 22; 64 over 264, three tiles, 14.3 and 11.9 undivided, 17.7
-  // divided).
+  // the SMs or more without an item, its keys over a cluster's CTAs, as many as run at once (see kSavedTiles).
   const int64_t alone = static_cast<int64_t>(a.qtiles) * num_heads * batch;
   a.paired = a.qpk % 2 == 0 && alone > sms;
   const int64_t items = a.paired ? alone / kStreams : alone;
@@ -138,14 +136,15 @@ extern "C" int nvk_fp8_paged_prefill(void* out, const void* query, const void* k
     return fail(NVK_ERR_UNSUPPORTED, "%s: %lld work items above the kernel's range", who, (long long)items);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int64_t most_tiles = (static_cast<int64_t>(max_blocks_per_seq) * block_size + kKeys - 1) / kKeys;
-  if (2 * items <= sms && most_tiles >= 2 * kLeastTiles) {
+  for (int ranks = 2 * items <= sms ? kMostParts : 1; ranks > 1; --ranks) {
+    const int64_t per = (most_tiles + ranks - 1) / ranks;
+    if (most_tiles - per < kSavedTiles) break;
+    if (items * ranks > sms) continue;
     rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&fp8_prefill_parts_kernel), kSmem);
     if (rc != NVK_OK) return rc;
-    for (int ranks = kMostParts; ranks > 1; --ranks)
-      if (items * ranks <= sms && most_tiles > (ranks - 1) * kLeastTiles && items <= clusters_at_once(dev, ranks)) {
-        ClusterLaunch at(static_cast<int>(items), ranks, st);
-        return check_cuda(cudaLaunchKernelEx(&at.cfg, fp8_prefill_parts_kernel, qm, a), "fp8_paged_prefill launch");
-      }
+    if (items > clusters_at_once(dev, ranks)) continue;
+    ClusterLaunch at(static_cast<int>(items), static_cast<int>((most_tiles + per - 1) / per), st);
+    return check_cuda(cudaLaunchKernelEx(&at.cfg, fp8_prefill_parts_kernel, qm, a), "fp8_paged_prefill launch");
   }
   if ((rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&fp8_prefill_kernel), kSmem)) != NVK_OK) return rc;
   const int grid = static_cast<int>(items < sms ? items : sms);

@@ -152,7 +152,7 @@ struct PrefillArgs {
 // (n_kv < 0: no further item).
 struct Item {
   int qt, h0, kvh, b, q0, lq, lk, kv_row0, n_kv;
-  int k0;  // split items: this CTA's first key, n_kv its tiles
+  int k0;  // divided items: this CTA's first key, n_kv its tiles
 };
 
 struct PrefillSmem {
@@ -177,7 +177,7 @@ struct PrefillSmem {
   uint64_t fin;
   uint32_t tmem_base;
   volatile int abort;
-  Item whole;                  // split items: the cluster's item
+  Item whole;                  // divided items: the cluster's item
   int parts;                   // and how many CTAs hold a part of it
 };
 
@@ -451,13 +451,18 @@ __device__ __forceinline__ void decode_chunks(Chunks& x, uint32_t tile, int r0, 
   }
 }
 
-// Split items (8-bit pool): where there are few items, a cluster of CTAs takes
+// Divided items (8-bit pool): where there are few items, a cluster of CTAs takes
 // one, each a run of its key tiles. Each leaves its O and softmax statistics in
 // its shared memory, over the K and V tiles; then every CTA puts a share of the
 // rows together, from all of them over distributed shared memory, the largest
-// reference first as within a tile. A run has kLeastTiles or more, since a tile
-// takes about 2.3 us and the two barriers and the join 3.
-constexpr int kLeastTiles = 2, kMostParts = 8;
+// reference first as within a tile. A tile takes 2.0 us, the clusters' start,
+// barriers and join 3 to 7: an item is divided where that saves kSavedTiles or
+// more. (45 items on clusters of three: 10 tiles each 20.9 us, undivided 26.1; 8
+// tiles 19.6 and 22.0; 6 tiles 18.2 and 18.0. Nine items on clusters of eight: 6
+// tiles 11.9 and 17.6, 20 tiles 15.8 and 45.9. 128 queries over 8192 keys, 16
+// heads on 8: 31.9 and 146; one query over 4097 19.6 and 78; 16 over 32784 100
+// and 612.)
+constexpr int kSavedTiles = 4, kMostParts = 8;
 struct Part {
   float m, exp, l, sc;
 };
@@ -466,8 +471,10 @@ __device__ __forceinline__ uint32_t part_chunk(int row, int c) {  // four dims o
 }
 
 // The output rows of this CTA, a share of the item's, by warps 0 to 7: a lane
-// takes a part's statistics (of eight at most), then four dims of all parts.
-__device__ __forceinline__ void join_parts(const PrefillArgs& a, PrefillSmem& sm, int rank, int ranks) {
+// takes a part's statistics (of eight at most), then four dims of all parts. Not
+// in line: its registers would be spilled in the softmax's loop (20 tiles of one
+// CTA 54.2 us instead of 46.1).
+[[maybe_unused]] static __device__ __noinline__ void join_parts(const PrefillArgs& a, PrefillSmem& sm, int rank, int ranks) {
   const Item& it = sm.whole;
   const int rows = min(kRows, it.lq - it.qt * kRows), share = (kRows + ranks - 1) / ranks, parts = sm.parts;
   const uint32_t o_at = smem_u32(sm.k), part_at = smem_u32(sm.v);
@@ -505,9 +512,9 @@ __device__ __forceinline__ void join_parts(const PrefillArgs& a, PrefillSmem& sm
   }
 }
 
-// kmap and vmap are read by the bf16 kernel only. kParts: launched in clusters,
+// kmap and vmap are read by the bf16 kernel only. kClusters: launched in clusters,
 // each of which has at most one item, of one stream.
-template <Held kHeld, bool kParts = false>
+template <Held kHeld, bool kClusters = false>
 __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                              const PrefillArgs& a) {
   constexpr bool kFp4 = kHeld == kHeldFp4;
@@ -515,8 +522,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
   constexpr bool kExps = kHeld == kHeldFp8;       // a tile's units have exponents
   pdl_launch_dependents();
   pdl_wait();
-  const int ns = kParts ? 1 : item_streams(a);
-  const int rank = kParts ? static_cast<int>(cluster_rank()) : 0, ranks = kParts ? static_cast<int>(cluster_size()) : 1;
+  const int ns = kClusters ? 1 : item_streams(a);
   const int total = a.qtiles * (a.num_heads / ns) * a.batch;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -543,7 +549,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
     for (int i = 0; i < kItemRing; ++i) mbar_init(&sm.item_full[i], 1);
     mbar_init(&sm.fin, 1);
     sm.abort = 0;
-    if constexpr (kParts) sm.parts = 0;
+    if constexpr (kClusters) sm.parts = 0;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -577,16 +583,18 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           *reinterpret_cast<uint4*>(row + (lane & 15) * 8) = make_uint4(0, 0, 0, 0);
         }
     };
-    const int step = kParts ? gridDim.x / ranks : gridDim.x;
-    int w = kParts ? blockIdx.x / ranks : blockIdx.x, qi = 0, g = 0, k_issued = 0, v_issued = 0;
+    const int rank = kClusters ? cluster_rank() : 0, ranks = kClusters ? cluster_size() : 1;
+    const int step = kClusters ? gridDim.x / ranks : gridDim.x;
+    int w = kClusters ? blockIdx.x / ranks : blockIdx.x, qi = 0, g = 0, k_issued = 0, v_issued = 0;
     int q_extra = 0;  // streams that have a load of item qi, where that is not all of them
     bool ok = true;
     while (true) {
       Item it;
       bool have = next_item<kDecoding>(a, w, step, total, it, zero_rows);
-      if constexpr (kParts) {
+      if constexpr (kClusters) {
         if (have) {
-          const int per = it.n_kv < 2 * kLeastTiles ? it.n_kv : max(kLeastTiles, (it.n_kv + ranks - 1) / ranks);
+          int per = (it.n_kv + ranks - 1) / ranks;
+          if (it.n_kv - per < kSavedTiles) per = it.n_kv;
           if (lane == 0) {
             sm.whole = it;
             sm.parts = (it.n_kv + per - 1) / per;
@@ -855,7 +863,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       } else {
         // One set of registers: K's chunks make room for V's of the same tile, those for K's of the next one.
         const int r0 = r & ~31;  // the warp's first token row
-        const int tok0 = kParts ? it.k0 + r0 : r0;
+        const int tok0 = kClusters ? it.k0 + r0 : r0;
         Chunks x;
         const uint8_t* unit[2] = {unit_of(tok0), unit_of(tok0 + 16)};
         int2 exps;  // lanes 0 and 1: of their unit
@@ -935,7 +943,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       }
       if (it.n_kv < 0) break;
       const int i = it.qt * kRows + r;
-      const int lim = (i < it.lq) ? (it.lk - it.lq + i) : (it.lk - 1);
+      const int lim = ((i < it.lq) ? (it.lk - it.lq + i) : (it.lk - 1)) - (kClusters ? it.k0 : 0);
       // 8-bit kernel: weights are relative to p 2^e, e the unit's exponent of V: to the exponent `exp` beside m, and
       // the sum l takes 2^-e back (see fp8_decode.cu).
       float exp = -INFINITY;
@@ -944,7 +952,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         // warp-uniform outcome: the tcgen05.ld/st below need a converged warp
         if (!__all_sync(0xffffffffu, mbar_wait(&sm.s_full[s], g & 1))) { ok = false; break; }
         tc_fence_after();
-        const int kbase = (kParts ? it.k0 : 0) + j * kKeys;
+        const int kbase = j * kKeys;
         uint32_t sr[4][32];
         // A decoding kernel masks in tensor memory, in a loop: masking all of the row's registers at once is code that
         // runs once an item, and fetching it took longer (the instruction caches are full of the decoders' code).
@@ -988,13 +996,13 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         };
         // The max is taken over raw scores (scale > 0), the scale folded into
         // the exponent's FMA below; max is exact, so its order is free.
-        constexpr int kParts = kExps ? kKeys / fp8::kUnitTokens : 4;  // units, or chunks
-        float mx[kParts];
+        constexpr int kRuns = kExps ? kKeys / fp8::kUnitTokens : 4;  // units, or chunks
+        float mx[kRuns];
 #pragma unroll
-        for (int u = 0; u < kParts; ++u) {
+        for (int u = 0; u < kRuns; ++u) {
           mx[u] = -INFINITY;
 #pragma unroll
-          for (int e = u * (kKeys / kParts); e < (u + 1) * (kKeys / kParts); e += 2)
+          for (int e = u * (kKeys / kRuns); e < (u + 1) * (kKeys / kRuns); e += 2)
             mx[u] = fmax3(mx[u], __uint_as_float(sr[e / 32][e % 32]), __uint_as_float(sr[e / 32][e % 32 + 1]));
         }
         bool resc;
@@ -1002,7 +1010,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         if constexpr (kExps) {
           float mt = -INFINITY, most = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < kParts; ++u) {
+          for (int u = 0; u < kRuns; ++u) {
             mx[u] *= k_pow2(u);
             mt = fmaxf(mt, mx[u]);
             most = fmaxf(most, fmaf(mx[u] - m, sc, v_exp(u) - exp));
@@ -1012,7 +1020,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
             const float to = exp == -INFINITY ? mt : fmaxf(m, mt), old = fmaf(m - to, sc, exp);
             most = old;
 #pragma unroll
-            for (int u = 0; u < kParts; ++u) most = fmaxf(most, fmaf(mx[u] - to, sc, v_exp(u)));
+            for (int u = 0; u < kRuns; ++u) most = fmaxf(most, fmaf(mx[u] - to, sc, v_exp(u)));
             alpha = fast_exp2(old - most);
             l *= alpha;
             m = to;
@@ -1120,7 +1128,6 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       if (!ok) break;
       const int rows = min(kRows, it.lq - it.qt * kRows);
       __nv_bfloat16* out = a.out + (static_cast<int64_t>(it.q0 + it.qt * kRows) * a.num_heads + it.h0 + s) * kD;
-      const float sc_done = sc;
       if (kDecoding && !begin_item(qi + 1)) {
         ok = false;
         break;
@@ -1137,7 +1144,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
       // (`it` is the next item by now; this one's slot is filled again only behind its output)
       const Item& done = sm.items[qi % kItemRing];
       const int seen = kDecoding ? done.lk - done.lq + done.qt * kRows + r : 0;  // this row's last key
-      if constexpr (kParts) {
+      if constexpr (kClusters) {
         if (sm.parts > 1) {
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
@@ -1150,7 +1157,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
           }
           if (seen >= sm.nan_from[qi % kItemRing][0]) l = __uint_as_float(0x7fffffffu);
           st_shared_v4(smem_u32(sm.v) + r * sizeof(Part), __float_as_uint(m), __float_as_uint(exp), __float_as_uint(l),
-                       __float_as_uint(sc_done));
+                       __float_as_uint(sc));  // (no item follows, so sc is still this one's)
           ++qi;
           continue;
         }
@@ -1202,9 +1209,9 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if constexpr (kParts) {  // (every wait above ends, so all threads of the cluster come here)
+  if constexpr (kClusters) {  // (every wait above ends, so all threads of the cluster come here)
     cluster_sync();
-    if (warp < kProducerWarp && sm.parts > 1) join_parts(a, sm, rank, ranks);
+    if (warp < kProducerWarp && sm.parts > 1) join_parts(a, sm, cluster_rank(), cluster_size());
     __syncwarp();
     cluster_sync();  // the others have read this CTA's part
   }
