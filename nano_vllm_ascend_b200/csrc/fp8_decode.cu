@@ -26,7 +26,7 @@
 // Measured: 256 contexts of 2048 to 6144 tokens (16 heads on 8, 2.16 GB) in 323
 // to 341 us, 0.97 to 1.02 of the measured copy rate; two of 40960 tokens (32 on
 // 8, 169 MB) in 33.3, 0.77: start, ends and the join of pieces; 77 ragged ones of
-// up to 1499 tokens (10 on 2) in 15.3 where their 33 MB take 5: a CTA's share is
+// up to 1499 tokens (10 on 2) in 14.0 where their 33 MB take 5: a CTA's share is
 // four units a warp. A kernel of one warp a unit and dot products by lanes took
 // 4900, 29200 and 1003 us.
 #include <type_traits>
@@ -238,14 +238,11 @@ struct Format {
   static __device__ __forceinline__ int dim(int j, int g) { return 16 * g + 2 * j; }
 };
 
-// Up to four heads a group 16 warps fit, above 12 (whose rings hold a stage more): 256 contexts of 2048 to 6144 tokens,
-// two heads a group, 331 us with 16 warps and 338 with 12; four short ones 7.4 and 8.1; two of 40960, four heads, 33.2
-// and 33.5.
-constexpr int kFewHeads = 4;
-using Few = Format<16, 1, 2>;
-using Many = Format<12, 1, 3>;
-static_assert(smem_bytes<Few>(kFewHeads) <= 232448 && smem_bytes<Many>(kMaxGroup) <= 232448,
-              "decode shared memory exceeds the 227 KB per-CTA limit");
+// 14 warps, a unit a tile, two tiles in flight a warp: 28 units (116 KB) an SM, and 128 registers a thread. 64 contexts of 4096 tokens of 8 KV heads with two, five and eight heads a group: 85.5,
+// 86.5 and 89.5 us; 16 warps (up to six heads fit) 89.2, 91.0 and none; 12 of three tiles 93.7 and 96.8 (five, eight); 10
+// of tiles of two units 87.2, 90.9 and 93.4. 77 ragged contexts, five heads: 14.0, 14.3, 15.2 and 14.5.
+using Only = Format<14, 1, 2>;
+static_assert(smem_bytes<Only>(kMaxGroup) <= 232448, "decode shared memory exceeds the 227 KB per-CTA limit");
 
 }  // namespace
 }  // namespace fp8
@@ -284,6 +281,5 @@ extern "C" int nvk_fp8_paged_decode(void* out, const void* query, const void* kv
   a.v_scale = 1.f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const char* what = "fp8_paged_decode launch";
-  return a.group <= kFewHeads ? launch<Few>(a, batch, ctas, kFewHeads, what, st)
-                              : launch<Many>(a, batch, ctas, kMaxGroup, what, st);
+  return launch<Only>(a, batch, ctas, kMaxGroup, what, st);
 }

@@ -16,7 +16,7 @@
 // five tiles ahead 98 to 101; with one stream, the idle softmax warpgroup as
 // second decoder 25.5 instead of 24.6 for five ragged requests. Those five (up to
 // 300 tokens over up to 1000, 9 heads on 3) are bound by latency: each walks up
-// to 10 tiles of 2.3 us, whatever their 1.7 us of operations.
+// to 9 tiles of 2.0 us, whatever their 1.7 us of operations.
 #include "prefill_core.cuh"
 
 #include <atomic>

@@ -67,7 +67,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
                 return half * math.log(length / (turns * 2 * math.pi)) / math.log(base)
 
             low = max(math.floor(pair_of(float(scaling.get("beta_fast", 32)))), 0)
-            high = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1)))), half - 1)
+            high = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
             ramp = ((torch.arange(half, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
             inv = inv / factor * ramp + inv * (1 - ramp)
             given_scale = scaling.get("attention_factor")
