@@ -260,6 +260,7 @@ class StepRunner:
         # sequence id -> row of the block manager and of the device table mirror
         self._rows: dict[int, int] = {}
         self._free_rows = list(range(max_num_seqs))
+        self._prepared_at: dict[int, int] = {}  # sequence id -> the block manager's moves when its prefix was looked up
         self._io = torch.empty(2 * max_num_seqs, dtype=torch.int64, pin_memory=True)  # ids | positions
         self._tokens = torch.empty(max(max_num_seqs, 1), dtype=torch.int64, pin_memory=True)
 
@@ -273,7 +274,7 @@ class StepRunner:
                                  f"{self.max_model_len}")
             seq.cached_block_ids = []
             seq.cached_prefix_len = 0
-            seq.block_moves = self.block_manager.moves
+            self._prepared_at[seq.seq_id] = self.block_manager.moves
             if self.enable_prefix_cache:
                 full = seq.estimated_prompt_len // self.block_size
                 limit = full - 1 if seq.estimated_prompt_len % self.block_size == 0 and full > 0 else full
@@ -318,8 +319,9 @@ class StepRunner:
         if not seqs:
             return
         self._check_greedy(seqs)
+        moves = self.block_manager.moves
         for seq in seqs:
-            if seq.cached_block_ids and getattr(seq, "block_moves", None) != self.block_manager.moves:
+            if seq.cached_block_ids and self._prepared_at.get(seq.seq_id, moves) != moves:
                 raise RuntimeError(f"seq {seq.seq_id} was prepared before compact() moved its cached prefix")
         rows = [self._row(seq) for seq in seqs]
         lens = [seq.runtime_prompt_len for seq in seqs]
@@ -410,6 +412,7 @@ class StepRunner:
 
     # ------------------------------------------------------------ the rest ---
     def free_seq(self, seq) -> None:
+        self._prepared_at.pop(seq.seq_id, None)
         row = self._rows.pop(seq.seq_id, None)
         if row is None:
             return
