@@ -3,8 +3,8 @@
 // prefill_core.cuh; the pool's format is in fp8_kv.cuh.
 //
 // Tensor-bound by its operations (4 * 128 a visible pair and head), in practice
-// by the chains of a tile: 98 us for 32 requests of 256 tokens over 768 cached
-// ones (16 heads on 8, blocks of 128; 60.2 GFLOP, 614 TF/s, tensor pipe 37 % of
+// by the chains of a tile: 97.2 us for 32 requests of 256 tokens over 768 cached
+// ones (16 heads on 8, blocks of 128; 60.2 GFLOP, 619 TF/s, tensor pipe 37 % of
 // its cycles), where the 4-bit kernel takes 80 to 82 and the bf16 one 71.5. The
 // decoders turn two codes a conversion (2 cycles a warp instruction, measured)
 // and a tile's 32768 codes pass four warps, beside 8 of softmax that take an

@@ -116,6 +116,7 @@ constexpr int kDecodeWarp0 = 12;          // quantised pools: warps 12-15
 constexpr int kThreadsDecoding = 16 * 32;
 // Registers a thread after the split of the decoding kernels' 512 x 128 (softmax, softmax, producer and MMA, decoders)
 constexpr int kRegsSoftmax = 176, kRegsIssue = 64, kRegsDecode = 96;
+// (8-bit: 184, 56 and 88 take 96.9 us for 97.4, 184, 48 and 96 108.8, 168, 64 and 112 106.7: what is spilled)
 static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsDecode <= 4 * 128, "setmaxnreg shares exceed the launch's registers");
 constexpr uint32_t kTmemCols = 512;       // S_0 | S_1 | O_0 | O_1, 128 columns each
 constexpr uint32_t kColO = 256;
@@ -1126,6 +1127,8 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         mbar_arrive(&sm.p_hi[s]);
       }
       if (!ok) break;
+      // (8-bit kernel: the descriptor is read again, since its fields would be spilled in the loop above: 98.0 -> 97.4 us)
+      if constexpr (kExps) it = sm.items[qi % kItemRing];
       const int rows = min(kRows, it.lq - it.qt * kRows);
       __nv_bfloat16* out = a.out + (static_cast<int64_t>(it.q0 + it.qt * kRows) * a.num_heads + it.h0 + s) * kD;
       if (kDecoding && !begin_item(qi + 1)) {
