@@ -104,13 +104,12 @@ template <typename T, bool kWide>
 __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a) {
   __shared__ int member[kMostChunk][kUnitTokens];  // the token that writes each offset of the unit, or -1
   __shared__ int64_t unit_of[kMostChunk];          // -1: no unit of the pool
-  __shared__ int owners[kMostChunk];
+  __shared__ int owners[kMostChunk];               // the block's tokens that own their unit, in order
   __shared__ int num_owners;
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int first = blockIdx.x * a.chunk, count = min(a.chunk, a.tokens - first);
-  if (tid == 0) num_owners = 0;
   if (tid < count) {
     const int64_t s = a.slots[first + tid];
     const bool ok = s >= 0 && s < a.num_slots;
@@ -136,11 +135,18 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a)
     }
   }
   __syncthreads();
-  if (tid < count) {
+  if (warp == 0) {
+    // Every block of the chunk (gridDim.y of them) makes this list for itself and takes a share of it by place, so the
+    // order has to be the same in all of them.
+    static_assert(kMostChunk <= 32, "a block's tokens are lanes of one warp");
     int low = -1;
-    for (int o = kUnitTokens - 1; o >= 0; --o)
-      if (member[tid][o] >= 0) low = member[tid][o];
-    if (low == first + tid) owners[atomicAdd(&num_owners, 1)] = tid;  // (the order does not matter)
+    if (lane < count)
+      for (int o = kUnitTokens - 1; o >= 0; --o)
+        if (member[lane][o] >= 0) low = member[lane][o];
+    const bool owns = lane < count && low == first + lane;
+    const uint32_t all = __ballot_sync(0xffffffffu, owns);
+    if (owns) owners[__popc(all & ((1u << lane) - 1))] = lane;
+    if (lane == 0) num_owners = __popc(all);
   }
   __syncthreads();
   const int per_unit = 2 * a.kvh, items = num_owners * per_unit;
