@@ -519,7 +519,8 @@ NVK_API int nvk_fp8_paged_prefill(void* out, const void* query, const void* kv_c
  * neither) each head is first divided by its root mean square (eps added to
  * the mean square) and multiplied by the weight. Rounded once, at the end. An
  * output may be its input (same pointer and stride). head_dim even, up to 512;
- * num_heads or num_kv_heads may be 0, whose pointers are then not used.
+ * num_heads or num_kv_heads may be 0, whose pointers, the weight among them, are
+ * then not used.
  */
 NVK_API int nvk_rotary(void* query_out, void* key_out, const void* query, const void* key, int64_t query_out_stride,
                        int64_t key_out_stride, int64_t query_stride, int64_t key_stride, const void* q_weight,

@@ -318,6 +318,8 @@ extern "C" int nvk_rotary(void* query_out, void* key_out, const void* query, con
   if (num_tokens == 0 || num_heads + num_kv_heads == 0) return NVK_OK;
   if (!inv_freq || !positions || (num_heads && (!query || !query_out)) || (num_kv_heads && (!key || !key_out)))
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (num_heads == 0) q_weight = nullptr;  // not used, whatever it is
+  if (num_kv_heads == 0) k_weight = nullptr;
   if (!q_weight != !k_weight && num_heads && num_kv_heads)
     return fail(NVK_ERR_INVALID_ARGUMENT, "%s: norm weights for only one of q and k", who);
   if (!aligned(inv_freq, 8) || !aligned(positions, 8) || !aligned(query, 2) || !aligned(key, 2) ||
