@@ -121,9 +121,10 @@ static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsDecode <= 4 * 128, "setmaxnre
 constexpr uint32_t kTmemCols = 512;       // S_0 | S_1 | O_0 | O_1, 128 columns each
 constexpr uint32_t kColO = 256;
 constexpr float kRescaleThreshold = 8.0f;
-// 8-bit kernel: bounds of the factor from products (of rows below 2^16 and codes, times 2^40 at most) to scores, such
-// that it stays normal times 2^-40 and that differences of products times it stay finite.
-constexpr float kLeastFactor = 0x1p-80f, kMostFactor = 0x1p53f;
+// 8-bit kernel: bounds of the factor from products to scores. Products are sums of 128 of rows below 2^16 and codes of
+// up to 448 * 2^40, so below 2^72: at the least factor, which is normal times 2^-40, all scores are within 2^-14 of 0
+// (weights round by 2^-11), and at the largest their differences stay finite.
+constexpr float kLeastFactor = 0x1p-86f, kMostFactor = 0x1p53f;
 constexpr float kFarScore = 1024.f;       // decoding kernels: scores whose rounding in fp32, 2^-14, would show in a weight
 constexpr int kItemRing = 4;              // item descriptors published ahead by the producer
 

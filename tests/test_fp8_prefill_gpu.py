@@ -114,3 +114,19 @@ def test_scores_of_any_magnitude(cuda_device, items):
     out = attend(pool, q, n, LOG2, items)
     want, a = fp4_oracle.attention(q, kr, vr, LOG2)
     base.check(out, want, a, n, float(vr.abs().max()), HOW)
+
+
+@pytest.mark.parametrize("items", ITEMS)
+@pytest.mark.parametrize("n", [32, 1024])
+def test_scores_next_to_zero_of_the_largest_keys(cuda_device, n, items):
+    """Keys at the format's end, +-448 * 2^40, and queries so small (2^-90) that all scores are within 2^-30 of 0: every
+    weight is the same, and values of both signs cancel."""
+    k = torch.full((n, 1, D), 448 * 2.0 ** 40)
+    k[1::2] *= -1
+    v = torch.ones(n, 1, D)
+    v[1::2] *= -1
+    pool, kr, vr = filled(cuda_device, k, v)
+    q = torch.full((1, 1, D), 1.9921875 * 2.0 ** -90, dtype=torch.bfloat16, device=cuda_device)
+    out = attend(pool, q, n, D ** -0.5, items)
+    want, a = fp4_oracle.attention(q, kr, vr, D ** -0.5)
+    base.check(out, want, a, n, float(vr.abs().max()), HOW)
