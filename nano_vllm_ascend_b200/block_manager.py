@@ -308,12 +308,19 @@ class BlockManager:
     # (the reference has neither). Both return the (source, destination) blocks
     # whose contents have to be copied, by the caches' copy_blocks(), before
     # the next step reads or writes the destinations.
-    def fork(self, slot: int, new_slot: int) -> list[tuple[int, int]]:
+    def fork(self, slot: int, new_slot: int, length: int | None = None) -> list[tuple[int, int]]:
         """Starts ``new_slot`` as a copy of ``slot``: full blocks are shared,
-        a last one that is partly filled gets a block of its own."""
+        a last one that is partly filled gets a block of its own. ``length``:
+        the tokens that the slot's blocks hold, where that is less than it has
+        been counted for (a step that failed behind its bookkeeping): both
+        sequences go on from there."""
         if new_slot in self.block_tables:
             raise ValueError(f"slot {new_slot} is in use")
-        table, length = self.block_tables[slot], self.seq_lens[slot]
+        table, counted = self.block_tables[slot], self.seq_lens[slot]
+        if length is None:
+            length = counted
+        elif not 0 <= length <= counted:
+            raise ValueError(f"cannot fork {length} tokens of slot {slot}, which has {counted}")
         full = length // self.block_size
         copies = []
         if length % self.block_size:

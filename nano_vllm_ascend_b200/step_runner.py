@@ -393,7 +393,7 @@ class StepRunner:
         source = self._rows[seq.seq_id]
         row = self._row(new_seq)
         try:
-            self.kv_cache.copy_blocks(self.block_manager.fork(source, row))
+            self.kv_cache.copy_blocks(self.block_manager.fork(source, row, seq.cache_position))
         except Exception:  # no free block, or an earlier step's error
             self.free_seq(new_seq)
             raise
