@@ -513,8 +513,9 @@ NVK_API int nvk_fp8_paged_prefill(void* out, const void* query, const void* kv_c
  * ELEMENTS between tokens, heads and dims packed), turned by their positions
  * over the first rotary_dim dims in pairs: dims (i, i + rotary_dim / 2), or (2 i,
  * 2 i + 1) where `interleaved`; pair i turns by position * inv_freq[i] radians
- * (double, rotary_dim / 2 of them), in 64 bits, so that no position loses
- * precision; the turned pair is multiplied by attention_scale. Dims from
+ * (double, rotary_dim / 2 of them), made in 64 bits: off by at most 2^-26 of a
+ * turn and 2^-52 of the angle itself (which stays below 2^-24 of a turn up to
+ * 2^30 radians); the turned pair is multiplied by attention_scale. Dims from
  * rotary_dim on pass. With q_weight and k_weight (`dtype` [head_dim], both or
  * neither) each head is first divided by its root mean square (eps added to
  * the mean square) and multiplied by the weight. Rounded once, at the end. An

@@ -1,10 +1,13 @@
-"""Calls of ``nvk_rotary`` that ``ops.rotary`` does not make, against the formula in 64 bits (see test_rotary_gpu)."""
+"""Calls of ``nvk_rotary`` that ``ops.rotary`` does not make, against the formula in 64 bits (see test_rotary_gpu), and
+its angles against exact ones."""
+
+import math
 
 import pytest
 import torch
 
-from nano_vllm_ascend_b200 import _lib
-from tests.test_rotary_gpu import check, formula, frequencies
+from nano_vllm_ascend_b200 import _lib, ops
+from tests.test_rotary_gpu import HALF, check, formula, frequencies
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +36,45 @@ def test_weights_of_an_absent_side_are_not_used(cuda_device, has, weights, inter
               *two(h), dim, rotated, interleaved, 0, torch.cuda.current_stream(dev).cuda_stream)
     want, mag = formula(x, w[side] if given[side] else None, 1e-6, inv, pos, bool(interleaved), 1.0)
     check(out, want, mag)
+
+
+PI = 31415926535897932384626433832795028841971693993751058209749445923078164062862089986280348253421170679  # times 10^-100
+
+
+def exact_angles(positions, inv):
+    """cos and sin of position * frequency [T, half], and the angles, from whole numbers."""
+    bits = 256
+    per_turn = (10 ** 100 << bits) // (2 * PI)  # 2^bits / (2 pi)
+    cos, sin, angle = [], [], []
+    for p in positions.tolist():
+        for f in inv.tolist():
+            m, d = f.as_integer_ratio()  # d a power of two
+            part = (p * m * per_turn) % (d << bits)  # of a turn, times d 2^bits
+            x = part / (d << bits) * 2 * math.pi
+            cos.append(math.cos(x))
+            sin.append(math.sin(x))
+            angle.append(abs(p) * f)
+    return (torch.tensor(t, dtype=torch.float64).view(len(positions), -1) for t in (cos, sin, angle))
+
+
+@pytest.mark.parametrize("top", [1, 12, 24, 28, 30, 36, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_an_angle_is_off_by_what_the_header_says(cuda_device, top, dtype):
+    """Turned rows (1, 0) against exact angles: the results near 0 (a few 2^-13 among so many) round by next to nothing,
+    so that the angle's own error shows. 2^-26 of a turn, 2^-52 of the angle, and in fp32 the cosine (2^-23)
+    and the product (2^-24)."""
+    half, t = 64, 2000
+    g = torch.Generator().manual_seed(top)
+    positions = torch.randint(-(1 << top), 1 << top, (t,), generator=g)
+    positions[0] = (1 << top) - 1
+    inv = frequencies(half)
+    x = torch.zeros(t, 1, 2 * half, dtype=dtype, device=cuda_device)
+    x[..., :half] = 1
+    got, _ = ops.rotary(x, x, inv.to(cuda_device), positions.to(cuda_device))
+    cos, sin, angle = exact_angles(positions, inv)
+    want = torch.cat((cos, sin), -1)
+    off = 2 * math.pi * 2.0 ** -26 + angle * 2.0 ** -52 + 2.0 ** -23 + 2.0 ** -24
+    err = (got[:, 0].double().cpu() - want).abs()
+    tol = want.abs() * HALF[dtype] + torch.cat((off, off), -1) + 2.0 ** -25 * (dtype == torch.float16)
+    assert bool((err <= tol).all()), float((err / tol).max())
+    assert top < 12 or float(want.abs().min()) < 2.0 ** -13
