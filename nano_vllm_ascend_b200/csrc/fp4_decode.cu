@@ -32,7 +32,8 @@
 // first bytes about 4 us, the pieces' meeting 1 to 2, a split pair's ticket and
 // join 2 (one context of 100 tokens 4.9 us, 32 of 256 to 2304 16.9). The last
 // comes from cuts inside pairs, which most are: 38 of 42 with 4 contexts up to
-// 513 tokens, 141 of 147 with those 32.#include <type_traits>
+// 513 tokens, 141 of 147 with those 32.
+#include <type_traits>
 
 #include "decode_core.cuh"
 

@@ -34,7 +34,6 @@ namespace fp8 {
 using fp4::e4m3_to_half2;
 using fp4::f32_to_pair;
 using fp4::floats_to_e4m3x2;
-using fp4::hmul2;
 using fp4::pair_to_f32;
 using fp4::units_log2;
 
