@@ -38,8 +38,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     and what the turned pairs are multiplied by. ``scaling``: {"type": one of the above, ...}, or None."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim {rotary_dim} is not even and positive")
-    if not base > 1:
-        raise ValueError(f"base {base} is not above 1")
+    if not 1 < base < math.inf:
+        raise ValueError(f"base {base} is not above 1 and finite")
     half = rotary_dim // 2
     pair = torch.arange(half, dtype=torch.float64) / half
     inv, scale = float(base) ** -pair, 1.0
@@ -53,27 +53,31 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
             raise ValueError(f"{kind} scaling takes {sorted(needed)}" + (f" and may have {sorted(more)}" if more else "")
                              + f", got {sorted(given)}")
         factor = float(scaling["factor"])
-        if not factor >= 1:
-            raise ValueError(f"scaling factor {factor} is below 1")
+        if not 1 <= factor < math.inf:
+            raise ValueError(f"scaling factor {factor} is below 1 or not finite")
+        length = float(scaling.get("original_max_position", 1))
+        if not 0 < length < math.inf:
+            raise ValueError(f"original_max_position {length} is not positive and finite")
         if kind == "linear":
             inv = inv / factor
         elif kind == "ntk":
             if half > 1:
                 inv = (base * factor ** (half / (half - 1))) ** -pair
         elif kind == "yarn":
-            length = float(scaling["original_max_position"])
+            fast, slow = float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
+            if not 0 < slow <= fast:
+                raise ValueError(f"beta_slow {slow} is not positive or above beta_fast {fast}")
 
             def pair_of(turns: float) -> float:  # the pair that turns so often within the length
                 return half * math.log(length / (turns * 2 * math.pi)) / math.log(base)
 
-            low = max(math.floor(pair_of(float(scaling.get("beta_fast", 32)))), 0)
-            high = min(math.ceil(pair_of(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
+            low = max(math.floor(pair_of(fast)), 0)
+            high = min(math.ceil(pair_of(slow)), rotary_dim - 1)
             ramp = ((torch.arange(half, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
             inv = inv / factor * ramp + inv * (1 - ramp)
             given_scale = scaling.get("attention_factor")
             scale = float(given_scale) if given_scale is not None else 0.1 * math.log(factor) + 1
         else:
-            length = float(scaling["original_max_position"])
             slow, fast = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
             if not 0 < slow < fast:
                 raise ValueError(f"low_freq_factor {slow} is not below high_freq_factor {fast}")
