@@ -500,7 +500,13 @@ NVK_API int nvk_fp8_paged_decode(void* out, const void* query, const void* kv_ca
                                  int head_dim, float scale, int num_ctas, void* workspace, size_t workspace_bytes,
                                  int* error_word, nvk_stream_t stream);
 
-/* nvk_paged_prefill over an 8-bit pool, with the conditions of nvk_fp4_paged_prefill. */
+/*
+ * nvk_paged_prefill over an 8-bit pool, with the conditions of
+ * nvk_fp4_paged_prefill. With few (query tile, head) items each one's keys are
+ * divided over several CTAs, by the number of items and max_blocks_per_seq: a
+ * call repeats bit for bit, but the same rows under a wider table, or among
+ * other sequences, may differ in the last bits.
+ */
 NVK_API int nvk_fp8_paged_prefill(void* out, const void* query, const void* kv_cache, int num_blocks, int block_size,
                                   const int32_t* block_tables, int block_table_stride, int max_blocks_per_seq,
                                   const int32_t* cu_seqlens_q, const int32_t* kv_lens, int batch, int total_q,

@@ -116,7 +116,8 @@ constexpr int kDecodeWarp0 = 12;          // quantised pools: warps 12-15
 constexpr int kThreadsDecoding = 16 * 32;
 // Registers a thread after the split of the decoding kernels' 512 x 128 (softmax, softmax, producer and MMA, decoders)
 constexpr int kRegsSoftmax = 176, kRegsIssue = 64, kRegsDecode = 96;
-// (8-bit: 184, 56 and 88 take 96.9 us for 97.4, 184, 48 and 96 108.8, 168, 64 and 112 106.7: what is spilled)
+// (8-bit: 184, 56 and 88 take 96.9 us for 97.4, within what repeats of one differ by, so that both kernels share one
+// split; 184, 48 and 96 108.8, 168, 64 and 112 106.7: what is spilled)
 static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsDecode <= 4 * 128, "setmaxnreg shares exceed the launch's registers");
 constexpr uint32_t kTmemCols = 512;       // S_0 | S_1 | O_0 | O_1, 128 columns each
 constexpr uint32_t kColO = 256;
@@ -255,7 +256,9 @@ __device__ __forceinline__ void flag_error(const PrefillArgs& a, PrefillSmem& sm
 }
 
 // The decoding kernels hold P as 2^7 p: p is at most 2^8 (see kRescaleThreshold),
-// so fp16 takes it, with 11 bits down to p = 2^-21.
+// so fp16 takes it, with 11 bits down to p = 2^-21. (8-bit kernel: p 2^e in p's
+// place. The largest one is held as 2^7 or more, so that a weight is off by
+// 2^-11 of itself or by 2^-32 of the largest one, half of fp16's least step.)
 template <bool kDecoding>
 constexpr float kPShift = kDecoding ? 7.f : 0.f;
 
@@ -462,7 +465,7 @@ __device__ __forceinline__ void decode_chunks(Chunks& x, uint32_t tile, int r0, 
 // more. (45 items on clusters of three: 10 tiles each 20.9 us, undivided 26.1; 8
 // tiles 19.6 and 22.0; 6 tiles 18.2 and 18.0. Nine items on clusters of eight: 6
 // tiles 11.9 and 17.6, 20 tiles 15.8 and 45.9. 128 queries over 8192 keys, 16
-// heads on 8: 31.9 and 146; one query over 4097 19.6 and 78; 16 over 32784 100
+// heads on 8: 31.9 and 146; one query over 4097 19.4 and 78; 16 over 32784 96
 // and 612.)
 constexpr int kSavedTiles = 4, kMostParts = 8;
 struct Part {
@@ -1128,7 +1131,7 @@ __device__ __forceinline__ void prefill_body(const CUtensorMap& qmap, const CUte
         mbar_arrive(&sm.p_hi[s]);
       }
       if (!ok) break;
-      // (8-bit kernel: the descriptor is read again, since its fields would be spilled in the loop above: 98.0 -> 97.4 us)
+      // (8-bit kernel: the descriptor is read again, since its fields would be spilled in the loop above: 98.0 -> 97.2 us)
       if constexpr (kExps) it = sm.items[qi % kItemRing];
       const int rows = min(kRows, it.lq - it.qt * kRows);
       __nv_bfloat16* out = a.out + (static_cast<int64_t>(it.q0 + it.qt * kRows) * a.num_heads + it.h0 + s) * kD;
