@@ -62,11 +62,12 @@ __global__ void __launch_bounds__(32 * kWarps) copy_kernel(const CopyArgs a) {
     const int part = static_cast<int>(w - block * a.parts), rest = static_cast<int>(block - pair * lt);
     const int tensor = rest / a.layers, layer = rest - tensor * a.layers;
     const int2 p = a.pairs[pair];
-    if (p.y == -1 || p.x == p.y) return;
+    if (p.y == -1) return;
     if (p.x < -1 || p.x >= a.num_blocks || p.y < 0 || p.y >= a.num_blocks) {
       if (a.err) atomicOr(a.err, kErrBadBlockId);
       return;
     }
+    if (p.x == p.y) return;
     const int64_t at = layer * a.layer_bytes + static_cast<int64_t>(part) * kPieceBytes;
     const uint64_t base = reinterpret_cast<uint64_t>(tensor ? a.base[1] : a.base[0]) + at;
     bytes = static_cast<int>(min(static_cast<int64_t>(kPieceBytes), a.block_bytes - static_cast<int64_t>(part) * kPieceBytes));
