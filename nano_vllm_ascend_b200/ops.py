@@ -128,11 +128,13 @@ def qk_norm_rope_append(
         query_out = torch.empty(tokens, num_heads, head_dim, dtype=_BF16, device=dev)
     elif query_out.shape != (tokens, num_heads, head_dim) or not query_out.is_contiguous() or query_out.dtype != _BF16:
         raise ValueError("qk_norm_rope_append: query_out must be a contiguous bf16 [tokens, heads, head_dim]")
+    # copies, where these make some, live until the launch
+    q_weight, k_weight, positions, slot_mapping = (t.contiguous() for t in (q_weight, k_weight, positions, slot_mapping))
     _lib.call(
         "nvk_qk_norm_rope_append", _ptr(query), _ptr(key), _ptr(value), query.stride(0), key.stride(0),
-        value.stride(0), _ptr(q_weight.contiguous()), _ptr(k_weight.contiguous()), float(eps), _ptr(cos_table),
-        _ptr(sin_table), cos_table.shape[0], _ptr(positions.contiguous()), _ptr(query_out), _ptr(key_cache),
-        _ptr(value_cache), _ptr(slot_mapping.contiguous()), tokens, num_blocks * block_size, num_heads, kvh,
+        value.stride(0), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos_table),
+        _ptr(sin_table), cos_table.shape[0], _ptr(positions), _ptr(query_out), _ptr(key_cache),
+        _ptr(value_cache), _ptr(slot_mapping), tokens, num_blocks * block_size, num_heads, kvh,
         head_dim, _ptr(error_word), _stream(dev),
     )
     return query_out
@@ -445,9 +447,10 @@ def paged_prefill(
         raise ValueError("paged_prefill: block_tables must be int32 [batch, max_blocks]")
     if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.numel() != batch + 1 or kv_lens.dtype != torch.int32:
         raise ValueError("paged_prefill: cu_seqlens_q must be int32 [batch+1] and kv_lens int32 [batch]")
+    cu_seqlens_q, kv_lens = cu_seqlens_q.contiguous(), kv_lens.contiguous()  # copies live until the launch
     _lib.call(
         "nvk_paged_prefill", _ptr(out), _ptr(query), _ptr(key_cache), _ptr(value_cache), num_blocks, block_size,
-        _ptr(block_tables), block_tables.stride(0), _ptr(cu_seqlens_q.contiguous()), _ptr(kv_lens.contiguous()),
+        _ptr(block_tables), block_tables.stride(0), _ptr(cu_seqlens_q), _ptr(kv_lens),
         batch, total_q, int(max_q_len), num_heads, kvh, head_dim, float(scale), _ptr(error_word), _stream(dev),
     )
     return out
@@ -478,9 +481,10 @@ def dense_prefill(
     batch = cu_seqlens_q.numel() - 1
     if d != head_dim or value.shape != key.shape or out.shape != query.shape or cu_seqlens_kv.numel() != batch + 1:
         raise ValueError("dense_prefill: shape mismatch")
+    cu_seqlens_q, cu_seqlens_kv = cu_seqlens_q.contiguous(), cu_seqlens_kv.contiguous()  # copies live until the launch
     _lib.call(
-        "nvk_dense_prefill", _ptr(out), _ptr(query), _ptr(key), _ptr(value), _ptr(cu_seqlens_q.contiguous()),
-        _ptr(cu_seqlens_kv.contiguous()), batch, total_q, total_kv, int(max_q_len), num_heads, kvh, head_dim,
+        "nvk_dense_prefill", _ptr(out), _ptr(query), _ptr(key), _ptr(value), _ptr(cu_seqlens_q),
+        _ptr(cu_seqlens_kv), batch, total_q, total_kv, int(max_q_len), num_heads, kvh, head_dim,
         float(scale), _ptr(error_word), _stream(dev),
     )
     return out
